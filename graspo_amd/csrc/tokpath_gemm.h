@@ -1,0 +1,289 @@
+// tokpath_gemm.h -- the matrix-core tile loop of the hidden-state losses (gfx950).
+//
+// One workgroup of 4 waves accumulates a 256 x 256 tile of A B^T in fp32 on
+// v_mfma_f32_32x32x16 (bf16 or fp16 operands), each wave 128 x 128 (4 x 4
+// blocks, 256 accumulators per lane).  K advances 64 at a time through two
+// LDS stages of 32 KB per operand, filled straight from global memory
+// (buffer_load_dwordx4 ... lds) while the matrix cores work on the other one.
+//
+// An operand lies in memory in one of two ways, and neither is copied or
+// transposed for the product:
+//
+// - kAlongK: a row per output index, K contiguous.  A stage holds 256 rows of
+//   128 bytes, whose eight 16-byte chunks are XOR-swizzled by bits 1-3 of the
+//   row, so that the 16 rows of a fragment read take all 16 bank groups.
+// - kAcrossK: a row per K index, output indices contiguous.  A stage holds 64
+//   rows of 512 bytes.  ds_read_b64_tr_b16 turns 4 rows x 16 columns around on
+//   the way out of LDS: of 16 lanes, lane i receives column i's 4 values.  The
+//   16-byte chunks are XOR-swizzled by 4 (row & 3), so that the 4 rows x 64
+//   bytes that half a wave reads take all 64 banks.
+//
+// Nothing past an operand's rows or its K is read: the buffer resource ends
+// with the last valid row, a chunk past K gets an offset past that end, and a
+// load out of range writes zeros to LDS.
+#pragma once
+
+#include "tokpath_stream.h"
+
+namespace gtp {
+namespace gemm {
+
+constexpr int kTile = 256;             // rows and columns of a tile
+constexpr int kBK = 64;                // K per stage
+constexpr int kWaves = 4;
+constexpr int kThreads = kWaves * 64;
+constexpr int kB = 4;                  // 32-wide blocks per wave along each side
+constexpr int kQ = 8;                  // 1 KB loads per wave, operand and K step
+constexpr int kStage = kTile * kBK / 8;  // 16-byte chunks per operand stage
+constexpr int kLds = 4 * kStage;         // chunks of all stages: 128 KB
+constexpr int kXcds = 8;
+constexpr int kMaxLd = (1 << 22) - 1;  // row strides (elements): 256 rows fit a buffer range
+constexpr int kRsrcWord3 = 0x00020000;  // raw buffer: 32-bit data format, no swizzle
+constexpr uint32_t kPast = 0x80000000u;  // an offset past every resource
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef __attribute__((address_space(3))) void lds_void;
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+
+enum Layout { kAlongK, kAcrossK };
+
+// 16-bit element types: product and rounding (nearest, ties to even)
+struct Bf16 {
+  __device__ static __forceinline__ f32x16 mfma(s16x8 a, s16x8 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a),
+                                                   __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  }
+  __device__ static __forceinline__ uint16_t from(float v) {
+    return __builtin_bit_cast(uint16_t, (__bf16)v);
+  }
+  __device__ static __forceinline__ float to(uint16_t v) { return u2f((uint32_t)v << 16); }
+};
+struct F16 {
+  __device__ static __forceinline__ f32x16 mfma(s16x8 a, s16x8 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a),
+                                                  __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  }
+  __device__ static __forceinline__ uint16_t from(float v) {
+    return __builtin_bit_cast(uint16_t, (_Float16)v);
+  }
+  __device__ static __forceinline__ float to(uint16_t v) { return f16_to_f32(v); }
+};
+
+// `outer` rows (kAlongK) or columns (kAcrossK) of 16-bit values; rows 16-byte
+// aligned and `ld` elements apart, ld and (kAcrossK) outer multiples of 8.
+struct Operand {
+  const uint16_t* p;
+  int64_t ld, outer;
+};
+
+// s_waitcnt vmcnt(0), the other counters untouched
+__device__ __forceinline__ void wait_vm0() { __builtin_amdgcn_s_waitcnt(0x0F70); }
+
+// An accumulator read straight from its AGPR (keeps the compiler from
+// copying every accumulator to VGPRs at once before an epilogue).
+__device__ __forceinline__ float acc_read(float a) {
+  float v;
+  asm volatile("v_accvgpr_read_b32 %0, %1" : "=v"(v) : "a"(a));
+  return v;
+}
+
+// Where one operand's K steps come from: wave w's load q of a step fills the
+// 1 KB of LDS from chunk (8w + q) * 64 on, 16 bytes per lane.
+template <Layout L>
+struct Source {
+  const uint16_t* base;  // the tile's first row (kAlongK) or column (kAcrossK)
+  int64_t ld, K;
+  uint32_t v0, v1;       // the lane's byte offset for even and odd q
+  int c0, c1;            // kAlongK: its chunk within the K step
+  uint32_t qstep;        // bytes from q to q + 2, halved
+  int64_t bytes;         // kAlongK: of the tile's valid rows; kAcrossK: valid columns
+  __device__ __forceinline__ Source(const Operand& o, int64_t first, int64_t K_, int wave,
+                                    int lane) {
+    ld = o.ld;
+    K = K_;
+    if constexpr (L == kAlongK) {
+      base = o.p + first * ld;
+      bytes = max((int64_t)0, min((int64_t)kTile, o.outer - first)) * ld * 2;
+      // LDS row 8 (8w + q) + lane / 8, chunk lane & 7 of it holding chunk
+      // (lane & 7) ^ ((row >> 1) & 7) of the row
+      const int row = wave * kQ * 8 + (lane >> 3);
+      c0 = (lane & 7) ^ ((lane >> 4) & 7);
+      c1 = (lane & 7) ^ ((4 + (lane >> 4)) & 7);
+      v0 = (uint32_t)((row * ld + c0 * 8) * 2);
+      v1 = (uint32_t)((row * ld + c1 * 8) * 2);
+      qstep = (uint32_t)(8 * ld * 2);
+    } else {
+      base = o.p + first;
+      bytes = max((int64_t)0, o.outer - first) * 2;
+      // LDS row 2 (8w + q) + lane / 32, chunk lane & 31 of it holding chunk
+      // (lane & 31) ^ 4 (row & 3) of the row
+      const int row = wave * kQ * 2 + (lane >> 5);
+      v0 = (uint32_t)((row * ld + ((lane & 31) ^ ((lane >> 5) << 2)) * 8) * 2);
+      v1 = (uint32_t)((row * ld + ((lane & 31) ^ ((2 + (lane >> 5)) << 2)) * 8) * 2);
+      c0 = c1 = 0;
+      qstep = (uint32_t)(2 * ld * 2);
+    }
+  }
+  __device__ __forceinline__ __amdgpu_buffer_rsrc_t rsrc(int64_t k0) const {
+    if constexpr (L == kAlongK) {
+      return __builtin_amdgcn_make_buffer_rsrc((void*)base, (short)0, (int)bytes, kRsrcWord3);
+    } else {
+      const int64_t rows = min((int64_t)kBK, K - k0);
+      const int64_t n = rows <= 0 || bytes <= 0 ? 0 : (rows - 1) * ld * 2 + bytes;
+      return __builtin_amdgcn_make_buffer_rsrc((void*)(base + (n ? k0 * ld : 0)), (short)0, (int)n,
+                                               kRsrcWord3);
+    }
+  }
+  // the whole offset goes in the VGPR operand: the range check covers it
+  __device__ __forceinline__ void issue(int q, __amdgpu_buffer_rsrc_t r, int64_t k0, uint4* stage,
+                                        int wave) const {
+    uint32_t v = ((q & 1) ? v1 : v0) + (uint32_t)q * qstep;
+    if constexpr (L == kAlongK) {
+      v += (uint32_t)(k0 * 2);
+      if (((q & 1) ? c1 : c0) * 8 >= K - k0) v = kPast;
+    }
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_void*)(stage + (wave * kQ + q) * 64), 16, v,
+                                             0, 0, 0);
+  }
+};
+
+// Fragment x (32 outer indices from side * 128 + 32 x on) of k16 step kk:
+// lane l holds index l & 31 of it and k = 8 (l / 32) .. + 7.
+template <Layout L>
+__device__ __forceinline__ s16x8 fragment(const uint4* stage, int side, int x, int kk, int lane) {
+  if constexpr (L == kAlongK) {
+    const int ch = (2 * kk + (lane >> 5)) ^ ((lane >> 1) & 7);
+    return __builtin_bit_cast(s16x8, stage[(side * 128 + x * 32 + (lane & 31)) * 8 + ch]);
+  } else {
+    // row 16 kk + 8 (l / 32) + 4 h + r, columns 32 (4 side + x) + 16 ((l / 16) & 1) + 4 (l & 3)
+    const int r = (lane & 15) >> 2;
+    const int at = (8 * (lane >> 5) + r) * 512 + side * 256 + ((x ^ r) * 64) +
+                   ((lane >> 4) & 1) * 32 + (lane & 3) * 8;
+    const char* p = reinterpret_cast<const char*>(stage) + at + kk * 16 * 512;
+    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)p);
+    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p + 4 * 512));
+    return s16x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+  }
+}
+
+// acc[x][y] += A rows (block x) times B rows (block y) over K steps
+// [k_first, k_first + K): lane l of a block holds B index l & 31 and the A
+// indices 8 (i / 4) + 4 (l / 32) + (i & 3) for i = 0 .. 15.  Ends with the
+// accumulators complete and every wave past its last LDS read.
+template <typename E, Layout LA, Layout LB>
+__device__ __forceinline__ void accumulate(const Source<LA>& a, const Source<LB>& b, int64_t k_first,
+                                           int64_t K, uint4* sm, int wave, int lane,
+                                           f32x16 (&acc)[kB][kB]) {
+  uint4 *sA0 = sm, *sA1 = sm + kStage, *sB0 = sm + 2 * kStage, *sB1 = sm + 3 * kStage;
+  const int wa = wave >> 1, wb = wave & 1;
+  // an even number of steps (the stages alternate); one past K adds zeros
+  const int total = 2 * (int)((K + 2 * kBK - 1) / (2 * kBK));
+  auto k_of = [&](int it) { return k_first + (int64_t)it * kBK; };
+  auto issue_one = [&](int j, __amdgpu_buffer_rsrc_t ra, __amdgpu_buffer_rsrc_t rb, int64_t k0,
+                       uint4* sa, uint4* sb) {
+    if (j & 1)
+      b.issue(j >> 1, rb, k0, sb, wave);
+    else
+      a.issue(j >> 1, ra, k0, sa, wave);
+  };
+  s16x8 fa[2][kB], fb[2][kB];
+  auto read_frags = [&](const uint4* sa, const uint4* sb, int kk, s16x8 (&f)[kB], s16x8 (&g)[kB]) {
+#pragma unroll
+    for (int x = 0; x < kB; ++x) f[x] = fragment<LA>(sa, wa, x, kk, lane);
+#pragma unroll
+    for (int y = 0; y < kB; ++y) g[y] = fragment<LB>(sb, wb, y, kk, lane);
+  };
+  // 16 MFMAs of one k16 step from fragment set c, with loads j0, j0 + 1, ...
+  // after every second one
+  auto mfma16 = [&](int c, bool load, int j0, __amdgpu_buffer_rsrc_t ra, __amdgpu_buffer_rsrc_t rb,
+                    int64_t k0, uint4* la, uint4* lb) {
+#pragma unroll
+    for (int x = 0; x < kB; ++x) {
+#pragma unroll
+      for (int y = 0; y < kB; ++y) {
+        acc[x][y] = E::mfma(fa[c][x], fb[c][y], acc[x][y]);
+        if (load && (y & 1)) issue_one(j0 + x * (kB / 2) + (y >> 1), ra, rb, k0, la, lb);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  // K step `it` from LDS stage (ca, cb), whose first k16 fragments are already
+  // in set 0.  Step it + 1 lives in (na, nb): its loads 0-7 went out during
+  // the last k16 of step it - 1, its loads 8-15 go out during the first k16
+  // here.  The barrier that publishes it sits before the last k16: every wave
+  // has read all of step it's fragments by then, so the loads 0-7 of step
+  // it + 2 into (ca, cb) go out during that last k16, while step it + 1's
+  // first fragments are read.
+  auto step = [&](int it, uint4* ca, uint4* cb, uint4* na, uint4* nb) {
+    const bool has1 = it + 1 < total, has2 = it + 2 < total;
+    const int64_t k1 = k_of(has1 ? it + 1 : it), k2 = k_of(has2 ? it + 2 : it);
+    const __amdgpu_buffer_rsrc_t a1 = a.rsrc(k1), b1 = b.rsrc(k1), a2 = a.rsrc(k2), b2 = b.rsrc(k2);
+    read_frags(ca, cb, 1, fa[1], fb[1]);
+    __builtin_amdgcn_sched_barrier(0);
+    mfma16(0, has1, kQ, a1, b1, k1, na, nb);
+    read_frags(ca, cb, 2, fa[0], fb[0]);
+    __builtin_amdgcn_sched_barrier(0);
+    mfma16(1, false, 0, a1, b1, 0, na, nb);
+    read_frags(ca, cb, 3, fa[1], fb[1]);
+    __builtin_amdgcn_sched_barrier(0);
+    mfma16(0, false, 0, a1, b1, 0, na, nb);
+    wait_vm0();
+    __syncthreads();
+    if (has1) read_frags(na, nb, 0, fa[0], fb[0]);
+    __builtin_amdgcn_sched_barrier(0);
+    mfma16(1, has2, 0, a2, b2, k2, ca, cb);
+  };
+  if (total > 0) {
+    const __amdgpu_buffer_rsrc_t a0 = a.rsrc(k_of(0)), b0 = b.rsrc(k_of(0));
+    const __amdgpu_buffer_rsrc_t a1 = a.rsrc(k_of(1)), b1 = b.rsrc(k_of(1));
+#pragma unroll
+    for (int j = 0; j < 2 * kQ; ++j) issue_one(j, a0, b0, k_of(0), sA0, sB0);
+#pragma unroll
+    for (int j = 0; j < kQ; ++j) issue_one(j, a1, b1, k_of(1), sA1, sB1);
+    wait_vm0();
+    __syncthreads();
+    read_frags(sA0, sB0, 0, fa[0], fb[0]);
+    for (int it = 0; it < total; it += 2) {
+      step(it, sA0, sB0, sA1, sB1);
+      step(it + 1, sA1, sB1, sA0, sB0);
+    }
+  }
+  __syncthreads();
+  // epilogues read the accumulators by inline asm, which the compiler's hazard
+  // checks do not see: no MFMA may be scheduled past this point, and 24 wait
+  // states after the last one cover its result latency (11 for an 8-pass MFMA)
+  __builtin_amdgcn_sched_barrier(0);
+  asm volatile("s_nop 7\n\ts_nop 7\n\ts_nop 7" ::: "memory");
+}
+
+// The order of a grid of tiles.  Workgroup b runs on XCD b mod 8; the 32 that
+// share an XCD's L2 at a time cover a block of h x 32 / h tiles: 8 x 4 where
+// the grid has that many (12 operand tiles per K step, the fewest for 32
+// workgroups), else as near as it goes.  h is picked on the host for the most
+// tiles that there can be, and fits any smaller grid.
+inline int block_rows(int64_t tm, int64_t tn) {
+  int h = 8;
+  while (h > 1 && h / 2 >= tm) h /= 2;
+  while (h < 32 && 32 / h / 2 >= tn) h *= 2;
+  return h;
+}
+inline int64_t grid_of(int64_t tm, int64_t tn, int h) {
+  const int64_t w = 32 / h, blocks = ((tm + h - 1) / h) * ((tn + w - 1) / w);
+  return (blocks + kXcds - 1) / kXcds * kXcds * 32;
+}
+// The tile (m, n) of workgroup b; false for one past the last.
+__device__ __forceinline__ bool tile_of(uint32_t b, int tm, int tn, int h, int& m, int& n) {
+  if (tm <= 0 || tn <= 0) return false;
+  const int w = 32 / h, rows = (tm + h - 1) / h;
+  const int i = b / kXcds, block = i / 32 * kXcds + b % kXcds, j = i % 32;
+  m = block % rows * h + j % h;
+  n = block / rows * w + j / h;
+  return m < tm && n < tn;
+}
+
+}  // namespace gemm
+}  // namespace gtp

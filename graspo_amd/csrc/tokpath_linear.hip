@@ -1,0 +1,861 @@
+// tokpath_linear.hip -- token logprobs from hidden states in pieces of the
+// vocabulary, without keeping the logits, and their gradients (gfx950).
+//
+//   x_nv  = h_n . w_v            lse_n = log sum_v exp(x_nv)
+//   lp_n  = x_{n,t_n} - lse_n    dx_nv = g_n ([v = t_n] - exp(x_nv - lse_n))
+//   dh_n  = sum_v dx_nv w_v      dw_v  = sum_n dx_nv h_n
+//
+// over bf16 or fp16 hidden states [B, S, K] and weight [V, K].  Four products
+// of 2 N K V operations (the logits, the logits again, dh, dw) on the matrix
+// cores, every one accumulated in fp32 by the tile loop of tokpath_gemm.h.
+//
+// - Forward: the logits of a 256 x 256 tile fold into (m, s) per token in
+//   registers; one partial state per (128 vocabulary rows, token), merged by
+//   a small kernel.
+// - Backward, piece by piece of the vocabulary: the piece's logits again,
+//   their gradient D rounded once to 16 bits (each element within half a step
+//   of its fp32 value; fp16 scaled by a power of two that puts the largest
+//   |g| just below 2^15, so that small probabilities keep their bits) and
+//   written vocabulary-major; then dh += D^T w and dw = D h from it, both
+//   accumulated in fp32 and rounded once.  A piece's D takes at most
+//   kPieceBytes whatever V is.
+//
+// Rows whose target is ignored, whose target lies outside [0, V) or (backward)
+// whose g is 0 are left out of every product: a first kernel lists the others
+// in order and a second gathers their hidden states, so the products run over
+// the listed rows alone.  Their number stays on the device; grids are sized
+// for all rows, and workgroups past the listed ones end at once.
+//
+// Nothing is summed with atomics: every sum has one order, fixed by the sizes
+// and the listed rows.
+//
+// Replaces the chunked F.linear + logsumexp + logaddexp loop of
+// _selected_token_log_probs_from_hidden
+// (src/graspo/backends/graspoflow/tensor_utils.py:167-186) under autograd,
+// which keeps every chunk's logits.
+#include "tokpath_gemm.h"
+
+namespace gtp {
+
+int64_t device_cus();  // compute units of the current device
+
+namespace lin {
+
+using namespace gemm;
+
+// Bytes of D at a time.
+constexpr int64_t kPieceBytes = (int64_t)512 << 20;
+
+struct Rows {
+  const void* targets;
+  int64_t V, S, T, tbstride, trstride, ignore;
+  int B, t64, has_ignore;
+  __device__ __forceinline__ int64_t target(int64_t b, int64_t s) const {
+    const int64_t at = b * tbstride + s * trstride;
+    return t64 ? reinterpret_cast<const int64_t*>(targets)[at]
+               : (int64_t)reinterpret_cast<const int32_t*>(targets)[at];
+  }
+};
+
+// What the listing kernel leaves for the others.
+struct Meta {
+  int32_t n;     // listed rows
+  int32_t bad;   // rows whose target lies outside [0, V)
+  float inv;     // 1 / the power of two in D
+  int32_t pad;
+};
+
+// One listed row.
+struct Listed {
+  int32_t* at;     // its index b * T + s
+  int32_t* target;
+  float* lse;      // backward only
+  float* g;        // backward only: times the power of two
+};
+
+// ------------------------------------------------------------ listing
+
+constexpr int kListBlock = 1024;
+
+// One workgroup; a thread takes a run of rows, counts those to list, and
+// lists them from where the threads before it end: the order stays.  out_lp
+// (forward): 0 for ignored rows and NaN for bad ones.  slot (backward): the
+// list index of each of the B x S positions, -1 for none.
+__global__ __launch_bounds__(kListBlock) void list_rows_kernel(
+    Rows a, Listed out, Meta* __restrict__ meta, float* __restrict__ out_lp,
+    float* __restrict__ out_lse, uint32_t* __restrict__ verdict, const float* __restrict__ grad,
+    const int64_t* __restrict__ mean_count, const float* __restrict__ lse_in,
+    int32_t* __restrict__ slot, int scaled) {
+  __shared__ uint32_t sums[kListBlock / kWave];
+  __shared__ float tops[kListBlock / kWave];
+  const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
+  const int64_t N = (int64_t)a.B * a.T, per = (N + kListBlock - 1) / kListBlock;
+  const int64_t first = min(N, tid * per), last = min(N, first + per);
+  const bool backward = grad != nullptr;
+  const float gm = backward && mean_count ? -grad[0] / (float)mean_count[0] : 0.0f;
+  auto g_of = [&](int64_t n) { return mean_count ? gm : grad[n]; };
+  uint32_t count = 0;
+  float top = 0.0f;
+  int bad = 0;
+  for (int64_t n = first; n < last; ++n) {
+    const int64_t b = n / a.T, s = n - b * a.T, t = a.target(b, s);
+    if (a.has_ignore && t == a.ignore) continue;
+    if (t < 0 || t >= a.V) {
+      bad = 1;
+      continue;
+    }
+    if (backward) {
+      const float g = g_of(n);
+      if (g == 0.0f) continue;
+      top = fmaxf(top, fabsf(g));
+    }
+    ++count;
+  }
+  uint32_t upto = wave_scan_u32(count);
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, kWave));
+  if (lane == 63) sums[wid] = upto;
+  if (lane == 0) tops[wid] = top;
+  const int any_bad = __syncthreads_or(bad);
+  uint32_t before = upto - count, all = 0;
+  top = 0.0f;
+#pragma unroll
+  for (int w = 0; w < kListBlock / kWave; ++w) {
+    before += w < wid ? sums[w] : 0;
+    all += sums[w];
+    top = fmaxf(top, tops[w]);
+  }
+  // fp16: 2^(15 - e) for 2^(e-1) <= top < 2^e (bounded, so that neither it nor
+  // its inverse leaves fp32's normal numbers)
+  float scale = 1.0f;
+  if (scaled && top > 0.0f && top < kPosInf) {
+    int e;
+    frexpf(top, &e);
+    scale = ldexpf(1.0f, min(max(15 - e, -100), 100));
+  }
+  if (tid == 0) {
+    *meta = Meta{(int32_t)all, any_bad, 1.0f / scale, 0};
+    if (verdict)
+      __hip_atomic_store(verdict, GTP_VERDICT_GOOD | (any_bad ? GTP_VERDICT_BAD : 0u),
+                         __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
+  }
+  uint32_t k = before;
+  for (int64_t n = first; n < last; ++n) {
+    const int64_t b = n / a.T, s = n - b * a.T, t = a.target(b, s);
+    const bool skip = a.has_ignore && t == a.ignore, out_of = t < 0 || t >= a.V;
+    float g = 0.0f;
+    if (backward && !skip && !out_of) g = g_of(n);
+    const bool take = !skip && !out_of && !(backward && g == 0.0f);
+    if (take) {
+      out.at[k] = (int32_t)n;
+      out.target[k] = (int32_t)t;
+      if (backward) {
+        out.lse[k] = lse_in[n];
+        out.g[k] = g * scale;
+      }
+    } else if (out_lp) {
+      const float v = skip ? 0.0f : __builtin_nanf("");
+      out_lp[n] = v;
+      out_lse[n] = v;
+    }
+    if (slot) slot[b * a.S + s] = take ? (int32_t)k : -1;
+    k += take;
+  }
+  if (slot) {  // positions without a target
+    const int64_t rest = a.S - a.T;
+    for (int64_t i = tid; i < a.B * rest; i += kListBlock) {
+      const int64_t b = i / rest;
+      slot[b * a.S + a.T + (i - b * rest)] = -1;
+    }
+  }
+}
+
+// The listed rows' hidden states, one after the other, padded with zeros to
+// ld elements (a multiple of 64): one workgroup per row, 16 bytes per thread
+// where the rows allow it.
+__global__ __launch_bounds__(256) void gather_rows_kernel(const uint16_t* __restrict__ hidden,
+                                                          int64_t hb, int64_t hs, int64_t T,
+                                                          int64_t K, const Meta* __restrict__ meta,
+                                                          const int32_t* __restrict__ at, int vec,
+                                                          uint16_t* __restrict__ out, int64_t ld) {
+  const int64_t k = blockIdx.x;
+  if (k >= meta->n) return;
+  const int64_t n = at[k], b = n / T, s = n - b * T;
+  const uint16_t* src = hidden + b * hb + s * hs;
+  uint16_t* dst = out + k * ld;
+  for (int64_t c = threadIdx.x; c < ld / 8; c += 256) {
+    uint4 v{0, 0, 0, 0};
+    if (vec) {
+      if (c * 8 < K) v = reinterpret_cast<const uint4*>(src)[c];
+    } else {
+      uint32_t e[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int64_t lo = c * 8 + 2 * i;
+        e[i] = lo < K ? src[lo] : 0u;
+        if (lo + 1 < K) e[i] |= (uint32_t)src[lo + 1] << 16;
+      }
+      v = uint4{e[0], e[1], e[2], e[3]};
+    }
+    reinterpret_cast<uint4*>(dst)[c] = v;
+  }
+}
+
+// ------------------------------------------------------------ forward
+
+struct LseArgs {
+  Operand w, h;  // [V, K], listed rows [., K]
+  int64_t K;
+  const Meta* meta;
+  const int32_t* target;  // of the listed rows
+  float2* partial;        // [2 * tiles of V][ldn]: (m, s)
+  float* xt;              // the target's logit of the listed rows
+  int64_t ldn;
+  int tm, h_order;        // tiles of V; block rows of the tile order
+};
+
+// merge of two (m, s) states; an empty one is (-inf, 0)
+__device__ __forceinline__ float2 merge_ms(float2 a, float2 b) {
+  const float m = fmaxf(a.x, b.x);
+  const float fa = a.x == m ? 1.0f : __builtin_amdgcn_exp2f((a.x - m) * kLog2e);
+  const float fb = b.x == m ? 1.0f : __builtin_amdgcn_exp2f((b.x - m) * kLog2e);
+  return float2{m, a.y * fa + b.y * fb};
+}
+
+// Vocabulary x tokens: lane l of a block holds token l & 31 and 16 vocabulary
+// rows, so that a token's values fold in registers.
+template <typename E>
+__global__ __launch_bounds__(kThreads, 1) void lse_kernel(LseArgs a) {
+  __shared__ __attribute__((aligned(16))) uint4 sm[kLds];
+  const int n_listed = a.meta->n;
+  int vt, tt;
+  if (!tile_of(blockIdx.x, a.tm, (n_listed + kTile - 1) / kTile, a.h_order, vt, tt)) return;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wv = wave >> 1, wt = wave & 1;
+  f32x16 acc[kB][kB];
+#pragma unroll
+  for (int x = 0; x < kB; ++x)
+#pragma unroll
+    for (int y = 0; y < kB; ++y) acc[x][y] = f32x16{};
+  Operand h = a.h;
+  h.outer = n_listed;
+  const Source<kAlongK> sa(a.w, (int64_t)vt * kTile, a.K, wave, lane);
+  const Source<kAlongK> sb(h, (int64_t)tt * kTile, a.K, wave, lane);
+  accumulate<E>(sa, sb, 0, a.K, sm, wave, lane, acc);
+
+  // the lane's vocabulary rows are v0 + 32 x + 8 (i / 4) + (i & 3)
+  const int64_t v0 = (int64_t)vt * kTile + wv * 128 + 4 * (lane >> 5);
+  const int64_t left = a.w.outer - v0;
+  const int lim = (int)min((int64_t)128, max(left, (int64_t)0));  // valid offsets are below
+#pragma unroll 1
+  for (int r = 0; r < kB; ++r) {  // token blocks, rotated through block 0
+    const int64_t k = (int64_t)tt * kTile + wt * 128 + r * 32 + (lane & 31);
+    const int64_t off = (k < n_listed ? (int64_t)a.target[k] : -1) - v0;
+    float2 st{kNegInf, 0.0f};
+#pragma unroll
+    for (int x = 0; x < kB; ++x) {
+      float v[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) v[i] = acc_read(acc[x][0][i]);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int o = x * 32 + 8 * (i >> 2) + (i & 3);
+        if (off == o) a.xt[k] = v[i];
+        if (o >= lim) v[i] = kNegInf;
+      }
+      float m = v[0];
+#pragma unroll
+      for (int i = 1; i < 16; i += 2) m = max3raw(m, v[i], i + 1 < 16 ? v[i + 1] : v[i]);
+      m = fmaxf(m, st.x);
+      // (the difference first: exact near the maximum, however large that is)
+      const float mb = m == kNegInf ? 0.0f : m;
+      float s = 0.0f;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s += __builtin_amdgcn_exp2f((v[i] - mb) * kLog2e);
+      const float f = st.x == m ? 1.0f : __builtin_amdgcn_exp2f((st.x - m) * kLog2e);
+      st = float2{m, __builtin_fmaf(st.y, f, s)};
+    }
+    const float2 other{__shfl_xor(st.x, 32, kWave), __shfl_xor(st.y, 32, kWave)};
+    st = merge_ms(st, other);
+    if (lane < 32 && k < n_listed) a.partial[(int64_t)(vt * 2 + wv) * a.ldn + k] = st;
+#pragma unroll
+    for (int y = 0; y < kB - 1; ++y)
+#pragma unroll
+      for (int x = 0; x < kB; ++x) acc[x][y] = acc[x][y + 1];
+  }
+}
+
+// The listed rows' logprob and lse from their partial states: 16 rows per
+// workgroup, 16 threads each merging every 16th state, then one merge in LDS.
+constexpr int kMergeTok = 16, kMergeGrp = 16;
+__global__ __launch_bounds__(256) void lse_merge_kernel(const float2* __restrict__ partial,
+                                                        int64_t ldn, int n_parts,
+                                                        const Meta* __restrict__ meta,
+                                                        const int32_t* __restrict__ at,
+                                                        const float* __restrict__ xt,
+                                                        float* __restrict__ out_lp,
+                                                        float* __restrict__ out_lse) {
+  __shared__ float2 red[kMergeGrp][kMergeTok];
+  const int lt = threadIdx.x % kMergeTok, g = threadIdx.x / kMergeTok;
+  const int64_t k = (int64_t)blockIdx.x * kMergeTok + lt;
+  const int n = meta->n;
+  if ((int64_t)blockIdx.x * kMergeTok >= n) return;
+  float2 st{kNegInf, 0.0f};
+  if (k < n) {
+#pragma unroll 4
+    for (int p = g; p < n_parts; p += kMergeGrp) st = merge_ms(st, partial[p * ldn + k]);
+  }
+  red[g][lt] = st;
+  __syncthreads();
+  if (g != 0 || k >= n) return;
+#pragma unroll
+  for (int q = 1; q < kMergeGrp; ++q) st = merge_ms(st, red[q][lt]);
+  const float ln_s = __builtin_amdgcn_logf(st.y) * kLn2;
+  out_lp[at[k]] = (xt[k] - st.x) - ln_s;
+  out_lse[at[k]] = st.x + ln_s;
+}
+
+// -sum(logprob) / count over the listed rows and the bad ones (whose NaN is
+// the mean then), in 64 bits, one workgroup.
+__global__ __launch_bounds__(1024) void mean_kernel(const Meta* __restrict__ meta,
+                                                    const int32_t* __restrict__ at,
+                                                    const float* __restrict__ lp,
+                                                    float* __restrict__ loss,
+                                                    int64_t* __restrict__ count) {
+  __shared__ double sums[1024 / kWave];
+  const int n = meta->n;
+  double sum = 0.0;
+  for (int k = threadIdx.x; k < n; k += 1024) sum += (double)lp[at[k]];
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, kWave);
+  if ((threadIdx.x & 63) == 0) sums[threadIdx.x >> 6] = sum;
+  __syncthreads();
+  if (threadIdx.x != 0) return;
+#pragma unroll
+  for (int w = 1; w < 1024 / kWave; ++w) sum += sums[w];
+  loss[0] = meta->bad ? __builtin_nanf("") : (float)(-sum / (double)n);
+  count[0] = n;
+}
+
+// ------------------------------------------------------------ backward
+
+// 32 rows x 128 columns of 16-bit values, held as lane = row and 4 columns in
+// a row per (x, j) by `value(x, j, e)`, written to `out` (row stride ld) as
+// whole 256-byte runs: through 8 KB of LDS of the wave's own, whose 16-byte
+// chunks are XOR-swizzled by the row.  `rows` and `cols` bound what is
+// written; vec: 16-byte stores (else 2-byte ones).
+template <typename Value>
+__device__ __forceinline__ void store_block(uint4* mine, int lane, uint16_t* out, int64_t ld,
+                                            int64_t rows, int64_t cols, bool vec, Value value) {
+  const int row = lane & 31;
+  uint2* half = reinterpret_cast<uint2*>(mine);
+#pragma unroll
+  for (int x = 0; x < kB; ++x)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      uint16_t e[4];
+      value(x, j, e);
+      // columns 32 x + 8 j + 4 (lane / 32): chunk 4 x + j, its half lane / 32
+      half[(row * 16 + ((4 * x + j) ^ (row & 15))) * 2 + (lane >> 5)] =
+          uint2{(uint32_t)e[0] | (uint32_t)e[1] << 16, (uint32_t)e[2] | (uint32_t)e[3] << 16};
+    }
+  wave_lds_sync();
+  const int c = lane & 15;
+#pragma unroll
+  for (int q = 0; q < 8; ++q) {
+    const int r = q * 4 + (lane >> 4);
+    const uint4 v = mine[r * 16 + (c ^ (r & 15))];
+    if (r < rows && c * 8 < cols) {
+      uint16_t* to = out + r * ld + c * 8;
+      if (vec) {
+        *reinterpret_cast<uint4*>(to) = v;
+      } else {
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (c * 8 + i < cols) to[i] = (uint16_t)(w[i >> 1] >> (16 * (i & 1)));
+      }
+    }
+  }
+  wave_lds_sync();
+}
+
+struct GradArgs {
+  Operand h, w;  // listed rows [., K]; the piece's weight rows [., K]
+  int64_t K, v_first;
+  const Meta* meta;
+  Listed rows;
+  uint16_t* d;   // [piece rows][ldn]
+  int64_t ldn;
+  int tn, h_order;
+};
+
+// The piece's D: tokens x vocabulary, lane l of a block holding vocabulary row
+// l & 31 and 16 tokens, whose lse, g and targets are in LDS.
+template <typename E>
+__global__ __launch_bounds__(kThreads, 1) void grad_logits_kernel(GradArgs a) {
+  __shared__ __attribute__((aligned(16))) uint4 sm[kLds];
+  __shared__ __attribute__((aligned(16))) float s_lse[kTile], s_g[kTile];
+  __shared__ __attribute__((aligned(16))) int s_t[kTile];
+  const int n_listed = a.meta->n;
+  int tt, vt;
+  if (!tile_of(blockIdx.x, (n_listed + kTile - 1) / kTile, a.tn, a.h_order, tt, vt)) return;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wt = wave >> 1, wv = wave & 1;
+  {
+    const int64_t k = (int64_t)tt * kTile + threadIdx.x;
+    const bool in = k < n_listed;
+    // a row past the last: exp(x - inf) = 0, times 0
+    s_lse[threadIdx.x] = in ? a.rows.lse[k] : kPosInf;
+    s_g[threadIdx.x] = in ? a.rows.g[k] : 0.0f;
+    s_t[threadIdx.x] = in ? (int)(a.rows.target[k] - a.v_first) : -1;
+  }
+  f32x16 acc[kB][kB];
+#pragma unroll
+  for (int x = 0; x < kB; ++x)
+#pragma unroll
+    for (int y = 0; y < kB; ++y) acc[x][y] = f32x16{};
+  Operand h = a.h;
+  h.outer = n_listed;
+  const Source<kAlongK> sa(h, (int64_t)tt * kTile, a.K, wave, lane);
+  const Source<kAlongK> sb(a.w, (int64_t)vt * kTile, a.K, wave, lane);
+  accumulate<E>(sa, sb, 0, a.K, sm, wave, lane, acc);
+
+#pragma unroll 1
+  for (int r = 0; r < kB; ++r) {
+    const int row0 = vt * kTile + wv * 128 + r * 32, v = row0 + (lane & 31);
+    const int64_t col0 = (int64_t)tt * kTile + wt * 128;
+    store_block(sm + wave * 512, lane, a.d + row0 * a.ldn + col0, a.ldn, a.w.outer - row0,
+                a.ldn - col0, true, [&](int x, int j, uint16_t (&e)[4]) {
+                  const int t0 = wt * 128 + x * 32 + j * 8 + 4 * (lane >> 5);
+                  const float4 l = *reinterpret_cast<const float4*>(s_lse + t0);
+                  const float4 g = *reinterpret_cast<const float4*>(s_g + t0);
+                  const int4 t = *reinterpret_cast<const int4*>(s_t + t0);
+                  const float ls[4] = {l.x, l.y, l.z, l.w}, gs[4] = {g.x, g.y, g.z, g.w};
+                  const int ts[4] = {t.x, t.y, t.z, t.w};
+#pragma unroll
+                  for (int i = 0; i < 4; ++i) {
+                    const float q = acc_read(acc[x][0][4 * j + i]);
+                    const float p = __builtin_amdgcn_exp2f((q - ls[i]) * kLog2e);
+                    e[i] = E::from(gs[i] * ((ts[i] == v ? 1.0f : 0.0f) - p));
+                  }
+                });
+#pragma unroll
+    for (int y = 0; y < kB - 1; ++y)
+#pragma unroll
+      for (int x = 0; x < kB; ++x) acc[x][y] = acc[x][y + 1];
+  }
+}
+
+struct HiddenArgs {
+  Operand d, w;  // D [piece rows][ldn] across K, the piece's weight rows across K
+  int64_t K;     // piece rows
+  const Meta* meta;
+  float* sum;    // [splits][N][width]
+  int64_t N, width;
+  int splits, first, tn, h_order;
+};
+
+// dh in fp32, summed over the pieces in place: a workgroup takes one tile's
+// share of the piece's rows.
+template <typename E>
+__global__ __launch_bounds__(kThreads, 1) void grad_hidden_kernel(HiddenArgs a) {
+  __shared__ __attribute__((aligned(16))) uint4 sm[kLds];
+  const int n_listed = a.meta->n;
+  int tt, ct;
+  if (!tile_of(blockIdx.x, (n_listed + kTile - 1) / kTile, a.tn, a.h_order, tt, ct)) return;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wt = wave >> 1, wc = wave & 1;
+  const int split = blockIdx.y;
+  const int64_t steps = (a.K + kBK - 1) / kBK, per = (steps + a.splits - 1) / a.splits * kBK;
+  const int64_t k0 = min(a.K, split * per), k1 = min(a.K, k0 + per);
+  f32x16 acc[kB][kB];
+#pragma unroll
+  for (int x = 0; x < kB; ++x)
+#pragma unroll
+    for (int y = 0; y < kB; ++y) acc[x][y] = f32x16{};
+  const Source<kAcrossK> sa(a.d, (int64_t)tt * kTile, k1, wave, lane);
+  const Source<kAcrossK> sb(a.w, (int64_t)ct * kTile, k1, wave, lane);
+  accumulate<E>(sa, sb, k0, k1 - k0, sm, wave, lane, acc);
+
+  float* sum = a.sum + (int64_t)split * a.N * a.width;
+#pragma unroll 1
+  for (int r = 0; r < kB; ++r) {
+    const int64_t col = (int64_t)ct * kTile + wc * 128 + r * 32 + (lane & 31);
+#pragma unroll
+    for (int x = 0; x < kB; ++x)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const float q = acc_read(acc[x][0][i]);
+        const int64_t k =
+            (int64_t)tt * kTile + wt * 128 + x * 32 + 8 * (i >> 2) + 4 * (lane >> 5) + (i & 3);
+        if (k < n_listed && col < a.width) {
+          float* to = sum + k * a.width + col;
+          *to = a.first ? q : *to + q;
+        }
+      }
+#pragma unroll
+    for (int y = 0; y < kB - 1; ++y)
+#pragma unroll
+      for (int x = 0; x < kB; ++x) acc[x][y] = acc[x][y + 1];
+  }
+}
+
+// grad_hidden [B x S, width] from the splits' sums; positions that were not
+// listed get zeros.
+template <typename E>
+__global__ __launch_bounds__(256) void grad_hidden_rows_kernel(const float* __restrict__ sum,
+                                                               int64_t N, int64_t width, int splits,
+                                                               const Meta* __restrict__ meta,
+                                                               const int32_t* __restrict__ slot,
+                                                               uint16_t* __restrict__ out) {
+  const int64_t pos = blockIdx.x;
+  const int k = slot[pos];
+  const float inv = meta->inv;
+  uint16_t* to = out + pos * width;
+  for (int64_t c = threadIdx.x; c < width; c += 256) {
+    float v = 0.0f;
+    if (k >= 0) {
+      for (int p = 0; p < splits; ++p) v += sum[(p * N + k) * width + c];
+      v *= inv;
+    }
+    to[c] = E::from(v);
+  }
+}
+
+struct WeightArgs {
+  Operand h, d;  // listed rows across K, D [piece rows][ldn] along K
+  const Meta* meta;
+  uint16_t* out;  // the piece's first row of grad_weight, row stride ld
+  int64_t ld, width;
+  int tm, tn, h_order, vec;
+};
+
+// dw of the piece's rows: hidden columns x vocabulary rows, over the listed
+// tokens.
+template <typename E>
+__global__ __launch_bounds__(kThreads, 1) void grad_weight_kernel(WeightArgs a) {
+  __shared__ __attribute__((aligned(16))) uint4 sm[kLds];
+  int ct, vt;
+  if (!tile_of(blockIdx.x, a.tm, a.tn, a.h_order, ct, vt)) return;
+  const int64_t K = a.meta->n;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wc = wave >> 1, wv = wave & 1;
+  f32x16 acc[kB][kB];
+#pragma unroll
+  for (int x = 0; x < kB; ++x)
+#pragma unroll
+    for (int y = 0; y < kB; ++y) acc[x][y] = f32x16{};
+  const Source<kAcrossK> sa(a.h, (int64_t)ct * kTile, K, wave, lane);
+  const Source<kAlongK> sb(a.d, (int64_t)vt * kTile, K, wave, lane);
+  accumulate<E>(sa, sb, 0, K, sm, wave, lane, acc);
+  const float inv = a.meta->inv;
+#pragma unroll 1
+  for (int r = 0; r < kB; ++r) {
+    const int64_t row0 = (int64_t)vt * kTile + wv * 128 + r * 32;
+    const int64_t col0 = (int64_t)ct * kTile + wc * 128;
+    store_block(sm + wave * 512, lane, a.out + row0 * a.ld + col0, a.ld, a.d.outer - row0,
+                a.width - col0, a.vec, [&](int x, int j, uint16_t (&e)[4]) {
+#pragma unroll
+                  for (int i = 0; i < 4; ++i) e[i] = E::from(acc_read(acc[x][0][4 * j + i]) * inv);
+                });
+#pragma unroll
+    for (int y = 0; y < kB - 1; ++y)
+#pragma unroll
+      for (int x = 0; x < kB; ++x) acc[x][y] = acc[x][y + 1];
+  }
+}
+
+// ------------------------------------------------------------ host
+
+inline size_t up(size_t n) { return (n + 255) / 256 * 256; }
+
+// A piece of the workspace, or its size alone where there is none.
+struct Carve {
+  unsigned char* base;
+  size_t at = 0;
+  template <typename T>
+  T* take(size_t count) {
+    T* p = base ? reinterpret_cast<T*>(base + at) : nullptr;
+    at += up(count * sizeof(T));
+    return p;
+  }
+};
+
+// The sizes that a call's kernels share.
+struct Shape {
+  int64_t N, K8, ldh, ldn;  // rows with a target; K to a multiple of 8; row strides
+  int n_vt, n_tt, n_ct;     // tiles of vocabulary, tokens and hidden columns
+};
+
+inline int tiles(int64_t n) { return (int)((n + kTile - 1) / kTile); }
+
+int shape_of(const gtp_linear_rows* r, Shape& s, Rows& a) {
+  if (!r || r->B < 0 || r->S < 0 || r->T < 0 || r->T > r->S || r->K <= 0 || r->V <= 0 ||
+      r->hidden_batch_stride < 0 || r->hidden_row_stride < 0 || r->weight_stride < r->K ||
+      r->target_batch_stride < 0 || r->target_row_stride < 0)
+    return GTP_ERR_INVALID_ARGUMENT;
+  if (r->dtype != GTP_DTYPE_BF16 && r->dtype != GTP_DTYPE_F16) return GTP_ERR_UNSUPPORTED;
+  if (r->B > kMaxLd || r->S > kMaxLd || r->B * r->S > kMaxLd - kTile || r->K > kMaxLd - 64 ||
+      r->V > 0x7FFFFFFFll - kTile)
+    return GTP_ERR_UNSUPPORTED;
+  s.N = r->B * r->T;
+  if (r->B * r->S > 0 && (!r->hidden || !r->weight || (s.N > 0 && !r->targets)))
+    return GTP_ERR_INVALID_ARGUMENT;
+  // the weight is read in place: whole 16-byte chunks of aligned rows
+  s.K8 = (r->K + 7) / 8 * 8;
+  if ((r->weight_stride & 7) || r->weight_stride < s.K8 || r->weight_stride > kMaxLd ||
+      (reinterpret_cast<uintptr_t>(r->weight) & 15u))
+    return GTP_ERR_UNSUPPORTED;
+  s.ldh = (r->K + 63) / 64 * 64;
+  s.ldn = (s.N + 7) / 8 * 8;
+  s.n_vt = tiles(r->V);
+  s.n_tt = tiles(s.N);
+  s.n_ct = tiles(s.K8);
+  // a launch holds fewer than 2^32 threads
+  if (grid_of(s.n_vt, s.n_tt, block_rows(s.n_vt, s.n_tt)) >= (int64_t)1 << 24 ||
+      grid_of(s.n_ct, s.n_vt, block_rows(s.n_ct, s.n_vt)) >= (int64_t)1 << 24)
+    return GTP_ERR_UNSUPPORTED;
+  a = Rows{r->targets, r->V, r->S, r->T, r->target_batch_stride, r->target_row_stride,
+           r->ignore_index, (int)r->B, r->targets_int64 ? 1 : 0, r->has_ignore ? 1 : 0};
+  return GTP_OK;
+}
+
+struct Forward {
+  Meta* meta;
+  int32_t *at, *target;
+  float* xt;
+  uint16_t* h;
+  float2* partial;
+  size_t bytes;
+};
+Forward forward_space(const Shape& s, void* ws) {
+  Carve c{reinterpret_cast<unsigned char*>(ws)};
+  Forward f;
+  f.meta = c.take<Meta>(1);
+  f.at = c.take<int32_t>(s.N);
+  f.target = c.take<int32_t>(s.N);
+  f.xt = c.take<float>(s.N);
+  f.h = c.take<uint16_t>(s.N * s.ldh);
+  f.partial = c.take<float2>((size_t)2 * s.n_vt * s.ldn);
+  f.bytes = c.at;
+  return f;
+}
+
+// Rows of the vocabulary per piece (a multiple of the tile), and the shares
+// that dh's products split a piece into, so that they fill the chip: rounds
+// of one workgroup per CU, each split costing a pass over its sums.
+struct Pieces {
+  int64_t rows;
+  int splits;
+};
+Pieces pieces_of(const Shape& s, int64_t V) {
+  Pieces p;
+  int64_t most = kPieceBytes / (s.ldn * 2) / kTile * kTile;
+  most = max(most, (int64_t)kTile);
+  const int64_t n = (V + most - 1) / most;
+  p.rows = min(most, ((V + n - 1) / n + kTile - 1) / kTile * kTile);
+  const int64_t cus = device_cus(), grid = (int64_t)s.n_tt * s.n_ct;
+  double best = 1e30;
+  p.splits = 1;
+  for (int k = 1; k <= 32 && p.rows / k >= 8 * kBK; ++k) {
+    const double cost = (double)((grid * k + cus - 1) / cus) / k + 0.01 * k;
+    if (cost < best) {
+      best = cost;
+      p.splits = k;
+    }
+  }
+  return p;
+}
+
+struct Backward {
+  Meta* meta;
+  Listed rows;
+  int32_t* slot;
+  uint16_t *h, *d;
+  float* sum;
+  size_t bytes;
+};
+Backward backward_space(const gtp_linear_rows* r, const Shape& s, const Pieces& p, void* ws) {
+  Carve c{reinterpret_cast<unsigned char*>(ws)};
+  Backward b;
+  b.meta = c.take<Meta>(1);
+  b.rows.at = c.take<int32_t>(s.N);
+  b.rows.target = c.take<int32_t>(s.N);
+  b.rows.lse = c.take<float>(s.N);
+  b.rows.g = c.take<float>(s.N);
+  b.slot = c.take<int32_t>(r->B * r->S);
+  b.h = c.take<uint16_t>(s.N * s.ldh);
+  b.d = c.take<uint16_t>(p.rows * s.ldn);
+  b.sum = c.take<float>((size_t)p.splits * s.N * r->K);
+  b.bytes = c.at;
+  return b;
+}
+
+void gather(const gtp_linear_rows* r, const Shape& s, const Meta* meta, const int32_t* at,
+            uint16_t* out, hipStream_t st) {
+  const int vec = ((reinterpret_cast<uintptr_t>(r->hidden) & 15u) == 0 &&
+                   (r->hidden_batch_stride & 7) == 0 && (r->hidden_row_stride & 7) == 0 &&
+                   (r->K & 7) == 0)
+                      ? 1
+                      : 0;
+  hipLaunchKernelGGL(gather_rows_kernel, dim3((unsigned)s.N), dim3(256), 0, st,
+                     reinterpret_cast<const uint16_t*>(r->hidden), r->hidden_batch_stride,
+                     r->hidden_row_stride, r->T, r->K, meta, at, vec, out, s.ldh);
+}
+
+template <typename E>
+void forward_launch(const gtp_linear_rows* r, const Shape& s, const Forward& f, hipStream_t st) {
+  LseArgs a;
+  a.w = Operand{reinterpret_cast<const uint16_t*>(r->weight), r->weight_stride, r->V};
+  a.h = Operand{f.h, s.ldh, s.N};
+  a.K = s.K8;
+  a.meta = f.meta;
+  a.target = f.target;
+  a.partial = f.partial;
+  a.xt = f.xt;
+  a.ldn = s.ldn;
+  a.tm = s.n_vt;
+  a.h_order = block_rows(s.n_vt, s.n_tt);
+  launch_timed(lse_kernel<E>, dim3((unsigned)grid_of(s.n_vt, s.n_tt, a.h_order)), dim3(kThreads),
+               st, a);
+}
+
+template <typename E>
+void backward_launch(const gtp_linear_rows* r, const Shape& s, const Pieces& p, const Backward& b,
+                     uint16_t* grad_hidden, uint16_t* grad_weight, hipStream_t st) {
+  const uint16_t* w = reinterpret_cast<const uint16_t*>(r->weight);
+  for (int64_t v0 = 0; s.N > 0 && v0 < r->V; v0 += p.rows) {
+    const int64_t rows = min(p.rows, r->V - v0);
+    const Operand piece{w + v0 * r->weight_stride, r->weight_stride, rows};
+    GradArgs g;
+    g.h = Operand{b.h, s.ldh, s.N};
+    g.w = piece;
+    g.K = s.K8;
+    g.v_first = v0;
+    g.meta = b.meta;
+    g.rows = b.rows;
+    g.d = b.d;
+    g.ldn = s.ldn;
+    g.tn = tiles(rows);
+    g.h_order = block_rows(s.n_tt, g.tn);
+    launch_timed(grad_logits_kernel<E>, dim3((unsigned)grid_of(s.n_tt, g.tn, g.h_order)),
+                 dim3(kThreads), st, g);
+    if (grad_hidden) {
+      HiddenArgs h;
+      h.d = Operand{b.d, s.ldn, s.ldn};
+      h.w = Operand{piece.p, piece.ld, s.K8};
+      h.K = rows;
+      h.meta = b.meta;
+      h.sum = b.sum;
+      h.N = s.N;
+      h.width = r->K;
+      h.splits = p.splits;
+      h.first = v0 == 0 ? 1 : 0;
+      h.tn = s.n_ct;
+      h.h_order = block_rows(s.n_tt, s.n_ct);
+      hipLaunchKernelGGL(grad_hidden_kernel<E>,
+                         dim3((unsigned)grid_of(s.n_tt, s.n_ct, h.h_order), (unsigned)p.splits),
+                         dim3(kThreads), 0, st, h);
+    }
+    if (grad_weight) {
+      WeightArgs q;
+      q.h = Operand{b.h, s.ldh, s.ldh};
+      q.d = Operand{b.d, s.ldn, rows};
+      q.meta = b.meta;
+      q.out = grad_weight + v0 * r->K;
+      q.ld = r->K;
+      q.width = r->K;
+      q.tm = s.n_ct;
+      q.tn = tiles(rows);
+      q.h_order = block_rows(q.tm, q.tn);
+      q.vec = (r->K & 7) == 0 && (reinterpret_cast<uintptr_t>(grad_weight) & 15u) == 0 ? 1 : 0;
+      hipLaunchKernelGGL(grad_weight_kernel<E>, dim3((unsigned)grid_of(q.tm, q.tn, q.h_order)),
+                         dim3(kThreads), 0, st, q);
+    }
+  }
+  if (grad_hidden)
+    hipLaunchKernelGGL(grad_hidden_rows_kernel<E>, dim3((unsigned)(r->B * r->S)), dim3(256), 0, st,
+                       b.sum, s.N, r->K, p.splits, b.meta, b.slot, grad_hidden);
+}
+
+}  // namespace lin
+}  // namespace gtp
+
+using namespace gtp;
+
+extern "C" size_t gtp_linear_logprob_workspace_bytes(const gtp_linear_rows* rows) {
+  lin::Shape s;
+  lin::Rows a;
+  if (lin::shape_of(rows, s, a) != GTP_OK) return 0;
+  return lin::forward_space(s, nullptr).bytes;
+}
+
+extern "C" int gtp_linear_logprob_rows(const gtp_linear_rows* rows, float* out_logprob,
+                                       float* out_lse, float* mean_loss, int64_t* mean_count,
+                                       uint32_t* verdict, void* workspace, size_t workspace_bytes,
+                                       void* stream) {
+  lin::Shape s;
+  lin::Rows a;
+  const int rc = lin::shape_of(rows, s, a);
+  if (rc != GTP_OK) return rc;
+  if ((s.N > 0 && (!out_logprob || !out_lse)) || !workspace || (!mean_loss != !mean_count))
+    return GTP_ERR_INVALID_ARGUMENT;
+  const lin::Forward f = lin::forward_space(s, workspace);
+  if (workspace_bytes < f.bytes) return GTP_ERR_INVALID_ARGUMENT;
+  hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  for (int i = 1; verdict && i < GTP_VERDICT_WORDS; ++i) verdict[i] = GTP_VERDICT_GOOD;
+  hipLaunchKernelGGL(lin::list_rows_kernel, dim3(1), dim3(lin::kListBlock), 0, st, a,
+                     lin::Listed{f.at, f.target, nullptr, nullptr}, f.meta, out_logprob, out_lse,
+                     verdict, nullptr, nullptr, nullptr, nullptr, 0);
+  if (s.N > 0) {
+    lin::gather(rows, s, f.meta, f.at, f.h, st);
+    if (rows->dtype == GTP_DTYPE_BF16)
+      lin::forward_launch<gemm::Bf16>(rows, s, f, st);
+    else
+      lin::forward_launch<gemm::F16>(rows, s, f, st);
+    hipLaunchKernelGGL(lin::lse_merge_kernel,
+                       dim3((unsigned)((s.N + lin::kMergeTok - 1) / lin::kMergeTok)), dim3(256), 0,
+                       st, f.partial, s.ldn, 2 * s.n_vt, f.meta, f.at, f.xt, out_logprob, out_lse);
+  }
+  if (mean_loss)
+    hipLaunchKernelGGL(lin::mean_kernel, dim3(1), dim3(1024), 0, st, f.meta, f.at, out_logprob,
+                       mean_loss, mean_count);
+  return hipGetLastError() == hipSuccess ? GTP_OK : GTP_ERR_LAUNCH;
+}
+
+extern "C" size_t gtp_linear_logprob_backward_workspace_bytes(const gtp_linear_rows* rows) {
+  lin::Shape s;
+  lin::Rows a;
+  if (lin::shape_of(rows, s, a) != GTP_OK || s.N == 0) return 0;
+  return lin::backward_space(rows, s, lin::pieces_of(s, rows->V), nullptr).bytes;
+}
+
+extern "C" int gtp_linear_logprob_backward(const gtp_linear_rows* rows, const float* lse,
+                                           const float* grad, const int64_t* mean_count,
+                                           void* grad_hidden, void* grad_weight, void* workspace,
+                                           size_t workspace_bytes, void* stream) {
+  lin::Shape s;
+  lin::Rows a;
+  const int rc = lin::shape_of(rows, s, a);
+  if (rc != GTP_OK) return rc;
+  // without a row there is nothing to list, and both gradients are zeros that
+  // the caller writes
+  if (s.N == 0) return GTP_ERR_UNSUPPORTED;
+  if (!lse || !grad || !workspace) return GTP_ERR_INVALID_ARGUMENT;
+  const lin::Pieces p = lin::pieces_of(s, rows->V);
+  const lin::Backward b = lin::backward_space(rows, s, p, workspace);
+  if (workspace_bytes < b.bytes) return GTP_ERR_INVALID_ARGUMENT;
+  hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  hipLaunchKernelGGL(lin::list_rows_kernel, dim3(1), dim3(lin::kListBlock), 0, st, a, b.rows,
+                     b.meta, nullptr, nullptr, nullptr, grad, mean_count, lse, b.slot,
+                     rows->dtype == GTP_DTYPE_F16 ? 1 : 0);
+  lin::gather(rows, s, b.meta, b.rows.at, b.h, st);
+  uint16_t* gh = reinterpret_cast<uint16_t*>(grad_hidden);
+  uint16_t* gw = reinterpret_cast<uint16_t*>(grad_weight);
+  if (rows->dtype == GTP_DTYPE_BF16)
+    lin::backward_launch<gemm::Bf16>(rows, s, p, b, gh, gw, st);
+  else
+    lin::backward_launch<gemm::F16>(rows, s, p, b, gh, gw, st);
+  return hipGetLastError() == hipSuccess ? GTP_OK : GTP_ERR_LAUNCH;
+}

@@ -4,7 +4,8 @@
 // logprob_entropy, token_logprob, token_logprob_backward, verdict_begin,
 // verdict_end, logprob_backward, graspo_loss_*, lse_partial, lse_finalize,
 // decode_update, to_bf16_exact, logprob_backward_split, time_next_launch,
-// lm_head_logprob, lm_head_logprob_save, softmax_grad_bf16}.  Each op validates
+// lm_head_logprob, lm_head_logprob_save, softmax_grad_bf16, linear_logprob,
+// linear_logprob_backward}.  Each op validates
 // its tensors (TORCH_CHECK surfaces as a Python RuntimeError), allocates the
 // outputs on the logits' device, and enqueues the HIP kernels on the stream handle passed in from Python
 // (torch.cuda.current_stream().cuda_stream), so work orders with the
@@ -771,7 +772,160 @@ std::tuple<at::Tensor, at::Tensor> softmax_grad_bf16(const at::Tensor& logits_t,
   return {out_t, out_n};
 }
 
+// ------------------------------------------------- the hidden-state losses
+
+// The weight with rows that the kernels read in place: unit column stride,
+// 16-byte aligned rows, whole 16-byte chunks.  Another one is copied into
+// such rows (zeros behind the last column).
+at::Tensor linear_weight(const at::Tensor& weight) {
+  const int64_t V = weight.size(0), K = weight.size(1);
+  const int64_t ld = V > 1 ? weight.stride(0) : K;
+  if ((K <= 1 || weight.stride(1) == 1) && K % 8 == 0 && ld >= K && ld % 8 == 0 && ld < (1 << 22) &&
+      (reinterpret_cast<uintptr_t>(weight.data_ptr()) & 15u) == 0)
+    return weight;
+  const int64_t K8 = (K + 7) / 8 * 8;
+  at::Tensor rows = at::empty({V, K8}, weight.options());
+  if (K8 > K) rows.narrow(1, K, K8 - K).zero_();
+  rows.narrow(1, 0, K).copy_(weight);
+  return rows;
+}
+
+// hidden [B, S, K] (unit column stride), weight [V, K] (linear_weight's) and
+// targets [B, T <= S]
+gtp_linear_rows linear_rows(const at::Tensor& hidden, const at::Tensor& weight, int64_t K,
+                            const at::Tensor& targets, const c10::optional<int64_t>& ignore_index) {
+  gtp_linear_rows r;
+  r.hidden = hidden.data_ptr();
+  r.weight = weight.data_ptr();
+  r.targets = targets.data_ptr();
+  r.dtype = dtype_code(hidden);
+  r.targets_int64 = targets.scalar_type() == at::kLong;
+  r.has_ignore = ignore_index.has_value();
+  r.ignore_index = ignore_index.value_or(0);
+  r.B = hidden.size(0);
+  r.S = hidden.size(1);
+  r.T = targets.size(1);
+  r.K = K;
+  r.V = weight.size(0);
+  r.hidden_batch_stride = hidden.stride(0);
+  r.hidden_row_stride = hidden.stride(1);
+  r.weight_stride = r.V > 1 ? weight.stride(0) : weight.size(1);
+  r.target_batch_stride = targets.stride(0);
+  r.target_row_stride = targets.stride(1);
+  return r;
+}
+
+void check_linear(const at::Tensor& hidden, const at::Tensor& weight, const at::Tensor& targets,
+                  const char* what) {
+  TORCH_CHECK(hidden.is_cuda() && hidden.dim() == 3 && weight.dim() == 2 && targets.dim() == 2,
+              "graspo_tokpath.", what, ": expected hidden [B, S, K], weight [V, K] and targets "
+              "[B, T] on a GPU");
+  check_same_device(hidden, weight, "weight");
+  check_same_device(hidden, targets, "targets");
+  TORCH_CHECK((hidden.scalar_type() == at::kBFloat16 || hidden.scalar_type() == at::kHalf) &&
+                  weight.scalar_type() == hidden.scalar_type(),
+              "graspo_tokpath.", what, ": hidden and weight must both be bfloat16 or both float16, "
+              "got ", hidden.scalar_type(), " and ", weight.scalar_type());
+  TORCH_CHECK(targets.scalar_type() == at::kInt || targets.scalar_type() == at::kLong,
+              "graspo_tokpath.", what, ": targets must be int32 or int64");
+  TORCH_CHECK(hidden.size(2) > 0 && weight.size(0) > 0 && weight.size(1) == hidden.size(2),
+              "graspo_tokpath.", what, ": hidden is [B, S, ", hidden.size(2), "] but weight is [",
+              weight.size(0), ", ", weight.size(1), "]");
+  TORCH_CHECK(targets.size(0) == hidden.size(0) && targets.size(1) <= hidden.size(1),
+              "graspo_tokpath.", what, ": targets must be [B, T] with T <= S");
+}
+
+at::Tensor unit_columns(const at::Tensor& t) {
+  return t.size(-1) <= 1 || t.stride(-1) == 1 ? t : t.contiguous();
+}
+
+// (logprob [B, T], lse [B, T], mean loss and count or empty tensors, whether a
+// target lies outside [0, V)).  Waits for the look at the targets, which runs
+// ahead of the products; a captured call does not (a bad target's logprob, and
+// the mean with it, is NaN).
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, bool> linear_logprob(
+    const at::Tensor& hidden_, const at::Tensor& weight_, const at::Tensor& targets,
+    c10::optional<int64_t> ignore_index, bool mean, int64_t stream) {
+  check_linear(hidden_, weight_, targets, "linear_logprob");
+  const c10::DeviceGuard guard(hidden_.device());
+  const at::Tensor hidden = unit_columns(hidden_), weight = linear_weight(weight_);
+  const gtp_linear_rows r = linear_rows(hidden, weight, hidden.size(2), targets, ignore_index);
+  void* st = reinterpret_cast<void*>(stream);
+  const auto f32 = hidden.options().dtype(at::kFloat);
+  at::Tensor lp = at::empty(targets.sizes(), f32), lse = at::empty(targets.sizes(), f32);
+  at::Tensor loss = at::empty({0}, f32), count = at::empty({0}, f32.dtype(at::kLong));
+  if (mean) {
+    loss = at::empty({}, f32);
+    count = at::empty({}, f32.dtype(at::kLong));
+  }
+  const size_t ws_bytes = gtp_linear_logprob_workspace_bytes(&r);
+  at::Tensor ws = at::empty({(int64_t)std::max<size_t>(ws_bytes, 256)},
+                            hidden.options().dtype(at::kByte));
+  at::Tensor words;
+  if (!gtp_stream_capturing(st)) words = verdict_words();
+  const int rc = gtp_linear_logprob_rows(
+      &r, lp.data_ptr<float>(), lse.data_ptr<float>(), mean ? loss.data_ptr<float>() : nullptr,
+      mean ? count.data_ptr<int64_t>() : nullptr, words.defined() ? verdict_ptr(words) : nullptr,
+      ws.data_ptr(), (size_t)ws.numel(), st);
+  // an argument error comes before any launch, a launch error after the look's
+  if (rc != GTP_OK && rc != GTP_ERR_LAUNCH) check_rc(rc, "gtp_linear_logprob_rows");
+  int bad = 0, wait_rc = GTP_OK;
+  if (words.defined()) wait_rc = verdict_wait(words, &bad, st);
+  check_rc(rc, "gtp_linear_logprob_rows");
+  check_rc(wait_rc, "gtp_verdict_wait");
+  return {lp, lse, loss, count, bad != 0};
+}
+
+// The gradients of sum(grad * logprob) (mean_count: of grad times the mean)
+// by hidden and weight, of their shapes and type, contiguous; an empty tensor
+// for one that is not asked for.
+std::tuple<at::Tensor, at::Tensor> linear_logprob_backward(
+    const at::Tensor& hidden_, const at::Tensor& weight_, const at::Tensor& targets,
+    const at::Tensor& lse, const at::Tensor& grad, const c10::optional<at::Tensor>& mean_count,
+    c10::optional<int64_t> ignore_index, bool need_hidden, bool need_weight, int64_t stream) {
+  check_linear(hidden_, weight_, targets, "linear_logprob_backward");
+  const bool is_mean = mean_count.has_value();
+  for (const at::Tensor* t : {&lse, &grad}) {
+    check_same_device(hidden_, *t, "lse / grad");
+    TORCH_CHECK(t->scalar_type() == at::kFloat && t->is_contiguous(),
+                "graspo_tokpath.linear_logprob_backward: lse and grad must be contiguous float32");
+  }
+  TORCH_CHECK(lse.numel() == targets.numel() && grad.numel() == (is_mean ? 1 : targets.numel()) &&
+                  (!is_mean || (mean_count->scalar_type() == at::kLong && mean_count->numel() == 1)),
+              "graspo_tokpath.linear_logprob_backward: lse, grad and mean_count must match the "
+              "targets");
+  if (is_mean) check_same_device(hidden_, *mean_count, "mean_count");
+  const c10::DeviceGuard guard(hidden_.device());
+  at::Tensor gh = need_hidden ? at::empty(hidden_.sizes(), hidden_.options())
+                              : at::empty({0}, hidden_.options());
+  at::Tensor gw = need_weight ? at::empty(weight_.sizes(), weight_.options())
+                              : at::empty({0}, weight_.options());
+  if (targets.numel() == 0) return {gh.zero_(), gw.zero_()};
+  if (!need_hidden && !need_weight) return {gh, gw};
+  const at::Tensor hidden = unit_columns(hidden_), weight = linear_weight(weight_);
+  const gtp_linear_rows r = linear_rows(hidden, weight, hidden.size(2), targets, ignore_index);
+  const size_t ws_bytes = gtp_linear_logprob_backward_workspace_bytes(&r);
+  at::Tensor ws = at::empty({(int64_t)std::max<size_t>(ws_bytes, 256)},
+                            hidden.options().dtype(at::kByte));
+  check_rc(gtp_linear_logprob_backward(
+               &r, lse.data_ptr<float>(), grad.data_ptr<float>(),
+               is_mean ? mean_count->data_ptr<int64_t>() : nullptr,
+               need_hidden ? gh.data_ptr() : nullptr, need_weight ? gw.data_ptr() : nullptr,
+               ws.data_ptr(), (size_t)ws.numel(), reinterpret_cast<void*>(stream)),
+           "gtp_linear_logprob_backward");
+  return {gh, gw};
+}
+
 TORCH_LIBRARY(graspo_tokpath, m) {
+  m.def(
+      "linear_logprob(Tensor hidden, Tensor weight, Tensor targets, int? ignore_index, bool mean, "
+      "int stream) -> (Tensor, Tensor, Tensor, Tensor, bool)",
+      &linear_logprob);
+  m.def(
+      "linear_logprob_backward(Tensor hidden, Tensor weight, Tensor targets, Tensor lse, "
+      "Tensor grad, Tensor? mean_count, int? ignore_index, bool need_hidden, bool need_weight, "
+      "int stream) -> (Tensor, Tensor)",
+      &linear_logprob_backward);
   m.def(
       "sample(Tensor logits, float temperature, int top_k, float top_p, float repetition_penalty, "
       "Tensor? history, Tensor? allow_mask, Tensor? uniforms, Tensor? finished, int pad_token_id, "

@@ -12,6 +12,7 @@ import torch
 from torch import nn
 
 from . import ops
+from .linear_loss import _LinearLogprob, check_operands
 
 
 def _token_rows(logits: torch.Tensor) -> torch.Tensor | None:
@@ -82,6 +83,36 @@ def sequence_log_probs_and_entropy_from_logits(
 ) -> tuple[torch.Tensor, torch.Tensor]:
     """(logprob, entropy) from the same single read of the logits (no grad)."""
     return _rows_logprob_entropy(logits, output_ids)
+
+
+def sequence_log_probs_from_hidden(
+    hidden_states: torch.Tensor,
+    lm_head_weight: torch.Tensor,
+    output_ids: torch.Tensor,
+    *,
+    ignore_index: int | None = None,
+) -> torch.Tensor:
+    """log_softmax(hidden_states @ lm_head_weight.T)[output_ids] in fp32, no
+    logits written or kept for the backward, which computes them again a piece
+    of the vocabulary at a time.  ``hidden_states`` [..., K] and
+    ``lm_head_weight`` [V, K] in bf16 or fp16, differentiable in both.  A
+    position whose id is ``ignore_index`` (off by default) has logprob 0 and
+    takes no part in any product; neither does, in the backward, one whose
+    gradient is 0 (an action mask's).  An id outside [0, V) raises
+    ``RuntimeError`` (in a graph capture, where nothing waits for the ids, its
+    logprob is NaN)."""
+    what = "sequence_log_probs_from_hidden"
+    check_operands(what, hidden_states, lm_head_weight)
+    lead = hidden_states.shape[:-1]
+    if output_ids.shape != lead:
+        raise ValueError(f"{what}: expected output ids {tuple(lead)}, got "
+                         f"{tuple(output_ids.shape)}")
+    h, t = hidden_states, output_ids
+    if h.dim() != 3:
+        h, t = h.reshape(1, -1, h.shape[-1]), t.reshape(1, -1)
+    lp = _LinearLogprob.apply(h, lm_head_weight, t,
+                              None if ignore_index is None else int(ignore_index), False, what)
+    return lp.reshape(lead)
 
 
 def masked_mean(

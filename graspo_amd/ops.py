@@ -2,7 +2,7 @@
 
 Each function validates nothing beyond what the native op checks, enqueues
 the HIP kernels on the caller's current stream and returns device tensors;
-none of them waits for the GPU except ``token_logprob`` and
+none of them waits for the GPU except ``token_logprob``, ``linear_logprob`` and
 ``TargetsVerdict.wait``, which wait for a look at the targets, so that a
 caller can raise on a bad one.
 """
@@ -312,6 +312,44 @@ def softmax_grad_bf16(logits_t: torch.Tensor, grad_logprob: torch.Tensor, lse: t
         lse.reshape(-1).to(torch.float32).contiguous(),
         (1 if vocab_major else 0) | (2 if token_major else 0), _stream(logits_t))
     return (gt if vocab_major else None), (gn if token_major else None)
+
+
+class LinearLogprob(NamedTuple):
+    logprob: torch.Tensor    # fp32, the targets' shape
+    lse: torch.Tensor        # fp32, the targets' shape
+    mean_loss: torch.Tensor  # fp32 scalar, -sum(logprob) / count (empty unless asked for)
+    count: torch.Tensor      # int64 scalar, rows in the mean (empty unless asked for)
+    bad_target: bool         # some target that is not ignored lies outside [0, V)
+
+
+def linear_logprob(hidden: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor, *,
+                   ignore_index: int | None = None, mean: bool = False) -> LinearLogprob:
+    """log_softmax(hidden @ weight.T)[targets] over bf16 or fp16 ``hidden``
+    [B, S, K] and ``weight`` [V, K], in pieces of the vocabulary, no logits
+    written.  ``targets`` [B, T <= S] are those of the first T positions.  A
+    row whose target is ``ignore_index`` has logprob 0 and no part in any
+    product; ``mean`` adds the mean loss over the others (NaN without one).
+    Waits for a look at the targets, which runs ahead of the products, to say
+    whether one is bad (its logprob, and the mean, is NaN); in a graph capture
+    it does not wait and says no."""
+    return LinearLogprob(*load().linear_logprob(hidden, weight, _targets(targets), ignore_index,
+                                                mean, _stream(hidden)))
+
+
+def linear_logprob_backward(hidden: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor,
+                            lse: torch.Tensor, grad: torch.Tensor, *,
+                            mean_count: torch.Tensor | None = None,
+                            ignore_index: int | None = None, need_hidden: bool = True,
+                            need_weight: bool = True):
+    """The gradients (hidden's, weight's; None for one not asked for) of
+    :func:`linear_logprob` from its ``lse`` and the fp32 ``grad`` per row, or
+    of its mean (``mean_count`` given, ``grad`` the loss's).  The logits are
+    computed again, a piece of the vocabulary at a time; rows with gradient 0
+    take no part.  A row whose target is bad has no gradient."""
+    gh, gw = load().linear_logprob_backward(
+        hidden, weight, _targets(targets), lse, grad.to(torch.float32).contiguous(), mean_count,
+        ignore_index, need_hidden, need_weight, _stream(hidden))
+    return (gh if need_hidden else None), (gw if need_weight else None)
 
 
 def decode_update(ids: torch.Tensor, status: torch.Tensor | None, finished: torch.Tensor,

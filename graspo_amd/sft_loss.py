@@ -6,6 +6,8 @@ logits over the labels that are not ``ignore_index``, as
 (sft_loss.py:12-34), without materialising the shifted copy or the [N, V]
 softmax: the forward is the logprob kernel (one read of the logits), the
 backward the logprob-gradient kernel (one read, one write).
+``sft_cross_entropy_loss_from_hidden`` is the same loss from the hidden states
+and the lm_head weight, for which no logits are kept.
 """
 
 from __future__ import annotations
@@ -13,6 +15,7 @@ from __future__ import annotations
 import torch
 
 from . import ops
+from .linear_loss import _LinearLogprob, check_operands
 
 
 class _SFTCrossEntropy(torch.autograd.Function):
@@ -54,3 +57,28 @@ def sft_cross_entropy_loss(
     if logits.stride(-1) != 1:
         logits = logits.contiguous()
     return _SFTCrossEntropy.apply(logits, labels, int(ignore_index))
+
+
+def sft_cross_entropy_loss_from_hidden(
+    hidden_states: torch.Tensor,
+    lm_head_weight: torch.Tensor,
+    labels: torch.Tensor,
+    *,
+    ignore_index: int = -100,
+) -> torch.Tensor:
+    """:func:`sft_cross_entropy_loss` of the logits ``hidden_states @
+    lm_head_weight.T``, which are not written: the mean cross-entropy of
+    positions 0 .. S - 2 against ``labels[:, 1:]``, skipping ``ignore_index``
+    (such positions take no part in any product).  ``hidden_states`` [B, S, K]
+    and ``lm_head_weight`` [V, K] in bf16 or fp16; the loss is an fp32 scalar,
+    differentiable in both.  A label outside [0, V) raises ``RuntimeError``
+    (in a graph capture, where nothing waits for the labels, it makes the loss
+    NaN)."""
+    what = "sft_cross_entropy_loss_from_hidden"
+    check_operands(what, hidden_states, lm_head_weight)
+    if hidden_states.dim() != 3 or labels.shape != hidden_states.shape[:2]:
+        raise ValueError(
+            f"{what}: expected hidden states [B, S, K] and labels [B, S], got "
+            f"{tuple(hidden_states.shape)} and {tuple(labels.shape)}")
+    return _LinearLogprob.apply(hidden_states, lm_head_weight, labels[:, 1:], int(ignore_index),
+                                True, what)

@@ -596,6 +596,63 @@ int gtp_stream_read_rows(const void* data, int64_t rows, int64_t row_bytes,
 /* Library version string, e.g. "graspo_tokpath 0.1 gfx950". */
 const char* gtp_version(void);
 
+/*
+ * The hidden-state losses: token logprobs from hidden states and the lm_head
+ * weight, in pieces of the vocabulary, without keeping the logits, and their
+ * gradients.  Replaces the chunk loop of _selected_token_log_probs_from_hidden
+ *   src/graspo/backends/graspoflow/tensor_utils.py:167-186
+ * under autograd (which keeps every chunk's logits), and F.cross_entropy over
+ * full logits of sft_cross_entropy_loss, src/graspo/core/sft_loss.py:12-34.
+ *
+ *   hidden   [B, S, K] bf16 or fp16 (`dtype`), unit column stride, any batch
+ *            and row strides (elements)
+ *   weight   [V, K] of the same type, rows 16-byte aligned, weight_stride a
+ *            multiple of 8, at least K rounded up to a multiple of 8 and below
+ *            2^22; values between K and that multiple must be zeros
+ *   targets  [B, T] int32 / int64 with T <= S: position s < T of a sequence
+ *            has target targets[b][s], the others have none
+ * A row whose target is ignore_index (has_ignore) has logprob 0, one whose
+ * target lies outside [0, V) NaN; neither takes part in a product, nor does,
+ * in the backward, a row with gradient 0.  B * S < 2^22 - 256, K < 2^22 - 64.
+ * Other sizes and types return GTP_ERR_UNSUPPORTED.
+ */
+typedef struct gtp_linear_rows {
+  const void* hidden;
+  const void* weight;
+  const void* targets;
+  int32_t dtype;
+  int32_t targets_int64;
+  int32_t has_ignore;
+  int64_t ignore_index;
+  int64_t B, S, T, K, V;
+  int64_t hidden_batch_stride, hidden_row_stride, weight_stride;
+  int64_t target_batch_stride, target_row_stride;
+} gtp_linear_rows;
+
+/*
+ * gtp_linear_logprob_rows -- out_logprob and out_lse [B * T] fp32 (both
+ * needed); with mean_loss and mean_count also -sum(logprob) / count over the
+ * rows that are not ignored (NaN without one, or with a bad target) and that
+ * count.  verdict: GTP_VERDICT_WORDS pinned words, each GTP_VERDICT_PENDING,
+ * answered ahead of the products (gtp_verdict_wait), or NULL.  The workspace
+ * (gtp_linear_logprob_workspace_bytes) carries nothing between calls.
+ */
+size_t gtp_linear_logprob_workspace_bytes(const gtp_linear_rows* rows);
+int gtp_linear_logprob_rows(const gtp_linear_rows* rows, float* out_logprob, float* out_lse,
+                            float* mean_loss, int64_t* mean_count, uint32_t* verdict,
+                            void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * gtp_linear_logprob_backward -- the gradients of sum_n grad[n] logprob[n]
+ * (grad fp32 [B * T]; with mean_count, as the forward wrote it, grad[0] times
+ * the mean loss): grad_hidden [B, S, K] and grad_weight [V, K], contiguous,
+ * of the operands' type, either NULL.  lse: the forward's.  Needs B * T > 0.
+ */
+size_t gtp_linear_logprob_backward_workspace_bytes(const gtp_linear_rows* rows);
+int gtp_linear_logprob_backward(const gtp_linear_rows* rows, const float* lse, const float* grad,
+                                const int64_t* mean_count, void* grad_hidden, void* grad_weight,
+                                void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
