@@ -25,7 +25,8 @@ EXT_NAME = "_graspo_tokpath_ops"
 
 HIP_SOURCES = ["tokpath_logprob.hip", "tokpath_sampler.hip", "tokpath_sampler_fast.hip",
                "tokpath_loss.hip", "tokpath_decode.hip",
-               "tokpath_narrow.hip", "tokpath_lmhead.hip", "tokpath_linear.hip"]
+               "tokpath_narrow.hip", "tokpath_lmhead.hip", "tokpath_linear.hip",
+               "tokpath_embedding.hip", "tokpath_gradnorm.hip"]
 HIP_FLAGS = [
     "--offload-arch=gfx950",
     "-O3",

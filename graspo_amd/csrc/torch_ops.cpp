@@ -5,7 +5,8 @@
 // verdict_end, logprob_backward, graspo_loss_*, lse_partial, lse_finalize,
 // decode_update, to_bf16_exact, logprob_backward_split, time_next_launch,
 // lm_head_logprob, lm_head_logprob_save, softmax_grad_bf16, linear_logprob,
-// linear_logprob_backward}.  Each op validates
+// linear_logprob_backward, embedding, embedding_backward, grad_norm,
+// clip_grads_, clip_grad_norm_}.  Each op validates
 // its tensors (TORCH_CHECK surfaces as a Python RuntimeError), allocates the
 // outputs on the logits' device, and enqueues the HIP kernels on the stream handle passed in from Python
 // (torch.cuda.current_stream().cuda_stream), so work orders with the
@@ -15,6 +16,7 @@
 #include <torch/library.h>
 
 #include <algorithm>
+#include <limits>
 #include <map>
 #include <mutex>
 #include <tuple>
@@ -916,7 +918,205 @@ std::tuple<at::Tensor, at::Tensor> linear_logprob_backward(
   return {gh, gw};
 }
 
+// ------------------------------------------------- embedding
+
+at::Tensor flat_ids(const at::Tensor& ids, const at::Tensor& like, const char* what) {
+  check_same_device(like, ids, "ids");
+  TORCH_CHECK(ids.scalar_type() == at::kInt || ids.scalar_type() == at::kLong, "graspo_tokpath.",
+              what, ": ids must be int32 or int64");
+  return ids.reshape({-1});
+}
+
+// (out [*ids.shape, H], whether an id lies outside [0, V): its row is NaN).
+// check: waits for a look at the ids, which runs ahead of the rows (not in a
+// captured call).
+std::tuple<at::Tensor, bool> embedding(const at::Tensor& ids_, const at::Tensor& weight,
+                                       double scale, bool check, int64_t stream) {
+  TORCH_CHECK(weight.is_cuda() && weight.dim() == 2 && weight.size(0) > 0 && weight.size(1) > 0,
+              "graspo_tokpath.embedding: weight must be a non-empty [V, H] GPU tensor");
+  const at::Tensor ids = flat_ids(ids_, weight, "embedding");
+  const c10::DeviceGuard guard(weight.device());
+  const int64_t N = ids.size(0), V = weight.size(0), H = weight.size(1);
+  const at::Tensor w = H == 1 || weight.stride(1) == 1 ? weight : weight.contiguous();
+  void* st = reinterpret_cast<void*>(stream);
+  auto shape = ids_.sizes().vec();
+  shape.push_back(H);
+  at::Tensor out = at::empty(shape, weight.options());
+  const int ids64 = ids.scalar_type() == at::kLong;
+  const int64_t ids_stride = N > 1 ? ids.stride(0) : 1;
+  at::Tensor words;
+  if (check && N > 0 && !gtp_stream_capturing(st)) {
+    words = verdict_words();
+    const int rc = gtp_targets_verdict(ids.data_ptr(), ids64, N, ids_stride, V, nullptr, nullptr,
+                                       verdict_ptr(words), st);
+    int found = 0;
+    if (rc == GTP_ERR_LAUNCH) verdict_wait(words, &found, st);
+    check_rc(rc, "gtp_targets_verdict");
+  }
+  const int rc = gtp_embedding_rows(ids.data_ptr(), ids64, N, ids_stride, w.data_ptr(),
+                                    dtype_code(w), V, H, V > 1 ? w.stride(0) : H, (float)scale,
+                                    out.data_ptr(), st);
+  int bad = 0, wait_rc = GTP_OK;
+  if (words.defined()) wait_rc = verdict_wait(words, &bad, st);
+  check_rc(rc, "gtp_embedding_rows");
+  check_rc(wait_rc, "gtp_verdict_wait");
+  return {out, (bad & 1) != 0};
+}
+
+// The gradient of the table from that of embedding()'s rows; out: added to.
+at::Tensor embedding_backward(const at::Tensor& ids_, const at::Tensor& grad_, int64_t V,
+                              double scale, int64_t padding_idx,
+                              const c10::optional<at::Tensor>& out, int64_t stream) {
+  TORCH_CHECK(grad_.is_cuda() && grad_.dim() >= 1 && grad_.size(-1) > 0 && V > 0,
+              "graspo_tokpath.embedding_backward: grad must be a [..., H] GPU tensor and V > 0");
+  const int64_t H = grad_.size(-1);
+  const at::Tensor ids = flat_ids(ids_, grad_, "embedding_backward");
+  const int64_t N = ids.size(0);
+  TORCH_CHECK(grad_.numel() == N * H,
+              "graspo_tokpath.embedding_backward: grad must be [*ids.shape, H]");
+  const c10::DeviceGuard guard(grad_.device());
+  at::Tensor grad = grad_.reshape({N, H});
+  if (H > 1 && grad.stride(1) != 1) grad = grad.contiguous();
+  at::Tensor to;
+  if (out.has_value()) {
+    to = *out;
+    check_same_device(grad, to, "out");
+    TORCH_CHECK(to.scalar_type() == grad.scalar_type() && to.dim() == 2 && to.size(0) == V &&
+                    to.size(1) == H && to.is_contiguous(),
+                "graspo_tokpath.embedding_backward: out must be a contiguous [V, H] of the "
+                "gradient's dtype");
+  } else {
+    to = at::empty({V, H}, grad.options());
+  }
+  const int dt = dtype_code(grad);
+  const size_t ws_bytes = gtp_embedding_backward_workspace_bytes(dt, N, H);
+  at::Tensor ws = at::empty({(int64_t)std::max<size_t>(ws_bytes, 256)},
+                            grad.options().dtype(at::kByte));
+  check_rc(gtp_embedding_backward(ids.data_ptr(), ids.scalar_type() == at::kLong, N,
+                                  N > 1 ? ids.stride(0) : 1, grad.data_ptr(), dt,
+                                  N > 1 ? grad.stride(0) : H, V, H, (float)scale, padding_idx,
+                                  out.has_value(), to.data_ptr(), ws.data_ptr(),
+                                  (size_t)ws.numel(), reinterpret_cast<void*>(stream)),
+           "gtp_embedding_backward");
+  return to;
+}
+
+// ------------------------------------------------- gradient norm and clipping
+
+// Tensors as address, size and type; one whose elements do not fill its
+// memory without gaps goes through a contiguous copy.
+struct GradList {
+  std::vector<void*> p;
+  std::vector<int64_t> n;
+  std::vector<int32_t> dtype;
+  std::vector<std::pair<at::Tensor, at::Tensor>> copies;  // (tensor, its copy)
+  explicit GradList(at::TensorList tensors, const char* what) {
+    TORCH_CHECK(!tensors.empty(), "graspo_tokpath.", what, ": no tensor");
+    p.reserve(tensors.size());
+    n.reserve(tensors.size());
+    dtype.reserve(tensors.size());
+    for (const at::Tensor& t : tensors) {
+      TORCH_CHECK(t.is_cuda(), "graspo_tokpath.", what, ": tensors must be on a GPU");
+      check_same_device(tensors[0], t, "every tensor");
+      const at::ScalarType s = t.scalar_type();
+      TORCH_CHECK(s == at::kFloat || s == at::kBFloat16 || s == at::kHalf, "graspo_tokpath.", what,
+                  ": tensors must be float32, bfloat16 or float16, got ", s);
+      const bool whole = t.is_contiguous() || t.is_non_overlapping_and_dense();
+      if (!whole) copies.emplace_back(t, t.contiguous());
+      p.push_back((whole ? t : copies.back().second).data_ptr());
+      n.push_back(t.numel());
+      dtype.push_back(s == at::kFloat ? GTP_DTYPE_F32
+                                      : s == at::kBFloat16 ? GTP_DTYPE_BF16 : GTP_DTYPE_F16);
+    }
+  }
+  int64_t size() const { return (int64_t)p.size(); }
+};
+
+// In-place products of overlapping tensors would race (and scale twice).
+void check_apart(at::TensorList tensors) {
+  std::vector<std::pair<uintptr_t, uintptr_t>> at;
+  at.reserve(tensors.size());
+  bool sorted = true;
+  for (const at::Tensor& t : tensors) {
+    if (t.numel() == 0) continue;
+    int64_t span = 1;
+    for (int64_t d = 0; d < t.dim(); ++d) {
+      TORCH_CHECK(t.size(d) <= 1 || t.stride(d) != 0,
+                  "graspo_tokpath.clip_grads_: a tensor overlaps itself");
+      span += (t.size(d) - 1) * t.stride(d);
+    }
+    const uintptr_t a = reinterpret_cast<uintptr_t>(t.data_ptr());
+    sorted = sorted && (at.empty() || at.back().first <= a);
+    at.emplace_back(a, a + span * t.element_size());
+  }
+  if (!sorted) std::sort(at.begin(), at.end());
+  for (size_t i = 1; i < at.size(); ++i)
+    TORCH_CHECK(at[i].first >= at[i - 1].second,
+                "graspo_tokpath.clip_grads_: tensors overlap in memory (the same one twice?)");
+}
+
+at::Tensor norm_of(const GradList& l, const at::Tensor& like, double norm_type, void* st) {
+  const int kind = norm_type == 1.0 ? 1 : norm_type == 2.0 ? 2 : 3;
+  TORCH_CHECK(kind < 3 || norm_type == std::numeric_limits<double>::infinity(),
+              "graspo_tokpath.grad_norm: norm_type must be 1, 2 or inf, got ", norm_type);
+  at::Tensor out = at::empty({}, like.options().dtype(at::kFloat));
+  const size_t ws_bytes = gtp_grad_norm_workspace_bytes(l.p.data(), l.n.data(), l.dtype.data(), l.size());
+  at::Tensor ws = at::empty({(int64_t)std::max<size_t>(ws_bytes, 256)},
+                            like.options().dtype(at::kByte));
+  check_rc(gtp_grad_norm(l.p.data(), l.n.data(), l.dtype.data(), l.size(), kind,
+                         out.data_ptr<float>(), ws.data_ptr(), (size_t)ws.numel(), st),
+           "gtp_grad_norm");
+  return out;
+}
+
+void clip_by(GradList& l, const at::Tensor& norm, double max_norm, void* st) {
+  check_rc(gtp_clip_grads(l.p.data(), l.n.data(), l.dtype.data(), l.size(), norm.data_ptr<float>(),
+                          (float)max_norm, st),
+           "gtp_clip_grads");
+  for (auto& c : l.copies) c.first.copy_(c.second);
+}
+
+at::Tensor grad_norm(at::TensorList tensors, double norm_type, int64_t stream) {
+  const GradList l(tensors, "grad_norm");
+  const c10::DeviceGuard guard(tensors[0].device());
+  return norm_of(l, tensors[0], norm_type, reinterpret_cast<void*>(stream));
+}
+
+void clip_grads_(at::TensorList tensors, const at::Tensor& norm, double max_norm, int64_t stream) {
+  GradList l(tensors, "clip_grads_");
+  check_apart(tensors);
+  check_same_device(tensors[0], norm, "norm");
+  TORCH_CHECK(norm.scalar_type() == at::kFloat && norm.numel() == 1,
+              "graspo_tokpath.clip_grads_: norm must be one float32");
+  const c10::DeviceGuard guard(tensors[0].device());
+  clip_by(l, norm, max_norm, reinterpret_cast<void*>(stream));
+}
+
+// Both, from one look at the list.
+at::Tensor clip_grad_norm_(at::TensorList tensors, double max_norm, double norm_type,
+                           int64_t stream) {
+  GradList l(tensors, "clip_grad_norm_");
+  check_apart(tensors);
+  const c10::DeviceGuard guard(tensors[0].device());
+  void* st = reinterpret_cast<void*>(stream);
+  const at::Tensor norm = norm_of(l, tensors[0], norm_type, st);
+  clip_by(l, norm, max_norm, st);
+  return norm;
+}
+
 TORCH_LIBRARY(graspo_tokpath, m) {
+  m.def("embedding(Tensor ids, Tensor weight, float scale, bool check, int stream) -> (Tensor, bool)",
+        &embedding);
+  m.def(
+      "embedding_backward(Tensor ids, Tensor grad, int vocab, float scale, int padding_idx, "
+      "Tensor(a!)? out, int stream) -> Tensor",
+      &embedding_backward);
+  m.def("grad_norm(Tensor[] tensors, float norm_type, int stream) -> Tensor", &grad_norm);
+  m.def("clip_grads_(Tensor(a!)[] tensors, Tensor norm, float max_norm, int stream) -> ()",
+        &clip_grads_);
+  m.def(
+      "clip_grad_norm_(Tensor(a!)[] tensors, float max_norm, float norm_type, int stream) -> Tensor",
+      &clip_grad_norm_);
   m.def(
       "linear_logprob(Tensor hidden, Tensor weight, Tensor targets, int? ignore_index, bool mean, "
       "int stream) -> (Tensor, Tensor, Tensor, Tensor, bool)",

@@ -2,9 +2,9 @@
 
 Each function validates nothing beyond what the native op checks, enqueues
 the HIP kernels on the caller's current stream and returns device tensors;
-none of them waits for the GPU except ``token_logprob``, ``linear_logprob`` and
-``TargetsVerdict.wait``, which wait for a look at the targets, so that a
-caller can raise on a bad one.
+none of them waits for the GPU except ``token_logprob``, ``linear_logprob``,
+``embedding`` (unless told not to) and ``TargetsVerdict.wait``, which wait for
+a look at the targets or ids, so that a caller can raise on a bad one.
 """
 
 from __future__ import annotations
@@ -350,6 +350,49 @@ def linear_logprob_backward(hidden: torch.Tensor, weight: torch.Tensor, targets:
         hidden, weight, _targets(targets), lse, grad.to(torch.float32).contiguous(), mean_count,
         ignore_index, need_hidden, need_weight, _stream(hidden))
     return (gh if need_hidden else None), (gw if need_weight else None)
+
+
+def embedding(ids: torch.Tensor, weight: torch.Tensor, *, scale: float = 1.0, check: bool = True):
+    """(``weight[ids] * scale``, whether an id lies outside [0, V)): rows of
+    the fp32, bf16 or fp16 table ``weight`` [V, H], the product in fp32 and
+    rounded once.  A bad id's row is NaN.  ``check`` waits for a look at the
+    ids, which runs ahead of the rows; without it, and in a graph capture,
+    nothing waits and the answer is no."""
+    return load().embedding(_targets(ids), weight, float(scale), check, _stream(weight))
+
+
+def embedding_backward(ids: torch.Tensor, grad: torch.Tensor, vocab: int, *, scale: float = 1.0,
+                       padding_idx: int | None = None,
+                       out: torch.Tensor | None = None) -> torch.Tensor:
+    """The gradient [V, H] of :func:`embedding`'s table from ``grad``
+    [*ids.shape, H], in its dtype: the tokens sorted by id, each row's sum in
+    fp32 in an order that the ids fix, rounded once.  Tokens of
+    ``padding_idx``, and bad ones, are left out.  With ``out`` (contiguous
+    [V, H] of that dtype, as a tied lm_head's gradient is) the sums are added
+    to it in place, and rows without a token are not touched."""
+    if padding_idx is not None and not 0 <= padding_idx < vocab:
+        raise ValueError(f"embedding_backward: padding_idx {padding_idx} outside [0, {vocab})")
+    return load().embedding_backward(_targets(ids), grad, int(vocab), float(scale),
+                                     -1 if padding_idx is None else int(padding_idx), out,
+                                     _stream(grad))
+
+
+def grad_norm(tensors, norm_type: float = 2.0) -> torch.Tensor:
+    """The fp32 norm (``norm_type`` 1, 2 or inf) of all elements of the fp32,
+    bf16 and fp16 ``tensors`` of one GPU, summed in 64 bits."""
+    return load().grad_norm(tensors, float(norm_type), _stream(tensors[0]))
+
+
+def clip_grads_(tensors, norm: torch.Tensor, max_norm: float) -> None:
+    """Multiplies ``tensors`` in place by min(1, max_norm / (norm + 1e-6)),
+    ``norm`` one fp32 on the device; nothing is read or written where that is
+    1."""
+    load().clip_grads_(tensors, norm, float(max_norm), _stream(tensors[0]))
+
+
+def clip_grad_norm_(tensors, max_norm: float, norm_type: float = 2.0) -> torch.Tensor:
+    """:func:`grad_norm`, then :func:`clip_grads_` by it; returns the norm."""
+    return load().clip_grad_norm_(tensors, float(max_norm), float(norm_type), _stream(tensors[0]))
 
 
 def decode_update(ids: torch.Tensor, status: torch.Tensor | None, finished: torch.Tensor,

@@ -653,6 +653,57 @@ int gtp_linear_logprob_backward(const gtp_linear_rows* rows, const float* lse, c
                                 const int64_t* mean_count, void* grad_hidden, void* grad_weight,
                                 void* workspace, size_t workspace_bytes, void* stream);
 
+/*
+ * The embedding of the vocabulary: out[n] = scale * weight[ids[n]], in fp32,
+ * rounded once, and the gradient of the table.
+ *
+ *   ids      [N] int32 / int64, ids_stride elements apart
+ *   weight   [V, H] fp32 / bf16 / fp16 (`dtype`), rows weight_stride apart
+ *   out      [N, H] contiguous, of the weight's type; an id outside [0, V)
+ *            gives a row of NaN
+ * N < 2^24, V < 2^31 - 1.
+ */
+int gtp_embedding_rows(const void* ids, int ids_int64, int64_t N, int64_t ids_stride,
+                       const void* weight, int dtype, int64_t V, int64_t H, int64_t weight_stride,
+                       float scale, void* out, void* stream);
+
+/*
+ * gtp_embedding_backward -- grad_weight[v] = scale * the sum of grad[n] over
+ * the n with ids[n] = v, in fp32, rounded once; the order of a sum depends on
+ * the ids alone.  Tokens whose id is padding_idx (negative: none) or outside
+ * [0, V) are left out.
+ *
+ *   grad         [N, H] of `dtype`, rows grad_stride apart
+ *   grad_weight  [V, H] contiguous of `dtype`, 16-byte aligned; accumulate:
+ *                added to what the rows hold, and rows without a token are
+ *                neither read nor written (any alignment)
+ * The workspace (gtp_embedding_backward_workspace_bytes) carries nothing
+ * between calls.
+ */
+size_t gtp_embedding_backward_workspace_bytes(int dtype, int64_t N, int64_t H);
+int gtp_embedding_backward(const void* ids, int ids_int64, int64_t N, int64_t ids_stride,
+                           const void* grad, int dtype, int64_t grad_stride, int64_t V, int64_t H,
+                           float scale, int64_t padding_idx, int accumulate, void* grad_weight,
+                           void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * gtp_grad_norm -- the norm of all elements of `count` tensors (tensors,
+ * sizes in elements and dtypes are HOST arrays, read during the call):
+ * norm_type 1 (sum of |x|), 2 (square root of the sum of squares, in 64 bits)
+ * or 3 (largest |x|; a NaN stays).  out_norm: one fp32.  No tensor: 0.
+ * gtp_clip_grads -- multiplies them, in place, by min(1, max_norm / (*norm +
+ * 1e-6)) (one fp32 product, one rounding; NaN where the norm is NaN); nothing
+ * is read or written where that is 1.  The tensors must not overlap.
+ * The workspace (gtp_grad_norm_workspace_bytes) carries nothing between calls.
+ */
+size_t gtp_grad_norm_workspace_bytes(const void* const* tensors, const int64_t* sizes,
+                                     const int32_t* dtypes, int64_t count);
+int gtp_grad_norm(const void* const* tensors, const int64_t* sizes, const int32_t* dtypes,
+                  int64_t count, int norm_type, float* out_norm, void* workspace,
+                  size_t workspace_bytes, void* stream);
+int gtp_clip_grads(void* const* tensors, const int64_t* sizes, const int32_t* dtypes,
+                   int64_t count, const float* norm, float max_norm, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
