@@ -35,7 +35,6 @@ constexpr int kThreads = kWaves * 64;
 constexpr int kB = 4;                  // 32-wide blocks per wave along each side
 constexpr int kQ = 8;                  // 1 KB loads per wave, operand and K step
 constexpr int kStage = kTile * kBK / 8;  // 16-byte chunks per operand stage
-constexpr int kLds = 4 * kStage;         // chunks of all stages: 128 KB
 constexpr int kXcds = 8;
 constexpr int kMaxLd = (1 << 22) - 1;  // row strides (elements): 256 rows fit a buffer range
 constexpr int kRsrcWord3 = 0x00020000;  // raw buffer: 32-bit data format, no swizzle
@@ -91,61 +90,72 @@ __device__ __forceinline__ float acc_read(float a) {
   return v;
 }
 
-// Where one operand's K steps come from: wave w's load q of a step fills the
-// 1 KB of LDS from chunk (8w + q) * 64 on, 16 bytes per lane.
+// One operand's K steps, in order: wave w's load q of a step fills the 1 KB of
+// LDS from chunk (8w + q) * 64 on, 16 bytes per lane.
 template <Layout L>
 struct Source {
-  const uint16_t* base;  // the tile's first row (kAlongK) or column (kAcrossK)
-  int64_t ld, K;
-  uint32_t v0, v1;       // the lane's byte offset for even and odd q
-  int c0, c1;            // kAlongK: its chunk within the K step
-  uint32_t qstep;        // bytes from q to q + 2, halved
-  int64_t bytes;         // kAlongK: of the tile's valid rows; kAcrossK: valid columns
-  __device__ __forceinline__ Source(const Operand& o, int64_t first, int64_t K_, int wave,
-                                    int lane) {
-    ld = o.ld;
-    K = K_;
+  const char* at;   // the next step's first byte
+  int64_t left;     // bytes from there to the operand's end; kAlongK: at least
+  int k_left;       // kAlongK: K from the next step on
+  uint32_t v0, v1;  // the lane's byte offset for even and odd q
+  int c0, c1;       // kAlongK: its first k within the step
+  uint32_t qstep;   // bytes from q to q + 2, halved
+  int64_t advance;  // bytes from step to step
+
+  // k_first: a multiple of 8; K: from there on
+  __device__ __forceinline__ Source(const Operand& o, int64_t first, int64_t k_first, int64_t K,
+                                    int wave, int lane) {
+    const int64_t ld = o.ld * 2, outer = max((int64_t)0, o.outer - first);
+    k_left = (int)K;
     if constexpr (L == kAlongK) {
-      base = o.p + first * ld;
-      bytes = max((int64_t)0, min((int64_t)kTile, o.outer - first)) * ld * 2;
+      at = reinterpret_cast<const char*>(o.p) + first * ld + k_first * 2;
+      left = min((int64_t)kTile, outer) * ld - k_first * 2;
+      advance = kBK * 2;
       // LDS row 8 (8w + q) + lane / 8, chunk lane & 7 of it holding chunk
       // (lane & 7) ^ ((row >> 1) & 7) of the row
       const int row = wave * kQ * 8 + (lane >> 3);
-      c0 = (lane & 7) ^ ((lane >> 4) & 7);
-      c1 = (lane & 7) ^ ((4 + (lane >> 4)) & 7);
-      v0 = (uint32_t)((row * ld + c0 * 8) * 2);
-      v1 = (uint32_t)((row * ld + c1 * 8) * 2);
-      qstep = (uint32_t)(8 * ld * 2);
+      c0 = ((lane & 7) ^ ((lane >> 4) & 7)) * 8;
+      c1 = ((lane & 7) ^ ((4 + (lane >> 4)) & 7)) * 8;
+      v0 = (uint32_t)(row * ld + c0 * 2);
+      v1 = (uint32_t)(row * ld + c1 * 2);
+      qstep = (uint32_t)(8 * ld);
     } else {
-      base = o.p + first;
-      bytes = max((int64_t)0, o.outer - first) * 2;
+      at = reinterpret_cast<const char*>(o.p + first) + k_first * ld;
+      left = outer > 0 && K > 0 ? (K - 1) * ld + outer * 2 : 0;
+      advance = kBK * ld;
       // LDS row 2 (8w + q) + lane / 32, chunk lane & 31 of it holding chunk
       // (lane & 31) ^ 4 (row & 3) of the row
       const int row = wave * kQ * 2 + (lane >> 5);
-      v0 = (uint32_t)((row * ld + ((lane & 31) ^ ((lane >> 5) << 2)) * 8) * 2);
-      v1 = (uint32_t)((row * ld + ((lane & 31) ^ ((2 + (lane >> 5)) << 2)) * 8) * 2);
+      v0 = (uint32_t)(row * ld + ((lane & 31) ^ ((lane >> 5) << 2)) * 16);
+      v1 = (uint32_t)(row * ld + ((lane & 31) ^ ((2 + (lane >> 5)) << 2)) * 16);
       c0 = c1 = 0;
-      qstep = (uint32_t)(2 * ld * 2);
+      qstep = (uint32_t)(2 * ld);
     }
   }
-  __device__ __forceinline__ __amdgpu_buffer_rsrc_t rsrc(int64_t k0) const {
+
+  struct Step {
+    const char* base;
+    int bytes;
+    uint32_t v0, v1;
+  };
+  // The next step; past the last one all its loads are out of range.
+  __device__ __forceinline__ Step next() {
+    const int n = (int)max((int64_t)0, min(left, (int64_t)kPast));
+    Step s{at, n, v0, v1};
     if constexpr (L == kAlongK) {
-      return __builtin_amdgcn_make_buffer_rsrc((void*)base, (short)0, (int)bytes, kRsrcWord3);
-    } else {
-      const int64_t rows = min((int64_t)kBK, K - k0);
-      const int64_t n = rows <= 0 || bytes <= 0 ? 0 : (rows - 1) * ld * 2 + bytes;
-      return __builtin_amdgcn_make_buffer_rsrc((void*)(base + (n ? k0 * ld : 0)), (short)0, (int)n,
-                                               kRsrcWord3);
+      s.v0 = c0 < k_left ? v0 : kPast;
+      s.v1 = c1 < k_left ? v1 : kPast;
+      k_left -= kBK;
     }
+    at += advance;
+    left -= advance;
+    return s;
   }
   // the whole offset goes in the VGPR operand: the range check covers it
-  __device__ __forceinline__ void issue(int q, __amdgpu_buffer_rsrc_t r, int64_t k0, uint4* stage,
-                                        int wave) const {
-    uint32_t v = ((q & 1) ? v1 : v0) + (uint32_t)q * qstep;
-    if constexpr (L == kAlongK) {
-      v += (uint32_t)(k0 * 2);
-      if (((q & 1) ? c1 : c0) * 8 >= K - k0) v = kPast;
-    }
+  __device__ __forceinline__ void issue(const Step& s, int q, uint4* stage, int wave) const {
+    const uint32_t v = ((q & 1) ? s.v1 : s.v0) + (uint32_t)q * qstep;
+    const __amdgpu_buffer_rsrc_t r =
+        __builtin_amdgcn_make_buffer_rsrc((void*)s.base, (short)0, s.bytes, kRsrcWord3);
     __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_void*)(stage + (wave * kQ + q) * 64), 16, v,
                                              0, 0, 0);
   }
@@ -170,25 +180,28 @@ __device__ __forceinline__ s16x8 fragment(const uint4* stage, int side, int x, i
   }
 }
 
-// acc[x][y] += A rows (block x) times B rows (block y) over K steps
-// [k_first, k_first + K): lane l of a block holds B index l & 31 and the A
-// indices 8 (i / 4) + 4 (l / 32) + (i & 3) for i = 0 .. 15.  Ends with the
-// accumulators complete and every wave past its last LDS read.
+// acc[x][y] += A rows (block x) times B rows (block y) over the sources' steps
+// of K: lane l of a block holds B index l & 31 and the A indices 8 (i / 4) +
+// 4 (l / 32) + (i & 3) for i = 0 .. 15.  Ends with the accumulators complete
+// and every wave past its last LDS access.
+//
+// The four stages are four arrays, so that the compiler sees that the loads in
+// flight write to others than it reads (from one array it waits for all loads
+// before every transposing read: 877 against 1040 TFLOP/s).
 template <typename E, Layout LA, Layout LB>
-__device__ __forceinline__ void accumulate(const Source<LA>& a, const Source<LB>& b, int64_t k_first,
-                                           int64_t K, uint4* sm, int wave, int lane,
+__device__ __forceinline__ void accumulate(Source<LA>& a, Source<LB>& b, int64_t K, uint4* sA0,
+                                           uint4* sA1, uint4* sB0, uint4* sB1, int wave, int lane,
                                            f32x16 (&acc)[kB][kB]) {
-  uint4 *sA0 = sm, *sA1 = sm + kStage, *sB0 = sm + 2 * kStage, *sB1 = sm + 3 * kStage;
   const int wa = wave >> 1, wb = wave & 1;
   // an even number of steps (the stages alternate); one past K adds zeros
   const int total = 2 * (int)((K + 2 * kBK - 1) / (2 * kBK));
-  auto k_of = [&](int it) { return k_first + (int64_t)it * kBK; };
-  auto issue_one = [&](int j, __amdgpu_buffer_rsrc_t ra, __amdgpu_buffer_rsrc_t rb, int64_t k0,
-                       uint4* sa, uint4* sb) {
+  typedef typename Source<LA>::Step StepA;
+  typedef typename Source<LB>::Step StepB;
+  auto issue_one = [&](int j, const StepA& ra, const StepB& rb, uint4* sa, uint4* sb) {
     if (j & 1)
-      b.issue(j >> 1, rb, k0, sb, wave);
+      b.issue(rb, j >> 1, sb, wave);
     else
-      a.issue(j >> 1, ra, k0, sa, wave);
+      a.issue(ra, j >> 1, sa, wave);
   };
   s16x8 fa[2][kB], fb[2][kB];
   auto read_frags = [&](const uint4* sa, const uint4* sb, int kk, s16x8 (&f)[kB], s16x8 (&g)[kB]) {
@@ -197,61 +210,62 @@ __device__ __forceinline__ void accumulate(const Source<LA>& a, const Source<LB>
 #pragma unroll
     for (int y = 0; y < kB; ++y) g[y] = fragment<LB>(sb, wb, y, kk, lane);
   };
-  // 16 MFMAs of one k16 step from fragment set c, with loads j0, j0 + 1, ...
-  // after every second one
-  auto mfma16 = [&](int c, bool load, int j0, __amdgpu_buffer_rsrc_t ra, __amdgpu_buffer_rsrc_t rb,
-                    int64_t k0, uint4* la, uint4* lb) {
+  // 16 MFMAs of one k16 step from fragment set c, with the loads j0 .. j0 + 7
+  // among them
+  auto mfma16 = [&](int c, int j0, const StepA& ra, const StepB& rb, uint4* la, uint4* lb) {
 #pragma unroll
     for (int x = 0; x < kB; ++x) {
 #pragma unroll
       for (int y = 0; y < kB; ++y) {
         acc[x][y] = E::mfma(fa[c][x], fb[c][y], acc[x][y]);
-        if (load && (y & 1)) issue_one(j0 + x * (kB / 2) + (y >> 1), ra, rb, k0, la, lb);
+        if (j0 >= 0 && (y & 1)) issue_one(j0 + x * (kB / 2) + (y >> 1), ra, rb, la, lb);
       }
       __builtin_amdgcn_sched_barrier(0);
     }
   };
-  // K step `it` from LDS stage (ca, cb), whose first k16 fragments are already
-  // in set 0.  Step it + 1 lives in (na, nb): its loads 0-7 went out during
-  // the last k16 of step it - 1, its loads 8-15 go out during the first k16
-  // here.  The barrier that publishes it sits before the last k16: every wave
-  // has read all of step it's fragments by then, so the loads 0-7 of step
-  // it + 2 into (ca, cb) go out during that last k16, while step it + 1's
-  // first fragments are read.
-  auto step = [&](int it, uint4* ca, uint4* cb, uint4* na, uint4* nb) {
-    const bool has1 = it + 1 < total, has2 = it + 2 < total;
-    const int64_t k1 = k_of(has1 ? it + 1 : it), k2 = k_of(has2 ? it + 2 : it);
-    const __amdgpu_buffer_rsrc_t a1 = a.rsrc(k1), b1 = b.rsrc(k1), a2 = a.rsrc(k2), b2 = b.rsrc(k2);
-    read_frags(ca, cb, 1, fa[1], fb[1]);
-    __builtin_amdgcn_sched_barrier(0);
-    mfma16(0, has1, kQ, a1, b1, k1, na, nb);
-    read_frags(ca, cb, 2, fa[0], fb[0]);
-    __builtin_amdgcn_sched_barrier(0);
-    mfma16(1, false, 0, a1, b1, 0, na, nb);
-    read_frags(ca, cb, 3, fa[1], fb[1]);
-    __builtin_amdgcn_sched_barrier(0);
-    mfma16(0, false, 0, a1, b1, 0, na, nb);
-    wait_vm0();
-    __syncthreads();
-    if (has1) read_frags(na, nb, 0, fa[0], fb[0]);
-    __builtin_amdgcn_sched_barrier(0);
-    mfma16(1, has2, 0, a2, b2, k2, ca, cb);
-  };
   if (total > 0) {
-    const __amdgpu_buffer_rsrc_t a0 = a.rsrc(k_of(0)), b0 = b.rsrc(k_of(0));
-    const __amdgpu_buffer_rsrc_t a1 = a.rsrc(k_of(1)), b1 = b.rsrc(k_of(1));
+    StepA ra = a.next();
+    StepB rb = b.next();
 #pragma unroll
-    for (int j = 0; j < 2 * kQ; ++j) issue_one(j, a0, b0, k_of(0), sA0, sB0);
+    for (int j = 0; j < 2 * kQ; ++j) issue_one(j, ra, rb, sA0, sB0);
+    ra = a.next();
+    rb = b.next();
 #pragma unroll
-    for (int j = 0; j < kQ; ++j) issue_one(j, a1, b1, k_of(1), sA1, sB1);
+    for (int j = 0; j < kQ; ++j) issue_one(j, ra, rb, sA1, sB1);
     wait_vm0();
     __syncthreads();
     read_frags(sA0, sB0, 0, fa[0], fb[0]);
+    // A K step from stage (ca, cb), whose first k16 fragments are already in
+    // set 0.  The next step lives in (na, nb): its loads 0-7 went out during
+    // the last k16 of the step before this one, its loads 8-15 go out during
+    // the first k16 here.  The barrier that publishes it sits before the last
+    // k16: every wave has read all of this step's fragments by then, so the
+    // loads 0-7 of the step after the next into (ca, cb) go out during that
+    // last k16, while the next step's first fragments are read.
+    auto step = [&](uint4* ca, uint4* cb, uint4* na, uint4* nb) {
+      read_frags(ca, cb, 1, fa[1], fb[1]);
+      __builtin_amdgcn_sched_barrier(0);
+      mfma16(0, kQ, ra, rb, na, nb);
+      read_frags(ca, cb, 2, fa[0], fb[0]);
+      __builtin_amdgcn_sched_barrier(0);
+      mfma16(1, -1, ra, rb, na, nb);
+      read_frags(ca, cb, 3, fa[1], fb[1]);
+      __builtin_amdgcn_sched_barrier(0);
+      mfma16(0, -1, ra, rb, na, nb);
+      ra = a.next();
+      rb = b.next();
+      wait_vm0();
+      __syncthreads();
+      read_frags(na, nb, 0, fa[0], fb[0]);
+      __builtin_amdgcn_sched_barrier(0);
+      mfma16(1, 0, ra, rb, ca, cb);
+    };
     for (int it = 0; it < total; it += 2) {
-      step(it, sA0, sB0, sA1, sB1);
-      step(it + 1, sA1, sB1, sA0, sB0);
+      step(sA0, sB0, sA1, sB1);
+      step(sA1, sB1, sA0, sB0);
     }
   }
+  wait_vm0();  // (the loads past the last step write their zeros)
   __syncthreads();
   // epilogues read the accumulators by inline asm, which the compiler's hazard
   // checks do not see: no MFMA may be scheduled past this point, and 24 wait
@@ -260,29 +274,40 @@ __device__ __forceinline__ void accumulate(const Source<LA>& a, const Source<LB>
   asm volatile("s_nop 7\n\ts_nop 7\n\ts_nop 7" ::: "memory");
 }
 
-// The order of a grid of tiles.  Workgroup b runs on XCD b mod 8; the 32 that
-// share an XCD's L2 at a time cover a block of h x 32 / h tiles: 8 x 4 where
-// the grid has that many (12 operand tiles per K step, the fewest for 32
-// workgroups), else as near as it goes.  h is picked on the host for the most
-// tiles that there can be, and fits any smaller grid.
-inline int block_rows(int64_t tm, int64_t tn) {
+// The order of tm x tn tiles (`shares` times over, for products whose K is
+// split).  Tiles are numbered through bands of h rows, down each column of a
+// band, so that a run of 32 covers a block of h x 32 / h.  Workgroup b runs on
+// XCD b mod 8: an XCD takes runs of 32 tiles, one per CU, whose 8 + 4 operand
+// tiles (12 is the fewest for 32 workgroups) its L2 serves; a smaller grid is
+// cut into eight runs.  h is picked on the host for the most tiles that there
+// can be and fits any smaller grid.
+inline int band_rows(int64_t tm, int64_t tn) {
   int h = 8;
   while (h > 1 && h / 2 >= tm) h /= 2;
   while (h < 32 && 32 / h / 2 >= tn) h *= 2;
   return h;
 }
-inline int64_t grid_of(int64_t tm, int64_t tn, int h) {
-  const int64_t w = 32 / h, blocks = ((tm + h - 1) / h) * ((tn + w - 1) / w);
-  return (blocks + kXcds - 1) / kXcds * kXcds * 32;
+__host__ __device__ __forceinline__ int run_of(int64_t tiles) {
+  return tiles >= 32 * kXcds ? 32 : (int)((tiles + kXcds - 1) / kXcds);
 }
-// The tile (m, n) of workgroup b; false for one past the last.
-__device__ __forceinline__ bool tile_of(uint32_t b, int tm, int tn, int h, int& m, int& n) {
-  if (tm <= 0 || tn <= 0) return false;
-  const int w = 32 / h, rows = (tm + h - 1) / h;
-  const int i = b / kXcds, block = i / 32 * kXcds + b % kXcds, j = i % 32;
-  m = block % rows * h + j % h;
-  n = block / rows * w + j / h;
-  return m < tm && n < tn;
+inline int64_t grid_of(int64_t tm, int64_t tn, int64_t shares = 1) {
+  const int64_t all = tm * tn * shares, round = (int64_t)kXcds * run_of(all);
+  return all <= 0 ? 0 : (all + round - 1) / round * round;
+}
+// The tile (m, n) and the share of workgroup b; false for one past the last.
+__device__ __forceinline__ bool tile_of(uint32_t b, int tm, int tn, int shares, int h, int& m,
+                                        int& n, int& share) {
+  const uint32_t each = (uint32_t)tm * tn, all = each * shares;
+  if (all == 0) return false;
+  const uint32_t run = run_of(all), i = b / kXcds;
+  const uint32_t at = (i / run * kXcds + b % kXcds) * run + i % run;
+  if (at >= all) return false;
+  share = at / each;
+  const uint32_t t = at - share * each, band = t / ((uint32_t)h * tn), q = t - band * h * tn;
+  const uint32_t rows = min((uint32_t)h, (uint32_t)tm - band * h);
+  m = band * h + q % rows;
+  n = q / rows;
+  return true;
 }
 
 }  // namespace gemm

@@ -211,7 +211,7 @@ struct LseArgs {
   float2* partial;        // [2 * tiles of V][ldn]: (m, s)
   float* xt;              // the target's logit of the listed rows
   int64_t ldn;
-  int tm, h_order;        // tiles of V; block rows of the tile order
+  int tm, band;           // tiles of V; rows of the tile order's bands
 };
 
 // merge of two (m, s) states; an empty one is (-inf, 0)
@@ -226,10 +226,10 @@ __device__ __forceinline__ float2 merge_ms(float2 a, float2 b) {
 // rows, so that a token's values fold in registers.
 template <typename E>
 __global__ __launch_bounds__(kThreads, 1) void lse_kernel(LseArgs a) {
-  __shared__ __attribute__((aligned(16))) uint4 sm[kLds];
+  __shared__ __attribute__((aligned(16))) uint4 sA0[kStage], sA1[kStage], sB0[kStage], sB1[kStage];
   const int n_listed = a.meta->n;
-  int vt, tt;
-  if (!tile_of(blockIdx.x, a.tm, (n_listed + kTile - 1) / kTile, a.h_order, vt, tt)) return;
+  int vt, tt, share;
+  if (!tile_of(blockIdx.x, a.tm, (n_listed + kTile - 1) / kTile, 1, a.band, vt, tt, share)) return;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wv = wave >> 1, wt = wave & 1;
   f32x16 acc[kB][kB];
@@ -239,9 +239,9 @@ __global__ __launch_bounds__(kThreads, 1) void lse_kernel(LseArgs a) {
     for (int y = 0; y < kB; ++y) acc[x][y] = f32x16{};
   Operand h = a.h;
   h.outer = n_listed;
-  const Source<kAlongK> sa(a.w, (int64_t)vt * kTile, a.K, wave, lane);
-  const Source<kAlongK> sb(h, (int64_t)tt * kTile, a.K, wave, lane);
-  accumulate<E>(sa, sb, 0, a.K, sm, wave, lane, acc);
+  Source<kAlongK> sa(a.w, (int64_t)vt * kTile, 0, a.K, wave, lane);
+  Source<kAlongK> sb(h, (int64_t)tt * kTile, 0, a.K, wave, lane);
+  accumulate<E>(sa, sb, a.K, sA0, sA1, sB0, sB1, wave, lane, acc);
 
   // the lane's vocabulary rows are v0 + 32 x + 8 (i / 4) + (i & 3)
   const int64_t v0 = (int64_t)vt * kTile + wv * 128 + 4 * (lane >> 5);
@@ -387,19 +387,19 @@ struct GradArgs {
   Listed rows;
   uint16_t* d;   // [piece rows][ldn]
   int64_t ldn;
-  int tn, h_order;
+  int tm, band;
 };
 
 // The piece's D: tokens x vocabulary, lane l of a block holding vocabulary row
 // l & 31 and 16 tokens, whose lse, g and targets are in LDS.
 template <typename E>
 __global__ __launch_bounds__(kThreads, 1) void grad_logits_kernel(GradArgs a) {
-  __shared__ __attribute__((aligned(16))) uint4 sm[kLds];
+  __shared__ __attribute__((aligned(16))) uint4 sA0[kStage], sA1[kStage], sB0[kStage], sB1[kStage];
   __shared__ __attribute__((aligned(16))) float s_lse[kTile], s_g[kTile];
   __shared__ __attribute__((aligned(16))) int s_t[kTile];
   const int n_listed = a.meta->n;
-  int tt, vt;
-  if (!tile_of(blockIdx.x, (n_listed + kTile - 1) / kTile, a.tn, a.h_order, tt, vt)) return;
+  int tt, vt, share;
+  if (!tile_of(blockIdx.x, a.tm, (n_listed + kTile - 1) / kTile, 1, a.band, vt, tt, share)) return;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wt = wave >> 1, wv = wave & 1;
   {
@@ -417,15 +417,15 @@ __global__ __launch_bounds__(kThreads, 1) void grad_logits_kernel(GradArgs a) {
     for (int y = 0; y < kB; ++y) acc[x][y] = f32x16{};
   Operand h = a.h;
   h.outer = n_listed;
-  const Source<kAlongK> sa(h, (int64_t)tt * kTile, a.K, wave, lane);
-  const Source<kAlongK> sb(a.w, (int64_t)vt * kTile, a.K, wave, lane);
-  accumulate<E>(sa, sb, 0, a.K, sm, wave, lane, acc);
+  Source<kAlongK> sa(h, (int64_t)tt * kTile, 0, a.K, wave, lane);
+  Source<kAlongK> sb(a.w, (int64_t)vt * kTile, 0, a.K, wave, lane);
+  accumulate<E>(sa, sb, a.K, sA0, sA1, sB0, sB1, wave, lane, acc);
 
 #pragma unroll 1
   for (int r = 0; r < kB; ++r) {
     const int row0 = vt * kTile + wv * 128 + r * 32, v = row0 + (lane & 31);
     const int64_t col0 = (int64_t)tt * kTile + wt * 128;
-    store_block(sm + wave * 512, lane, a.d + row0 * a.ldn + col0, a.ldn, a.w.outer - row0,
+    store_block(sA0 + wave * 512, lane, a.d + row0 * a.ldn + col0, a.ldn, a.w.outer - row0,
                 a.ldn - col0, true, [&](int x, int j, uint16_t (&e)[4]) {
                   const int t0 = wt * 128 + x * 32 + j * 8 + 4 * (lane >> 5);
                   const float4 l = *reinterpret_cast<const float4*>(s_lse + t0);
@@ -453,20 +453,20 @@ struct HiddenArgs {
   const Meta* meta;
   float* sum;    // [splits][N][width]
   int64_t N, width;
-  int splits, first, tn, h_order;
+  int splits, first, tn, band;
 };
 
 // dh in fp32, summed over the pieces in place: a workgroup takes one tile's
 // share of the piece's rows.
 template <typename E>
 __global__ __launch_bounds__(kThreads, 1) void grad_hidden_kernel(HiddenArgs a) {
-  __shared__ __attribute__((aligned(16))) uint4 sm[kLds];
+  __shared__ __attribute__((aligned(16))) uint4 sA0[kStage], sA1[kStage], sB0[kStage], sB1[kStage];
   const int n_listed = a.meta->n;
-  int tt, ct;
-  if (!tile_of(blockIdx.x, (n_listed + kTile - 1) / kTile, a.tn, a.h_order, tt, ct)) return;
+  int tt, ct, split;
+  if (!tile_of(blockIdx.x, (n_listed + kTile - 1) / kTile, a.tn, a.splits, a.band, tt, ct, split))
+    return;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wt = wave >> 1, wc = wave & 1;
-  const int split = blockIdx.y;
   const int64_t steps = (a.K + kBK - 1) / kBK, per = (steps + a.splits - 1) / a.splits * kBK;
   const int64_t k0 = min(a.K, split * per), k1 = min(a.K, k0 + per);
   f32x16 acc[kB][kB];
@@ -474,9 +474,9 @@ __global__ __launch_bounds__(kThreads, 1) void grad_hidden_kernel(HiddenArgs a) 
   for (int x = 0; x < kB; ++x)
 #pragma unroll
     for (int y = 0; y < kB; ++y) acc[x][y] = f32x16{};
-  const Source<kAcrossK> sa(a.d, (int64_t)tt * kTile, k1, wave, lane);
-  const Source<kAcrossK> sb(a.w, (int64_t)ct * kTile, k1, wave, lane);
-  accumulate<E>(sa, sb, k0, k1 - k0, sm, wave, lane, acc);
+  Source<kAcrossK> sa(a.d, (int64_t)tt * kTile, k0, k1 - k0, wave, lane);
+  Source<kAcrossK> sb(a.w, (int64_t)ct * kTile, k0, k1 - k0, wave, lane);
+  accumulate<E>(sa, sb, k1 - k0, sA0, sA1, sB0, sB1, wave, lane, acc);
 
   float* sum = a.sum + (int64_t)split * a.N * a.width;
 #pragma unroll 1
@@ -528,16 +528,16 @@ struct WeightArgs {
   const Meta* meta;
   uint16_t* out;  // the piece's first row of grad_weight, row stride ld
   int64_t ld, width;
-  int tm, tn, h_order, vec;
+  int tm, tn, band, vec;
 };
 
 // dw of the piece's rows: hidden columns x vocabulary rows, over the listed
 // tokens.
 template <typename E>
 __global__ __launch_bounds__(kThreads, 1) void grad_weight_kernel(WeightArgs a) {
-  __shared__ __attribute__((aligned(16))) uint4 sm[kLds];
-  int ct, vt;
-  if (!tile_of(blockIdx.x, a.tm, a.tn, a.h_order, ct, vt)) return;
+  __shared__ __attribute__((aligned(16))) uint4 sA0[kStage], sA1[kStage], sB0[kStage], sB1[kStage];
+  int ct, vt, share;
+  if (!tile_of(blockIdx.x, a.tm, a.tn, 1, a.band, vt, ct, share)) return;
   const int64_t K = a.meta->n;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wc = wave >> 1, wv = wave & 1;
@@ -546,15 +546,15 @@ __global__ __launch_bounds__(kThreads, 1) void grad_weight_kernel(WeightArgs a) 
   for (int x = 0; x < kB; ++x)
 #pragma unroll
     for (int y = 0; y < kB; ++y) acc[x][y] = f32x16{};
-  const Source<kAcrossK> sa(a.h, (int64_t)ct * kTile, K, wave, lane);
-  const Source<kAlongK> sb(a.d, (int64_t)vt * kTile, K, wave, lane);
-  accumulate<E>(sa, sb, 0, K, sm, wave, lane, acc);
+  Source<kAcrossK> sa(a.h, (int64_t)ct * kTile, 0, K, wave, lane);
+  Source<kAlongK> sb(a.d, (int64_t)vt * kTile, 0, K, wave, lane);
+  accumulate<E>(sa, sb, K, sA0, sA1, sB0, sB1, wave, lane, acc);
   const float inv = a.meta->inv;
 #pragma unroll 1
   for (int r = 0; r < kB; ++r) {
     const int64_t row0 = (int64_t)vt * kTile + wv * 128 + r * 32;
     const int64_t col0 = (int64_t)ct * kTile + wc * 128;
-    store_block(sm + wave * 512, lane, a.out + row0 * a.ld + col0, a.ld, a.d.outer - row0,
+    store_block(sA0 + wave * 512, lane, a.out + row0 * a.ld + col0, a.ld, a.d.outer - row0,
                 a.width - col0, a.vec, [&](int x, int j, uint16_t (&e)[4]) {
 #pragma unroll
                   for (int i = 0; i < 4; ++i) e[i] = E::from(acc_read(acc[x][0][4 * j + i]) * inv);
@@ -613,8 +613,7 @@ int shape_of(const gtp_linear_rows* r, Shape& s, Rows& a) {
   s.n_tt = tiles(s.N);
   s.n_ct = tiles(s.K8);
   // a launch holds fewer than 2^32 threads
-  if (grid_of(s.n_vt, s.n_tt, block_rows(s.n_vt, s.n_tt)) >= (int64_t)1 << 24 ||
-      grid_of(s.n_ct, s.n_vt, block_rows(s.n_ct, s.n_vt)) >= (int64_t)1 << 24)
+  if (grid_of(s.n_vt, s.n_tt) >= (int64_t)1 << 24 || grid_of(s.n_ct, s.n_vt) >= (int64_t)1 << 24)
     return GTP_ERR_UNSUPPORTED;
   a = Rows{r->targets, r->V, r->S, r->T, r->target_batch_stride, r->target_row_stride,
            r->ignore_index, (int)r->B, r->targets_int64 ? 1 : 0, r->has_ignore ? 1 : 0};
@@ -716,63 +715,78 @@ void forward_launch(const gtp_linear_rows* r, const Shape& s, const Forward& f, 
   a.xt = f.xt;
   a.ldn = s.ldn;
   a.tm = s.n_vt;
-  a.h_order = block_rows(s.n_vt, s.n_tt);
-  launch_timed(lse_kernel<E>, dim3((unsigned)grid_of(s.n_vt, s.n_tt, a.h_order)), dim3(kThreads),
-               st, a);
+  a.band = band_rows(s.n_vt, s.n_tt);
+  launch_timed(lse_kernel<E>, dim3((unsigned)grid_of(s.n_vt, s.n_tt)), dim3(kThreads), st, a);
+}
+
+// The three products of a piece of `rows` vocabulary rows from v0 on.
+inline Operand piece_of(const gtp_linear_rows* r, int64_t v0, int64_t rows) {
+  return Operand{reinterpret_cast<const uint16_t*>(r->weight) + v0 * r->weight_stride,
+                 r->weight_stride, rows};
+}
+
+template <typename E>
+void grad_logits_launch(const gtp_linear_rows* r, const Shape& s, const Backward& b, int64_t v0,
+                        int64_t rows, hipStream_t st) {
+  GradArgs a;
+  a.h = Operand{b.h, s.ldh, s.N};
+  a.w = piece_of(r, v0, rows);
+  a.K = s.K8;
+  a.v_first = v0;
+  a.meta = b.meta;
+  a.rows = b.rows;
+  a.d = b.d;
+  a.ldn = s.ldn;
+  a.tm = tiles(rows);
+  a.band = band_rows(a.tm, s.n_tt);
+  launch_timed(grad_logits_kernel<E>, dim3((unsigned)grid_of(a.tm, s.n_tt)), dim3(kThreads), st, a);
+}
+
+template <typename E>
+void grad_hidden_launch(const gtp_linear_rows* r, const Shape& s, const Pieces& p,
+                        const Backward& b, int64_t v0, int64_t rows, hipStream_t st) {
+  HiddenArgs a;
+  a.d = Operand{b.d, s.ldn, s.ldn};
+  a.w = piece_of(r, v0, s.K8);
+  a.K = rows;
+  a.meta = b.meta;
+  a.sum = b.sum;
+  a.N = s.N;
+  a.width = r->K;
+  a.splits = p.splits;
+  a.first = v0 == 0 ? 1 : 0;
+  a.tn = s.n_ct;
+  a.band = band_rows(s.n_tt, s.n_ct);
+  hipLaunchKernelGGL(grad_hidden_kernel<E>, dim3((unsigned)grid_of(s.n_tt, s.n_ct, p.splits)),
+                     dim3(kThreads), 0, st, a);
+}
+
+template <typename E>
+void grad_weight_launch(const gtp_linear_rows* r, const Shape& s, const Backward& b, int64_t v0,
+                        int64_t rows, uint16_t* grad_weight, hipStream_t st) {
+  WeightArgs a;
+  a.h = Operand{b.h, s.ldh, s.ldh};
+  a.d = Operand{b.d, s.ldn, rows};
+  a.meta = b.meta;
+  a.out = grad_weight + v0 * r->K;
+  a.ld = r->K;
+  a.width = r->K;
+  a.tm = tiles(rows);
+  a.tn = s.n_ct;
+  a.band = band_rows(a.tm, a.tn);
+  a.vec = (r->K & 7) == 0 && (reinterpret_cast<uintptr_t>(grad_weight) & 15u) == 0 ? 1 : 0;
+  hipLaunchKernelGGL(grad_weight_kernel<E>, dim3((unsigned)grid_of(a.tm, a.tn)), dim3(kThreads), 0,
+                     st, a);
 }
 
 template <typename E>
 void backward_launch(const gtp_linear_rows* r, const Shape& s, const Pieces& p, const Backward& b,
                      uint16_t* grad_hidden, uint16_t* grad_weight, hipStream_t st) {
-  const uint16_t* w = reinterpret_cast<const uint16_t*>(r->weight);
-  for (int64_t v0 = 0; s.N > 0 && v0 < r->V; v0 += p.rows) {
+  for (int64_t v0 = 0; v0 < r->V; v0 += p.rows) {
     const int64_t rows = min(p.rows, r->V - v0);
-    const Operand piece{w + v0 * r->weight_stride, r->weight_stride, rows};
-    GradArgs g;
-    g.h = Operand{b.h, s.ldh, s.N};
-    g.w = piece;
-    g.K = s.K8;
-    g.v_first = v0;
-    g.meta = b.meta;
-    g.rows = b.rows;
-    g.d = b.d;
-    g.ldn = s.ldn;
-    g.tn = tiles(rows);
-    g.h_order = block_rows(s.n_tt, g.tn);
-    launch_timed(grad_logits_kernel<E>, dim3((unsigned)grid_of(s.n_tt, g.tn, g.h_order)),
-                 dim3(kThreads), st, g);
-    if (grad_hidden) {
-      HiddenArgs h;
-      h.d = Operand{b.d, s.ldn, s.ldn};
-      h.w = Operand{piece.p, piece.ld, s.K8};
-      h.K = rows;
-      h.meta = b.meta;
-      h.sum = b.sum;
-      h.N = s.N;
-      h.width = r->K;
-      h.splits = p.splits;
-      h.first = v0 == 0 ? 1 : 0;
-      h.tn = s.n_ct;
-      h.h_order = block_rows(s.n_tt, s.n_ct);
-      hipLaunchKernelGGL(grad_hidden_kernel<E>,
-                         dim3((unsigned)grid_of(s.n_tt, s.n_ct, h.h_order), (unsigned)p.splits),
-                         dim3(kThreads), 0, st, h);
-    }
-    if (grad_weight) {
-      WeightArgs q;
-      q.h = Operand{b.h, s.ldh, s.ldh};
-      q.d = Operand{b.d, s.ldn, rows};
-      q.meta = b.meta;
-      q.out = grad_weight + v0 * r->K;
-      q.ld = r->K;
-      q.width = r->K;
-      q.tm = s.n_ct;
-      q.tn = tiles(rows);
-      q.h_order = block_rows(q.tm, q.tn);
-      q.vec = (r->K & 7) == 0 && (reinterpret_cast<uintptr_t>(grad_weight) & 15u) == 0 ? 1 : 0;
-      hipLaunchKernelGGL(grad_weight_kernel<E>, dim3((unsigned)grid_of(q.tm, q.tn, q.h_order)),
-                         dim3(kThreads), 0, st, q);
-    }
+    grad_logits_launch<E>(r, s, b, v0, rows, st);
+    if (grad_hidden) grad_hidden_launch<E>(r, s, p, b, v0, rows, st);
+    if (grad_weight) grad_weight_launch<E>(r, s, b, v0, rows, grad_weight, st);
   }
   if (grad_hidden)
     hipLaunchKernelGGL(grad_hidden_rows_kernel<E>, dim3((unsigned)(r->B * r->S)), dim3(256), 0, st,
