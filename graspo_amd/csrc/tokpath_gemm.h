@@ -90,26 +90,39 @@ __device__ __forceinline__ float acc_read(float a) {
   return v;
 }
 
+// Where an operand's K steps for one tile lie (uniform over the workgroup).
+struct Cursor {
+  const char* at;  // the next step's first byte
+  int64_t left;    // bytes from there to the end of what the tile may read
+  int k_left;      // kAlongK: K from there on
+};
+// Of the tile whose first row (kAlongK) or column (kAcrossK) is `first`, for K
+// values of K from k_first (a multiple of 8) on.
+template <Layout L>
+__device__ __forceinline__ Cursor cursor_of(const Operand& o, int64_t first, int64_t k_first,
+                                            int64_t K) {
+  const int64_t ld = o.ld * 2, outer = max((int64_t)0, o.outer - first);
+  if constexpr (L == kAlongK)
+    return Cursor{reinterpret_cast<const char*>(o.p) + first * ld + k_first * 2,
+                  min((int64_t)kTile, outer) * ld - k_first * 2, (int)K};
+  else
+    return Cursor{reinterpret_cast<const char*>(o.p + first) + k_first * ld,
+                  outer > 0 && K > 0 ? (K - 1) * ld + outer * 2 : 0, (int)K};
+}
+
 // One operand's K steps, in order: wave w's load q of a step fills the 1 KB of
 // LDS from chunk (8w + q) * 64 on, 16 bytes per lane.
 template <Layout L>
 struct Source {
-  const char* at;   // the next step's first byte
-  int64_t left;     // bytes from there to the operand's end; kAlongK: at least
-  int k_left;       // kAlongK: K from the next step on
+  Cursor c;
   uint32_t v0, v1;  // the lane's byte offset for even and odd q
   int c0, c1;       // kAlongK: its first k within the step
   uint32_t qstep;   // bytes from q to q + 2, halved
   int64_t advance;  // bytes from step to step
 
-  // k_first: a multiple of 8; K: from there on
-  __device__ __forceinline__ Source(const Operand& o, int64_t first, int64_t k_first, int64_t K,
-                                    int wave, int lane) {
-    const int64_t ld = o.ld * 2, outer = max((int64_t)0, o.outer - first);
-    k_left = (int)K;
+  __device__ __forceinline__ Source(int64_t ld_elements, int wave, int lane) : c{nullptr, 0, 0} {
+    const int64_t ld = ld_elements * 2;
     if constexpr (L == kAlongK) {
-      at = reinterpret_cast<const char*>(o.p) + first * ld + k_first * 2;
-      left = min((int64_t)kTile, outer) * ld - k_first * 2;
       advance = kBK * 2;
       // LDS row 8 (8w + q) + lane / 8, chunk lane & 7 of it holding chunk
       // (lane & 7) ^ ((row >> 1) & 7) of the row
@@ -120,8 +133,6 @@ struct Source {
       v1 = (uint32_t)(row * ld + c1 * 2);
       qstep = (uint32_t)(8 * ld);
     } else {
-      at = reinterpret_cast<const char*>(o.p + first) + k_first * ld;
-      left = outer > 0 && K > 0 ? (K - 1) * ld + outer * 2 : 0;
       advance = kBK * ld;
       // LDS row 2 (8w + q) + lane / 32, chunk lane & 31 of it holding chunk
       // (lane & 31) ^ 4 (row & 3) of the row
@@ -140,15 +151,15 @@ struct Source {
   };
   // The next step; past the last one all its loads are out of range.
   __device__ __forceinline__ Step next() {
-    const int n = (int)max((int64_t)0, min(left, (int64_t)kPast));
-    Step s{at, n, v0, v1};
+    const int n = (int)max((int64_t)0, min(c.left, (int64_t)kPast));
+    Step s{c.at, n, v0, v1};
     if constexpr (L == kAlongK) {
-      s.v0 = c0 < k_left ? v0 : kPast;
-      s.v1 = c1 < k_left ? v1 : kPast;
-      k_left -= kBK;
+      s.v0 = c0 < c.k_left ? v0 : kPast;
+      s.v1 = c1 < c.k_left ? v1 : kPast;
+      c.k_left -= kBK;
     }
-    at += advance;
-    left -= advance;
+    c.at += advance;
+    c.left -= advance;
     return s;
   }
   // the whole offset goes in the VGPR operand: the range check covers it
@@ -180,107 +191,138 @@ __device__ __forceinline__ s16x8 fragment(const uint4* stage, int side, int x, i
   }
 }
 
-// acc[x][y] += A rows (block x) times B rows (block y) over the sources' steps
-// of K: lane l of a block holds B index l & 31 and the A indices 8 (i / 4) +
-// 4 (l / 32) + (i & 3) for i = 0 .. 15.  Ends with the accumulators complete
-// and every wave past its last LDS access.
+// The tile loop of a workgroup: acc[x][y] = A rows (block x) times B rows
+// (block y), lane l of a block holding B index l & 31 and the A indices
+// 8 (i / 4) + 4 (l / 32) + (i & 3) for i = 0 .. 15.
+//
+// The loop runs on from tile to tile: the last two K steps of a tile load the
+// first two of the next one, so that its operands come in while the epilogue
+// works on the accumulators (a tile started anew cost 12 us of 110 at K =
+// 4096).
 //
 // The four stages are four arrays, so that the compiler sees that the loads in
 // flight write to others than it reads (from one array it waits for all loads
-// before every transposing read: 877 against 1040 TFLOP/s).
+// before every transposing read: 877 against 1225 TFLOP/s).
 template <typename E, Layout LA, Layout LB>
-__device__ __forceinline__ void accumulate(Source<LA>& a, Source<LB>& b, int64_t K, uint4* sA0,
-                                           uint4* sA1, uint4* sB0, uint4* sB1, int wave, int lane,
-                                           f32x16 (&acc)[kB][kB]) {
-  const int wa = wave >> 1, wb = wave & 1;
-  // an even number of steps (the stages alternate); one past K adds zeros
-  const int total = 2 * (int)((K + 2 * kBK - 1) / (2 * kBK));
+struct TileLoop {
   typedef typename Source<LA>::Step StepA;
   typedef typename Source<LB>::Step StepB;
-  auto issue_one = [&](int j, const StepA& ra, const StepB& rb, uint4* sa, uint4* sb) {
+  Source<LA> a;
+  Source<LB> b;
+  uint4 *sA0, *sA1, *sB0, *sB1;
+  int wave, lane;
+  StepA na;  // the step whose loads are going out
+  StepB nb;
+  f32x16 acc[kB][kB];
+  // fragments of the k16 step at work and of the next one, [0, kB) of A and
+  // [kB, 2 kB) of B
+  s16x8 f[2][2 * kB];
+
+  __device__ __forceinline__ TileLoop(int64_t lda, int64_t ldb, uint4* sA0_, uint4* sA1_,
+                                      uint4* sB0_, uint4* sB1_, int wave_, int lane_)
+      : a(lda, wave_, lane_), b(ldb, wave_, lane_), sA0(sA0_), sA1(sA1_), sB0(sB0_), sB1(sB1_),
+        wave(wave_), lane(lane_) {}
+
+  __device__ __forceinline__ void issue_one(int j, uint4* sa, uint4* sb) {
     if (j & 1)
-      b.issue(rb, j >> 1, sb, wave);
+      b.issue(nb, j >> 1, sb, wave);
     else
-      a.issue(ra, j >> 1, sa, wave);
-  };
-  s16x8 fa[2][kB], fb[2][kB];
-  auto read_frags = [&](const uint4* sa, const uint4* sb, int kk, s16x8 (&f)[kB], s16x8 (&g)[kB]) {
+      a.issue(na, j >> 1, sa, wave);
+  }
+  // read i of a k16 step, in the order in which the MFMAs want them
+  __device__ __forceinline__ void read_one(int set, int i, const uint4* sa, const uint4* sb, int kk) {
+    if (i == 0)
+      f[set][0] = fragment<LA>(sa, wave >> 1, 0, kk, lane);
+    else if (i <= kB)
+      f[set][kB + i - 1] = fragment<LB>(sb, wave & 1, i - 1, kk, lane);
+    else
+      f[set][i - kB] = fragment<LA>(sa, wave >> 1, i - kB, kk, lane);
+  }
+  // 16 MFMAs of one k16 step from fragment set c.  Among them, one after the
+  // other so that neither queue holds the matrix cores up: the reads of the
+  // next k16 step (kk of stage (ra, rb)) and, with j0 >= 0, the loads j0 ..
+  // j0 + 7 into stage (la, lb).
+  __device__ __forceinline__ void mfma16(int c, const uint4* ra, const uint4* rb, int kk, int j0,
+                                         uint4* la, uint4* lb) {
 #pragma unroll
-    for (int x = 0; x < kB; ++x) f[x] = fragment<LA>(sa, wa, x, kk, lane);
-#pragma unroll
-    for (int y = 0; y < kB; ++y) g[y] = fragment<LB>(sb, wb, y, kk, lane);
-  };
-  // 16 MFMAs of one k16 step from fragment set c, with the loads j0 .. j0 + 7
-  // among them
-  auto mfma16 = [&](int c, int j0, const StepA& ra, const StepB& rb, uint4* la, uint4* lb) {
-#pragma unroll
-    for (int x = 0; x < kB; ++x) {
+    for (int x = 0; x < kB; ++x)
 #pragma unroll
       for (int y = 0; y < kB; ++y) {
-        acc[x][y] = E::mfma(fa[c][x], fb[c][y], acc[x][y]);
-        if (j0 >= 0 && (y & 1)) issue_one(j0 + x * (kB / 2) + (y >> 1), ra, rb, la, lb);
+        const int i = x * kB + y;
+        acc[x][y] = E::mfma(f[c][x], f[c][kB + y], acc[x][y]);
+        if (i % 2 == 0) read_one(c ^ 1, i / 2, ra, rb, kk);
+        if (i % 2 == 1 && j0 >= 0) issue_one(j0 + i / 2, la, lb);
+        __builtin_amdgcn_sched_barrier(0);
       }
-      __builtin_amdgcn_sched_barrier(0);
-    }
-  };
-  if (total > 0) {
-    StepA ra = a.next();
-    StepB rb = b.next();
-#pragma unroll
-    for (int j = 0; j < 2 * kQ; ++j) issue_one(j, ra, rb, sA0, sB0);
-    ra = a.next();
-    rb = b.next();
-#pragma unroll
-    for (int j = 0; j < kQ; ++j) issue_one(j, ra, rb, sA1, sB1);
+  }
+  // A K step from stage (ca, cb), whose first k16 fragments are already in
+  // set 0.  The next step lives in (sa, sb): its loads 0-7 went out during the
+  // last k16 of the step before this one, its loads 8-15 go out during the
+  // first k16 here.  The barrier that publishes it sits before the last k16:
+  // every wave has read all of this step's fragments by then, so the loads 0-7
+  // of the step after the next into (ca, cb) go out during that last k16,
+  // while the next step's first fragments are read.
+  __device__ __forceinline__ void step(uint4* ca, uint4* cb, uint4* sa, uint4* sb) {
+    mfma16(0, ca, cb, 1, kQ, sa, sb);
+    mfma16(1, ca, cb, 2, -1, sa, sb);
+    mfma16(0, ca, cb, 3, -1, sa, sb);
+    na = a.next();
+    nb = b.next();
     wait_vm0();
     __syncthreads();
-    read_frags(sA0, sB0, 0, fa[0], fb[0]);
-    // A K step from stage (ca, cb), whose first k16 fragments are already in
-    // set 0.  The next step lives in (na, nb): its loads 0-7 went out during
-    // the last k16 of the step before this one, its loads 8-15 go out during
-    // the first k16 here.  The barrier that publishes it sits before the last
-    // k16: every wave has read all of this step's fragments by then, so the
-    // loads 0-7 of the step after the next into (ca, cb) go out during that
-    // last k16, while the next step's first fragments are read.
-    auto step = [&](uint4* ca, uint4* cb, uint4* na, uint4* nb) {
-      read_frags(ca, cb, 1, fa[1], fb[1]);
-      __builtin_amdgcn_sched_barrier(0);
-      mfma16(0, kQ, ra, rb, na, nb);
-      read_frags(ca, cb, 2, fa[0], fb[0]);
-      __builtin_amdgcn_sched_barrier(0);
-      mfma16(1, -1, ra, rb, na, nb);
-      read_frags(ca, cb, 3, fa[1], fb[1]);
-      __builtin_amdgcn_sched_barrier(0);
-      mfma16(0, -1, ra, rb, na, nb);
-      ra = a.next();
-      rb = b.next();
-      wait_vm0();
-      __syncthreads();
-      read_frags(na, nb, 0, fa[0], fb[0]);
-      __builtin_amdgcn_sched_barrier(0);
-      mfma16(1, 0, ra, rb, ca, cb);
-    };
-    for (int it = 0; it < total; it += 2) {
+    mfma16(1, sa, sb, 0, 0, ca, cb);
+  }
+  // Ahead of the first tile.
+  __device__ __forceinline__ void start(const Cursor& ca, const Cursor& cb) {
+    a.c = ca;
+    b.c = cb;
+    na = a.next();
+    nb = b.next();
+#pragma unroll
+    for (int j = 0; j < 2 * kQ; ++j) issue_one(j, sA0, sB0);
+    na = a.next();
+    nb = b.next();
+#pragma unroll
+    for (int j = 0; j < kQ; ++j) issue_one(j, sA1, sB1);
+    wait_vm0();
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 2 * kB; ++i) read_one(0, i, sA0, sB0, 0);
+  }
+  // One tile over K (at least its first two steps; past K they are zeros),
+  // then on to the tile of the cursors given (empty ones behind the last).
+  __device__ __forceinline__ void tile(int64_t K, const Cursor& next_a, const Cursor& next_b) {
+#pragma unroll
+    for (int x = 0; x < kB; ++x)
+#pragma unroll
+      for (int y = 0; y < kB; ++y) acc[x][y] = f32x16{};
+    // an even number of steps (the stages alternate)
+    int pairs = (int)((K + 2 * kBK - 1) / (2 * kBK));
+    pairs = pairs < 1 ? 1 : pairs;
+    for (int p = 0; p < pairs; ++p) {
+      if (p + 1 == pairs) {
+        a.c = next_a;
+        b.c = next_b;
+      }
       step(sA0, sB0, sA1, sB1);
       step(sA1, sB1, sA0, sB0);
     }
+    // epilogues read the accumulators by inline asm, which the compiler's
+    // hazard checks do not see: no MFMA may be scheduled past this point, and
+    // 24 wait states after the last one cover its result latency (11 for an
+    // 8-pass MFMA)
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("s_nop 7\n\ts_nop 7\n\ts_nop 7" ::: "memory");
   }
-  wait_vm0();  // (the loads past the last step write their zeros)
-  __syncthreads();
-  // epilogues read the accumulators by inline asm, which the compiler's hazard
-  // checks do not see: no MFMA may be scheduled past this point, and 24 wait
-  // states after the last one cover its result latency (11 for an 8-pass MFMA)
-  __builtin_amdgcn_sched_barrier(0);
-  asm volatile("s_nop 7\n\ts_nop 7\n\ts_nop 7" ::: "memory");
-}
+};
 
 // The order of tm x tn tiles (`shares` times over, for products whose K is
 // split).  Tiles are numbered through bands of h rows, down each column of a
 // band, so that a run of 32 covers a block of h x 32 / h.  Workgroup b runs on
-// XCD b mod 8: an XCD takes runs of 32 tiles, one per CU, whose 8 + 4 operand
-// tiles (12 is the fewest for 32 workgroups) its L2 serves; a smaller grid is
-// cut into eight runs.  h is picked on the host for the most tiles that there
-// can be and fits any smaller grid.
+// XCD b mod 8: an XCD takes every eighth run of 32 tiles, one tile per
+// workgroup, whose 8 + 4 operand tiles (12 is the fewest for 32 workgroups)
+// its L2 serves; up to 256 tiles are cut into eight runs.  h is picked on the
+// host for the most tiles that there can be and fits any smaller number.
 inline int band_rows(int64_t tm, int64_t tn) {
   int h = 8;
   while (h > 1 && h / 2 >= tm) h /= 2;
@@ -290,25 +332,30 @@ inline int band_rows(int64_t tm, int64_t tn) {
 __host__ __device__ __forceinline__ int run_of(int64_t tiles) {
   return tiles >= 32 * kXcds ? 32 : (int)((tiles + kXcds - 1) / kXcds);
 }
-inline int64_t grid_of(int64_t tm, int64_t tn, int64_t shares = 1) {
-  const int64_t all = tm * tn * shares, round = (int64_t)kXcds * run_of(all);
-  return all <= 0 ? 0 : (all + round - 1) / round * round;
+// Workgroups: one per tile up to one per CU of the whole chip.
+inline unsigned grid_of(int64_t tm, int64_t tn, int64_t shares = 1) {
+  return (unsigned)(kXcds * run_of(tm * tn * shares));
 }
-// The tile (m, n) and the share of workgroup b; false for one past the last.
-__device__ __forceinline__ bool tile_of(uint32_t b, int tm, int tn, int shares, int h, int& m,
-                                        int& n, int& share) {
-  const uint32_t each = (uint32_t)tm * tn, all = each * shares;
-  if (all == 0) return false;
-  const uint32_t run = run_of(all), i = b / kXcds;
-  const uint32_t at = (i / run * kXcds + b % kXcds) * run + i % run;
-  if (at >= all) return false;
-  share = at / each;
-  const uint32_t t = at - share * each, band = t / ((uint32_t)h * tn), q = t - band * h * tn;
-  const uint32_t rows = min((uint32_t)h, (uint32_t)tm - band * h);
-  m = band * h + q % rows;
-  n = q / rows;
-  return true;
-}
+// Walks the tiles of one workgroup.
+struct Tiles {
+  uint32_t all, each, run, at, tn, h, tm;
+  __device__ __forceinline__ Tiles(uint32_t b, int tm_, int tn_, int shares, int h_)
+      : each((uint32_t)tm_ * tn_), tn(tn_), h(h_), tm(tm_) {
+    all = each * shares;
+    run = run_of(all);
+    const uint32_t i = b / kXcds;
+    at = i < run ? b % kXcds * run + i : all;
+  }
+  __device__ __forceinline__ bool more() const { return at < all; }
+  __device__ __forceinline__ void step() { at += kXcds * run; }
+  __device__ __forceinline__ void place(int& m, int& n, int& share) const {
+    share = at / each;
+    const uint32_t t = at - share * each, band = t / (h * tn), q = t - band * h * tn;
+    const uint32_t rows = min(h, tm - band * h);
+    m = band * h + q % rows;
+    n = q / rows;
+  }
+};
 
 }  // namespace gemm
 }  // namespace gtp

@@ -43,8 +43,10 @@ namespace lin {
 
 using namespace gemm;
 
-// Bytes of D at a time.
-constexpr int64_t kPieceBytes = (int64_t)512 << 20;
+// Bytes of D at a time.  A piece costs dh a pass over its fp32 sums and a
+// drain of the chip: at 8192 x 4096 x 131072 dh takes 6.6 ms in one piece of 2
+// GiB, 6.7 in two, 7.1 in four, 8.3 in eight; the other products do not care.
+constexpr int64_t kPieceBytes = (int64_t)1 << 30;
 
 struct Rows {
   const void* targets;
@@ -228,61 +230,76 @@ template <typename E>
 __global__ __launch_bounds__(kThreads, 1) void lse_kernel(LseArgs a) {
   __shared__ __attribute__((aligned(16))) uint4 sA0[kStage], sA1[kStage], sB0[kStage], sB1[kStage];
   const int n_listed = a.meta->n;
-  int vt, tt, share;
-  if (!tile_of(blockIdx.x, a.tm, (n_listed + kTile - 1) / kTile, 1, a.band, vt, tt, share)) return;
+  Tiles at(blockIdx.x, a.tm, (n_listed + kTile - 1) / kTile, 1, a.band);
+  if (!at.more()) return;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wv = wave >> 1, wt = wave & 1;
-  f32x16 acc[kB][kB];
-#pragma unroll
-  for (int x = 0; x < kB; ++x)
-#pragma unroll
-    for (int y = 0; y < kB; ++y) acc[x][y] = f32x16{};
   Operand h = a.h;
   h.outer = n_listed;
-  Source<kAlongK> sa(a.w, (int64_t)vt * kTile, 0, a.K, wave, lane);
-  Source<kAlongK> sb(h, (int64_t)tt * kTile, 0, a.K, wave, lane);
-  accumulate<E>(sa, sb, a.K, sA0, sA1, sB0, sB1, wave, lane, acc);
-
-  // the lane's vocabulary rows are v0 + 32 x + 8 (i / 4) + (i & 3)
-  const int64_t v0 = (int64_t)vt * kTile + wv * 128 + 4 * (lane >> 5);
-  const int64_t left = a.w.outer - v0;
-  const int lim = (int)min((int64_t)128, max(left, (int64_t)0));  // valid offsets are below
-#pragma unroll 1
-  for (int r = 0; r < kB; ++r) {  // token blocks, rotated through block 0
-    const int64_t k = (int64_t)tt * kTile + wt * 128 + r * 32 + (lane & 31);
-    const int64_t off = (k < n_listed ? (int64_t)a.target[k] : -1) - v0;
-    float2 st{kNegInf, 0.0f};
-#pragma unroll
-    for (int x = 0; x < kB; ++x) {
-      float v[16];
-#pragma unroll
-      for (int i = 0; i < 16; ++i) v[i] = acc_read(acc[x][0][i]);
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const int o = x * 32 + 8 * (i >> 2) + (i & 3);
-        if (off == o) a.xt[k] = v[i];
-        if (o >= lim) v[i] = kNegInf;
-      }
-      float m = v[0];
-#pragma unroll
-      for (int i = 1; i < 16; i += 2) m = max3raw(m, v[i], i + 1 < 16 ? v[i + 1] : v[i]);
-      m = fmaxf(m, st.x);
-      // (the difference first: exact near the maximum, however large that is)
-      const float mb = m == kNegInf ? 0.0f : m;
-      float s = 0.0f;
-#pragma unroll
-      for (int i = 0; i < 16; ++i) s += __builtin_amdgcn_exp2f((v[i] - mb) * kLog2e);
-      const float f = st.x == m ? 1.0f : __builtin_amdgcn_exp2f((st.x - m) * kLog2e);
-      st = float2{m, __builtin_fmaf(st.y, f, s)};
+  TileLoop<E, kAlongK, kAlongK> loop(a.w.ld, h.ld, sA0, sA1, sB0, sB1, wave, lane);
+  int vt, tt, share;
+  at.place(vt, tt, share);
+  loop.start(cursor_of<kAlongK>(a.w, (int64_t)vt * kTile, 0, a.K),
+             cursor_of<kAlongK>(h, (int64_t)tt * kTile, 0, a.K));
+  for (bool more = true; more;) {
+    at.step();
+    more = at.more();
+    int vt2 = 0, tt2 = 0;
+    Cursor ca{nullptr, 0, 0}, cb = ca;
+    if (more) {
+      at.place(vt2, tt2, share);
+      ca = cursor_of<kAlongK>(a.w, (int64_t)vt2 * kTile, 0, a.K);
+      cb = cursor_of<kAlongK>(h, (int64_t)tt2 * kTile, 0, a.K);
     }
-    const float2 other{__shfl_xor(st.x, 32, kWave), __shfl_xor(st.y, 32, kWave)};
-    st = merge_ms(st, other);
-    if (lane < 32 && k < n_listed) a.partial[(int64_t)(vt * 2 + wv) * a.ldn + k] = st;
+    loop.tile(a.K, ca, cb);
+
+    // the lane's vocabulary rows are v0 + 32 x + 8 (i / 4) + (i & 3)
+    const int64_t v0 = (int64_t)vt * kTile + wv * 128 + 4 * (lane >> 5);
+    const int64_t left = a.w.outer - v0;
+    const int lim = (int)min((int64_t)128, max(left, (int64_t)0));  // valid offsets are below
+#pragma unroll 1
+    for (int r = 0; r < kB; ++r) {  // token blocks, rotated through block 0
+      const int64_t k = (int64_t)tt * kTile + wt * 128 + r * 32 + (lane & 31);
+      const int64_t off = (k < n_listed ? (int64_t)a.target[k] : -1) - v0;
+      const int want = off >= 0 && off < lim ? (int)off : -1;
+      float2 st{kNegInf, 0.0f};
+      float xt = 0.0f;
 #pragma unroll
-    for (int y = 0; y < kB - 1; ++y)
+      for (int x = 0; x < kB; ++x) {
+        float v[16];
 #pragma unroll
-      for (int x = 0; x < kB; ++x) acc[x][y] = acc[x][y + 1];
+        for (int i = 0; i < 16; ++i) {
+          const int o = x * 32 + 8 * (i >> 2) + (i & 3);
+          const float q = acc_read(loop.acc[x][0][i]);
+          xt = want == o ? q : xt;
+          v[i] = o < lim ? q : kNegInf;
+        }
+        float m = v[0];
+#pragma unroll
+        for (int i = 1; i < 16; i += 2) m = max3raw(m, v[i], i + 1 < 16 ? v[i + 1] : v[i]);
+        m = fmaxf(m, st.x);
+        // (the difference first: exact near the maximum, however large that is)
+        const float mb = m == kNegInf ? 0.0f : m;
+        float s = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s += __builtin_amdgcn_exp2f((v[i] - mb) * kLog2e);
+        const float f = st.x == m ? 1.0f : __builtin_amdgcn_exp2f((st.x - m) * kLog2e);
+        st = float2{m, __builtin_fmaf(st.y, f, s)};
+      }
+      // (the lane halves hold offsets with bit 2 clear and set)
+      if (want >= 0 && (want & 4) == 0) a.xt[k] = xt;
+      const float2 other{__shfl_xor(st.x, 32, kWave), __shfl_xor(st.y, 32, kWave)};
+      st = merge_ms(st, other);
+      if (lane < 32 && k < n_listed) a.partial[(int64_t)(vt * 2 + wv) * a.ldn + k] = st;
+#pragma unroll
+      for (int y = 0; y < kB - 1; ++y)
+#pragma unroll
+        for (int x = 0; x < kB; ++x) loop.acc[x][y] = loop.acc[x][y + 1];
+    }
+    vt = vt2;
+    tt = tt2;
   }
+  wait_vm0();  // the loads past the last tile write their zeros
 }
 
 // The listed rows' logprob and lse from their partial states: 16 rows per
@@ -340,44 +357,48 @@ __global__ __launch_bounds__(1024) void mean_kernel(const Meta* __restrict__ met
 // ------------------------------------------------------------ backward
 
 // 32 rows x 128 columns of 16-bit values, held as lane = row and 4 columns in
-// a row per (x, j) by `value(x, j, e)`, written to `out` (row stride ld) as
-// whole 256-byte runs: through 8 KB of LDS of the wave's own, whose 16-byte
-// chunks are XOR-swizzled by the row.  `rows` and `cols` bound what is
-// written; vec: 16-byte stores (else 2-byte ones).
+// a row per (x, j) by `value(x, j, e)`, written to `out` (row stride ld) in
+// whole 128-byte lines: 64 columns at a time through 4 KB of LDS of the wave's
+// own, whose 16-byte chunks are XOR-swizzled by the row.  `rows` and `cols`
+// bound what is written; vec: 16-byte stores (else 2-byte ones).
+constexpr int kStoreLds = 256;  // chunks per wave
 template <typename Value>
 __device__ __forceinline__ void store_block(uint4* mine, int lane, uint16_t* out, int64_t ld,
                                             int64_t rows, int64_t cols, bool vec, Value value) {
   const int row = lane & 31;
   uint2* half = reinterpret_cast<uint2*>(mine);
 #pragma unroll
-  for (int x = 0; x < kB; ++x)
+  for (int h = 0; h < 2; ++h) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      uint16_t e[4];
-      value(x, j, e);
-      // columns 32 x + 8 j + 4 (lane / 32): chunk 4 x + j, its half lane / 32
-      half[(row * 16 + ((4 * x + j) ^ (row & 15))) * 2 + (lane >> 5)] =
-          uint2{(uint32_t)e[0] | (uint32_t)e[1] << 16, (uint32_t)e[2] | (uint32_t)e[3] << 16};
-    }
-  wave_lds_sync();
-  const int c = lane & 15;
+    for (int x = 0; x < kB / 2; ++x)
 #pragma unroll
-  for (int q = 0; q < 8; ++q) {
-    const int r = q * 4 + (lane >> 4);
-    const uint4 v = mine[r * 16 + (c ^ (r & 15))];
-    if (r < rows && c * 8 < cols) {
-      uint16_t* to = out + r * ld + c * 8;
-      if (vec) {
-        *reinterpret_cast<uint4*>(to) = v;
-      } else {
-        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+      for (int j = 0; j < 4; ++j) {
+        uint16_t e[4];
+        value(h * (kB / 2) + x, j, e);
+        // columns 32 x + 8 j + 4 (lane / 32): chunk 4 x + j, its half lane / 32
+        half[(row * 8 + ((4 * x + j) ^ ((row >> 1) & 7))) * 2 + (lane >> 5)] =
+            uint2{(uint32_t)e[0] | (uint32_t)e[1] << 16, (uint32_t)e[2] | (uint32_t)e[3] << 16};
+      }
+    wave_lds_sync();
+    const int c = lane & 7, col = h * 64 + c * 8;
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (c * 8 + i < cols) to[i] = (uint16_t)(w[i >> 1] >> (16 * (i & 1)));
+    for (int q = 0; q < 4; ++q) {
+      const int r = q * 8 + (lane >> 3);
+      const uint4 v = mine[r * 8 + (c ^ ((r >> 1) & 7))];
+      if (r < rows && col < cols) {
+        uint16_t* to = out + r * ld + col;
+        if (vec) {
+          *reinterpret_cast<uint4*>(to) = v;
+        } else {
+          const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (col + i < cols) to[i] = (uint16_t)(w[i >> 1] >> (16 * (i & 1)));
+        }
       }
     }
+    wave_lds_sync();
   }
-  wave_lds_sync();
 }
 
 struct GradArgs {
@@ -391,60 +412,75 @@ struct GradArgs {
 };
 
 // The piece's D: tokens x vocabulary, lane l of a block holding vocabulary row
-// l & 31 and 16 tokens, whose lse, g and targets are in LDS.
+// l & 31 and 16 tokens, whose lse, g and targets are in LDS (twice: a wave may
+// be a tile ahead of another).
 template <typename E>
 __global__ __launch_bounds__(kThreads, 1) void grad_logits_kernel(GradArgs a) {
   __shared__ __attribute__((aligned(16))) uint4 sA0[kStage], sA1[kStage], sB0[kStage], sB1[kStage];
-  __shared__ __attribute__((aligned(16))) float s_lse[kTile], s_g[kTile];
-  __shared__ __attribute__((aligned(16))) int s_t[kTile];
+  __shared__ __attribute__((aligned(16))) uint4 s_out[kWaves * kStoreLds];
+  __shared__ __attribute__((aligned(16))) float s_lse[2][kTile], s_g[2][kTile];
+  __shared__ __attribute__((aligned(16))) int s_t[2][kTile];
   const int n_listed = a.meta->n;
-  int tt, vt, share;
-  if (!tile_of(blockIdx.x, a.tm, (n_listed + kTile - 1) / kTile, 1, a.band, vt, tt, share)) return;
+  Tiles at(blockIdx.x, a.tm, (n_listed + kTile - 1) / kTile, 1, a.band);
+  if (!at.more()) return;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wt = wave >> 1, wv = wave & 1;
-  {
-    const int64_t k = (int64_t)tt * kTile + threadIdx.x;
-    const bool in = k < n_listed;
-    // a row past the last: exp(x - inf) = 0, times 0
-    s_lse[threadIdx.x] = in ? a.rows.lse[k] : kPosInf;
-    s_g[threadIdx.x] = in ? a.rows.g[k] : 0.0f;
-    s_t[threadIdx.x] = in ? (int)(a.rows.target[k] - a.v_first) : -1;
-  }
-  f32x16 acc[kB][kB];
-#pragma unroll
-  for (int x = 0; x < kB; ++x)
-#pragma unroll
-    for (int y = 0; y < kB; ++y) acc[x][y] = f32x16{};
   Operand h = a.h;
   h.outer = n_listed;
-  Source<kAlongK> sa(h, (int64_t)tt * kTile, 0, a.K, wave, lane);
-  Source<kAlongK> sb(a.w, (int64_t)vt * kTile, 0, a.K, wave, lane);
-  accumulate<E>(sa, sb, a.K, sA0, sA1, sB0, sB1, wave, lane, acc);
-
+  TileLoop<E, kAlongK, kAlongK> loop(h.ld, a.w.ld, sA0, sA1, sB0, sB1, wave, lane);
+  int vt, tt, share;
+  at.place(vt, tt, share);
+  loop.start(cursor_of<kAlongK>(h, (int64_t)tt * kTile, 0, a.K),
+             cursor_of<kAlongK>(a.w, (int64_t)vt * kTile, 0, a.K));
+  int odd = 0;
+  for (bool more = true; more; odd ^= 1) {
+    at.step();
+    more = at.more();
+    int vt2 = 0, tt2 = 0;
+    Cursor ca{nullptr, 0, 0}, cb = ca;
+    if (more) {
+      at.place(vt2, tt2, share);
+      ca = cursor_of<kAlongK>(h, (int64_t)tt2 * kTile, 0, a.K);
+      cb = cursor_of<kAlongK>(a.w, (int64_t)vt2 * kTile, 0, a.K);
+    }
+    {
+      // (the tile's barriers publish them)
+      const int64_t k = (int64_t)tt * kTile + threadIdx.x;
+      const bool in = k < n_listed;
+      // a row past the last: exp(x - inf) = 0, times 0
+      s_lse[odd][threadIdx.x] = in ? a.rows.lse[k] : kPosInf;
+      s_g[odd][threadIdx.x] = in ? a.rows.g[k] : 0.0f;
+      s_t[odd][threadIdx.x] = in ? (int)(a.rows.target[k] - a.v_first) : -1;
+    }
+    loop.tile(a.K, ca, cb);
 #pragma unroll 1
-  for (int r = 0; r < kB; ++r) {
-    const int row0 = vt * kTile + wv * 128 + r * 32, v = row0 + (lane & 31);
-    const int64_t col0 = (int64_t)tt * kTile + wt * 128;
-    store_block(sA0 + wave * 512, lane, a.d + row0 * a.ldn + col0, a.ldn, a.w.outer - row0,
-                a.ldn - col0, true, [&](int x, int j, uint16_t (&e)[4]) {
-                  const int t0 = wt * 128 + x * 32 + j * 8 + 4 * (lane >> 5);
-                  const float4 l = *reinterpret_cast<const float4*>(s_lse + t0);
-                  const float4 g = *reinterpret_cast<const float4*>(s_g + t0);
-                  const int4 t = *reinterpret_cast<const int4*>(s_t + t0);
-                  const float ls[4] = {l.x, l.y, l.z, l.w}, gs[4] = {g.x, g.y, g.z, g.w};
-                  const int ts[4] = {t.x, t.y, t.z, t.w};
+    for (int r = 0; r < kB; ++r) {
+      const int row0 = vt * kTile + wv * 128 + r * 32, v = row0 + (lane & 31);
+      const int64_t col0 = (int64_t)tt * kTile + wt * 128;
+      store_block(s_out + wave * kStoreLds, lane, a.d + row0 * a.ldn + col0, a.ldn,
+                  a.w.outer - row0, a.ldn - col0, true, [&](int x, int j, uint16_t (&e)[4]) {
+                    const int t0 = wt * 128 + x * 32 + j * 8 + 4 * (lane >> 5);
+                    const float4 l = *reinterpret_cast<const float4*>(&s_lse[odd][t0]);
+                    const float4 g = *reinterpret_cast<const float4*>(&s_g[odd][t0]);
+                    const int4 t = *reinterpret_cast<const int4*>(&s_t[odd][t0]);
+                    const float ls[4] = {l.x, l.y, l.z, l.w}, gs[4] = {g.x, g.y, g.z, g.w};
+                    const int ts[4] = {t.x, t.y, t.z, t.w};
 #pragma unroll
-                  for (int i = 0; i < 4; ++i) {
-                    const float q = acc_read(acc[x][0][4 * j + i]);
-                    const float p = __builtin_amdgcn_exp2f((q - ls[i]) * kLog2e);
-                    e[i] = E::from(gs[i] * ((ts[i] == v ? 1.0f : 0.0f) - p));
-                  }
-                });
+                    for (int i = 0; i < 4; ++i) {
+                      const float q = acc_read(loop.acc[x][0][4 * j + i]);
+                      const float p = __builtin_amdgcn_exp2f((q - ls[i]) * kLog2e);
+                      e[i] = E::from(gs[i] * ((ts[i] == v ? 1.0f : 0.0f) - p));
+                    }
+                  });
 #pragma unroll
-    for (int y = 0; y < kB - 1; ++y)
+      for (int y = 0; y < kB - 1; ++y)
 #pragma unroll
-      for (int x = 0; x < kB; ++x) acc[x][y] = acc[x][y + 1];
+        for (int x = 0; x < kB; ++x) loop.acc[x][y] = loop.acc[x][y + 1];
+    }
+    vt = vt2;
+    tt = tt2;
   }
+  wait_vm0();
 }
 
 struct HiddenArgs {
@@ -456,49 +492,84 @@ struct HiddenArgs {
   int splits, first, tn, band;
 };
 
-// dh in fp32, summed over the pieces in place: a workgroup takes one tile's
-// share of the piece's rows.
+// dh in fp32, summed over the pieces in place: a tile's share of the piece's
+// rows at a time.
 template <typename E>
 __global__ __launch_bounds__(kThreads, 1) void grad_hidden_kernel(HiddenArgs a) {
   __shared__ __attribute__((aligned(16))) uint4 sA0[kStage], sA1[kStage], sB0[kStage], sB1[kStage];
   const int n_listed = a.meta->n;
-  int tt, ct, split;
-  if (!tile_of(blockIdx.x, (n_listed + kTile - 1) / kTile, a.tn, a.splits, a.band, tt, ct, split))
-    return;
+  Tiles at(blockIdx.x, (n_listed + kTile - 1) / kTile, a.tn, a.splits, a.band);
+  if (!at.more()) return;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wt = wave >> 1, wc = wave & 1;
   const int64_t steps = (a.K + kBK - 1) / kBK, per = (steps + a.splits - 1) / a.splits * kBK;
-  const int64_t k0 = min(a.K, split * per), k1 = min(a.K, k0 + per);
-  f32x16 acc[kB][kB];
-#pragma unroll
-  for (int x = 0; x < kB; ++x)
-#pragma unroll
-    for (int y = 0; y < kB; ++y) acc[x][y] = f32x16{};
-  Source<kAcrossK> sa(a.d, (int64_t)tt * kTile, k0, k1 - k0, wave, lane);
-  Source<kAcrossK> sb(a.w, (int64_t)ct * kTile, k0, k1 - k0, wave, lane);
-  accumulate<E>(sa, sb, k1 - k0, sA0, sA1, sB0, sB1, wave, lane, acc);
+  auto k_of = [&](int split) { return min(a.K, split * per); };
+  auto cursor_a = [&](int tt, int split) {
+    return cursor_of<kAcrossK>(a.d, (int64_t)tt * kTile, k_of(split), k_of(split + 1) - k_of(split));
+  };
+  auto cursor_b = [&](int ct, int split) {
+    return cursor_of<kAcrossK>(a.w, (int64_t)ct * kTile, k_of(split), k_of(split + 1) - k_of(split));
+  };
+  TileLoop<E, kAcrossK, kAcrossK> loop(a.d.ld, a.w.ld, sA0, sA1, sB0, sB1, wave, lane);
+  int tt, ct, split;
+  at.place(tt, ct, split);
+  loop.start(cursor_a(tt, split), cursor_b(ct, split));
+  for (bool more = true; more;) {
+    at.step();
+    more = at.more();
+    int tt2 = 0, ct2 = 0, split2 = 0;
+    Cursor ca{nullptr, 0, 0}, cb = ca;
+    if (more) {
+      at.place(tt2, ct2, split2);
+      ca = cursor_a(tt2, split2);
+      cb = cursor_b(ct2, split2);
+    }
+    loop.tile(k_of(split + 1) - k_of(split), ca, cb);
 
-  float* sum = a.sum + (int64_t)split * a.N * a.width;
+    float* sum = a.sum + (int64_t)split * a.N * a.width;
 #pragma unroll 1
-  for (int r = 0; r < kB; ++r) {
-    const int64_t col = (int64_t)ct * kTile + wc * 128 + r * 32 + (lane & 31);
+    for (int r = 0; r < kB; ++r) {
+      const int64_t col = (int64_t)ct * kTile + wc * 128 + r * 32 + (lane & 31);
 #pragma unroll
-    for (int x = 0; x < kB; ++x)
+      for (int x = 0; x < kB; ++x) {
+        // values i = 4 j .. 4 j + 3 are rows k0 + 8 j and the three behind it
+        const int k0 = tt * kTile + wt * 128 + x * 32 + 4 * (lane >> 5);
+        const int rows = col < a.width ? n_listed - k0 : 0;
+        float* to = sum + k0 * a.width + col;
+        float q[16];
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const float q = acc_read(acc[x][0][i]);
-        const int64_t k =
-            (int64_t)tt * kTile + wt * 128 + x * 32 + 8 * (i >> 2) + 4 * (lane >> 5) + (i & 3);
-        if (k < n_listed && col < a.width) {
-          float* to = sum + k * a.width + col;
-          *to = a.first ? q : *to + q;
+        for (int i = 0; i < 16; ++i) q[i] = acc_read(loop.acc[x][0][i]);
+        // one running address (the compiler would hold them all), through the
+        // sixteen loads and again through the stores
+        if (!a.first) {
+          const float* from = to;
+          float old[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            old[i] = 8 * (i >> 2) + (i & 3) < rows ? *from : 0.0f;
+            from += (i & 3) == 3 ? 5 * a.width : a.width;
+            asm volatile("" : "+v"(from));
+          }
+#pragma unroll
+          for (int i = 0; i < 16; ++i) q[i] += old[i];
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          if (8 * (i >> 2) + (i & 3) < rows) *to = q[i];
+          to += (i & 3) == 3 ? 5 * a.width : a.width;
+          asm volatile("" : "+v"(to));
         }
       }
 #pragma unroll
-    for (int y = 0; y < kB - 1; ++y)
+      for (int y = 0; y < kB - 1; ++y)
 #pragma unroll
-      for (int x = 0; x < kB; ++x) acc[x][y] = acc[x][y + 1];
+        for (int x = 0; x < kB; ++x) loop.acc[x][y] = loop.acc[x][y + 1];
+    }
+    tt = tt2;
+    ct = ct2;
+    split = split2;
   }
+  wait_vm0();
 }
 
 // grad_hidden [B x S, width] from the splits' sums; positions that were not
@@ -536,34 +607,48 @@ struct WeightArgs {
 template <typename E>
 __global__ __launch_bounds__(kThreads, 1) void grad_weight_kernel(WeightArgs a) {
   __shared__ __attribute__((aligned(16))) uint4 sA0[kStage], sA1[kStage], sB0[kStage], sB1[kStage];
-  int ct, vt, share;
-  if (!tile_of(blockIdx.x, a.tm, a.tn, 1, a.band, vt, ct, share)) return;
+  __shared__ __attribute__((aligned(16))) uint4 s_out[kWaves * kStoreLds];
+  Tiles at(blockIdx.x, a.tm, a.tn, 1, a.band);
+  if (!at.more()) return;
   const int64_t K = a.meta->n;
+  const float inv = a.meta->inv;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wc = wave >> 1, wv = wave & 1;
-  f32x16 acc[kB][kB];
-#pragma unroll
-  for (int x = 0; x < kB; ++x)
-#pragma unroll
-    for (int y = 0; y < kB; ++y) acc[x][y] = f32x16{};
-  Source<kAcrossK> sa(a.h, (int64_t)ct * kTile, 0, K, wave, lane);
-  Source<kAlongK> sb(a.d, (int64_t)vt * kTile, 0, K, wave, lane);
-  accumulate<E>(sa, sb, K, sA0, sA1, sB0, sB1, wave, lane, acc);
-  const float inv = a.meta->inv;
+  TileLoop<E, kAcrossK, kAlongK> loop(a.h.ld, a.d.ld, sA0, sA1, sB0, sB1, wave, lane);
+  int vt, ct, share;
+  at.place(vt, ct, share);
+  loop.start(cursor_of<kAcrossK>(a.h, (int64_t)ct * kTile, 0, K),
+             cursor_of<kAlongK>(a.d, (int64_t)vt * kTile, 0, K));
+  for (bool more = true; more;) {
+    at.step();
+    more = at.more();
+    int vt2 = 0, ct2 = 0;
+    Cursor ca{nullptr, 0, 0}, cb = ca;
+    if (more) {
+      at.place(vt2, ct2, share);
+      ca = cursor_of<kAcrossK>(a.h, (int64_t)ct2 * kTile, 0, K);
+      cb = cursor_of<kAlongK>(a.d, (int64_t)vt2 * kTile, 0, K);
+    }
+    loop.tile(K, ca, cb);
 #pragma unroll 1
-  for (int r = 0; r < kB; ++r) {
-    const int64_t row0 = (int64_t)vt * kTile + wv * 128 + r * 32;
-    const int64_t col0 = (int64_t)ct * kTile + wc * 128;
-    store_block(sA0 + wave * 512, lane, a.out + row0 * a.ld + col0, a.ld, a.d.outer - row0,
-                a.width - col0, a.vec, [&](int x, int j, uint16_t (&e)[4]) {
+    for (int r = 0; r < kB; ++r) {
+      const int64_t row0 = (int64_t)vt * kTile + wv * 128 + r * 32;
+      const int64_t col0 = (int64_t)ct * kTile + wc * 128;
+      store_block(s_out + wave * kStoreLds, lane, a.out + row0 * a.ld + col0, a.ld,
+                  a.d.outer - row0, a.width - col0, a.vec, [&](int x, int j, uint16_t (&e)[4]) {
 #pragma unroll
-                  for (int i = 0; i < 4; ++i) e[i] = E::from(acc_read(acc[x][0][4 * j + i]) * inv);
-                });
+                    for (int i = 0; i < 4; ++i)
+                      e[i] = E::from(acc_read(loop.acc[x][0][4 * j + i]) * inv);
+                  });
 #pragma unroll
-    for (int y = 0; y < kB - 1; ++y)
+      for (int y = 0; y < kB - 1; ++y)
 #pragma unroll
-      for (int x = 0; x < kB; ++x) acc[x][y] = acc[x][y + 1];
+        for (int x = 0; x < kB; ++x) loop.acc[x][y] = loop.acc[x][y + 1];
+    }
+    vt = vt2;
+    ct = ct2;
   }
+  wait_vm0();
 }
 
 // ------------------------------------------------------------ host
@@ -612,8 +697,9 @@ int shape_of(const gtp_linear_rows* r, Shape& s, Rows& a) {
   s.n_vt = tiles(r->V);
   s.n_tt = tiles(s.N);
   s.n_ct = tiles(s.K8);
-  // a launch holds fewer than 2^32 threads
-  if (grid_of(s.n_vt, s.n_tt) >= (int64_t)1 << 24 || grid_of(s.n_ct, s.n_vt) >= (int64_t)1 << 24)
+  // the tiles are numbered in 32 bits
+  if ((int64_t)s.n_vt * s.n_tt >= (int64_t)1 << 24 || (int64_t)s.n_ct * s.n_vt >= (int64_t)1 << 24 ||
+      (int64_t)s.n_ct * s.n_tt >= (int64_t)1 << 24)
     return GTP_ERR_UNSUPPORTED;
   a = Rows{r->targets, r->V, r->S, r->T, r->target_batch_stride, r->target_row_stride,
            r->ignore_index, (int)r->B, r->targets_int64 ? 1 : 0, r->has_ignore ? 1 : 0};
@@ -641,26 +727,31 @@ Forward forward_space(const Shape& s, void* ws) {
   return f;
 }
 
-// Rows of the vocabulary per piece (a multiple of the tile), and the shares
-// that dh's products split a piece into, so that they fill the chip: rounds
-// of one workgroup per CU, each split costing a pass over its sums.
+// Rows of the vocabulary per piece, a multiple of 8 tiles where there are as
+// many (a multiple of 8 keeps the grids whole), and the shares that dh's
+// products split a piece's rows into, so that few tiles fill the chip: rounds
+// of one tile per CU at 1.7 us a K step, against three passes over the shares'
+// sums at 4.5 TB/s.
 struct Pieces {
   int64_t rows;
   int splits;
 };
-Pieces pieces_of(const Shape& s, int64_t V) {
+Pieces pieces_of(const Shape& s, int64_t V, int64_t width) {
   Pieces p;
-  int64_t most = kPieceBytes / (s.ldn * 2) / kTile * kTile;
-  most = max(most, (int64_t)kTile);
-  const int64_t n = (V + most - 1) / most;
-  p.rows = min(most, ((V + n - 1) / n + kTile - 1) / kTile * kTile);
+  const int64_t fit = max(kPieceBytes / (s.ldn * 2), (int64_t)kTile);
+  const int64_t unit = fit >= 8 * kTile ? 8 * kTile : kTile;
+  const int64_t most = fit / unit * unit, n = (V + most - 1) / most;
+  p.rows = min(most, ((V + n - 1) / n + unit - 1) / unit * unit);
   const int64_t cus = device_cus(), grid = (int64_t)s.n_tt * s.n_ct;
-  double best = 1e30;
-  p.splits = 1;
-  for (int k = 1; k <= 32 && p.rows / k >= 8 * kBK; ++k) {
-    const double cost = (double)((grid * k + cus - 1) / cus) / k + 0.01 * k;
-    if (cost < best) {
-      best = cost;
+  const int64_t steps = (min(p.rows, V) + kBK - 1) / kBK;
+  double best = 0.0;
+  p.splits = 0;
+  for (int k = 1; k <= 32 && (k == 1 || steps / k >= 8); ++k) {
+    const double rounds = (double)((grid * k + cus - 1) / cus);
+    const double us = rounds * (double)((steps + k - 1) / k) * 1.7 +
+                      (double)(k * s.N * width) * 12.0 / 4.5e6;
+    if (p.splits == 0 || us < best) {
+      best = us;
       p.splits = k;
     }
   }
@@ -716,7 +807,7 @@ void forward_launch(const gtp_linear_rows* r, const Shape& s, const Forward& f, 
   a.ldn = s.ldn;
   a.tm = s.n_vt;
   a.band = band_rows(s.n_vt, s.n_tt);
-  launch_timed(lse_kernel<E>, dim3((unsigned)grid_of(s.n_vt, s.n_tt)), dim3(kThreads), st, a);
+  launch_timed(lse_kernel<E>, dim3(grid_of(s.n_vt, s.n_tt)), dim3(kThreads), st, a);
 }
 
 // The three products of a piece of `rows` vocabulary rows from v0 on.
@@ -739,7 +830,7 @@ void grad_logits_launch(const gtp_linear_rows* r, const Shape& s, const Backward
   a.ldn = s.ldn;
   a.tm = tiles(rows);
   a.band = band_rows(a.tm, s.n_tt);
-  launch_timed(grad_logits_kernel<E>, dim3((unsigned)grid_of(a.tm, s.n_tt)), dim3(kThreads), st, a);
+  launch_timed(grad_logits_kernel<E>, dim3(grid_of(a.tm, s.n_tt)), dim3(kThreads), st, a);
 }
 
 template <typename E>
@@ -757,7 +848,7 @@ void grad_hidden_launch(const gtp_linear_rows* r, const Shape& s, const Pieces& 
   a.first = v0 == 0 ? 1 : 0;
   a.tn = s.n_ct;
   a.band = band_rows(s.n_tt, s.n_ct);
-  hipLaunchKernelGGL(grad_hidden_kernel<E>, dim3((unsigned)grid_of(s.n_tt, s.n_ct, p.splits)),
+  hipLaunchKernelGGL(grad_hidden_kernel<E>, dim3(grid_of(s.n_tt, s.n_ct, p.splits)),
                      dim3(kThreads), 0, st, a);
 }
 
@@ -775,7 +866,7 @@ void grad_weight_launch(const gtp_linear_rows* r, const Shape& s, const Backward
   a.tn = s.n_ct;
   a.band = band_rows(a.tm, a.tn);
   a.vec = (r->K & 7) == 0 && (reinterpret_cast<uintptr_t>(grad_weight) & 15u) == 0 ? 1 : 0;
-  hipLaunchKernelGGL(grad_weight_kernel<E>, dim3((unsigned)grid_of(a.tm, a.tn)), dim3(kThreads), 0,
+  hipLaunchKernelGGL(grad_weight_kernel<E>, dim3(grid_of(a.tm, a.tn)), dim3(kThreads), 0,
                      st, a);
 }
 
@@ -842,7 +933,7 @@ extern "C" size_t gtp_linear_logprob_backward_workspace_bytes(const gtp_linear_r
   lin::Shape s;
   lin::Rows a;
   if (lin::shape_of(rows, s, a) != GTP_OK || s.N == 0) return 0;
-  return lin::backward_space(rows, s, lin::pieces_of(s, rows->V), nullptr).bytes;
+  return lin::backward_space(rows, s, lin::pieces_of(s, rows->V, rows->K), nullptr).bytes;
 }
 
 extern "C" int gtp_linear_logprob_backward(const gtp_linear_rows* rows, const float* lse,
@@ -857,7 +948,7 @@ extern "C" int gtp_linear_logprob_backward(const gtp_linear_rows* rows, const fl
   // the caller writes
   if (s.N == 0) return GTP_ERR_UNSUPPORTED;
   if (!lse || !grad || !workspace) return GTP_ERR_INVALID_ARGUMENT;
-  const lin::Pieces p = lin::pieces_of(s, rows->V);
+  const lin::Pieces p = lin::pieces_of(s, rows->V, rows->K);
   const lin::Backward b = lin::backward_space(rows, s, p, workspace);
   if (workspace_bytes < b.bytes) return GTP_ERR_INVALID_ARGUMENT;
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);

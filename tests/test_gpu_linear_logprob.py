@@ -286,14 +286,14 @@ def test_large_and_infinite_logits():
 
 
 def test_pieces_of_the_vocabulary():
-    """More than one piece (a piece's gradient takes at most 512 MiB)."""
-    N, V, K = 2100, 140001, 64
+    """More than one piece (a piece's gradient takes at most 1 GiB)."""
+    N, V, K = 4200, 140001, 64
     gen = torch.Generator(device="cuda").manual_seed(3)
     w = (torch.randn(V, K, generator=gen, device="cuda") * 2 / K ** 0.5).to(BF)
     t = torch.randint(0, V, (N,), generator=gen, device="cuda")
     h = (torch.randn(N, K, generator=gen, device="cuda") + w[t].float()).to(BF)
     g = torch.randn(N, generator=gen, device="cuda")
-    assert 2 * N * V > 512 << 20
+    assert 2 * N * V > 1 << 30
     lp, lp_e, gh, gh_e, gw, gw_e = expect(h, w, t, g, BF)
     hd, wd = h.requires_grad_(), w.requires_grad_()
     got = sequence_log_probs_from_hidden(hd, wd, t)
@@ -306,7 +306,7 @@ def test_pieces_of_the_vocabulary():
 
 
 def test_memory_is_bounded_by_a_piece():
-    N, V, K = 4096, 151936, 64
+    N, V, K = 8192, 151936, 64
     h = torch.randn(N, K, device="cuda").to(BF).requires_grad_()
     w = torch.randn(V, K, device="cuda").to(BF).requires_grad_()
     t = torch.randint(0, V, (N,), device="cuda")
@@ -316,8 +316,8 @@ def test_memory_is_bounded_by_a_piece():
     lp = sequence_log_probs_from_hidden(h, w, t)
     assert torch.cuda.memory_allocated() - before < 1 << 20  # kept for the backward
     lp.sum().backward()
-    # the logits in 16 bits alone would take 1.2 GB
-    assert torch.cuda.max_memory_allocated() - before < 800 << 20
+    # the logits in 16 bits alone would take 2.5 GB
+    assert torch.cuda.max_memory_allocated() - before < 1200 << 20
 
 
 def test_other_stream():
