@@ -1,7 +1,7 @@
 // tokpath_gemm.h -- the matrix-core tile loop of the hidden-state losses (gfx950).
 //
 // One workgroup of 4 waves accumulates a 256 x 256 tile of A B^T in fp32 on
-// v_mfma_f32_32x32x16 (bf16 or fp16 operands), each wave 128 x 128 (4 x 4
+// v_mfma_f32_16x16x32 (bf16 or fp16 operands), each wave 128 x 128 (8 x 8
 // blocks, 256 accumulators per lane).  K advances 64 at a time through two
 // LDS stages of 32 KB per operand, filled straight from global memory
 // (buffer_load_dwordx4 ... lds) while the matrix cores work on the other one.
@@ -15,12 +15,29 @@
 // - kAcrossK: a row per K index, output indices contiguous.  A stage holds 64
 //   rows of 512 bytes.  ds_read_b64_tr_b16 turns 4 rows x 16 columns around on
 //   the way out of LDS: of 16 lanes, lane i receives column i's 4 values.  The
-//   16-byte chunks are XOR-swizzled by 4 (row & 3), so that the 4 rows x 64
-//   bytes that half a wave reads take all 64 banks.
+//   16-byte chunks are XOR-swizzled by 4 (row & 3) + 2 (row / 8 & 1), so that
+//   the 8 rows x 32 bytes that half a wave reads take all 64 banks.
 //
 // Nothing past an operand's rows or its K is read: the buffer resource ends
 // with the last valid row, a chunk past K gets an offset past that end, and a
 // load out of range writes zeros to LDS.
+//
+// What bounds it: the part's power.  The matrix cores run 70% of the cycles at
+// 1.7-1.9 GHz; at 8192 x 4096 x 131072 the four products reach 1350-1500
+// TFLOP/s, the library's product of the same sizes 1490-1590 on such a card.
+// What brought it there from 880-1170, each measured on one box:
+// - a stage per array (the compiler waits for all loads in flight before a
+//   transposing read of an array that one of them writes): 877 -> 1225 TFLOP/s
+//   with both operands across K;
+// - the reads and loads one by one among the MFMAs, not ahead of them: +2-6%;
+// - tile after tile without a stop (TileLoop): +1-5%, more with a short K;
+// - 16 x 16 x 32 in place of 32 x 32 x 16 (half the accumulator traffic per
+//   product, so a higher clock), fragments in halves of a side, and the
+//   accumulators held in place by inline asm (the compiler moved them between
+//   register files): +3-7%;
+// - each K step's lines brought into L2 a step ahead of its loads, every line
+//   by one of the workgroups that share it: +4-8% (a step's loads alone took
+//   1.5 us from behind L2 and 0.7 us from L2, against 1.1 us of products).
 #pragma once
 
 #include "tokpath_stream.h"
@@ -32,7 +49,8 @@ constexpr int kTile = 256;             // rows and columns of a tile
 constexpr int kBK = 64;                // K per stage
 constexpr int kWaves = 4;
 constexpr int kThreads = kWaves * 64;
-constexpr int kB = 4;                  // 32-wide blocks per wave along each side
+constexpr int kB = 8;                  // 16-wide blocks per wave along each side
+constexpr int kH = kB / 2;             // half a side
 constexpr int kQ = 8;                  // 1 KB loads per wave, operand and K step
 constexpr int kStage = kTile * kBK / 8;  // 16-byte chunks per operand stage
 constexpr int kXcds = 8;
@@ -40,36 +58,35 @@ constexpr int kMaxLd = (1 << 22) - 1;  // row strides (elements): 256 rows fit a
 constexpr int kRsrcWord3 = 0x00020000;  // raw buffer: 32-bit data format, no swizzle
 constexpr uint32_t kPast = 0x80000000u;  // an offset past every resource
 
-typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x8 __attribute__((ext_vector_type(8)));
-typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) void lds_void;
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 
 enum Layout { kAlongK, kAcrossK };
 
-// 16-bit element types: product and rounding (nearest, ties to even)
+// 16-bit element types: product and rounding (nearest, ties to even).  The
+// product is inline asm so that an accumulator stays in its registers: from
+// the builtins the compiler made 250 moves between register files per 256
+// products.  It does not see the asm's wait states: its operands come from LDS
+// (which it waits for) and never from a vector instruction, and TileLoop keeps
+// what writes or reads an accumulator away from the products.
 struct Bf16 {
-  __device__ static __forceinline__ f32x16 mfma(s16x8 a, s16x8 b, f32x16 c) {
-    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a),
-                                                   __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  __device__ static __forceinline__ void mfma(f32x4& c, s16x8 a, s16x8 b) {
+    asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
   }
   __device__ static __forceinline__ uint16_t from(float v) {
     return __builtin_bit_cast(uint16_t, (__bf16)v);
   }
-  __device__ static __forceinline__ float to(uint16_t v) { return u2f((uint32_t)v << 16); }
 };
 struct F16 {
-  __device__ static __forceinline__ f32x16 mfma(s16x8 a, s16x8 b, f32x16 c) {
-    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a),
-                                                  __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  __device__ static __forceinline__ void mfma(f32x4& c, s16x8 a, s16x8 b) {
+    asm volatile("v_mfma_f32_16x16x32_f16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
   }
   __device__ static __forceinline__ uint16_t from(float v) {
     return __builtin_bit_cast(uint16_t, (_Float16)v);
   }
-  __device__ static __forceinline__ float to(uint16_t v) { return f16_to_f32(v); }
 };
 
 // `outer` rows (kAlongK) or columns (kAcrossK) of 16-bit values; rows 16-byte
@@ -79,8 +96,11 @@ struct Operand {
   int64_t ld, outer;
 };
 
-// s_waitcnt vmcnt(0), the other counters untouched
-__device__ __forceinline__ void wait_vm0() { __builtin_amdgcn_s_waitcnt(0x0F70); }
+// s_waitcnt vmcnt(n), the other counters untouched
+template <int kLeft>
+__device__ __forceinline__ void wait_vm() {
+  __builtin_amdgcn_s_waitcnt(0x0F70 | kLeft);
+}
 
 // An accumulator read straight from its AGPR (keeps the compiler from
 // copying every accumulator to VGPRs at once before an epilogue).
@@ -115,12 +135,15 @@ __device__ __forceinline__ Cursor cursor_of(const Operand& o, int64_t first, int
 template <Layout L>
 struct Source {
   Cursor c;
-  uint32_t v0, v1;  // the lane's byte offset for even and odd q
-  int c0, c1;       // kAlongK: its first k within the step
-  uint32_t qstep;   // bytes from q to q + 2, halved
-  int64_t advance;  // bytes from step to step
+  uint32_t v[2][2];  // the lane's byte offset for (q & 1, q / 4)
+  int c0, c1;        // kAlongK: its first k within the step, for even and odd q
+  uint32_t qstep;    // bytes from q to q + 2, halved
+  uint32_t line;     // the line of a step that this lane brings into L2
+  int64_t advance;   // bytes from step to step
 
-  __device__ __forceinline__ Source(int64_t ld_elements, int wave, int lane) : c{nullptr, 0, 0} {
+  // part of parts: this workgroup's share of the lines
+  __device__ __forceinline__ Source(int64_t ld_elements, int parts, int part, int wave, int lane)
+      : c{nullptr, 0, 0} {
     const int64_t ld = ld_elements * 2;
     if constexpr (L == kAlongK) {
       advance = kBK * 2;
@@ -129,33 +152,42 @@ struct Source {
       const int row = wave * kQ * 8 + (lane >> 3);
       c0 = ((lane & 7) ^ ((lane >> 4) & 7)) * 8;
       c1 = ((lane & 7) ^ ((4 + (lane >> 4)) & 7)) * 8;
-      v0 = (uint32_t)(row * ld + c0 * 2);
-      v1 = (uint32_t)(row * ld + c1 * 2);
+      v[0][0] = v[0][1] = (uint32_t)(row * ld + c0 * 2);
+      v[1][0] = v[1][1] = (uint32_t)(row * ld + c1 * 2);
       qstep = (uint32_t)(8 * ld);
+      line = (uint32_t)((wave * 64 + lane) * ld);
     } else {
       advance = kBK * ld;
       // LDS row 2 (8w + q) + lane / 32, chunk lane & 31 of it holding chunk
-      // (lane & 31) ^ 4 (row & 3) of the row
+      // (lane & 31) ^ (4 (row & 3) + 2 (row / 8 & 1)) of the row
       const int row = wave * kQ * 2 + (lane >> 5);
-      v0 = (uint32_t)(row * ld + ((lane & 31) ^ ((lane >> 5) << 2)) * 16);
-      v1 = (uint32_t)(row * ld + ((lane & 31) ^ ((2 + (lane >> 5)) << 2)) * 16);
+#pragma unroll
+      for (int odd = 0; odd < 2; ++odd)
+#pragma unroll
+        for (int high = 0; high < 2; ++high)
+          v[odd][high] = (uint32_t)(
+              row * ld + ((lane & 31) ^ ((2 * odd + (lane >> 5)) << 2) ^ (high << 1)) * 16);
       c0 = c1 = 0;
       qstep = (uint32_t)(2 * ld);
+      line = (uint32_t)((wave * 16 + (lane >> 2)) * ld + (lane & 3) * 128);
     }
+    if ((wave * 64 + lane) * parts / 256 != part) line = kPast;
   }
 
   struct Step {
     const char* base;
     int bytes;
-    uint32_t v0, v1;
+    uint32_t v[2][2];
   };
+  __device__ __forceinline__ int bytes_left() const {
+    return (int)max((int64_t)0, min(c.left, (int64_t)kPast));
+  }
   // The next step; past the last one all its loads are out of range.
   __device__ __forceinline__ Step next() {
-    const int n = (int)max((int64_t)0, min(c.left, (int64_t)kPast));
-    Step s{c.at, n, v0, v1};
+    Step s{c.at, bytes_left(), {{v[0][0], v[0][1]}, {v[1][0], v[1][1]}}};
     if constexpr (L == kAlongK) {
-      s.v0 = c0 < c.k_left ? v0 : kPast;
-      s.v1 = c1 < c.k_left ? v1 : kPast;
+      s.v[0][0] = s.v[0][1] = c0 < c.k_left ? v[0][0] : kPast;
+      s.v[1][0] = s.v[1][1] = c1 < c.k_left ? v[1][0] : kPast;
       c.k_left -= kBK;
     }
     c.at += advance;
@@ -164,27 +196,33 @@ struct Source {
   }
   // the whole offset goes in the VGPR operand: the range check covers it
   __device__ __forceinline__ void issue(const Step& s, int q, uint4* stage, int wave) const {
-    const uint32_t v = ((q & 1) ? s.v1 : s.v0) + (uint32_t)q * qstep;
     const __amdgpu_buffer_rsrc_t r =
         __builtin_amdgcn_make_buffer_rsrc((void*)s.base, (short)0, s.bytes, kRsrcWord3);
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_void*)(stage + (wave * kQ + q) * 64), 16, v,
-                                             0, 0, 0);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_void*)(stage + (wave * kQ + q) * 64), 16,
+                                             s.v[q & 1][q >> 2] + (uint32_t)q * qstep, 0, 0, 0);
+  }
+  // The lines of the step that next() will give, into L2 (4 bytes of each go
+  // to LDS that nothing reads: a load without a register).
+  __device__ __forceinline__ void ahead(uint32_t* unread, int wave) const {
+    const __amdgpu_buffer_rsrc_t r =
+        __builtin_amdgcn_make_buffer_rsrc((void*)c.at, (short)0, bytes_left(), kRsrcWord3);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_void*)(unread + wave * 64), 4, line, 0, 0, 0);
   }
 };
 
-// Fragment x (32 outer indices from side * 128 + 32 x on) of k16 step kk:
-// lane l holds index l & 31 of it and k = 8 (l / 32) .. + 7.
+// Fragment x (16 outer indices from side * 128 + 16 x on) of k32 step kk:
+// lane l holds index l & 15 of it and k = 8 (l / 16) .. + 7.
 template <Layout L>
 __device__ __forceinline__ s16x8 fragment(const uint4* stage, int side, int x, int kk, int lane) {
   if constexpr (L == kAlongK) {
-    const int ch = (2 * kk + (lane >> 5)) ^ ((lane >> 1) & 7);
-    return __builtin_bit_cast(s16x8, stage[(side * 128 + x * 32 + (lane & 31)) * 8 + ch]);
+    const int ch = (4 * kk + (lane >> 4)) ^ ((lane >> 1) & 7);
+    return __builtin_bit_cast(s16x8, stage[(side * 128 + x * 16 + (lane & 15)) * 8 + ch]);
   } else {
-    // row 16 kk + 8 (l / 32) + 4 h + r, columns 32 (4 side + x) + 16 ((l / 16) & 1) + 4 (l & 3)
-    const int r = (lane & 15) >> 2;
-    const int at = (8 * (lane >> 5) + r) * 512 + side * 256 + ((x ^ r) * 64) +
-                   ((lane >> 4) & 1) * 32 + (lane & 3) * 8;
-    const char* p = reinterpret_cast<const char*>(stage) + at + kk * 16 * 512;
+    // row 32 kk + 8 g + 4 h + r, columns 128 side + 16 x + 4 (l & 3)
+    const int r = (lane & 15) >> 2, g = lane >> 4;
+    const int chunk = (2 * x + ((lane & 3) >> 1)) ^ (r << 2) ^ ((g & 1) << 1);
+    const int at = (8 * g + r) * 512 + side * 256 + chunk * 16 + (lane & 1) * 8;
+    const char* p = reinterpret_cast<const char*>(stage) + at + kk * 32 * 512;
     const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)p);
     const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p + 4 * 512));
     return s16x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
@@ -192,17 +230,17 @@ __device__ __forceinline__ s16x8 fragment(const uint4* stage, int side, int x, i
 }
 
 // The tile loop of a workgroup: acc[x][y] = A rows (block x) times B rows
-// (block y), lane l of a block holding B index l & 31 and the A indices
-// 8 (i / 4) + 4 (l / 32) + (i & 3) for i = 0 .. 15.
+// (block y), lane l of a block holding B index l & 15 and the A indices
+// 4 (l / 16) + i for i = 0 .. 3.
 //
 // The loop runs on from tile to tile: the last two K steps of a tile load the
 // first two of the next one, so that its operands come in while the epilogue
-// works on the accumulators (a tile started anew cost 12 us of 110 at K =
-// 4096).
+// works on the accumulators.
 //
-// The four stages are four arrays, so that the compiler sees that the loads in
-// flight write to others than it reads (from one array it waits for all loads
-// before every transposing read: 877 against 1225 TFLOP/s).
+// A k32 step is four quadrants of 16 products, walked so that each changes one
+// side's half, and the fragments of a half are read one quadrant ahead into
+// the registers that the other half's quadrant has left: 64 registers of
+// fragments in place of 128.
 template <typename E, Layout LA, Layout LB>
 struct TileLoop {
   typedef typename Source<LA>::Step StepA;
@@ -210,18 +248,18 @@ struct TileLoop {
   Source<LA> a;
   Source<LB> b;
   uint4 *sA0, *sA1, *sB0, *sB1;
+  uint32_t* unread;  // 256 words of LDS
   int wave, lane;
   StepA na;  // the step whose loads are going out
   StepB nb;
-  f32x16 acc[kB][kB];
-  // fragments of the k16 step at work and of the next one, [0, kB) of A and
-  // [kB, 2 kB) of B
-  s16x8 f[2][2 * kB];
+  f32x4 acc[kB][kB];
+  s16x8 fa[kB], fb[kB];
 
-  __device__ __forceinline__ TileLoop(int64_t lda, int64_t ldb, uint4* sA0_, uint4* sA1_,
-                                      uint4* sB0_, uint4* sB1_, int wave_, int lane_)
-      : a(lda, wave_, lane_), b(ldb, wave_, lane_), sA0(sA0_), sA1(sA1_), sB0(sB0_), sB1(sB1_),
-        wave(wave_), lane(lane_) {}
+  __device__ __forceinline__ TileLoop(const Source<LA>& a_, const Source<LB>& b_, uint4* sA0_,
+                                      uint4* sA1_, uint4* sB0_, uint4* sB1_, uint32_t* unread_,
+                                      int wave_, int lane_)
+      : a(a_), b(b_), sA0(sA0_), sA1(sA1_), sB0(sB0_), sB1(sB1_), unread(unread_), wave(wave_),
+        lane(lane_) {}
 
   __device__ __forceinline__ void issue_one(int j, uint4* sa, uint4* sb) {
     if (j & 1)
@@ -229,48 +267,62 @@ struct TileLoop {
     else
       a.issue(na, j >> 1, sa, wave);
   }
-  // read i of a k16 step, in the order in which the MFMAs want them
-  __device__ __forceinline__ void read_one(int set, int i, const uint4* sa, const uint4* sb, int kk) {
-    if (i == 0)
-      f[set][0] = fragment<LA>(sa, wave >> 1, 0, kk, lane);
-    else if (i <= kB)
-      f[set][kB + i - 1] = fragment<LB>(sb, wave & 1, i - 1, kk, lane);
-    else
-      f[set][i - kB] = fragment<LA>(sa, wave >> 1, i - kB, kk, lane);
+  __device__ __forceinline__ void read_a(int x, const uint4* sa, int kk) {
+    fa[x] = fragment<LA>(sa, wave >> 1, x, kk, lane);
   }
-  // 16 MFMAs of one k16 step from fragment set c.  Among them, one after the
-  // other so that neither queue holds the matrix cores up: the reads of the
-  // next k16 step (kk of stage (ra, rb)) and, with j0 >= 0, the loads j0 ..
-  // j0 + 7 into stage (la, lb).
-  __device__ __forceinline__ void mfma16(int c, const uint4* ra, const uint4* rb, int kk, int j0,
-                                         uint4* la, uint4* lb) {
+  __device__ __forceinline__ void read_b(int y, const uint4* sb, int kk) {
+    fb[y] = fragment<LB>(sb, wave & 1, y, kk, lane);
+  }
+  // Quadrant (kX, kY).  Among its products, one after the other so that
+  // neither queue holds the matrix cores up: the reads of A's half kReadA (of
+  // k32 step ka of sa) and B's half kReadB (kb of sb), -1 for none, and the
+  // loads kFirst .. kLast - 1 into (la, lb).
+  template <int kX, int kY, int kReadA, int kReadB, int kFirst, int kLast>
+  __device__ __forceinline__ void quadrant(const uint4* sa, int ka, const uint4* sb, int kb,
+                                           uint4* la, uint4* lb) {
+    constexpr int n = kLast - kFirst;
 #pragma unroll
-    for (int x = 0; x < kB; ++x)
+    for (int x = 0; x < kH; ++x)
 #pragma unroll
-      for (int y = 0; y < kB; ++y) {
-        const int i = x * kB + y;
-        acc[x][y] = E::mfma(f[c][x], f[c][kB + y], acc[x][y]);
-        if (i % 2 == 0) read_one(c ^ 1, i / 2, ra, rb, kk);
-        if (i % 2 == 1 && j0 >= 0) issue_one(j0 + i / 2, la, lb);
+      for (int y = 0; y < kH; ++y) {
+        const int i = x * kH + y;
+        E::mfma(acc[kX * kH + x][kY * kH + y], fa[kX * kH + x], fb[kY * kH + y]);
+        if (kReadB >= 0 && i % 4 == 0) read_b(kReadB * kH + i / 4, sb, kb);
+        if (kReadA >= 0 && i % 4 == (kReadB >= 0 ? 2 : 0)) read_a(kReadA * kH + i / 4, sa, ka);
+        if ((i + 1) * n / 16 != i * n / 16) issue_one(kFirst + i * n / 16, la, lb);
         __builtin_amdgcn_sched_barrier(0);
       }
   }
-  // A K step from stage (ca, cb), whose first k16 fragments are already in
-  // set 0.  The next step lives in (sa, sb): its loads 0-7 went out during the
-  // last k16 of the step before this one, its loads 8-15 go out during the
-  // first k16 here.  The barrier that publishes it sits before the last k16:
-  // every wave has read all of this step's fragments by then, so the loads 0-7
-  // of the step after the next into (ca, cb) go out during that last k16,
-  // while the next step's first fragments are read.
+  // A K step from stage (ca, cb), with half 0 of both sides of its first k32
+  // step read.  The next step lives in (sa, sb): its loads 0-7 went out in the
+  // last two quadrants of the step before this one, its loads 8-15 go out in
+  // the first two here.  The barrier that publishes it sits before the last
+  // two quadrants: every wave has read all of this step's fragments by then,
+  // so the loads 0-7 of the step after the next into (ca, cb) go out during
+  // those, while the next step's first fragments are read.  The wait leaves
+  // out the two loads of `ahead`, which are behind all of the next step's.
   __device__ __forceinline__ void step(uint4* ca, uint4* cb, uint4* sa, uint4* sb) {
-    mfma16(0, ca, cb, 1, kQ, sa, sb);
-    mfma16(1, ca, cb, 2, -1, sa, sb);
-    mfma16(0, ca, cb, 3, -1, sa, sb);
+    quadrant<0, 0, -1, 1, 8, 12>(ca, 0, cb, 0, sa, sb);
+    quadrant<0, 1, 1, -1, 12, 16>(ca, 0, cb, 0, sa, sb);
+    a.ahead(unread, wave);
+    b.ahead(unread, wave);
+    quadrant<1, 1, 0, -1, 0, 0>(ca, 1, cb, 0, sa, sb);
+    quadrant<1, 0, -1, 1, 0, 0>(ca, 0, cb, 1, sa, sb);
+    quadrant<0, 1, 1, 0, 0, 0>(ca, 1, cb, 1, sa, sb);
+    quadrant<0, 0, -1, -1, 0, 0>(ca, 0, cb, 0, sa, sb);
     na = a.next();
     nb = b.next();
-    wait_vm0();
-    __syncthreads();
-    mfma16(1, sa, sb, 0, 0, ca, cb);
+    publish<2>();
+    quadrant<1, 0, 0, -1, 0, 4>(sa, 0, sb, 0, ca, cb);
+    quadrant<1, 1, -1, 0, 4, 8>(sa, 0, sb, 0, ca, cb);
+  }
+  // Waits until at most kLeft of the wave's vector-memory accesses are out and
+  // its LDS reads are done, then for the other waves.
+  template <int kLeft>
+  __device__ __forceinline__ void publish() {
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(kLeft) : "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
   }
   // Ahead of the first tile.
   __device__ __forceinline__ void start(const Cursor& ca, const Cursor& cb) {
@@ -284,10 +336,12 @@ struct TileLoop {
     nb = b.next();
 #pragma unroll
     for (int j = 0; j < kQ; ++j) issue_one(j, sA1, sB1);
-    wait_vm0();
-    __syncthreads();
+    publish<0>();
 #pragma unroll
-    for (int i = 0; i < 2 * kB; ++i) read_one(0, i, sA0, sB0, 0);
+    for (int i = 0; i < kH; ++i) {
+      read_a(i, sA0, 0);
+      read_b(i, sB0, 0);
+    }
   }
   // One tile over K (at least its first two steps; past K they are zeros),
   // then on to the tile of the cursors given (empty ones behind the last).
@@ -295,7 +349,14 @@ struct TileLoop {
 #pragma unroll
     for (int x = 0; x < kB; ++x)
 #pragma unroll
-      for (int y = 0; y < kB; ++y) acc[x][y] = f32x16{};
+      for (int y = 0; y < kB; ++y) acc[x][y] = f32x4{};
+    // the zeros are written here, and 8 wait states before the first product
+#pragma unroll
+    for (int x = 0; x < kB; ++x)
+      asm volatile(""
+                   : "+a"(acc[x][0]), "+a"(acc[x][1]), "+a"(acc[x][2]), "+a"(acc[x][3]),
+                     "+a"(acc[x][4]), "+a"(acc[x][5]), "+a"(acc[x][6]), "+a"(acc[x][7]));
+    asm volatile("s_nop 7" ::: "memory");
     // an even number of steps (the stages alternate)
     int pairs = (int)((K + 2 * kBK - 1) / (2 * kBK));
     pairs = pairs < 1 ? 1 : pairs;
@@ -307,10 +368,8 @@ struct TileLoop {
       step(sA0, sB0, sA1, sB1);
       step(sA1, sB1, sA0, sB0);
     }
-    // epilogues read the accumulators by inline asm, which the compiler's
-    // hazard checks do not see: no MFMA may be scheduled past this point, and
-    // 24 wait states after the last one cover its result latency (11 for an
-    // 8-pass MFMA)
+    // 24 wait states cover the last product's latency before its accumulators
+    // are read
     __builtin_amdgcn_sched_barrier(0);
     asm volatile("s_nop 7\n\ts_nop 7\n\ts_nop 7" ::: "memory");
   }
@@ -346,6 +405,12 @@ struct Tiles {
     const uint32_t i = b / kXcds;
     at = i < run ? b % kXcds * run + i : all;
   }
+  // Of the 32 workgroups of a run, those with the same m (or n) share that
+  // operand's lines.
+  __device__ __forceinline__ int parts_m() const { return max(1u, run / h); }
+  __device__ __forceinline__ int part_m() const { return blockIdx.x / kXcds / h % parts_m(); }
+  __device__ __forceinline__ int parts_n() const { return min(h, run); }
+  __device__ __forceinline__ int part_n() const { return blockIdx.x / kXcds % parts_n(); }
   __device__ __forceinline__ bool more() const { return at < all; }
   __device__ __forceinline__ void step() { at += kXcds * run; }
   __device__ __forceinline__ void place(int& m, int& n, int& share) const {

@@ -64,7 +64,31 @@ struct Meta {
   int32_t n;     // listed rows
   int32_t bad;   // rows whose target lies outside [0, V)
   float inv;     // 1 / the power of two in D
-  int32_t pad;
+  int32_t splits;  // shares of dh's products (backward)
+};
+
+// What dh's products split their K into.  A share writes sums of its own (one
+// row of `width` floats per listed row, `most` rows in all), so that few tiles
+// fill the chip: rounds of one tile per CU at 1.5 us a K step, against three
+// passes over the sums at 4.5 TB/s.  Picked for the rows that are listed, on
+// the device.
+struct Shares {
+  int32_t column_tiles, cus;
+  int64_t steps, width, most;
+  __host__ __device__ int64_t best(int64_t rows) const {
+    const int64_t tiles = (rows + kTile - 1) / kTile * column_tiles;
+    int64_t found = 1;
+    float least = 0.0f;
+    for (int64_t k = 1; k <= 32 && (k == 1 || (steps / k >= 8 && k * rows <= most)); ++k) {
+      const float us = (float)((tiles * k + cus - 1) / cus * ((steps + k - 1) / k)) * 1.5f +
+                       (float)(k * rows * width) * (12.0f / 4.5e6f);
+      if (k == 1 || us < least) {
+        least = us;
+        found = k;
+      }
+    }
+    return found;
+  }
 };
 
 // One listed row.
@@ -87,7 +111,7 @@ __global__ __launch_bounds__(kListBlock) void list_rows_kernel(
     Rows a, Listed out, Meta* __restrict__ meta, float* __restrict__ out_lp,
     float* __restrict__ out_lse, uint32_t* __restrict__ verdict, const float* __restrict__ grad,
     const int64_t* __restrict__ mean_count, const float* __restrict__ lse_in,
-    int32_t* __restrict__ slot, int scaled) {
+    int32_t* __restrict__ slot, int scaled, Shares shares) {
   __shared__ uint32_t sums[kListBlock / kWave];
   __shared__ float tops[kListBlock / kWave];
   const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
@@ -136,7 +160,7 @@ __global__ __launch_bounds__(kListBlock) void list_rows_kernel(
     scale = ldexpf(1.0f, min(max(15 - e, -100), 100));
   }
   if (tid == 0) {
-    *meta = Meta{(int32_t)all, any_bad, 1.0f / scale, 0};
+    *meta = Meta{(int32_t)all, any_bad, 1.0f / scale, backward ? (int32_t)shares.best(all) : 0};
     if (verdict)
       __hip_atomic_store(verdict, GTP_VERDICT_GOOD | (any_bad ? GTP_VERDICT_BAD : 0u),
                          __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
@@ -224,11 +248,18 @@ __device__ __forceinline__ float2 merge_ms(float2 a, float2 b) {
   return float2{m, a.y * fa + b.y * fb};
 }
 
-// Vocabulary x tokens: lane l of a block holds token l & 31 and 16 vocabulary
+// The stages and the scratch of a tile loop.
+#define GTP_LOOP_LDS                                                                      \
+  __shared__ __attribute__((aligned(16))) uint4 sA0[kStage], sA1[kStage], sB0[kStage],    \
+      sB1[kStage];                                                                        \
+  __shared__ uint32_t s_unread[256]
+
+// Vocabulary x tokens: lane l of a block holds token l & 15 and 4 vocabulary
 // rows, so that a token's values fold in registers.
 template <typename E>
 __global__ __launch_bounds__(kThreads, 1) void lse_kernel(LseArgs a) {
-  __shared__ __attribute__((aligned(16))) uint4 sA0[kStage], sA1[kStage], sB0[kStage], sB1[kStage];
+  GTP_LOOP_LDS;
+  __shared__ int s_t[2][kTile];  // (twice: a wave may be a tile ahead of another)
   const int n_listed = a.meta->n;
   Tiles at(blockIdx.x, a.tm, (n_listed + kTile - 1) / kTile, 1, a.band);
   if (!at.more()) return;
@@ -236,12 +267,16 @@ __global__ __launch_bounds__(kThreads, 1) void lse_kernel(LseArgs a) {
   const int wv = wave >> 1, wt = wave & 1;
   Operand h = a.h;
   h.outer = n_listed;
-  TileLoop<E, kAlongK, kAlongK> loop(a.w.ld, h.ld, sA0, sA1, sB0, sB1, wave, lane);
+  TileLoop<E, kAlongK, kAlongK> loop(
+      Source<kAlongK>(a.w.ld, at.parts_m(), at.part_m(), wave, lane),
+      Source<kAlongK>(h.ld, at.parts_n(), at.part_n(), wave, lane), sA0, sA1, sB0, sB1, s_unread,
+      wave, lane);
   int vt, tt, share;
   at.place(vt, tt, share);
   loop.start(cursor_of<kAlongK>(a.w, (int64_t)vt * kTile, 0, a.K),
              cursor_of<kAlongK>(h, (int64_t)tt * kTile, 0, a.K));
-  for (bool more = true; more;) {
+  int odd = 0;
+  for (bool more = true; more; odd ^= 1) {
     at.step();
     more = at.more();
     int vt2 = 0, tt2 = 0;
@@ -251,61 +286,60 @@ __global__ __launch_bounds__(kThreads, 1) void lse_kernel(LseArgs a) {
       ca = cursor_of<kAlongK>(a.w, (int64_t)vt2 * kTile, 0, a.K);
       cb = cursor_of<kAlongK>(h, (int64_t)tt2 * kTile, 0, a.K);
     }
+    {
+      // (the tile's barriers publish them)
+      const int64_t k = (int64_t)tt * kTile + threadIdx.x;
+      s_t[odd][threadIdx.x] = k < n_listed ? a.target[k] : -1;
+    }
     loop.tile(a.K, ca, cb);
 
-    // the lane's vocabulary rows are v0 + 32 x + 8 (i / 4) + (i & 3)
-    const int64_t v0 = (int64_t)vt * kTile + wv * 128 + 4 * (lane >> 5);
+    // the lane's vocabulary rows are v0 + 16 x + i
+    const int64_t v0 = (int64_t)vt * kTile + wv * 128 + 4 * (lane >> 4);
     const int64_t left = a.w.outer - v0;
     const int lim = (int)min((int64_t)128, max(left, (int64_t)0));  // valid offsets are below
-#pragma unroll 1
-    for (int r = 0; r < kB; ++r) {  // token blocks, rotated through block 0
-      const int64_t k = (int64_t)tt * kTile + wt * 128 + r * 32 + (lane & 31);
-      const int64_t off = (k < n_listed ? (int64_t)a.target[k] : -1) - v0;
-      const int want = off >= 0 && off < lim ? (int)off : -1;
-      float2 st{kNegInf, 0.0f};
-      float xt = 0.0f;
+    // (the epilogues are unrolled: a loop over the blocks moves accumulators,
+    // and the compiler then also moves some in the products' loop, where it
+    // does not see the asm's wait states)
 #pragma unroll
-      for (int x = 0; x < kB; ++x) {
-        float v[16];
+    for (int y = 0; y < kB; ++y) {
+        const int token = wt * 128 + y * 16 + (lane & 15);
+        const int64_t k = (int64_t)tt * kTile + token;
+        const int64_t off = (int64_t)s_t[odd][token] - v0;
+        const int want = off >= 0 && off < lim ? (int)off : -1;
+        float v[4 * kB], xt = 0.0f;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int o = x * 32 + 8 * (i >> 2) + (i & 3);
-          const float q = acc_read(loop.acc[x][0][i]);
-          xt = want == o ? q : xt;
-          v[i] = o < lim ? q : kNegInf;
-        }
+        for (int x = 0; x < kB; ++x)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float q = acc_read(loop.acc[x][y][i]);
+            xt = want == x * 16 + i ? q : xt;
+            v[4 * x + i] = x * 16 + i < lim ? q : kNegInf;
+          }
         float m = v[0];
 #pragma unroll
-        for (int i = 1; i < 16; i += 2) m = max3raw(m, v[i], i + 1 < 16 ? v[i + 1] : v[i]);
-        m = fmaxf(m, st.x);
+        for (int i = 1; i < 4 * kB; i += 2) m = max3raw(m, v[i], i + 1 < 4 * kB ? v[i + 1] : v[i]);
         // (the difference first: exact near the maximum, however large that is)
         const float mb = m == kNegInf ? 0.0f : m;
         float s = 0.0f;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) s += __builtin_amdgcn_exp2f((v[i] - mb) * kLog2e);
-        const float f = st.x == m ? 1.0f : __builtin_amdgcn_exp2f((st.x - m) * kLog2e);
-        st = float2{m, __builtin_fmaf(st.y, f, s)};
-      }
-      // (the lane halves hold offsets with bit 2 clear and set)
-      if (want >= 0 && (want & 4) == 0) a.xt[k] = xt;
-      const float2 other{__shfl_xor(st.x, 32, kWave), __shfl_xor(st.y, 32, kWave)};
-      st = merge_ms(st, other);
-      if (lane < 32 && k < n_listed) a.partial[(int64_t)(vt * 2 + wv) * a.ldn + k] = st;
-#pragma unroll
-      for (int y = 0; y < kB - 1; ++y)
-#pragma unroll
-        for (int x = 0; x < kB; ++x) loop.acc[x][y] = loop.acc[x][y + 1];
+        for (int i = 0; i < 4 * kB; ++i) s += __builtin_amdgcn_exp2f((v[i] - mb) * kLog2e);
+        // (a target's bits 2 and 3 say which of the lane's four groups has it)
+        if (want >= 0 && (want & 12) == 0) a.xt[k] = xt;
+        float2 st{m, s};
+        st = merge_ms(st, float2{__shfl_xor(st.x, 16, kWave), __shfl_xor(st.y, 16, kWave)});
+        st = merge_ms(st, float2{__shfl_xor(st.x, 32, kWave), __shfl_xor(st.y, 32, kWave)});
+        if (lane < 16 && k < n_listed) a.partial[(int64_t)(vt * 2 + wv) * a.ldn + k] = st;
     }
     vt = vt2;
     tt = tt2;
   }
-  wait_vm0();  // the loads past the last tile write their zeros
+  wait_vm<0>();  // the loads past the last tile write their zeros
 }
 
 // The listed rows' logprob and lse from their partial states: 16 rows per
-// workgroup, 16 threads each merging every 16th state, then one merge in LDS.
-constexpr int kMergeTok = 16, kMergeGrp = 16;
-__global__ __launch_bounds__(256) void lse_merge_kernel(const float2* __restrict__ partial,
+// workgroup, 64 threads each merging every 64th state, then one merge in LDS.
+constexpr int kMergeTok = 16, kMergeGrp = 64;
+__global__ __launch_bounds__(kMergeTok * kMergeGrp) void lse_merge_kernel(const float2* __restrict__ partial,
                                                         int64_t ldn, int n_parts,
                                                         const Meta* __restrict__ meta,
                                                         const int32_t* __restrict__ at,
@@ -356,49 +390,44 @@ __global__ __launch_bounds__(1024) void mean_kernel(const Meta* __restrict__ met
 
 // ------------------------------------------------------------ backward
 
-// 32 rows x 128 columns of 16-bit values, held as lane = row and 4 columns in
-// a row per (x, j) by `value(x, j, e)`, written to `out` (row stride ld) in
-// whole 128-byte lines: 64 columns at a time through 4 KB of LDS of the wave's
-// own, whose 16-byte chunks are XOR-swizzled by the row.  `rows` and `cols`
-// bound what is written; vec: 16-byte stores (else 2-byte ones).
+// 16 rows x 128 columns of 16-bit values, held as lane & 15 = row and 4 columns
+// in a row per x by `value(x, e)`, written to `out` (row stride ld) in whole
+// 256-byte runs: through 4 KB of LDS of the wave's own, whose 16-byte chunks
+// are XOR-swizzled by the row.  `rows` and `cols` bound what is written; vec:
+// 16-byte stores (else 2-byte ones).
 constexpr int kStoreLds = 256;  // chunks per wave
 template <typename Value>
 __device__ __forceinline__ void store_block(uint4* mine, int lane, uint16_t* out, int64_t ld,
                                             int64_t rows, int64_t cols, bool vec, Value value) {
-  const int row = lane & 31;
+  const int row = lane & 15;
   uint2* half = reinterpret_cast<uint2*>(mine);
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
+  for (int x = 0; x < kB; ++x) {
+    uint16_t e[4];
+    value(x, e);
+    // columns 16 x + 4 (lane / 16): chunk 2 x + lane / 32, its half lane / 16 & 1
+    half[(row * 16 + ((2 * x + (lane >> 5)) ^ row)) * 2 + ((lane >> 4) & 1)] =
+        uint2{(uint32_t)e[0] | (uint32_t)e[1] << 16, (uint32_t)e[2] | (uint32_t)e[3] << 16};
+  }
+  wave_lds_sync();
+  const int c = lane & 15, col = c * 8;
 #pragma unroll
-    for (int x = 0; x < kB / 2; ++x)
+  for (int q = 0; q < 4; ++q) {
+    const int r = q * 4 + (lane >> 4);
+    const uint4 v = mine[r * 16 + (c ^ r)];
+    if (r < rows && col < cols) {
+      uint16_t* to = out + r * ld + col;
+      if (vec) {
+        *reinterpret_cast<uint4*>(to) = v;
+      } else {
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        uint16_t e[4];
-        value(h * (kB / 2) + x, j, e);
-        // columns 32 x + 8 j + 4 (lane / 32): chunk 4 x + j, its half lane / 32
-        half[(row * 8 + ((4 * x + j) ^ ((row >> 1) & 7))) * 2 + (lane >> 5)] =
-            uint2{(uint32_t)e[0] | (uint32_t)e[1] << 16, (uint32_t)e[2] | (uint32_t)e[3] << 16};
-      }
-    wave_lds_sync();
-    const int c = lane & 7, col = h * 64 + c * 8;
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const int r = q * 8 + (lane >> 3);
-      const uint4 v = mine[r * 8 + (c ^ ((r >> 1) & 7))];
-      if (r < rows && col < cols) {
-        uint16_t* to = out + r * ld + col;
-        if (vec) {
-          *reinterpret_cast<uint4*>(to) = v;
-        } else {
-          const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
-            if (col + i < cols) to[i] = (uint16_t)(w[i >> 1] >> (16 * (i & 1)));
-        }
+        for (int i = 0; i < 8; ++i)
+          if (col + i < cols) to[i] = (uint16_t)(w[i >> 1] >> (16 * (i & 1)));
       }
     }
-    wave_lds_sync();
   }
+  wave_lds_sync();
 }
 
 struct GradArgs {
@@ -412,11 +441,10 @@ struct GradArgs {
 };
 
 // The piece's D: tokens x vocabulary, lane l of a block holding vocabulary row
-// l & 31 and 16 tokens, whose lse, g and targets are in LDS (twice: a wave may
-// be a tile ahead of another).
+// l & 15 and 4 tokens, whose lse, g and targets are in LDS.
 template <typename E>
 __global__ __launch_bounds__(kThreads, 1) void grad_logits_kernel(GradArgs a) {
-  __shared__ __attribute__((aligned(16))) uint4 sA0[kStage], sA1[kStage], sB0[kStage], sB1[kStage];
+  GTP_LOOP_LDS;
   __shared__ __attribute__((aligned(16))) uint4 s_out[kWaves * kStoreLds];
   __shared__ __attribute__((aligned(16))) float s_lse[2][kTile], s_g[2][kTile];
   __shared__ __attribute__((aligned(16))) int s_t[2][kTile];
@@ -427,7 +455,10 @@ __global__ __launch_bounds__(kThreads, 1) void grad_logits_kernel(GradArgs a) {
   const int wt = wave >> 1, wv = wave & 1;
   Operand h = a.h;
   h.outer = n_listed;
-  TileLoop<E, kAlongK, kAlongK> loop(h.ld, a.w.ld, sA0, sA1, sB0, sB1, wave, lane);
+  TileLoop<E, kAlongK, kAlongK> loop(
+      Source<kAlongK>(h.ld, at.parts_n(), at.part_n(), wave, lane),
+      Source<kAlongK>(a.w.ld, at.parts_m(), at.part_m(), wave, lane), sA0, sA1, sB0, sB1, s_unread,
+      wave, lane);
   int vt, tt, share;
   at.place(vt, tt, share);
   loop.start(cursor_of<kAlongK>(h, (int64_t)tt * kTile, 0, a.K),
@@ -444,7 +475,6 @@ __global__ __launch_bounds__(kThreads, 1) void grad_logits_kernel(GradArgs a) {
       cb = cursor_of<kAlongK>(a.w, (int64_t)vt2 * kTile, 0, a.K);
     }
     {
-      // (the tile's barriers publish them)
       const int64_t k = (int64_t)tt * kTile + threadIdx.x;
       const bool in = k < n_listed;
       // a row past the last: exp(x - inf) = 0, times 0
@@ -453,56 +483,52 @@ __global__ __launch_bounds__(kThreads, 1) void grad_logits_kernel(GradArgs a) {
       s_t[odd][threadIdx.x] = in ? (int)(a.rows.target[k] - a.v_first) : -1;
     }
     loop.tile(a.K, ca, cb);
-#pragma unroll 1
-    for (int r = 0; r < kB; ++r) {
-      const int row0 = vt * kTile + wv * 128 + r * 32, v = row0 + (lane & 31);
-      const int64_t col0 = (int64_t)tt * kTile + wt * 128;
-      store_block(s_out + wave * kStoreLds, lane, a.d + row0 * a.ldn + col0, a.ldn,
-                  a.w.outer - row0, a.ldn - col0, true, [&](int x, int j, uint16_t (&e)[4]) {
-                    const int t0 = wt * 128 + x * 32 + j * 8 + 4 * (lane >> 5);
-                    const float4 l = *reinterpret_cast<const float4*>(&s_lse[odd][t0]);
-                    const float4 g = *reinterpret_cast<const float4*>(&s_g[odd][t0]);
-                    const int4 t = *reinterpret_cast<const int4*>(&s_t[odd][t0]);
-                    const float ls[4] = {l.x, l.y, l.z, l.w}, gs[4] = {g.x, g.y, g.z, g.w};
-                    const int ts[4] = {t.x, t.y, t.z, t.w};
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                      const float q = acc_read(loop.acc[x][0][4 * j + i]);
-                      const float p = __builtin_amdgcn_exp2f((q - ls[i]) * kLog2e);
-                      e[i] = E::from(gs[i] * ((ts[i] == v ? 1.0f : 0.0f) - p));
-                    }
-                  });
+    for (int y = 0; y < kB; ++y) {
+        const int row0 = vt * kTile + wv * 128 + y * 16, v = row0 + (lane & 15);
+        const int64_t col0 = (int64_t)tt * kTile + wt * 128;
+        store_block(s_out + wave * kStoreLds, lane, a.d + row0 * a.ldn + col0, a.ldn,
+                    a.w.outer - row0, a.ldn - col0, true, [&](int x, uint16_t (&e)[4]) {
+                      const int t0 = wt * 128 + x * 16 + 4 * (lane >> 4);
+                      const float4 l = *reinterpret_cast<const float4*>(&s_lse[odd][t0]);
+                      const float4 g = *reinterpret_cast<const float4*>(&s_g[odd][t0]);
+                      const int4 t = *reinterpret_cast<const int4*>(&s_t[odd][t0]);
+                      const float ls[4] = {l.x, l.y, l.z, l.w}, gs[4] = {g.x, g.y, g.z, g.w};
+                      const int ts[4] = {t.x, t.y, t.z, t.w};
 #pragma unroll
-      for (int y = 0; y < kB - 1; ++y)
-#pragma unroll
-        for (int x = 0; x < kB; ++x) loop.acc[x][y] = loop.acc[x][y + 1];
+                      for (int i = 0; i < 4; ++i) {
+                        const float q = acc_read(loop.acc[x][y][i]);
+                        const float p = __builtin_amdgcn_exp2f((q - ls[i]) * kLog2e);
+                        e[i] = E::from(gs[i] * ((ts[i] == v ? 1.0f : 0.0f) - p));
+                      }
+                    });
     }
     vt = vt2;
     tt = tt2;
   }
-  wait_vm0();
+  wait_vm<0>();
 }
 
 struct HiddenArgs {
   Operand d, w;  // D [piece rows][ldn] across K, the piece's weight rows across K
   int64_t K;     // piece rows
   const Meta* meta;
-  float* sum;    // [splits][N][width]
-  int64_t N, width;
-  int splits, first, tn, band;
+  float* sum;    // [shares][listed rows][width]
+  int64_t width;
+  int first, tn, band;
 };
 
 // dh in fp32, summed over the pieces in place: a tile's share of the piece's
 // rows at a time.
 template <typename E>
 __global__ __launch_bounds__(kThreads, 1) void grad_hidden_kernel(HiddenArgs a) {
-  __shared__ __attribute__((aligned(16))) uint4 sA0[kStage], sA1[kStage], sB0[kStage], sB1[kStage];
-  const int n_listed = a.meta->n;
-  Tiles at(blockIdx.x, (n_listed + kTile - 1) / kTile, a.tn, a.splits, a.band);
+  GTP_LOOP_LDS;
+  const int n_listed = a.meta->n, splits = a.meta->splits;
+  Tiles at(blockIdx.x, (n_listed + kTile - 1) / kTile, a.tn, splits, a.band);
   if (!at.more()) return;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wt = wave >> 1, wc = wave & 1;
-  const int64_t steps = (a.K + kBK - 1) / kBK, per = (steps + a.splits - 1) / a.splits * kBK;
+  const int64_t steps = (a.K + kBK - 1) / kBK, per = (steps + splits - 1) / splits * kBK;
   auto k_of = [&](int split) { return min(a.K, split * per); };
   auto cursor_a = [&](int tt, int split) {
     return cursor_of<kAcrossK>(a.d, (int64_t)tt * kTile, k_of(split), k_of(split + 1) - k_of(split));
@@ -510,7 +536,10 @@ __global__ __launch_bounds__(kThreads, 1) void grad_hidden_kernel(HiddenArgs a) 
   auto cursor_b = [&](int ct, int split) {
     return cursor_of<kAcrossK>(a.w, (int64_t)ct * kTile, k_of(split), k_of(split + 1) - k_of(split));
   };
-  TileLoop<E, kAcrossK, kAcrossK> loop(a.d.ld, a.w.ld, sA0, sA1, sB0, sB1, wave, lane);
+  TileLoop<E, kAcrossK, kAcrossK> loop(
+      Source<kAcrossK>(a.d.ld, at.parts_m(), at.part_m(), wave, lane),
+      Source<kAcrossK>(a.w.ld, at.parts_n(), at.part_n(), wave, lane), sA0, sA1, sB0, sB1, s_unread,
+      wave, lane);
   int tt, ct, split;
   at.place(tt, ct, split);
   loop.start(cursor_a(tt, split), cursor_b(ct, split));
@@ -526,72 +555,64 @@ __global__ __launch_bounds__(kThreads, 1) void grad_hidden_kernel(HiddenArgs a) 
     }
     loop.tile(k_of(split + 1) - k_of(split), ca, cb);
 
-    float* sum = a.sum + (int64_t)split * a.N * a.width;
-#pragma unroll 1
-    for (int r = 0; r < kB; ++r) {
-      const int64_t col = (int64_t)ct * kTile + wc * 128 + r * 32 + (lane & 31);
+    float* sum = a.sum + (int64_t)split * n_listed * a.width;
 #pragma unroll
-      for (int x = 0; x < kB; ++x) {
-        // values i = 4 j .. 4 j + 3 are rows k0 + 8 j and the three behind it
-        const int k0 = tt * kTile + wt * 128 + x * 32 + 4 * (lane >> 5);
-        const int rows = col < a.width ? n_listed - k0 : 0;
-        float* to = sum + k0 * a.width + col;
-        float q[16];
+    for (int y = 0; y < kB; ++y) {
+        const int64_t col = (int64_t)ct * kTile + wc * 128 + y * 16 + (lane & 15);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) q[i] = acc_read(loop.acc[x][0][i]);
-        // one running address (the compiler would hold them all), through the
-        // sixteen loads and again through the stores
-        if (!a.first) {
-          const float* from = to;
-          float old[16];
+        for (int x = 0; x < kB; ++x) {
+          const int k0 = tt * kTile + wt * 128 + x * 16 + 4 * (lane >> 4);
+          const int rows = col < a.width ? n_listed - k0 : 0;
+          float* to = sum + k0 * a.width + col;
+          float q[4];
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            old[i] = 8 * (i >> 2) + (i & 3) < rows ? *from : 0.0f;
-            from += (i & 3) == 3 ? 5 * a.width : a.width;
-            asm volatile("" : "+v"(from));
+          for (int i = 0; i < 4; ++i) q[i] = acc_read(loop.acc[x][y][i]);
+          if (!a.first) {
+            float old[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) old[i] = i < rows ? to[i * a.width] : 0.0f;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) q[i] += old[i];
           }
 #pragma unroll
-          for (int i = 0; i < 16; ++i) q[i] += old[i];
+          for (int i = 0; i < 4; ++i)
+            if (i < rows) to[i * a.width] = q[i];
+          // (one block's addresses at a time)
+          asm volatile("" ::: "memory");
         }
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          if (8 * (i >> 2) + (i & 3) < rows) *to = q[i];
-          to += (i & 3) == 3 ? 5 * a.width : a.width;
-          asm volatile("" : "+v"(to));
-        }
-      }
-#pragma unroll
-      for (int y = 0; y < kB - 1; ++y)
-#pragma unroll
-        for (int x = 0; x < kB; ++x) loop.acc[x][y] = loop.acc[x][y + 1];
     }
     tt = tt2;
     ct = ct2;
     split = split2;
   }
-  wait_vm0();
+  wait_vm<0>();
 }
 
-// grad_hidden [B x S, width] from the splits' sums; positions that were not
-// listed get zeros.
+// grad_hidden [B x S, width] from the shares' sums; positions that were not
+// listed get zeros.  One workgroup per position and 1024 columns.
 template <typename E>
 __global__ __launch_bounds__(256) void grad_hidden_rows_kernel(const float* __restrict__ sum,
-                                                               int64_t N, int64_t width, int splits,
+                                                               int64_t width,
                                                                const Meta* __restrict__ meta,
                                                                const int32_t* __restrict__ slot,
                                                                uint16_t* __restrict__ out) {
   const int64_t pos = blockIdx.x;
-  const int k = slot[pos];
+  const int k = slot[pos], n = meta->n, splits = meta->splits;
   const float inv = meta->inv;
   uint16_t* to = out + pos * width;
-  for (int64_t c = threadIdx.x; c < width; c += 256) {
-    float v = 0.0f;
-    if (k >= 0) {
-      for (int p = 0; p < splits; ++p) v += sum[(p * N + k) * width + c];
-      v *= inv;
-    }
-    to[c] = E::from(v);
+  const int64_t c0 = (int64_t)blockIdx.y * 1024 + threadIdx.x;
+  float v[4] = {};
+  if (k >= 0) {
+    const float* row = sum + k * width;
+#pragma unroll 2
+    for (int p = 0; p < splits; ++p, row += n * width)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (c0 + i * 256 < width) v[i] += row[c0 + i * 256];
   }
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (c0 + i * 256 < width) to[c0 + i * 256] = E::from(v[i] * inv);
 }
 
 struct WeightArgs {
@@ -606,7 +627,7 @@ struct WeightArgs {
 // tokens.
 template <typename E>
 __global__ __launch_bounds__(kThreads, 1) void grad_weight_kernel(WeightArgs a) {
-  __shared__ __attribute__((aligned(16))) uint4 sA0[kStage], sA1[kStage], sB0[kStage], sB1[kStage];
+  GTP_LOOP_LDS;
   __shared__ __attribute__((aligned(16))) uint4 s_out[kWaves * kStoreLds];
   Tiles at(blockIdx.x, a.tm, a.tn, 1, a.band);
   if (!at.more()) return;
@@ -614,7 +635,10 @@ __global__ __launch_bounds__(kThreads, 1) void grad_weight_kernel(WeightArgs a) 
   const float inv = a.meta->inv;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wc = wave >> 1, wv = wave & 1;
-  TileLoop<E, kAcrossK, kAlongK> loop(a.h.ld, a.d.ld, sA0, sA1, sB0, sB1, wave, lane);
+  TileLoop<E, kAcrossK, kAlongK> loop(
+      Source<kAcrossK>(a.h.ld, at.parts_n(), at.part_n(), wave, lane),
+      Source<kAlongK>(a.d.ld, at.parts_m(), at.part_m(), wave, lane), sA0, sA1, sB0, sB1, s_unread,
+      wave, lane);
   int vt, ct, share;
   at.place(vt, ct, share);
   loop.start(cursor_of<kAcrossK>(a.h, (int64_t)ct * kTile, 0, K),
@@ -630,25 +654,21 @@ __global__ __launch_bounds__(kThreads, 1) void grad_weight_kernel(WeightArgs a) 
       cb = cursor_of<kAlongK>(a.d, (int64_t)vt2 * kTile, 0, K);
     }
     loop.tile(K, ca, cb);
-#pragma unroll 1
-    for (int r = 0; r < kB; ++r) {
-      const int64_t row0 = (int64_t)vt * kTile + wv * 128 + r * 32;
-      const int64_t col0 = (int64_t)ct * kTile + wc * 128;
-      store_block(s_out + wave * kStoreLds, lane, a.out + row0 * a.ld + col0, a.ld,
-                  a.d.outer - row0, a.width - col0, a.vec, [&](int x, int j, uint16_t (&e)[4]) {
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                      e[i] = E::from(acc_read(loop.acc[x][0][4 * j + i]) * inv);
-                  });
+    for (int y = 0; y < kB; ++y) {
+        const int64_t row0 = (int64_t)vt * kTile + wv * 128 + y * 16;
+        const int64_t col0 = (int64_t)ct * kTile + wc * 128;
+        store_block(s_out + wave * kStoreLds, lane, a.out + row0 * a.ld + col0, a.ld,
+                    a.d.outer - row0, a.width - col0, a.vec, [&](int x, uint16_t (&e)[4]) {
 #pragma unroll
-      for (int y = 0; y < kB - 1; ++y)
-#pragma unroll
-        for (int x = 0; x < kB; ++x) loop.acc[x][y] = loop.acc[x][y + 1];
+                      for (int i = 0; i < 4; ++i)
+                        e[i] = E::from(acc_read(loop.acc[x][y][i]) * inv);
+                    });
     }
     vt = vt2;
     ct = ct2;
   }
-  wait_vm0();
+  wait_vm<0>();
 }
 
 // ------------------------------------------------------------ host
@@ -698,6 +718,7 @@ int shape_of(const gtp_linear_rows* r, Shape& s, Rows& a) {
   s.n_tt = tiles(s.N);
   s.n_ct = tiles(s.K8);
   // the tiles are numbered in 32 bits
+  // (dh's 32 times over)
   if ((int64_t)s.n_vt * s.n_tt >= (int64_t)1 << 24 || (int64_t)s.n_ct * s.n_vt >= (int64_t)1 << 24 ||
       (int64_t)s.n_ct * s.n_tt >= (int64_t)1 << 24)
     return GTP_ERR_UNSUPPORTED;
@@ -728,13 +749,11 @@ Forward forward_space(const Shape& s, void* ws) {
 }
 
 // Rows of the vocabulary per piece, a multiple of 8 tiles where there are as
-// many (a multiple of 8 keeps the grids whole), and the shares that dh's
-// products split a piece's rows into, so that few tiles fill the chip: rounds
-// of one tile per CU at 1.7 us a K step, against three passes over the shares'
-// sums at 4.5 TB/s.
+// many (which keeps the grids whole), and the room for dh's shares: what all
+// rows would take, or three times as many rows in up to 256 MiB.
 struct Pieces {
   int64_t rows;
-  int splits;
+  Shares shares;
 };
 Pieces pieces_of(const Shape& s, int64_t V, int64_t width) {
   Pieces p;
@@ -742,19 +761,9 @@ Pieces pieces_of(const Shape& s, int64_t V, int64_t width) {
   const int64_t unit = fit >= 8 * kTile ? 8 * kTile : kTile;
   const int64_t most = fit / unit * unit, n = (V + most - 1) / most;
   p.rows = min(most, ((V + n - 1) / n + unit - 1) / unit * unit);
-  const int64_t cus = device_cus(), grid = (int64_t)s.n_tt * s.n_ct;
-  const int64_t steps = (min(p.rows, V) + kBK - 1) / kBK;
-  double best = 0.0;
-  p.splits = 0;
-  for (int k = 1; k <= 32 && (k == 1 || steps / k >= 8); ++k) {
-    const double rounds = (double)((grid * k + cus - 1) / cus);
-    const double us = rounds * (double)((steps + k - 1) / k) * 1.7 +
-                      (double)(k * s.N * width) * 12.0 / 4.5e6;
-    if (p.splits == 0 || us < best) {
-      best = us;
-      p.splits = k;
-    }
-  }
+  p.shares = Shares{s.n_ct, (int32_t)device_cus(), (min(p.rows, V) + kBK - 1) / kBK, width,
+                    32 * s.N};
+  p.shares.most = max(p.shares.best(s.N) * s.N, min(3 * s.N, ((int64_t)1 << 26) / width));
   return p;
 }
 
@@ -777,7 +786,7 @@ Backward backward_space(const gtp_linear_rows* r, const Shape& s, const Pieces& 
   b.slot = c.take<int32_t>(r->B * r->S);
   b.h = c.take<uint16_t>(s.N * s.ldh);
   b.d = c.take<uint16_t>(p.rows * s.ldn);
-  b.sum = c.take<float>((size_t)p.splits * s.N * r->K);
+  b.sum = c.take<float>((size_t)p.shares.most * r->K);
   b.bytes = c.at;
   return b;
 }
@@ -834,22 +843,20 @@ void grad_logits_launch(const gtp_linear_rows* r, const Shape& s, const Backward
 }
 
 template <typename E>
-void grad_hidden_launch(const gtp_linear_rows* r, const Shape& s, const Pieces& p,
-                        const Backward& b, int64_t v0, int64_t rows, hipStream_t st) {
+void grad_hidden_launch(const gtp_linear_rows* r, const Shape& s, const Backward& b, int64_t v0,
+                        int64_t rows, hipStream_t st) {
   HiddenArgs a;
   a.d = Operand{b.d, s.ldn, s.ldn};
   a.w = piece_of(r, v0, s.K8);
   a.K = rows;
   a.meta = b.meta;
   a.sum = b.sum;
-  a.N = s.N;
   a.width = r->K;
-  a.splits = p.splits;
   a.first = v0 == 0 ? 1 : 0;
   a.tn = s.n_ct;
   a.band = band_rows(s.n_tt, s.n_ct);
-  hipLaunchKernelGGL(grad_hidden_kernel<E>, dim3(grid_of(s.n_tt, s.n_ct, p.splits)),
-                     dim3(kThreads), 0, st, a);
+  // (the shares are picked on the device: as many workgroups as there can be)
+  hipLaunchKernelGGL(grad_hidden_kernel<E>, dim3(kXcds * 32), dim3(kThreads), 0, st, a);
 }
 
 template <typename E>
@@ -876,12 +883,13 @@ void backward_launch(const gtp_linear_rows* r, const Shape& s, const Pieces& p, 
   for (int64_t v0 = 0; v0 < r->V; v0 += p.rows) {
     const int64_t rows = min(p.rows, r->V - v0);
     grad_logits_launch<E>(r, s, b, v0, rows, st);
-    if (grad_hidden) grad_hidden_launch<E>(r, s, p, b, v0, rows, st);
+    if (grad_hidden) grad_hidden_launch<E>(r, s, b, v0, rows, st);
     if (grad_weight) grad_weight_launch<E>(r, s, b, v0, rows, grad_weight, st);
   }
   if (grad_hidden)
-    hipLaunchKernelGGL(grad_hidden_rows_kernel<E>, dim3((unsigned)(r->B * r->S)), dim3(256), 0, st,
-                       b.sum, s.N, r->K, p.splits, b.meta, b.slot, grad_hidden);
+    hipLaunchKernelGGL(grad_hidden_rows_kernel<E>,
+                       dim3((unsigned)(r->B * r->S), (unsigned)((r->K + 1023) / 1024)), dim3(256), 0,
+                       st, b.sum, r->K, b.meta, b.slot, grad_hidden);
 }
 
 }  // namespace lin
@@ -912,7 +920,7 @@ extern "C" int gtp_linear_logprob_rows(const gtp_linear_rows* rows, float* out_l
   for (int i = 1; verdict && i < GTP_VERDICT_WORDS; ++i) verdict[i] = GTP_VERDICT_GOOD;
   hipLaunchKernelGGL(lin::list_rows_kernel, dim3(1), dim3(lin::kListBlock), 0, st, a,
                      lin::Listed{f.at, f.target, nullptr, nullptr}, f.meta, out_logprob, out_lse,
-                     verdict, nullptr, nullptr, nullptr, nullptr, 0);
+                     verdict, nullptr, nullptr, nullptr, nullptr, 0, lin::Shares{});
   if (s.N > 0) {
     lin::gather(rows, s, f.meta, f.at, f.h, st);
     if (rows->dtype == GTP_DTYPE_BF16)
@@ -920,8 +928,8 @@ extern "C" int gtp_linear_logprob_rows(const gtp_linear_rows* rows, float* out_l
     else
       lin::forward_launch<gemm::F16>(rows, s, f, st);
     hipLaunchKernelGGL(lin::lse_merge_kernel,
-                       dim3((unsigned)((s.N + lin::kMergeTok - 1) / lin::kMergeTok)), dim3(256), 0,
-                       st, f.partial, s.ldn, 2 * s.n_vt, f.meta, f.at, f.xt, out_logprob, out_lse);
+                       dim3((unsigned)((s.N + lin::kMergeTok - 1) / lin::kMergeTok)),
+                       dim3(lin::kMergeTok * lin::kMergeGrp), 0, st, f.partial, s.ldn, 2 * s.n_vt, f.meta, f.at, f.xt, out_logprob, out_lse);
   }
   if (mean_loss)
     hipLaunchKernelGGL(lin::mean_kernel, dim3(1), dim3(1024), 0, st, f.meta, f.at, out_logprob,
@@ -954,7 +962,7 @@ extern "C" int gtp_linear_logprob_backward(const gtp_linear_rows* rows, const fl
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   hipLaunchKernelGGL(lin::list_rows_kernel, dim3(1), dim3(lin::kListBlock), 0, st, a, b.rows,
                      b.meta, nullptr, nullptr, nullptr, grad, mean_count, lse, b.slot,
-                     rows->dtype == GTP_DTYPE_F16 ? 1 : 0);
+                     rows->dtype == GTP_DTYPE_F16 ? 1 : 0, p.shares);
   lin::gather(rows, s, b.meta, b.rows.at, b.h, st);
   uint16_t* gh = reinterpret_cast<uint16_t*>(grad_hidden);
   uint16_t* gw = reinterpret_cast<uint16_t*>(grad_weight);
