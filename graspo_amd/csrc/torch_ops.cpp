@@ -13,6 +13,8 @@
 // caller's other torch work exactly as the reference's ATen ops did.
 #include <ATen/ATen.h>
 #include <ATen/EmptyTensor.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/library.h>
 
 #include <algorithm>
@@ -927,11 +929,13 @@ at::Tensor flat_ids(const at::Tensor& ids, const at::Tensor& like, const char* w
   return ids.reshape({-1});
 }
 
-// (out [*ids.shape, H], whether an id lies outside [0, V): its row is NaN).
-// check: waits for a look at the ids, which runs ahead of the rows (not in a
-// captured call).
-std::tuple<at::Tensor, bool> embedding(const at::Tensor& ids_, const at::Tensor& weight,
-                                       double scale, bool check, int64_t stream) {
+// (out [*ids.shape, H], whether an id lies outside [0, V): its row is NaN, the
+// tokens' order).  check: waits for a look at the ids, which runs ahead of the
+// rows (not in a captured call).  ordered: sorts the tokens but padding_idx's
+// beside the rows, for the backward; else the order is empty.
+std::tuple<at::Tensor, bool, at::Tensor> embedding(const at::Tensor& ids_, const at::Tensor& weight,
+                                                   double scale, bool check, bool ordered,
+                                                   int64_t padding_idx, int64_t stream) {
   TORCH_CHECK(weight.is_cuda() && weight.dim() == 2 && weight.size(0) > 0 && weight.size(1) > 0,
               "graspo_tokpath.embedding: weight must be a non-empty [V, H] GPU tensor");
   const at::Tensor ids = flat_ids(ids_, weight, "embedding");
@@ -953,27 +957,45 @@ std::tuple<at::Tensor, bool> embedding(const at::Tensor& ids_, const at::Tensor&
     if (rc == GTP_ERR_LAUNCH) verdict_wait(words, &found, st);
     check_rc(rc, "gtp_targets_verdict");
   }
-  const int rc = gtp_embedding_rows(ids.data_ptr(), ids64, N, ids_stride, w.data_ptr(),
-                                    dtype_code(w), V, H, V > 1 ? w.stride(0) : H, (float)scale,
-                                    out.data_ptr(), st);
+  const int64_t ld = V > 1 ? w.stride(0) : H;
+  const size_t order_bytes = ordered ? gtp_embedding_order_bytes(N, V) : 0;
+  at::Tensor order = at::empty({(int64_t)order_bytes / 4}, weight.options().dtype(at::kInt));
+  const int rc =
+      ordered ? gtp_embedding_rows_ordered(ids.data_ptr(), ids64, N, ids_stride, w.data_ptr(),
+                                           dtype_code(w), V, H, ld, (float)scale, out.data_ptr(),
+                                           padding_idx, order.data_ptr(), order_bytes, st)
+              : gtp_embedding_rows(ids.data_ptr(), ids64, N, ids_stride, w.data_ptr(),
+                                   dtype_code(w), V, H, ld, (float)scale, out.data_ptr(), st);
   int bad = 0, wait_rc = GTP_OK;
   if (words.defined()) wait_rc = verdict_wait(words, &bad, st);
   check_rc(rc, "gtp_embedding_rows");
   check_rc(wait_rc, "gtp_verdict_wait");
-  return {out, (bad & 1) != 0};
+  return {out, (bad & 1) != 0, order};
 }
 
 // The gradient of the table from that of embedding()'s rows; out: added to.
-at::Tensor embedding_backward(const at::Tensor& ids_, const at::Tensor& grad_, int64_t V,
-                              double scale, int64_t padding_idx,
-                              const c10::optional<at::Tensor>& out, int64_t stream) {
+// order: embedding()'s, in the ids' place.
+at::Tensor embedding_backward(const c10::optional<at::Tensor>& ids_, const at::Tensor& grad_,
+                              int64_t V, double scale, int64_t padding_idx,
+                              const c10::optional<at::Tensor>& out,
+                              const c10::optional<at::Tensor>& order, int64_t stream) {
   TORCH_CHECK(grad_.is_cuda() && grad_.dim() >= 1 && grad_.size(-1) > 0 && V > 0,
               "graspo_tokpath.embedding_backward: grad must be a [..., H] GPU tensor and V > 0");
   const int64_t H = grad_.size(-1);
-  const at::Tensor ids = flat_ids(ids_, grad_, "embedding_backward");
-  const int64_t N = ids.size(0);
-  TORCH_CHECK(grad_.numel() == N * H,
-              "graspo_tokpath.embedding_backward: grad must be [*ids.shape, H]");
+  const int64_t N = grad_.numel() / H;
+  at::Tensor ids;
+  if (order.has_value()) {
+    check_same_device(grad_, *order, "order");
+    TORCH_CHECK(order->scalar_type() == at::kInt && order->is_contiguous() &&
+                    (size_t)order->numel() * 4 == gtp_embedding_order_bytes(N, V),
+                "graspo_tokpath.embedding_backward: the order is not one of ", N, " tokens of ", V,
+                " rows");
+  } else {
+    TORCH_CHECK(ids_.has_value(), "graspo_tokpath.embedding_backward: neither ids nor an order");
+    ids = flat_ids(*ids_, grad_, "embedding_backward");
+    TORCH_CHECK(ids.size(0) == N,
+                "graspo_tokpath.embedding_backward: grad must be [*ids.shape, H]");
+  }
   const c10::DeviceGuard guard(grad_.device());
   at::Tensor grad = grad_.reshape({N, H});
   if (H > 1 && grad.stride(1) != 1) grad = grad.contiguous();
@@ -989,16 +1011,68 @@ at::Tensor embedding_backward(const at::Tensor& ids_, const at::Tensor& grad_, i
     to = at::empty({V, H}, grad.options());
   }
   const int dt = dtype_code(grad);
-  const size_t ws_bytes = gtp_embedding_backward_workspace_bytes(dt, N, H);
+  const size_t ws_bytes = order.has_value()
+                              ? gtp_embedding_backward_ordered_workspace_bytes(dt, N, H)
+                              : gtp_embedding_backward_workspace_bytes(dt, N, V, H);
   at::Tensor ws = at::empty({(int64_t)std::max<size_t>(ws_bytes, 256)},
                             grad.options().dtype(at::kByte));
-  check_rc(gtp_embedding_backward(ids.data_ptr(), ids.scalar_type() == at::kLong, N,
-                                  N > 1 ? ids.stride(0) : 1, grad.data_ptr(), dt,
-                                  N > 1 ? grad.stride(0) : H, V, H, (float)scale, padding_idx,
-                                  out.has_value(), to.data_ptr(), ws.data_ptr(),
-                                  (size_t)ws.numel(), reinterpret_cast<void*>(stream)),
-           "gtp_embedding_backward");
+  const int64_t ld = N > 1 ? grad.stride(0) : H;
+  void* st = reinterpret_cast<void*>(stream);
+  const int rc =
+      order.has_value()
+          ? gtp_embedding_backward_ordered(order->data_ptr(), (size_t)order->numel() * 4, N,
+                                           grad.data_ptr(), dt, ld, V, H, (float)scale,
+                                           out.has_value(), to.data_ptr(), ws.data_ptr(),
+                                           (size_t)ws.numel(), st)
+          : gtp_embedding_backward(ids.data_ptr(), ids.scalar_type() == at::kLong, N,
+                                   N > 1 ? ids.stride(0) : 1, grad.data_ptr(), dt, ld, V, H,
+                                   (float)scale, padding_idx, out.has_value(), to.data_ptr(),
+                                   ws.data_ptr(), (size_t)ws.numel(), st);
+  check_rc(rc, "gtp_embedding_backward");
   return to;
+}
+
+// embedding() with its gradient.  A C++ node: for few tokens Python's part of
+// a forward and a backward is most of what they take (999 tokens of a 206 MB
+// table: 102 us with a Python function, 66 so).
+struct TokenEmbedding : torch::autograd::Function<TokenEmbedding> {
+  static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& ids,
+                            const at::Tensor& weight, double scale, int64_t padding_idx, bool check,
+                            int64_t stream) {
+    auto [out, bad, order] = embedding(ids, weight, scale, check, true, padding_idx, stream);
+    TORCH_CHECK(!bad, "token_embedding: an id is outside [0, vocab_size)");
+    // the tokens' order is kept, not the ids: a loader may refill its batch
+    // before the backward
+    ctx->save_for_backward({order});
+    ctx->saved_data["vocab"] = weight.size(0);
+    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["stream"] = stream;
+    return out;
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                 torch::autograd::variable_list grads) {
+    const at::Tensor& grad = grads[0];
+    // (the engine runs a node on its forward's stream)
+    at::Tensor out = embedding_backward(
+        c10::nullopt, grad.detach(), ctx->saved_data["vocab"].toInt(),
+        ctx->saved_data["scale"].toDouble(), -1, c10::nullopt, ctx->get_saved_variables()[0],
+        ctx->saved_data["stream"].toInt());
+    if (at::GradMode::is_enabled() && grad.requires_grad()) {
+      out.requires_grad_();
+      out = (*std::make_shared<torch::autograd::DelayedError>(
+          "token_embedding is differentiable once only", 1))({out})[0];
+    }
+    return {at::Tensor(), out, at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()};
+  }
+};
+
+at::Tensor token_embedding(const at::Tensor& ids, const at::Tensor& weight, double scale,
+                           int64_t padding_idx, bool check, int64_t stream) {
+  if (at::GradMode::is_enabled() && weight.requires_grad())
+    return TokenEmbedding::apply(ids, weight, scale, padding_idx, check, stream);
+  auto [out, bad, order] = embedding(ids, weight, scale, check, false, padding_idx, stream);
+  TORCH_CHECK(!bad, "token_embedding: an id is outside [0, vocab_size)");
+  return out;
 }
 
 // ------------------------------------------------- gradient norm and clipping
@@ -1105,12 +1179,16 @@ at::Tensor clip_grad_norm_(at::TensorList tensors, double max_norm, double norm_
 }
 
 TORCH_LIBRARY(graspo_tokpath, m) {
-  m.def("embedding(Tensor ids, Tensor weight, float scale, bool check, int stream) -> (Tensor, bool)",
+  m.def("embedding(Tensor ids, Tensor weight, float scale, bool check, bool ordered, int padding_idx, "
+        "int stream) -> (Tensor, bool, Tensor)",
         &embedding);
   m.def(
-      "embedding_backward(Tensor ids, Tensor grad, int vocab, float scale, int padding_idx, "
-      "Tensor(a!)? out, int stream) -> Tensor",
+      "embedding_backward(Tensor? ids, Tensor grad, int vocab, float scale, int padding_idx, "
+      "Tensor(a!)? out, Tensor? order, int stream) -> Tensor",
       &embedding_backward);
+  m.def("token_embedding(Tensor ids, Tensor weight, float scale, int padding_idx, bool check, "
+        "int stream) -> Tensor",
+        &token_embedding);
   m.def("grad_norm(Tensor[] tensors, float norm_type, int stream) -> Tensor", &grad_norm);
   m.def("clip_grads_(Tensor(a!)[] tensors, Tensor norm, float max_norm, int stream) -> ()",
         &clip_grads_);

@@ -13,24 +13,6 @@ import torch
 from . import ops
 
 
-class _TokenEmbedding(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, ids, weight, scale, padding_idx, check):
-        out, bad = ops.embedding(ids, weight, scale=scale, check=check)
-        if bad:
-            raise RuntimeError("token_embedding: an id is outside [0, vocab_size)")
-        # a copy of the ids: a loader may refill its batch before the backward
-        ctx.save_for_backward(ids.clone() if ctx.needs_input_grad[1] else None)
-        ctx.vocab, ctx.scale, ctx.padding_idx = weight.shape[0], scale, padding_idx
-        return out
-
-    @staticmethod
-    def backward(ctx, grad):
-        (ids,) = ctx.saved_tensors
-        return None, ops.embedding_backward(ids, grad, ctx.vocab, scale=ctx.scale,
-                                            padding_idx=ctx.padding_idx), None, None, None
-
-
 def token_embedding(
     input_ids: torch.Tensor,
     weight: torch.Tensor,
@@ -59,4 +41,5 @@ def token_embedding(
             raise ValueError(f"token_embedding: padding_idx {padding_idx} outside the table's {V} "
                              f"rows")
         padding_idx %= V
-    return _TokenEmbedding.apply(input_ids, weight, float(scale), padding_idx, bool(check_status))
+    return ops.token_embedding(input_ids, weight, scale=scale, padding_idx=padding_idx,
+                               check=bool(check_status))

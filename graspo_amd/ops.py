@@ -40,7 +40,8 @@ def _stream(t: torch.Tensor) -> int:
     if t.device.type != "cuda":
         raise RuntimeError(
             f"graspo_tokpath: tensors must be on a GPU (got {t.device}); there is no CPU path")
-    return torch.cuda.current_stream(t.device).cuda_stream
+    # (the handle alone: a Stream object for it takes 2 us)
+    return torch._C._cuda_getCurrentRawStream(t.device.index)
 
 
 def _as_rows(logits: torch.Tensor) -> torch.Tensor:
@@ -352,29 +353,58 @@ def linear_logprob_backward(hidden: torch.Tensor, weight: torch.Tensor, targets:
     return (gh if need_hidden else None), (gw if need_weight else None)
 
 
+def _padding(name: str, padding_idx: int | None, vocab: int) -> int:
+    if padding_idx is not None and not 0 <= padding_idx < vocab:
+        raise ValueError(f"{name}: padding_idx {padding_idx} outside [0, {vocab})")
+    return -1 if padding_idx is None else int(padding_idx)
+
+
 def embedding(ids: torch.Tensor, weight: torch.Tensor, *, scale: float = 1.0, check: bool = True):
     """(``weight[ids] * scale``, whether an id lies outside [0, V)): rows of
     the fp32, bf16 or fp16 table ``weight`` [V, H], the product in fp32 and
     rounded once.  A bad id's row is NaN.  ``check`` waits for a look at the
     ids, which runs ahead of the rows; without it, and in a graph capture,
     nothing waits and the answer is no."""
-    return load().embedding(_targets(ids), weight, float(scale), check, _stream(weight))
+    out, bad, _ = load().embedding(_targets(ids), weight, float(scale), check, False, -1,
+                                   _stream(weight))
+    return out, bad
 
 
-def embedding_backward(ids: torch.Tensor, grad: torch.Tensor, vocab: int, *, scale: float = 1.0,
-                       padding_idx: int | None = None,
-                       out: torch.Tensor | None = None) -> torch.Tensor:
+def embedding_ordered(ids: torch.Tensor, weight: torch.Tensor, *, scale: float = 1.0,
+                      padding_idx: int | None = None, check: bool = True):
+    """:func:`embedding`'s two and the tokens' order by id, which is made in
+    the same launch beside the rows: an int32 tensor for
+    :func:`embedding_backward` to take in the ids' place.  Tokens of
+    ``padding_idx``, and bad ones, are not in it."""
+    pad = _padding("embedding_ordered", padding_idx, weight.shape[0])
+    return load().embedding(_targets(ids), weight, float(scale), check, True, pad,
+                            _stream(weight))
+
+
+def token_embedding(ids: torch.Tensor, weight: torch.Tensor, *, scale: float = 1.0,
+                    padding_idx: int | None = None, check: bool = True) -> torch.Tensor:
+    """:func:`embedding`'s rows, differentiable (once) in ``weight``; a bad id
+    that ``check`` finds raises ``RuntimeError``."""
+    pad = _padding("token_embedding", padding_idx, weight.shape[0])
+    return load().token_embedding(_targets(ids), weight, float(scale), pad, check,
+                                  _stream(weight))
+
+
+def embedding_backward(ids: torch.Tensor | None, grad: torch.Tensor, vocab: int, *,
+                       scale: float = 1.0, padding_idx: int | None = None,
+                       out: torch.Tensor | None = None,
+                       order: torch.Tensor | None = None) -> torch.Tensor:
     """The gradient [V, H] of :func:`embedding`'s table from ``grad``
     [*ids.shape, H], in its dtype: the tokens sorted by id, each row's sum in
     fp32 in an order that the ids fix, rounded once.  Tokens of
     ``padding_idx``, and bad ones, are left out.  With ``out`` (contiguous
     [V, H] of that dtype, as a tied lm_head's gradient is) the sums are added
-    to it in place, and rows without a token are not touched."""
-    if padding_idx is not None and not 0 <= padding_idx < vocab:
-        raise ValueError(f"embedding_backward: padding_idx {padding_idx} outside [0, {vocab})")
-    return load().embedding_backward(_targets(ids), grad, int(vocab), float(scale),
-                                     -1 if padding_idx is None else int(padding_idx), out,
-                                     _stream(grad))
+    to it in place, and rows without a token are not touched.  ``order``:
+    what :func:`embedding_ordered` made of the ids and the padding; ``ids``
+    may then be None."""
+    pad = _padding("embedding_backward", padding_idx, vocab)
+    return load().embedding_backward(ids if ids is None else _targets(ids), grad, int(vocab),
+                                     float(scale), pad, out, order, _stream(grad))
 
 
 def grad_norm(tensors, norm_type: float = 2.0) -> torch.Tensor:

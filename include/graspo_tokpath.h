@@ -674,17 +674,34 @@ int gtp_embedding_rows(const void* ids, int ids_int64, int64_t N, int64_t ids_st
  * [0, V) are left out.
  *
  *   grad         [N, H] of `dtype`, rows grad_stride apart
- *   grad_weight  [V, H] contiguous of `dtype`, 16-byte aligned; accumulate:
- *                added to what the rows hold, and rows without a token are
- *                neither read nor written (any alignment)
+ *   grad_weight  [V, H] contiguous of `dtype`; accumulate: added to what the
+ *                rows hold, and rows without a token are neither read nor
+ *                written
  * The workspace (gtp_embedding_backward_workspace_bytes) carries nothing
  * between calls.
  */
-size_t gtp_embedding_backward_workspace_bytes(int dtype, int64_t N, int64_t H);
+size_t gtp_embedding_backward_workspace_bytes(int dtype, int64_t N, int64_t V, int64_t H);
 int gtp_embedding_backward(const void* ids, int ids_int64, int64_t N, int64_t ids_stride,
                            const void* grad, int dtype, int64_t grad_stride, int64_t V, int64_t H,
                            float scale, int64_t padding_idx, int accumulate, void* grad_weight,
                            void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * The same pair for a training step: the lookup also sorts the tokens, beside
+ * its rows, into `order` (gtp_embedding_order_bytes, 4-byte aligned), which
+ * the backward takes in the ids' place, any number of times.  padding_idx is
+ * the lookup's to give here.
+ */
+size_t gtp_embedding_order_bytes(int64_t N, int64_t V);
+int gtp_embedding_rows_ordered(const void* ids, int ids_int64, int64_t N, int64_t ids_stride,
+                               const void* weight, int dtype, int64_t V, int64_t H,
+                               int64_t weight_stride, float scale, void* out, int64_t padding_idx,
+                               void* order, size_t order_bytes, void* stream);
+size_t gtp_embedding_backward_ordered_workspace_bytes(int dtype, int64_t N, int64_t H);
+int gtp_embedding_backward_ordered(const void* order, size_t order_bytes, int64_t N,
+                                   const void* grad, int dtype, int64_t grad_stride, int64_t V,
+                                   int64_t H, float scale, int accumulate, void* grad_weight,
+                                   void* workspace, size_t workspace_bytes, void* stream);
 
 /*
  * gtp_grad_norm -- the norm of all elements of `count` tensors (tensors,

@@ -65,7 +65,7 @@ def _embedding_lib():
     L.gtp_embedding_rows.argtypes = [VP, I32, I64, I64, VP, I32, I64, I64, I64, ctypes.c_float, VP, VP]
     L.gtp_embedding_backward.argtypes = [VP, I32, I64, I64, VP, I32, I64, I64, I64, ctypes.c_float,
                                          I64, I32, VP, VP, SZ, VP]
-    L.gtp_embedding_backward_workspace_bytes.argtypes = [I32, I64, I64]
+    L.gtp_embedding_backward_workspace_bytes.argtypes = [I32, I64, I64, I64]
     L.gtp_embedding_backward_workspace_bytes.restype = SZ
     return L
 
@@ -88,15 +88,41 @@ def test_embedding_entry_points(change, code):
 
 def test_embedding_buffers():
     L = _embedding_lib()
-    need = L.gtp_embedding_backward_workspace_bytes(1, 8, 64)
+    need = L.gtp_embedding_backward_workspace_bytes(1, 8, 100, 64)
     assert need > 0
     call = lambda out, ws, n, add=0: L.gtp_embedding_backward(  # noqa: E731
         4096, 1, 8, 1, 4096, 1, 64, 100, 64, 1.0, -1, add, out, ws, n, None)
     assert call(4096, 4096, need - 1) == INVALID
     assert call(4096, None, need) == INVALID
     assert call(4097, 4096, need) == INVALID      # no whole element
-    assert call(4098, 4096, need) == UNSUPPORTED  # zeros go in 16-byte vectors
+    assert call(4096, 4097, need) == INVALID
     assert L.gtp_embedding_rows(4096, 1, 8, 1, 4096, 1, 100, 64, 63, 1.0, 4096, None) == INVALID
+
+
+def test_ordered_entry_points():
+    L = _embedding_lib()
+    L.gtp_embedding_order_bytes.argtypes = [I64, I64]
+    L.gtp_embedding_order_bytes.restype = SZ
+    L.gtp_embedding_backward_ordered_workspace_bytes.argtypes = [I32, I64, I64]
+    L.gtp_embedding_backward_ordered_workspace_bytes.restype = SZ
+    L.gtp_embedding_rows_ordered.argtypes = [VP, I32, I64, I64, VP, I32, I64, I64, I64,
+                                             ctypes.c_float, VP, I64, VP, SZ, VP]
+    L.gtp_embedding_backward_ordered.argtypes = [VP, SZ, I64, VP, I32, I64, I64, I64,
+                                                 ctypes.c_float, I32, VP, VP, SZ, VP]
+    need = L.gtp_embedding_order_bytes(8, 100)
+    assert need == 4 * (4 * 8 + 4)  # two buffers of keys and places, and 100 bits
+    assert L.gtp_embedding_order_bytes(0, 100) == L.gtp_embedding_order_bytes(8, 0) == 0
+    rows = lambda order, n, N=8: L.gtp_embedding_rows_ordered(  # noqa: E731
+        4096, 1, N, 1, 4096, 1, 100, 64, 64, 1.0, 4096, -1, order, n, None)
+    ws = L.gtp_embedding_backward_ordered_workspace_bytes(1, 8, 64)
+    grad = lambda order, n, N=8, w=4096, b=ws, out=4096: L.gtp_embedding_backward_ordered(  # noqa: E731
+        order, n, N, 4096, 1, 64, 100, 64, 1.0, 0, out, w, b, None)
+    for call in (rows, grad):
+        assert call(None, need) == call(4097, need) == call(4096, need - 1) == INVALID
+        assert call(4096, need, N=-1) == INVALID
+        assert call(4096, 1 << 40, N=1 << 24) == UNSUPPORTED
+    assert grad(4096, need, b=ws - 1) == grad(4096, need, w=None) == INVALID
+    assert grad(4096, need, w=4098) == grad(4096, need, out=None) == INVALID
 
 
 def test_norm_entry_points():

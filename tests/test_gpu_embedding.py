@@ -145,6 +145,57 @@ def test_added_to_a_tied_gradient(dtype):
     check(odd, *expect(ids, grad, V, 1.0))
 
 
+@pytest.mark.parametrize("dtype", [BF, HF, FP], ids=IDS)
+@pytest.mark.parametrize("N,V,H", SIZES)
+def test_the_order_stands_for_the_ids(N, V, H, dtype):
+    """To the bit, twice from one order, into new memory and onto old."""
+    ids = ids_of(N, V, N + H).cuda()
+    if N > 3:
+        ids[1], ids[-1] = -1, V
+    w, grad = torch.randn(V, H).to(dtype).cuda(), torch.randn(N, H).to(dtype).cuda()
+    out, bad, order = ops.embedding_ordered(ids, w, scale=3.0, padding_idx=V // 2, check=False)
+    assert not bad and order.dtype == torch.int32
+    assert torch.equal(out.nan_to_num(7.0), ops.embedding(ids, w, scale=3.0, check=False)[0].nan_to_num(7.0))
+    want = ops.embedding_backward(ids, grad, V, scale=3.0, padding_idx=V // 2)
+    ids.zero_()
+    for _ in range(2):
+        assert torch.equal(ops.embedding_backward(None, grad, V, scale=3.0, order=order), want)
+    onto = torch.zeros(V, H, dtype=dtype, device="cuda")
+    ops.embedding_backward(None, grad, V, scale=3.0, order=order, out=onto)
+    assert torch.equal(onto, want)
+
+
+def test_rows_without_tokens_are_zeros():
+    """Whatever the memory held, at every alignment of a row; nothing behind
+    the last row is written."""
+    for H in (1, 3, 7, 9, 64, 129, 1027):
+        for dtype in (BF, FP):
+            V, N = 203, 3
+            ids = torch.tensor([0, V - 1, 77], device="cuda")
+            w = torch.zeros(V, H, dtype=dtype, device="cuda")
+            grad = torch.ones(N, H, dtype=dtype, device="cuda")
+            order = ops.embedding_ordered(ids, w)[2]
+            dirty = torch.full((V * H + 1024,), float("nan"), dtype=dtype, device="cuda")
+            del dirty  # the allocator hands this block out next
+            for got in (ops.embedding_backward(ids, grad, V),
+                        ops.embedding_backward(None, grad, V, order=order)):
+                want = torch.zeros(V, H)
+                want[ids.cpu()] = 1.0
+                assert torch.equal(got.cpu().float(), want)
+
+
+def test_orders_of_other_sizes_are_refused():
+    w = torch.zeros(40, 8, device="cuda")
+    order = ops.embedding_ordered(torch.arange(5, device="cuda"), w)[2]
+    grad = torch.zeros(5, 8, device="cuda")
+    for g, V, o in ((grad[:4], 40, order), (grad, 99, order), (grad, 40, order.long()),
+                    (grad, 40, order[:-1]), (grad, 40, order.cpu())):
+        with pytest.raises(RuntimeError, match="order"):
+            ops.embedding_backward(None, g, V, order=o)
+    with pytest.raises(RuntimeError, match="neither"):
+        ops.embedding_backward(None, grad, 40)
+
+
 def test_layouts():
     N, V, H = 90, 200, 64
     ids = ids_of(N, V, 7)
@@ -212,7 +263,10 @@ def test_captured_and_replayed():
         w.normal_(), grad.normal_()
 
     def step():
-        return ops.embedding(ids, w, scale=3.0)[0], ops.embedding_backward(ids, grad, V, scale=3.0)
+        out, _, order = ops.embedding_ordered(ids, w, scale=3.0)
+        return (ops.embedding(ids, w, scale=3.0)[0], out,
+                ops.embedding_backward(ids, grad, V, scale=3.0),
+                ops.embedding_backward(None, grad, V, scale=3.0, order=order))
 
     fill(0)
     s = torch.cuda.Stream()
