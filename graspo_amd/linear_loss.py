@@ -13,6 +13,7 @@ fp32 logits: one product more, and 4 N V bytes less (8.1 GB at 8192 tokens of
 from __future__ import annotations
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import ops
 
@@ -34,6 +35,7 @@ class _LinearLogprob(torch.autograd.Function):
         return out.mean_loss if mean else out.logprob
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, grad):
         hidden, weight, targets, lse, count = ctx.saved_tensors
         gh, gw = ops.linear_logprob_backward(

@@ -187,6 +187,30 @@ def test_max_norm_of_zero_and_no_gradient():
     assert float(get_total_norm([torch.empty(0, device="cuda")])) == 0.0
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_views_of_a_bucket(dtype):
+    """Neighbours in any order, empty ones and gaps between: each element of
+    the listed views counts and is scaled once, the others stay."""
+    sizes = [5, 0, 4096, 1, 70001, 33, 16384, 9, 2, 65536]
+    bucket = torch.randn(sum(sizes) + 7, generator=torch.Generator().manual_seed(3)).to(dtype).cuda()
+    before, at, views = bucket.clone(), 3, []
+    for n in sizes:
+        views.append(bucket[at : at + n])
+        at += n
+    for order in (range(10), [9, 8, 7, 6, 5, 4, 3, 2, 1, 0], [0, 1, 2, 4, 5, 3, 7, 8], [6, 7, 9]):
+        listed = [views[i] for i in order]
+        bucket.copy_(before)
+        want = exact_norm([v.clone() for v in listed], 2.0)
+        norm = clip_grad_norm_([_as_param(v) for v in listed], 1.0)
+        assert abs(float(norm) - float(want)) <= 2 * 2.0 ** -24 * float(want)
+        # the same products one tensor at a time
+        alone = before.clone()
+        for v in listed:
+            w = alone[v.storage_offset() : v.storage_offset() + v.numel()]
+            clip_grads_with_norm_([_as_param(w)], 1.0, norm)
+        assert torch.equal(bucket, alone)
+
+
 def _as_param(g):
     p = torch.nn.Parameter(torch.zeros_like(g))
     p.grad = g
