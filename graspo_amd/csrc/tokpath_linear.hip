@@ -63,7 +63,7 @@ struct Rows {
 struct Meta {
   int32_t n;     // listed rows
   int32_t bad;   // rows whose target lies outside [0, V)
-  float inv;     // 1 / the power of two in D
+  float inv;     // what D lacks: 1 / a power of two, or the mean's gradient
   int32_t splits;  // shares of dh's products (backward)
 };
 
@@ -96,7 +96,7 @@ struct Listed {
   int32_t* at;     // its index b * T + s
   int32_t* target;
   float* lse;      // backward only
-  float* g;        // backward only: times the power of two
+  float* g;        // backward only: over Meta::inv
 };
 
 // ------------------------------------------------------------ listing
@@ -152,15 +152,23 @@ __global__ __launch_bounds__(kListBlock) void list_rows_kernel(
     top = fmaxf(top, tops[w]);
   }
   // fp16: 2^(15 - e) for 2^(e-1) <= top < 2^e (bounded, so that neither it nor
-  // its inverse leaves fp32's normal numbers)
-  float scale = 1.0f;
-  if (scaled && top > 0.0f && top < kPosInf) {
+  // its inverse leaves fp32's normal numbers).  The mean's gradient is one for
+  // all rows and left out of D altogether: a target's element g (1 - p) is
+  // nearly g in most rows, and one rounding shared by all of them would not
+  // average out (4096 tokens of 151936: the error against 64 bits was 0.0027,
+  // and is 0.0018 so, of which rounding the results takes 0.0017).
+  float scale = 1.0f, inv = 1.0f;
+  if (mean_count) {
+    scale = scaled ? 16384.0f : 1.0f;
+    inv = gm / scale;
+  } else if (scaled && top > 0.0f && top < kPosInf) {
     int e;
     frexpf(top, &e);
     scale = ldexpf(1.0f, min(max(15 - e, -100), 100));
+    inv = 1.0f / scale;
   }
   if (tid == 0) {
-    *meta = Meta{(int32_t)all, any_bad, 1.0f / scale, backward ? (int32_t)shares.best(all) : 0};
+    *meta = Meta{(int32_t)all, any_bad, inv, backward ? (int32_t)shares.best(all) : 0};
     if (verdict)
       __hip_atomic_store(verdict, GTP_VERDICT_GOOD | (any_bad ? GTP_VERDICT_BAD : 0u),
                          __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
@@ -177,7 +185,7 @@ __global__ __launch_bounds__(kListBlock) void list_rows_kernel(
       out.target[k] = (int32_t)t;
       if (backward) {
         out.lse[k] = lse_in[n];
-        out.g[k] = g * scale;
+        out.g[k] = mean_count ? scale : g * scale;
       }
     } else if (out_lp) {
       const float v = skip ? 0.0f : __builtin_nanf("");
