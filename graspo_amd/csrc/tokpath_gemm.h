@@ -76,6 +76,11 @@ struct Bf16 {
   __device__ static __forceinline__ void mfma(f32x4& c, s16x8 a, s16x8 b) {
     asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
   }
+  typedef __bf16 x8 __attribute__((ext_vector_type(8)));
+  __device__ static __forceinline__ f32x4 mul(s16x8 a, s16x8 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(x8, a),
+                                                   __builtin_bit_cast(x8, b), c, 0, 0, 0);
+  }
   __device__ static __forceinline__ uint16_t from(float v) {
     return __builtin_bit_cast(uint16_t, (__bf16)v);
   }
@@ -83,6 +88,11 @@ struct Bf16 {
 struct F16 {
   __device__ static __forceinline__ void mfma(f32x4& c, s16x8 a, s16x8 b) {
     asm volatile("v_mfma_f32_16x16x32_f16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
+  }
+  typedef _Float16 x8 __attribute__((ext_vector_type(8)));
+  __device__ static __forceinline__ f32x4 mul(s16x8 a, s16x8 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(x8, a),
+                                                  __builtin_bit_cast(x8, b), c, 0, 0, 0);
   }
   __device__ static __forceinline__ uint16_t from(float v) {
     return __builtin_bit_cast(uint16_t, (_Float16)v);

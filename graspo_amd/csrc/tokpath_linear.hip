@@ -33,6 +33,7 @@
 // _selected_token_log_probs_from_hidden
 // (src/graspo/backends/graspoflow/tensor_utils.py:167-186) under autograd,
 // which keeps every chunk's logits.
+#include "tokpath_few.h"
 #include "tokpath_gemm.h"
 
 namespace gtp {
@@ -344,6 +345,53 @@ __global__ __launch_bounds__(kThreads, 1) void lse_kernel(LseArgs a) {
   wait_vm<0>();  // the loads past the last tile write their zeros
 }
 
+// The same partial states for at most 16 kNB rows: a workgroup's 128 vocabulary
+// rows in one.
+template <typename E, int kNB>
+__global__ __launch_bounds__(few::kThreads, 2) void few_lse_kernel(LseArgs a) {
+  constexpr int kTok = 16 * kNB;
+  __shared__ __attribute__((aligned(16))) uint4 s_h[2][kTok * few::kChunks<kNB>];
+  __shared__ float2 s_ms[few::kWaves][kTok];
+  const int n = a.meta->n;
+  if (n == 0) return;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t first = (int64_t)blockIdx.x * few::kRows + wave * few::kWaveRows;
+  few::Product<E, kNB, false> x;
+  x.run(a.w, first, a.h, n, a.K, s_h);
+  const int64_t v0 = first + 4 * (lane >> 4);
+  const int lim = (int)min((int64_t)few::kWaveRows, max(a.w.outer - v0, (int64_t)0));
+#pragma unroll
+  for (int y = 0; y < kNB; ++y) {
+    const int k = y * 16 + (lane & 15);
+    const int64_t off = (k < n ? (int64_t)a.target[k] : -1) - v0;
+    const int want = off >= 0 && off < lim ? (int)off : -1;
+    float v[8], xt = 0.0f, m = kNegInf, s = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int o = (i / 4) * 16 + (i & 3);
+      const float q = x.acc[i / 4][y][i & 3];
+      xt = want == o ? q : xt;
+      v[i] = o < lim ? q : kNegInf;
+      m = max3raw(m, v[i], v[i]);
+    }
+    const float mb = m == kNegInf ? 0.0f : m;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) s += __builtin_amdgcn_exp2f((v[i] - mb) * kLog2e);
+    if (want >= 0 && (want & 12) == 0) a.xt[k] = xt;
+    float2 st{m, s};
+    st = merge_ms(st, float2{__shfl_xor(st.x, 16, kWave), __shfl_xor(st.y, 16, kWave)});
+    st = merge_ms(st, float2{__shfl_xor(st.x, 32, kWave), __shfl_xor(st.y, 32, kWave)});
+    if (lane < 16) s_ms[wave][k] = st;
+  }
+  __syncthreads();
+  const int k = threadIdx.x;
+  if (k >= n) return;
+  float2 st = s_ms[0][k];
+#pragma unroll
+  for (int w = 1; w < few::kWaves; ++w) st = merge_ms(st, s_ms[w][k]);
+  a.partial[(int64_t)blockIdx.x * a.ldn + k] = st;
+}
+
 // The listed rows' logprob and lse from their partial states: 16 rows per
 // workgroup, 64 threads each merging every 64th state, then one merge in LDS.
 constexpr int kMergeTok = 16, kMergeGrp = 64;
@@ -515,6 +563,44 @@ __global__ __launch_bounds__(kThreads, 1) void grad_logits_kernel(GradArgs a) {
     tt = tt2;
   }
   wait_vm<0>();
+}
+
+// The piece's D for at most 16 kNB rows, ldn = 16 kNB of them (past the last:
+// zeros, whatever the weight holds).
+template <typename E, int kNB>
+__global__ __launch_bounds__(few::kThreads, 2) void few_grad_logits_kernel(GradArgs a) {
+  constexpr int kTok = 16 * kNB;
+  __shared__ __attribute__((aligned(16))) uint4 s_h[2][kTok * few::kChunks<kNB>];
+  __shared__ __attribute__((aligned(16))) float s_lse[kTok], s_g[kTok];
+  __shared__ __attribute__((aligned(16))) int s_t[kTok];
+  const int n = a.meta->n, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  if (threadIdx.x < kTok) {  // (the product's barriers publish them)
+    const int k = threadIdx.x;
+    s_lse[k] = k < n ? a.rows.lse[k] : kPosInf;
+    s_g[k] = k < n ? a.rows.g[k] : 0.0f;
+    s_t[k] = k < n ? (int)(a.rows.target[k] - a.v_first) : -1;
+  }
+  const int64_t first = (int64_t)blockIdx.x * few::kRows + wave * few::kWaveRows;
+  few::Product<E, kNB, true> x;
+  x.run(a.w, first, a.h, n, a.K, s_h);
+#pragma unroll
+  for (int b = 0; b < 2; ++b) {
+    const int64_t v = first + 16 * b + (lane & 15);
+    if (v >= a.w.outer) continue;
+#pragma unroll
+    for (int y = 0; y < kNB; ++y) {
+      const int t0 = 16 * y + 4 * (lane >> 4);
+      uint16_t e[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float g = s_g[t0 + i];
+        const float p = __builtin_amdgcn_exp2f((x.acc[b][y][i] - s_lse[t0 + i]) * kLog2e);
+        const float d = g * ((s_t[t0 + i] == v ? 1.0f : 0.0f) - p);
+        e[i] = E::from(g == 0.0f ? 0.0f : d);
+      }
+      *reinterpret_cast<uint2*>(a.d + v * a.ldn + t0) = __builtin_bit_cast(uint2, e);
+    }
+  }
 }
 
 struct HiddenArgs {
@@ -721,7 +807,7 @@ int shape_of(const gtp_linear_rows* r, Shape& s, Rows& a) {
       (reinterpret_cast<uintptr_t>(r->weight) & 15u))
     return GTP_ERR_UNSUPPORTED;
   s.ldh = (r->K + 63) / 64 * 64;
-  s.ldn = (s.N + 7) / 8 * 8;
+  s.ldn = s.N <= few::kMostRows ? (s.N + 63) / 64 * 64 : (s.N + 7) / 8 * 8;
   s.n_vt = tiles(r->V);
   s.n_tt = tiles(s.N);
   s.n_ct = tiles(s.K8);
@@ -824,6 +910,12 @@ void forward_launch(const gtp_linear_rows* r, const Shape& s, const Forward& f, 
   a.ldn = s.ldn;
   a.tm = s.n_vt;
   a.band = band_rows(s.n_vt, s.n_tt);
+  if (s.N <= few::kMostRows) {
+    const dim3 grid((unsigned)(2 * s.n_vt)), block(few::kThreads);
+    s.N <= 64 ? launch_timed(few_lse_kernel<E, 4>, grid, block, st, a)
+              : launch_timed(few_lse_kernel<E, 8>, grid, block, st, a);
+    return;
+  }
   launch_timed(lse_kernel<E>, dim3(grid_of(s.n_vt, s.n_tt)), dim3(kThreads), st, a);
 }
 
@@ -847,6 +939,12 @@ void grad_logits_launch(const gtp_linear_rows* r, const Shape& s, const Backward
   a.ldn = s.ldn;
   a.tm = tiles(rows);
   a.band = band_rows(a.tm, s.n_tt);
+  if (s.N <= few::kMostRows) {
+    const dim3 grid((unsigned)((rows + few::kRows - 1) / few::kRows)), block(few::kThreads);
+    s.N <= 64 ? launch_timed(few_grad_logits_kernel<E, 4>, grid, block, st, a)
+              : launch_timed(few_grad_logits_kernel<E, 8>, grid, block, st, a);
+    return;
+  }
   launch_timed(grad_logits_kernel<E>, dim3(grid_of(a.tm, s.n_tt)), dim3(kThreads), st, a);
 }
 
@@ -870,6 +968,31 @@ void grad_hidden_launch(const gtp_linear_rows* r, const Shape& s, const Backward
 template <typename E>
 void grad_weight_launch(const gtp_linear_rows* r, const Shape& s, const Backward& b, int64_t v0,
                         int64_t rows, uint16_t* grad_weight, hipStream_t st) {
+  const int vec = (r->K & 7) == 0 && (reinterpret_cast<uintptr_t>(grad_weight) & 15u) == 0 ? 1 : 0;
+  if (s.N <= few::kMostRows) {
+    few::WeightArgs a;
+    a.h = Operand{b.h, s.ldh, s.N};
+    a.d = Operand{b.d, s.ldn, rows};
+    a.n_listed = &b.meta->n;
+    a.inv = &b.meta->inv;
+    a.out = grad_weight + v0 * r->K;
+    a.ld = r->K;
+    a.width = r->K;
+    const int cols = few::kWaves * (s.N <= 64 ? few::kWaveCols<4> : few::kWaveCols<8>);
+    a.slabs = (int)((r->K + cols - 1) / cols);
+    // three workgroups per CU (what their registers allow at once), each of 16
+    // vocabulary rows at least
+    const int64_t ranges = max((int64_t)3 * device_cus() / a.slabs, (int64_t)1);
+    a.range = ((rows + ranges - 1) / ranges + 15) / 16 * 16;
+    const int64_t each = ((rows + a.range - 1) / a.range + 7) / 8;
+    const dim3 grid((unsigned)(8 * each * a.slabs)), block(few::kThreads);
+    auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, block, 0, st, a); };
+    if (s.N <= 64)
+      vec ? launch(few::few_weight_kernel<E, 4, true>) : launch(few::few_weight_kernel<E, 4, false>);
+    else
+      vec ? launch(few::few_weight_kernel<E, 8, true>) : launch(few::few_weight_kernel<E, 8, false>);
+    return;
+  }
   WeightArgs a;
   a.h = Operand{b.h, s.ldh, s.ldh};
   a.d = Operand{b.d, s.ldn, rows};
@@ -880,7 +1003,7 @@ void grad_weight_launch(const gtp_linear_rows* r, const Shape& s, const Backward
   a.tm = tiles(rows);
   a.tn = s.n_ct;
   a.band = band_rows(a.tm, a.tn);
-  a.vec = (r->K & 7) == 0 && (reinterpret_cast<uintptr_t>(grad_weight) & 15u) == 0 ? 1 : 0;
+  a.vec = vec;
   hipLaunchKernelGGL(grad_weight_kernel<E>, dim3(grid_of(a.tm, a.tn)), dim3(kThreads), 0,
                      st, a);
 }
