@@ -76,19 +76,35 @@ struct Meta {
 struct Shares {
   int32_t column_tiles, cus;
   int64_t steps, width, most;
-  __host__ __device__ int64_t best(int64_t rows) const {
+  __host__ __device__ float us(int64_t rows, int64_t k) const {
     const int64_t tiles = (rows + kTile - 1) / kTile * column_tiles;
+    return (float)((tiles * k + cus - 1) / cus * ((steps + k - 1) / k)) * 1.5f +
+           (float)(k * rows * width) * (12.0f / 4.5e6f);
+  }
+  __host__ __device__ bool possible(int64_t rows, int64_t k) const {
+    return k == 1 || (k <= 32 && steps / k >= 8 && k * rows <= most);
+  }
+  int64_t best(int64_t rows) const {
     int64_t found = 1;
-    float least = 0.0f;
-    for (int64_t k = 1; k <= 32 && (k == 1 || (steps / k >= 8 && k * rows <= most)); ++k) {
-      const float us = (float)((tiles * k + cus - 1) / cus * ((steps + k - 1) / k)) * 1.5f +
-                       (float)(k * rows * width) * (12.0f / 4.5e6f);
-      if (k == 1 || us < least) {
-        least = us;
+    for (int64_t k = 2; possible(rows, k); ++k)
+      if (us(rows, k) < us(rows, found)) found = k;
+    return found;
+  }
+  // The same by a whole wave.
+  __device__ int best_of(int64_t rows) const {
+    const int lane = threadIdx.x & 63;
+    float least = lane < 32 && possible(rows, lane + 1) ? us(rows, lane + 1) : kPosInf;
+    int found = lane + 1;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const float u = __shfl_xor(least, o, kWave);
+      const int k = __shfl_xor(found, o, kWave);
+      if (u < least || (u == least && k < found)) {
+        least = u;
         found = k;
       }
     }
-    return found;
+    return __shfl(found, 0, kWave);
   }
 };
 
@@ -168,8 +184,9 @@ __global__ __launch_bounds__(kListBlock) void list_rows_kernel(
     scale = ldexpf(1.0f, min(max(15 - e, -100), 100));
     inv = 1.0f / scale;
   }
+  const int splits = backward && wid == 0 ? shares.best_of(all) : 0;
   if (tid == 0) {
-    *meta = Meta{(int32_t)all, any_bad, inv, backward ? (int32_t)shares.best(all) : 0};
+    *meta = Meta{(int32_t)all, any_bad, inv, splits};
     if (verdict)
       __hip_atomic_store(verdict, GTP_VERDICT_GOOD | (any_bad ? GTP_VERDICT_BAD : 0u),
                          __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
@@ -392,31 +409,33 @@ __global__ __launch_bounds__(few::kThreads, 2) void few_lse_kernel(LseArgs a) {
   a.partial[(int64_t)blockIdx.x * a.ldn + k] = st;
 }
 
-// The listed rows' logprob and lse from their partial states: 16 rows per
-// workgroup, 64 threads each merging every 64th state, then one merge in LDS.
-constexpr int kMergeTok = 16, kMergeGrp = 64;
-__global__ __launch_bounds__(kMergeTok * kMergeGrp) void lse_merge_kernel(const float2* __restrict__ partial,
-                                                        int64_t ldn, int n_parts,
-                                                        const Meta* __restrict__ meta,
-                                                        const int32_t* __restrict__ at,
-                                                        const float* __restrict__ xt,
-                                                        float* __restrict__ out_lp,
-                                                        float* __restrict__ out_lse) {
-  __shared__ float2 red[kMergeGrp][kMergeTok];
-  const int lt = threadIdx.x % kMergeTok, g = threadIdx.x / kMergeTok;
-  const int64_t k = (int64_t)blockIdx.x * kMergeTok + lt;
+// The listed rows' logprob and lse from their partial states: kTok rows per
+// workgroup, the other threads merging every so many states of them each.
+constexpr int kMergeBlock = 1024;
+template <int kTok>
+__global__ __launch_bounds__(kMergeBlock) void lse_merge_kernel(
+    const float2* __restrict__ partial, int64_t ldn, int n_parts, const Meta* __restrict__ meta,
+    const int32_t* __restrict__ at, const float* __restrict__ xt, float* __restrict__ out_lp,
+    float* __restrict__ out_lse) {
+  constexpr int kGroups = kMergeBlock / kTok;
+  __shared__ float2 red[kMergeBlock / kWave][kTok];
+  const int lt = threadIdx.x % kTok, g = threadIdx.x / kTok;
+  const int64_t k = (int64_t)blockIdx.x * kTok + lt;
   const int n = meta->n;
-  if ((int64_t)blockIdx.x * kMergeTok >= n) return;
+  if ((int64_t)blockIdx.x * kTok >= n) return;
   float2 st{kNegInf, 0.0f};
   if (k < n) {
 #pragma unroll 4
-    for (int p = g; p < n_parts; p += kMergeGrp) st = merge_ms(st, partial[p * ldn + k]);
+    for (int p = g; p < n_parts; p += kGroups) st = merge_ms(st, partial[p * ldn + k]);
   }
-  red[g][lt] = st;
+#pragma unroll
+  for (int o = kTok; o < kWave; o <<= 1)
+    st = merge_ms(st, float2{__shfl_xor(st.x, o, kWave), __shfl_xor(st.y, o, kWave)});
+  if ((threadIdx.x & 63) < kTok) red[threadIdx.x >> 6][lt] = st;
   __syncthreads();
   if (g != 0 || k >= n) return;
 #pragma unroll
-  for (int q = 1; q < kMergeGrp; ++q) st = merge_ms(st, red[q][lt]);
+  for (int w = 1; w < kMergeBlock / kWave; ++w) st = merge_ms(st, red[w][lt]);
   const float ln_s = __builtin_amdgcn_logf(st.y) * kLn2;
   out_lp[at[k]] = (xt[k] - st.x) - ln_s;
   out_lse[at[k]] = st.x + ln_s;
@@ -698,11 +717,13 @@ __global__ __launch_bounds__(256) void grad_hidden_rows_kernel(const float* __re
   float v[4] = {};
   if (k >= 0) {
     const float* row = sum + k * width;
-#pragma unroll 2
+    int64_t c[4];  // (no branch around a load: columns past the last read the last)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) c[i] = min(c0 + i * 256, width - 1);
+#pragma unroll 8
     for (int p = 0; p < splits; ++p, row += n * width)
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (c0 + i * 256 < width) v[i] += row[c0 + i * 256];
+      for (int i = 0; i < 4; ++i) v[i] += row[c[i]];
   }
 #pragma unroll
   for (int i = 0; i < 4; ++i)
@@ -1058,9 +1079,13 @@ extern "C" int gtp_linear_logprob_rows(const gtp_linear_rows* rows, float* out_l
       lin::forward_launch<gemm::Bf16>(rows, s, f, st);
     else
       lin::forward_launch<gemm::F16>(rows, s, f, st);
-    hipLaunchKernelGGL(lin::lse_merge_kernel,
-                       dim3((unsigned)((s.N + lin::kMergeTok - 1) / lin::kMergeTok)),
-                       dim3(lin::kMergeTok * lin::kMergeGrp), 0, st, f.partial, s.ldn, 2 * s.n_vt, f.meta, f.at, f.xt, out_logprob, out_lse);
+    auto merge = [&](auto kernel, int64_t rows_each) {
+      hipLaunchKernelGGL(kernel, dim3((unsigned)((s.N + rows_each - 1) / rows_each)),
+                         dim3(lin::kMergeBlock), 0, st, f.partial, s.ldn, 2 * s.n_vt, f.meta, f.at,
+                         f.xt, out_logprob, out_lse);
+    };
+    // few rows: more threads for each
+    s.N <= few::kMostRows ? merge(lin::lse_merge_kernel<4>, 4) : merge(lin::lse_merge_kernel<16>, 16);
   }
   if (mean_loss)
     hipLaunchKernelGGL(lin::mean_kernel, dim3(1), dim3(1024), 0, st, f.meta, f.at, out_logprob,
