@@ -12,7 +12,7 @@ import torch
 from torch import nn
 
 from . import ops
-from .linear_loss import _LinearLogprob, check_operands
+from .linear_loss import check_operands
 
 
 def _token_rows(logits: torch.Tensor) -> torch.Tensor | None:
@@ -110,8 +110,8 @@ def sequence_log_probs_from_hidden(
     h, t = hidden_states, output_ids
     if h.dim() != 3:
         h, t = h.reshape(1, -1, h.shape[-1]), t.reshape(1, -1)
-    lp = _LinearLogprob.apply(h, lm_head_weight, t,
-                              None if ignore_index is None else int(ignore_index), False, what)
+    lp = ops.linear_loss(h, lm_head_weight, t, what=what,
+                         ignore_index=None if ignore_index is None else int(ignore_index))
     return lp.reshape(lead)
 
 

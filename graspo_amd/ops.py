@@ -353,6 +353,16 @@ def linear_logprob_backward(hidden: torch.Tensor, weight: torch.Tensor, targets:
     return (gh if need_hidden else None), (gw if need_weight else None)
 
 
+def linear_loss(hidden: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor, *,
+                ignore_index: int | None = None, mean: bool = False,
+                what: str = "linear_loss") -> torch.Tensor:
+    """:func:`linear_logprob`'s logprobs, or their mean loss, differentiable
+    (once) in both operands.  A bad target raises ``RuntimeError`` (in a graph
+    capture its logprob, and the mean, is NaN)."""
+    return load().linear_loss(hidden, weight, _targets(targets), ignore_index, mean, what,
+                              _stream(hidden))
+
+
 def _padding(name: str, padding_idx: int | None, vocab: int) -> int:
     if padding_idx is not None and not 0 <= padding_idx < vocab:
         raise ValueError(f"{name}: padding_idx {padding_idx} outside [0, {vocab})")

@@ -15,7 +15,7 @@ from __future__ import annotations
 import torch
 
 from . import ops
-from .linear_loss import _LinearLogprob, check_operands
+from .linear_loss import check_operands
 
 
 class _SFTCrossEntropy(torch.autograd.Function):
@@ -80,5 +80,5 @@ def sft_cross_entropy_loss_from_hidden(
         raise ValueError(
             f"{what}: expected hidden states [B, S, K] and labels [B, S], got "
             f"{tuple(hidden_states.shape)} and {tuple(labels.shape)}")
-    return _LinearLogprob.apply(hidden_states, lm_head_weight, labels[:, 1:], int(ignore_index),
-                                True, what)
+    return ops.linear_loss(hidden_states, lm_head_weight, labels[:, 1:], mean=True, what=what,
+                           ignore_index=int(ignore_index))

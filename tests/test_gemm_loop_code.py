@@ -14,18 +14,24 @@ from graspo_amd import build as B
 
 
 @pytest.fixture(scope="module")
-def kernels(tmp_path_factory):
+def every_kernel(tmp_path_factory):
     out = tmp_path_factory.mktemp("asm") / "linear.s"
     flags = [f for f in B.HIP_FLAGS if f != "-fPIC"]
     subprocess.run([B._hipcc(), *flags, "-S", "--cuda-device-only",
                     os.path.join(B.CSRC, "tokpath_linear.hip"), "-o", str(out)], check=True,
                    capture_output=True)
-    found = re.findall(r"^(_ZN3gtp3lin\w+):(.*?)s_endpgm", out.read_text(), re.S | re.M)
+    found = re.findall(r"^(_ZN3gtp3(?:lin|few)\w+):(.*?)\.Lfunc_end", out.read_text(), re.S | re.M)
     code = {}
     for name, body in found:
         lines = [x.strip() for x in body.split("\n")]
         code[name] = [x for x in lines if x and not x.startswith((";", "."))]
     return {k: v for k, v in code.items() if any("v_mfma" in x for x in v)}
+
+
+@pytest.fixture(scope="module")
+def kernels(every_kernel):
+    # (those for few rows leave their products to the compiler)
+    return {k: v for k, v in every_kernel.items() if "few_" not in k}
 
 
 def registers(token):
@@ -84,3 +90,20 @@ def test_fragments_come_from_lds(kernels):
                 to = operands(y)[0]
                 wrote = registers(to) or ({int(to[1:])} if re.match(r"v\d+$", to) else set())
                 assert not wrote & wanted, (name, y, x)
+
+
+def test_few_rows_stores_that_a_stage_leaves(every_kernel):
+    """The wait for a stage's loads lets a full stage's stores be: as many as a
+    block has, times its blocks, all of them behind the loads."""
+    found = {k: v for k, v in every_kernel.items() if "few_weight_kernel" in k and "Lb1" in k}
+    assert len(found) == 4
+    for name, body in found.items():
+        stores, blocks = (4, 8) if "ELi4E" in name else (2, 4)
+        at = [i for i, x in enumerate(body) if x.startswith("buffer_store_dwordx4")]
+        loads = [i for i, x in enumerate(body) if x.startswith("buffer_load_dwordx4") and " lds" in x]
+        # two stages, each with one loop over its blocks
+        assert len(at) == 2 * stores and len(loads) == 3 * 4, (name, len(at), len(loads))
+        assert loads[7] < at[0] and at[stores - 1] < loads[8] < at[stores], name
+        waits = [x for x in body if x.startswith("s_waitcnt vmcnt(%d) lgkmcnt(0)" % (stores * blocks))]
+        assert len(waits) == 2, name
+        assert not any(x.startswith("scratch") for x in body), name

@@ -100,6 +100,47 @@ def test_logprob_and_gradients(N, V, K, dtype):
 
 
 @pytest.mark.parametrize("dtype", [BF, HF], ids=["bf16", "fp16"])
+@pytest.mark.parametrize("N,V,K", [
+    (64, 129, 256), (65, 128, 64), (127, 1000, 30), (128, 513, 1032), (129, 300, 72), (100, 33, 7),
+    (64, 1, 520), (16, 4097, 1),
+])
+def test_few_rows(N, V, K, dtype):
+    test_logprob_and_gradients(N, V, K, dtype)
+
+
+@pytest.mark.parametrize("N", [61, 100])
+def test_few_rows_over_many_vocabulary_rows(N):
+    """More of them per workgroup than it stages at once, a ragged end."""
+    V, K = 30011, 4104
+    h, w, t, g = (x.cuda() for x in inputs(N, V, K, BF, seed=N))
+    lp, lp_e, gh, gh_e, gw, gw_e = expect(h, w, t, g, BF)
+    h.requires_grad_(), w.requires_grad_()
+    got = sequence_log_probs_from_hidden(h, w, t)
+    within(got.detach(), lp, lp_e, "logprob")
+    a, b = torch.autograd.grad(got, [h, w], g)
+    within(a, gh, gh_e, "hidden's gradient")
+    within(b, gw, gw_e, "weight's gradient")
+
+
+def test_few_rows_beside_a_masked_vocabulary_row():
+    """A vocabulary row of -inf logits takes no part, and the rows of the
+    16-row blocks that are not there make no NaN of it."""
+    for N in (5, 70):
+        h, w, t, g = inputs(N, 40, 64, BF, seed=N)
+        h = h.abs() + 0.5
+        w[7], w[7, 3] = 0.0, float("-inf")
+        t[t == 7] = 8
+        keep = torch.arange(40) != 7
+        small = torch.where(t > 7, t - 1, t)
+        lp, lp_e, *_ = expect(h, w[keep], small, g, BF)
+        hd, wd = h.cuda(), w.cuda().requires_grad_()
+        got = sequence_log_probs_from_hidden(hd, wd, t.cuda())
+        within(got.detach().cpu(), lp, lp_e, "logprob")
+        (gw,) = torch.autograd.grad(got, [wd], g.cuda())
+        assert bool((gw[7] == 0).all()) and bool(gw.isfinite().all())
+
+
+@pytest.mark.parametrize("dtype", [BF, HF], ids=["bf16", "fp16"])
 def test_mean_loss_skips_ignored(dtype):
     B, S, V, K = 3, 90, 611, 96
     h, w, t, _ = inputs(B * S, V, K, dtype, seed=5)
