@@ -8,6 +8,9 @@ extension (``torch.ops.graspo_tokpath``).
 * :mod:`graspo_amd.ops` -- tensor-level entry points.
 * :mod:`graspo_amd.tensor_utils` / :mod:`graspo_amd.graspo_loss` -- drop-ins
   with the reference's names and signatures.
+* :mod:`graspo_amd.embedding` / :mod:`graspo_amd.grad_clip` -- the other ends
+  of a training step: the embedding lookup with its table's gradient, and the
+  global gradient norm with clipping.
 * :mod:`graspo_amd.integration` -- installs the drop-ins into an imported
   ``graspo`` package without editing its call sites.
 

@@ -4,9 +4,16 @@
 // of 256 x 256 leave the cores to rows that are not there, and one workgroup
 // per CU waits for each step's loads.  So here a wave streams its own rows of
 // the weight from memory straight into the operands of the products (each is
-// used once, by this wave alone), two stages ahead, and only the few rows of
-// the other operand go through LDS, where the workgroup's waves share them.
+// used once, by this wave alone), two stages in flight, and only the few rows
+// of the other operand go through LDS, where the workgroup's waves share them.
 // Several workgroups per CU hide each other's waits.
+//
+// 61 rows of 4096, 151936 of the vocabulary, bf16 (1.24 GB; a plain read of it
+// in this pattern takes 225 us, a fill 190): the lse 411 us with the tiles and
+// 320 so (50 of them the write-back of what ran before), D 381 and 291, dw 385
+// and 269; forward and backward 1.39 and 1.14 ms.  At 127 rows 1.39 ms; the
+// tiles take 1.52 at 129.  (With D in one part 1.11 and 1.28 ms, and gradients
+// off by 0.0024 instead of 0.0017: see few_grad_logits_kernel.)
 #pragma once
 #include "tokpath_gemm.h"
 
@@ -135,14 +142,14 @@ struct Product {
   }
 };
 
-// dw[v][c] = inv * sum over the rows of D[v][.] h[.][c]: a wave holds its 128
+// dw[v][c] = inv * sum over the rows of D[v][.] h[.][c], D in two parts: a wave holds its 128
 // (more than 64 rows: 64) columns of h as first operands and walks the vocabulary 16 rows at a time.
 // Bound by the writes.
 template <int kNB>
 constexpr int kWaveCols = kNB == 4 ? 128 : 64;
 
 struct WeightArgs {
-  gemm::Operand h, d;  // listed rows [., ld]; D [piece rows][16 kNB]
+  gemm::Operand h, d;  // listed rows [., ld]; D [piece rows][2][16 kNB], rounded and the rest
   const int32_t* n_listed;
   const float* inv;
   uint16_t* out;  // row stride ld
@@ -153,11 +160,12 @@ struct WeightArgs {
 
 // D goes through LDS, kStaged rows at a time and a stage ahead: loads wait in
 // the memory pipeline behind the stores before them (61 rows of 4096, 151936
-// of the vocabulary: 353 us with each block's D loaded a block ahead, 320 with
-// stages loaded where they are due, 216 with one stage alone).
+// of the vocabulary, D in one part: 353 us with each block's D loaded a block
+// ahead, 320 with stages loaded where they are due, 238 so, 216 with one stage
+// alone).
 // kVec: 16-byte stores.
 template <int kNB>
-constexpr int kStaged = kNB == 4 ? 128 : 64;
+constexpr int kStaged = kNB == 4 ? 96 : 48;
 
 // Two chunks of a stage, and the wait for them.  (In asm: a read that the
 // compiler sees waits for the other stage's loads and the stores before them.)
@@ -185,10 +193,10 @@ __global__ __launch_bounds__(kThreads, 2) void few_weight_kernel(WeightArgs a) {
   const int64_t c0 = ((int64_t)(in_xcd % a.slabs) * kWaves + wave) * kWaveCols<kNB>;
   const int64_t last = min(first + a.range, a.d.outer);
   if (first >= last) return;
-  constexpr int kC = 2 * kNB;  // 16-byte chunks of a row of D
+  constexpr int kC = 4 * kNB;  // 16-byte chunks of a row of D
   constexpr int kLoads = kStaged<kNB> * kC / kThreads;  // per thread and stage
   __shared__ __attribute__((aligned(16))) uint4 s_d0[kStaged<kNB> * kC], s_d1[kStaged<kNB> * kC];
-  auto place = [](int t, int c) { return t * kC + (c ^ (kC == 16 ? t & 15 : (t >> 1) & 7)); };
+  auto place = [](int t, int c) { return t * kC + (c ^ (t & 15)); };
   const int n = *a.n_listed;
   const float inv = *a.inv;
   // blocks 2 j and 2 j + 1 hold columns 32 j + 8 (m / 4) + m % 4 and 4 more in
@@ -215,17 +223,21 @@ __global__ __launch_bounds__(kThreads, 2) void few_weight_kernel(WeightArgs a) {
     col_at[x] = c < a.width ? 2 * (uint32_t)(r * a.ld + c) : kNowhere;
   }
   auto block = [&](int64_t v0, int row, const uint4* s_d) {
-    s16x8 d[kS];
-#pragma unroll
-    for (int s = 0; s < kS; s += 2)
-      read2(&s_d[place(row + r, 4 * s + q)], &s_d[place(row + r, 4 * s + 4 + q)], d[s], d[s + 1]);
     f32x4 acc[kX];
 #pragma unroll
     for (int x = 0; x < kX; ++x) acc[x] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-    for (int s = 0; s < kS; ++s)
+    for (int part = kC / 2; part >= 0; part -= kC / 2) {
+      s16x8 d[kS];
 #pragma unroll
-      for (int x = 0; x < kX; ++x) acc[x] = E::mul(h[x][s], d[s], acc[x]);
+      for (int s = 0; s < kS; s += 2)
+        read2(&s_d[place(row + r, part + 4 * s + q)], &s_d[place(row + r, part + 4 * s + 4 + q)],
+              d[s], d[s + 1]);
+#pragma unroll
+      for (int s = 0; s < kS; ++s)
+#pragma unroll
+        for (int x = 0; x < kX; ++x) acc[x] = E::mul(h[x][s], d[s], acc[x]);
+    }
     // (rows past the last: none of the buffer)
     const __amdgpu_buffer_rsrc_t out =
         buffer(a.out + v0 * a.ld, min(last - v0, (int64_t)16) * a.ld);

@@ -22,9 +22,10 @@
 // with the last valid row, a chunk past K gets an offset past that end, and a
 // load out of range writes zeros to LDS.
 //
-// What bounds it: the part's power.  The matrix cores run 70% of the cycles at
-// 1.7-1.9 GHz; at 8192 x 4096 x 131072 the four products reach 1350-1500
-// TFLOP/s, the library's product of the same sizes 1490-1590 on such a card.
+// What bounds it: the part's power (the library's product keeps the matrix
+// cores busy 93% of the cycles, at 1.58 GHz).  At 8192 x 4096 x 131072 the four
+// products (the lse, D, dh, dw) reach 1434, 1421, 1514 and 1510 TFLOP/s, the
+// library's of the same sizes 1538-1630 on that card; cards differ by 7-10%.
 // What brought it there from 880-1170, each measured on one box:
 // - a stage per array (the compiler waits for all loads in flight before a
 //   transposing read of an array that one of them writes): 877 -> 1225 TFLOP/s
@@ -84,6 +85,7 @@ struct Bf16 {
   __device__ static __forceinline__ uint16_t from(float v) {
     return __builtin_bit_cast(uint16_t, (__bf16)v);
   }
+  __device__ static __forceinline__ float to(uint16_t v) { return u2f((uint32_t)v << 16); }
 };
 struct F16 {
   __device__ static __forceinline__ void mfma(f32x4& c, s16x8 a, s16x8 b) {
@@ -97,6 +99,7 @@ struct F16 {
   __device__ static __forceinline__ uint16_t from(float v) {
     return __builtin_bit_cast(uint16_t, (_Float16)v);
   }
+  __device__ static __forceinline__ float to(uint16_t v) { return f16_to_f32(v); }
 };
 
 // `outer` rows (kAlongK) or columns (kAcrossK) of 16-bit values; rows 16-byte

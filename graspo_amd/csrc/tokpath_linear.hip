@@ -15,10 +15,14 @@
 // - Backward, piece by piece of the vocabulary: the piece's logits again,
 //   their gradient D rounded once to 16 bits (each element within half a step
 //   of its fp32 value; fp16 scaled by a power of two that puts the largest
-//   |g| just below 2^15, so that small probabilities keep their bits) and
+//   |g| just below 2^15, so that small probabilities keep their bits; the
+//   mean's g, one for all rows, left for the end) and
 //   written vocabulary-major; then dh += D^T w and dw = D h from it, both
 //   accumulated in fp32 and rounded once.  A piece's D takes at most
 //   kPieceBytes whatever V is.
+//
+//   With at most 128 rows the weight's bytes bound the call, the products but
+//   dh's run in the kernels of tokpath_few.h, and D is two 16-bit parts.
 //
 // Rows whose target is ignored, whose target lies outside [0, V) or (backward)
 // whose g is 0 are left out of every product: a first kernel lists the others
@@ -75,7 +79,12 @@ struct Meta {
 // the device.
 struct Shares {
   int32_t column_tiles, cus;
+  int32_t low;  // D in two parts: the second one's first row in the sums
   int64_t steps, width, most;
+  // rows of the sums
+  __host__ __device__ int64_t rows(int64_t listed) const {
+    return low > 0 && listed > 0 ? low + listed : listed;
+  }
   __host__ __device__ float us(int64_t rows, int64_t k) const {
     const int64_t tiles = (rows + kTile - 1) / kTile * column_tiles;
     return (float)((tiles * k + cus - 1) / cus * ((steps + k - 1) / k)) * 1.5f +
@@ -184,7 +193,7 @@ __global__ __launch_bounds__(kListBlock) void list_rows_kernel(
     scale = ldexpf(1.0f, min(max(15 - e, -100), 100));
     inv = 1.0f / scale;
   }
-  const int splits = backward && wid == 0 ? shares.best_of(all) : 0;
+  const int splits = backward && wid == 0 ? shares.best_of(shares.rows(all)) : 0;
   if (tid == 0) {
     *meta = Meta{(int32_t)all, any_bad, inv, splits};
     if (verdict)
@@ -584,8 +593,12 @@ __global__ __launch_bounds__(kThreads, 1) void grad_logits_kernel(GradArgs a) {
   wait_vm<0>();
 }
 
-// The piece's D for at most 16 kNB rows, ldn = 16 kNB of them (past the last:
-// zeros, whatever the weight holds).
+// The piece's D for at most 16 kNB rows (past the last: zeros, whatever the
+// weight holds), rounded to 16 bits and, 16 kNB elements on, what that left
+// out.  With few rows the roundings of D do not average out against the
+// results' own (56 rows of 2944: the gradients were off by 0.0026 against 64
+// bits, rounding them alone takes 0.0017), the products are not what bounds
+// them, and dh's tile has room for as many rows again.
 template <typename E, int kNB>
 __global__ __launch_bounds__(few::kThreads, 2) void few_grad_logits_kernel(GradArgs a) {
   constexpr int kTok = 16 * kNB;
@@ -609,15 +622,19 @@ __global__ __launch_bounds__(few::kThreads, 2) void few_grad_logits_kernel(GradA
 #pragma unroll
     for (int y = 0; y < kNB; ++y) {
       const int t0 = 16 * y + 4 * (lane >> 4);
-      uint16_t e[4];
+      uint16_t high[4], low[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const float g = s_g[t0 + i];
         const float p = __builtin_amdgcn_exp2f((x.acc[b][y][i] - s_lse[t0 + i]) * kLog2e);
-        const float d = g * ((s_t[t0 + i] == v ? 1.0f : 0.0f) - p);
-        e[i] = E::from(g == 0.0f ? 0.0f : d);
+        const float d = g == 0.0f ? 0.0f : g * ((s_t[t0 + i] == v ? 1.0f : 0.0f) - p);
+        high[i] = E::from(d);
+        const float h = E::to(high[i]);
+        low[i] = E::from(fabsf(h) < kPosInf ? d - h : 0.0f);
       }
-      *reinterpret_cast<uint2*>(a.d + v * a.ldn + t0) = __builtin_bit_cast(uint2, e);
+      uint16_t* to = a.d + v * a.ldn + t0;
+      *reinterpret_cast<uint2*>(to) = __builtin_bit_cast(uint2, high);
+      *reinterpret_cast<uint2*>(to + kTok) = __builtin_bit_cast(uint2, low);
     }
   }
 }
@@ -626,7 +643,8 @@ struct HiddenArgs {
   Operand d, w;  // D [piece rows][ldn] across K, the piece's weight rows across K
   int64_t K;     // piece rows
   const Meta* meta;
-  float* sum;    // [shares][listed rows][width]
+  float* sum;    // [shares][rows of the sums][width]
+  Shares shares;
   int64_t width;
   int first, tn, band;
 };
@@ -636,8 +654,8 @@ struct HiddenArgs {
 template <typename E>
 __global__ __launch_bounds__(kThreads, 1) void grad_hidden_kernel(HiddenArgs a) {
   GTP_LOOP_LDS;
-  const int n_listed = a.meta->n, splits = a.meta->splits;
-  Tiles at(blockIdx.x, (n_listed + kTile - 1) / kTile, a.tn, splits, a.band);
+  const int n_rows = (int)a.shares.rows(a.meta->n), splits = a.meta->splits;
+  Tiles at(blockIdx.x, (n_rows + kTile - 1) / kTile, a.tn, splits, a.band);
   if (!at.more()) return;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wt = wave >> 1, wc = wave & 1;
@@ -668,14 +686,14 @@ __global__ __launch_bounds__(kThreads, 1) void grad_hidden_kernel(HiddenArgs a) 
     }
     loop.tile(k_of(split + 1) - k_of(split), ca, cb);
 
-    float* sum = a.sum + (int64_t)split * n_listed * a.width;
+    float* sum = a.sum + (int64_t)split * n_rows * a.width;
 #pragma unroll
     for (int y = 0; y < kB; ++y) {
         const int64_t col = (int64_t)ct * kTile + wc * 128 + y * 16 + (lane & 15);
 #pragma unroll
         for (int x = 0; x < kB; ++x) {
           const int k0 = tt * kTile + wt * 128 + x * 16 + 4 * (lane >> 4);
-          const int rows = col < a.width ? n_listed - k0 : 0;
+          const int rows = col < a.width ? n_rows - k0 : 0;
           float* to = sum + k0 * a.width + col;
           float q[4];
 #pragma unroll
@@ -705,25 +723,28 @@ __global__ __launch_bounds__(kThreads, 1) void grad_hidden_kernel(HiddenArgs a) 
 // listed get zeros.  One workgroup per position and 1024 columns.
 template <typename E>
 __global__ __launch_bounds__(256) void grad_hidden_rows_kernel(const float* __restrict__ sum,
-                                                               int64_t width,
+                                                               int64_t width, Shares shares,
                                                                const Meta* __restrict__ meta,
                                                                const int32_t* __restrict__ slot,
                                                                uint16_t* __restrict__ out) {
-  const int64_t pos = blockIdx.x;
-  const int k = slot[pos], n = meta->n, splits = meta->splits;
+  const int64_t pos = blockIdx.x, n_rows = shares.rows(meta->n);
+  const int k = slot[pos], splits = meta->splits;
   const float inv = meta->inv;
   uint16_t* to = out + pos * width;
   const int64_t c0 = (int64_t)blockIdx.y * 1024 + threadIdx.x;
   float v[4] = {};
   if (k >= 0) {
-    const float* row = sum + k * width;
     int64_t c[4];  // (no branch around a load: columns past the last read the last)
 #pragma unroll
     for (int i = 0; i < 4; ++i) c[i] = min(c0 + i * 256, width - 1);
+    for (int64_t at = shares.low + k; at >= 0; at -= shares.low) {  // the low part first
+      const float* row = sum + at * width;
 #pragma unroll 8
-    for (int p = 0; p < splits; ++p, row += n * width)
+      for (int p = 0; p < splits; ++p, row += n_rows * width)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) v[i] += row[c[i]];
+        for (int i = 0; i < 4; ++i) v[i] += row[c[i]];
+      if (at == k) break;
+    }
   }
 #pragma unroll
   for (int i = 0; i < 4; ++i)
@@ -806,6 +827,7 @@ struct Carve {
 struct Shape {
   int64_t N, K8, ldh, ldn;  // rows with a target; K to a multiple of 8; row strides
   int n_vt, n_tt, n_ct;     // tiles of vocabulary, tokens and hidden columns
+  int low;                  // few rows: where D's second part begins, else 0
 };
 
 inline int tiles(int64_t n) { return (int)((n + kTile - 1) / kTile); }
@@ -828,7 +850,9 @@ int shape_of(const gtp_linear_rows* r, Shape& s, Rows& a) {
       (reinterpret_cast<uintptr_t>(r->weight) & 15u))
     return GTP_ERR_UNSUPPORTED;
   s.ldh = (r->K + 63) / 64 * 64;
-  s.ldn = s.N <= few::kMostRows ? (s.N + 63) / 64 * 64 : (s.N + 7) / 8 * 8;
+  // (few rows: D's two parts, 64 or 128 of them each)
+  s.low = s.N <= few::kMostRows ? (int)(s.N + 63) / 64 * 64 : 0;
+  s.ldn = s.low ? 2 * s.low : (s.N + 7) / 8 * 8;
   s.n_vt = tiles(r->V);
   s.n_tt = tiles(s.N);
   s.n_ct = tiles(s.K8);
@@ -872,13 +896,14 @@ struct Pieces {
 };
 Pieces pieces_of(const Shape& s, int64_t V, int64_t width) {
   Pieces p;
+  const int64_t rows = s.low ? s.low + s.N : s.N;
   const int64_t fit = max(kPieceBytes / (s.ldn * 2), (int64_t)kTile);
   const int64_t unit = fit >= 8 * kTile ? 8 * kTile : kTile;
   const int64_t most = fit / unit * unit, n = (V + most - 1) / most;
   p.rows = min(most, ((V + n - 1) / n + unit - 1) / unit * unit);
-  p.shares = Shares{s.n_ct, (int32_t)device_cus(), (min(p.rows, V) + kBK - 1) / kBK, width,
-                    32 * s.N};
-  p.shares.most = max(p.shares.best(s.N) * s.N, min(3 * s.N, ((int64_t)1 << 26) / width));
+  p.shares = Shares{s.n_ct, (int32_t)device_cus(), s.low, (min(p.rows, V) + kBK - 1) / kBK, width,
+                    32 * rows};
+  p.shares.most = max(p.shares.best(rows) * rows, min(3 * rows, ((int64_t)1 << 26) / width));
   return p;
 }
 
@@ -970,7 +995,8 @@ void grad_logits_launch(const gtp_linear_rows* r, const Shape& s, const Backward
 }
 
 template <typename E>
-void grad_hidden_launch(const gtp_linear_rows* r, const Shape& s, const Backward& b, int64_t v0,
+void grad_hidden_launch(const gtp_linear_rows* r, const Shape& s, const Pieces& p,
+                        const Backward& b, int64_t v0,
                         int64_t rows, hipStream_t st) {
   HiddenArgs a;
   a.d = Operand{b.d, s.ldn, s.ldn};
@@ -978,6 +1004,7 @@ void grad_hidden_launch(const gtp_linear_rows* r, const Shape& s, const Backward
   a.K = rows;
   a.meta = b.meta;
   a.sum = b.sum;
+  a.shares = p.shares;
   a.width = r->K;
   a.first = v0 == 0 ? 1 : 0;
   a.tn = s.n_ct;
@@ -1035,13 +1062,13 @@ void backward_launch(const gtp_linear_rows* r, const Shape& s, const Pieces& p, 
   for (int64_t v0 = 0; v0 < r->V; v0 += p.rows) {
     const int64_t rows = min(p.rows, r->V - v0);
     grad_logits_launch<E>(r, s, b, v0, rows, st);
-    if (grad_hidden) grad_hidden_launch<E>(r, s, b, v0, rows, st);
+    if (grad_hidden) grad_hidden_launch<E>(r, s, p, b, v0, rows, st);
     if (grad_weight) grad_weight_launch<E>(r, s, b, v0, rows, grad_weight, st);
   }
   if (grad_hidden)
     hipLaunchKernelGGL(grad_hidden_rows_kernel<E>,
                        dim3((unsigned)(r->B * r->S), (unsigned)((r->K + 1023) / 1024)), dim3(256), 0,
-                       st, b.sum, r->K, b.meta, b.slot, grad_hidden);
+                       st, b.sum, r->K, p.shares, b.meta, b.slot, grad_hidden);
 }
 
 }  // namespace lin

@@ -11,6 +11,11 @@
  *   2. gtp_logprob_entropy_rows / gtp_lse_partial_rows: the per-token
  *      selective log-softmax gather and the softmax entropy, fp32 accumulation.
  *
+ * and, at the end of this file, those of a training step around the vocabulary
+ * matrix: gtp_linear_logprob_* (token losses from hidden states with both
+ * gradients), gtp_embedding_* (the lookup and its table's gradient),
+ * gtp_grad_norm / gtp_clip_grads.
+ *
  * Conventions shared by every entry point:
  *   - All array pointers are DEVICE pointers owned by the caller.  The library
  *     never allocates and is reentrant, with one exception:

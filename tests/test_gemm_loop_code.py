@@ -98,12 +98,12 @@ def test_few_rows_stores_that_a_stage_leaves(every_kernel):
     found = {k: v for k, v in every_kernel.items() if "few_weight_kernel" in k and "Lb1" in k}
     assert len(found) == 4
     for name, body in found.items():
-        stores, blocks = (4, 8) if "ELi4E" in name else (2, 4)
+        stores, blocks = (4, 6) if "ELi4E" in name else (2, 3)
         at = [i for i, x in enumerate(body) if x.startswith("buffer_store_dwordx4")]
         loads = [i for i, x in enumerate(body) if x.startswith("buffer_load_dwordx4") and " lds" in x]
         # two stages, each with one loop over its blocks
-        assert len(at) == 2 * stores and len(loads) == 3 * 4, (name, len(at), len(loads))
-        assert loads[7] < at[0] and at[stores - 1] < loads[8] < at[stores], name
+        assert len(at) == 2 * stores and len(loads) == 3 * 6, (name, len(at), len(loads))
+        assert loads[11] < at[0] and at[stores - 1] < loads[12] < at[stores], name
         waits = [x for x in body if x.startswith("s_waitcnt vmcnt(%d) lgkmcnt(0)" % (stores * blocks))]
         assert len(waits) == 2, name
         assert not any(x.startswith("scratch") for x in body), name

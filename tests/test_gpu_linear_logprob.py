@@ -12,6 +12,8 @@ and w = 2^-24 (fp32):
 - an element of the logits' gradient d = g ([v = t] - p) is rounded once to
   the operands' type: u |d|, plus g p times twice the logits' error, plus, for
   fp16, half its smallest step at the power of two in it;
+- (up to 128 rows D is kept in two parts of the type, the second one rounded:
+  u^2 |d|, test_few_rows_keep_d_whole);
 - a gradient sums N or V such products in fp32 and is rounded once: n w
   sum|d||x| and u |result| (and half the smallest step of the type).
 """
@@ -45,8 +47,9 @@ def inputs(N, V, K, dtype, seed, spread=2.0):
     return h, w, t, grad
 
 
-def expect(h, w, t, g, dtype):
-    """(logprob, its bound, dh, its bound, dw, its bound) in 64 bits."""
+def expect(h, w, t, g, dtype, parts=1):
+    """(logprob, its bound, dh, its bound, dw, its bound) in 64 bits; D in
+    `parts` of the type."""
     u, K, V = half_step(dtype), h.shape[1], w.shape[0]
     h, w, g = h.double(), w.double(), g.double()
     x, mag = h @ w.T, h.abs() @ w.abs().T
@@ -57,7 +60,7 @@ def expect(h, w, t, g, dtype):
     p = (x - lse[:, None]).exp()
     d = -g[:, None] * p
     d.scatter_add_(1, t[:, None], g[:, None])
-    d_err = u * d.abs() + (1 + u) * g.abs()[:, None] * p * 2 * (x_err + 64 * W)[:, None]
+    d_err = u ** parts * d.abs() + (1 + u) * g.abs()[:, None] * p * 2 * (x_err + 64 * W)[:, None]
     # (1 - p and the product are fp32 operations too)
     d_err += 2 * W * g.abs()[:, None] * (t[:, None] == torch.arange(V, device=t.device)[None, :])
     if dtype == HF:
@@ -106,6 +109,17 @@ def test_logprob_and_gradients(N, V, K, dtype):
 ])
 def test_few_rows(N, V, K, dtype):
     test_logprob_and_gradients(N, V, K, dtype)
+
+
+@pytest.mark.parametrize("dtype", [BF, HF], ids=["bf16", "fp16"])
+@pytest.mark.parametrize("N", [1, 64, 65, 128])
+def test_few_rows_keep_d_whole(N, dtype):
+    h, w, t, g = inputs(N, 777, 96, dtype, seed=N)
+    _, _, gh, gh_e, gw, gw_e = expect(h, w, t, g, dtype, parts=2)
+    hd, wd = h.cuda().requires_grad_(), w.cuda().requires_grad_()
+    a, b = torch.autograd.grad(sequence_log_probs_from_hidden(hd, wd, t.cuda()), [hd, wd], g.cuda())
+    within(a.cpu(), gh, gh_e, "hidden's gradient")
+    within(b.cpu(), gw, gw_e, "weight's gradient")
 
 
 @pytest.mark.parametrize("N", [61, 100])
