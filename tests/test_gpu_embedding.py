@@ -253,6 +253,38 @@ def test_bad_ids(bad):
     assert bool((gw[:20][rest] == 1).all()) and bool((gw[4] == 0).all()) and bool((gw[20:] == 0).all())
 
 
+def test_a_table_past_32_bit_offsets():
+    V, H = (1 << 31) // 1024 + 1000, 1024
+    ids = torch.tensor([V - 1, 0, V - 2, (1 << 31) // 1024, V - 1], device="cuda")
+    w = torch.zeros(V, H, dtype=BF, device="cuda")
+    w[ids] = torch.arange(1.0, 6.0, device="cuda", dtype=BF)[:, None]
+    w[V - 1] = 7.0
+    w.requires_grad_()
+    out = token_embedding(ids, w)
+    assert out.detach()[:, 5].tolist() == [7.0, 2.0, 3.0, 4.0, 7.0]
+    (gw,) = torch.autograd.grad(out, [w], torch.ones_like(out))
+    assert gw[ids].float().mean(1).tolist() == [2.0, 1.0, 1.0, 1.0, 2.0]
+    gw[ids] = 0
+    assert not bool(gw.any())
+
+
+def test_one_order_on_two_streams():
+    ids, w = ids_of(3000, 500, 21).cuda(), torch.randn(500, 96, device="cuda")
+    grads = [torch.randn(3000, 96, device="cuda") for _ in range(2)]
+    order = ops.embedding_ordered(ids, w)[2]
+    want = [ops.embedding_backward(ids, g, 500) for g in grads]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(5):
+        for s, g in zip(streams, grads):
+            with torch.cuda.stream(s):
+                got.append(ops.embedding_backward(None, g, 500, order=order))
+    torch.cuda.synchronize()
+    for i, x in enumerate(got):
+        assert torch.equal(x, want[i % 2])
+
+
 def test_captured_and_replayed():
     N, V, H = 300, 700, 64
     ids = torch.zeros(N, dtype=torch.int64, device="cuda")

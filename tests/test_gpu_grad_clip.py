@@ -211,6 +211,14 @@ def test_views_of_a_bucket(dtype):
         assert torch.equal(bucket, alone)
 
 
+def test_a_tensor_past_32_bit_offsets():
+    n = (1 << 31) + 4099
+    x = torch.ones(n, dtype=BF, device="cuda")
+    norm = clip_grad_norm_([_as_param(x)], 0.25 * math.sqrt(n))
+    assert abs(float(norm) - math.sqrt(n)) <= 2 * W * math.sqrt(n)
+    assert bool((x == 0.25).all())
+
+
 def _as_param(g):
     p = torch.nn.Parameter(torch.zeros_like(g))
     p.grad = g

@@ -154,6 +154,46 @@ def test_few_rows_beside_a_masked_vocabulary_row():
         assert bool((gw[7] == 0).all()) and bool(gw.isfinite().all())
 
 
+@pytest.mark.parametrize("N", [3, 130])
+def test_a_weight_past_32_bit_offsets(N):
+    """Zero rows but a few: logits 0 there, so the sums are known."""
+    V, K = (1 << 31) // 4096 + 777, 4096
+    w = torch.zeros(V, K, dtype=BF, device="cuda")
+    rows = torch.tensor([0, 1 << 19, V - 300, V - 1], device="cuda")
+    g = torch.Generator().manual_seed(2)
+    w[rows] = (torch.randn(4, K, generator=g) * 0.05).to(BF).cuda()
+    h = torch.randn(N, K, generator=g).to(BF).cuda()
+    t = rows[torch.arange(N, device="cuda") % 4]
+    x = h.double() @ w[rows].double().T
+    lse = torch.log(x.exp().sum(1) + (V - 4))
+    grad = torch.linspace(0.5, 1.0, N, device="cuda")
+    hd, wd = h.requires_grad_(), w.requires_grad_()
+    lp = sequence_log_probs_from_hidden(hd, wd, t)
+    want = x[torch.arange(N), torch.arange(N) % 4] - lse
+    mag = (h.double().abs() @ w[rows].double().abs().T).amax(1)
+    err = 2 * (K * W * mag + 4 * W * (1 + x.abs().amax(1))) + 64 * W + 2 * W * want.abs()
+    within(lp.detach(), want.detach(), err.detach(), "logprob")
+    gh, gw = torch.autograd.grad(lp, [hd, wd], grad)
+    p = (x - lse[:, None]).exp().detach()
+    d = -p * grad[:, None]
+    d[torch.arange(N), torch.arange(N) % 4] += grad
+    u = half_step(BF)
+    d_err = u * d.abs() + (1 + u) * grad[:, None] * p * 2 * err.detach()[:, None] + 4 * W
+    tiny = torch.finfo(BF).smallest_normal * torch.finfo(BF).eps / 2
+    for got, a, e, b in ((gw[rows], d.T, d_err.T, h), (gh, d, d_err, w.detach()[rows])):
+        b = b.detach().double()
+        r = a @ b
+        e = e @ b.abs() + (V + N) * W * ((a.abs() + e) @ b.abs())
+        within(got, r, e + u * (r.abs() + e) + tiny, "gradient")
+    # a zero row's gradient: -sum g_n h_n / exp(lse_n); D is off by u and by
+    # twice the logprobs' error, the sum by N w, the result rounded once
+    one = gw[V - 2].double()
+    r = -(grad.double()[:, None] * h.detach().double() * (-lse.detach())[:, None].exp()).sum(0)
+    mag = (grad.double()[:, None] * h.detach().double().abs() * (-lse.detach())[:, None].exp()).sum(0)
+    rel = 2 * u + 2 * float(err.max()) + N * W
+    within(one, r, rel * mag + tiny, "a zero row's gradient")
+
+
 @pytest.mark.parametrize("dtype", [BF, HF], ids=["bf16", "fp16"])
 def test_mean_loss_skips_ignored(dtype):
     B, S, V, K = 3, 90, 611, 96

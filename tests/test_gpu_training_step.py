@@ -135,6 +135,35 @@ def test_steps_on_another_stream_repeat_to_the_bit():
         assert torch.equal(x, y) and bool(x.isfinite().all())
 
 
+def test_steps_of_two_streams_at_once():
+    """Neither waits for the other, and both get what they get alone."""
+    sizes = [(2, 80, 3000, 256), (1, 200, 1500, 384)]
+    made = []
+    for i, (B, S, V, H) in enumerate(sizes):
+        ids, w, grad = batch(B, S, V, H, BF, seed=60 + i)
+        made.append((ids.cuda(), w.cuda().requires_grad_(), grad.cuda()))
+
+    def step(ids, w, grad):
+        _, lp = policy(ids, w)
+        (g,) = torch.autograd.grad(lp, [w], grad)
+        p = torch.nn.Parameter(w.detach(), requires_grad=False)
+        p.grad = g
+        return lp.detach(), clip_grad_norm_([p], 1e-3), g
+
+    want = [[x.clone() for x in step(*m)] for m in made]
+    streams = [torch.cuda.Stream() for _ in made]
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(6):
+        for m, s in zip(made, streams):
+            with torch.cuda.stream(s):
+                got.append(step(*m))
+    torch.cuda.synchronize()
+    for i, out in enumerate(got):
+        for x, y in zip(out, want[i % 2]):
+            assert torch.equal(x, y)
+
+
 def test_step_captured_and_replayed():
     B, S, V, H = 2, 60, 700, 64
     ids = torch.zeros(B, S, dtype=torch.int64, device="cuda")
