@@ -13,8 +13,10 @@
 // caller's other torch work exactly as the reference's ATen ops did.
 #include <ATen/ATen.h>
 #include <ATen/EmptyTensor.h>
+#include <c10/core/impl/VirtualGuardImpl.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/variable.h>
 #include <torch/library.h>
 
 #include <algorithm>
@@ -929,6 +931,23 @@ at::Tensor once_only(at::Tensor grad, const at::Tensor& from, const char* what) 
       std::string(what) + " is differentiable once only", 1))({grad})[0];
 }
 
+// In a graph capture: the accumulator of a leaf's gradient runs on the stream
+// that it was made on, so while an eager graph of the leaf lives a captured
+// backward would leave the capture there, which ends the process.
+void check_leaf(const at::Tensor& leaf, const char* what, int64_t stream) {
+  if (!leaf.requires_grad() || !leaf.is_leaf() ||
+      !gtp_stream_capturing(reinterpret_cast<void*>(stream)))
+    return;
+  const auto node = torch::autograd::impl::try_get_grad_accumulator(leaf);
+  if (!node) return;
+  const auto made_on = node->stream();
+  const c10::Stream now =
+      c10::impl::VirtualGuardImpl(leaf.device().type()).getStream(leaf.device());
+  TORCH_CHECK(!made_on.has_value() || *made_on == now, what,
+              ": an eager graph of the same parameter is alive on another stream; a backward "
+              "cannot be captured beside it (drop the graph first)");
+}
+
 // linear_logprob() as a node of the C++ engine (8 tokens of 512, 32000 of the
 // vocabulary, forward and backward: 135 us with a Python function, 95 so).
 struct LinearLoss : torch::autograd::Function<LinearLoss> {
@@ -971,8 +990,10 @@ struct LinearLoss : torch::autograd::Function<LinearLoss> {
 at::Tensor linear_loss(const at::Tensor& hidden, const at::Tensor& weight,
                        const at::Tensor& targets, c10::optional<int64_t> ignore_index, bool mean,
                        std::string what, int64_t stream) {
-  if (at::GradMode::is_enabled() && (hidden.requires_grad() || weight.requires_grad()))
+  if (at::GradMode::is_enabled() && (hidden.requires_grad() || weight.requires_grad())) {
+    for (const at::Tensor* t : {&hidden, &weight}) check_leaf(*t, what.c_str(), stream);
     return LinearLoss::apply(hidden, weight, targets, ignore_index, mean, what, stream);
+  }
   auto [lp, lse, loss, count, bad] =
       linear_logprob(hidden, weight, targets, ignore_index, mean, stream);
   TORCH_CHECK(!bad, what, ": a target is outside [0, vocab_size)");
@@ -1123,8 +1144,10 @@ struct TokenEmbedding : torch::autograd::Function<TokenEmbedding> {
 
 at::Tensor token_embedding(const at::Tensor& ids, const at::Tensor& weight, double scale,
                            int64_t padding_idx, bool check, int64_t stream) {
-  if (at::GradMode::is_enabled() && weight.requires_grad())
+  if (at::GradMode::is_enabled() && weight.requires_grad()) {
+    check_leaf(weight, "token_embedding", stream);
     return TokenEmbedding::apply(ids, weight, scale, padding_idx, check, stream);
+  }
   auto [out, bad, order] = embedding(ids, weight, scale, check, false, padding_idx, stream);
   TORCH_CHECK(!bad, "token_embedding: an id is outside [0, vocab_size)");
   return out;

@@ -206,6 +206,36 @@ def test_step_captured_and_replayed():
                 assert torch.equal(a, b)
 
 
+def test_captures_beside_an_eager_graph_are_refused():
+    ids = torch.arange(8, device="cuda").view(2, 4)
+    w = torch.randn(20, 16, device="cuda").to(BF).requires_grad_()
+    calls = [lambda: token_embedding(ids, w), lambda: sequence_log_probs_from_hidden(hidden, w, ids)]
+    hidden = torch.randn(2, 4, 16, device="cuda").to(BF)
+    for call in calls:
+        eager = call()
+        seen = []
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            kept = hidden * 1.0  # (a graph is not captured empty)
+            try:
+                call()
+            except RuntimeError as e:
+                seen.append(str(e))
+        assert len(seen) == 1 and "eager graph" in seen[0]
+        del eager
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = call()
+            (g,) = torch.autograd.grad(out, [w], torch.ones_like(out))
+        for _ in range(2):
+            graph.replay()
+        torch.cuda.synchronize()
+        want_out = call()
+        (want,) = torch.autograd.grad(want_out, [w], torch.ones_like(want_out))
+        assert torch.equal(out.detach(), want_out.detach()) and torch.equal(g, want)
+        del out, want_out, kept
+
+
 def test_second_derivatives_are_refused():
     w = torch.randn(20, 8, device="cuda").requires_grad_()
     scale = torch.ones((), device="cuda", requires_grad=True)
