@@ -473,12 +473,13 @@ struct Order {
 };
 inline Order order(int64_t N, int64_t V, void* p) {
   uint32_t* w = reinterpret_cast<uint32_t*>(p);
+  auto at = [&](int64_t words) { return w ? w + words : nullptr; };
   Order o;
   for (int i = 0; i < 2; ++i) {
-    o.key[i] = w + 2 * i * N;
-    o.pos[i] = reinterpret_cast<int32_t*>(w + (2 * i + 1) * N);
+    o.key[i] = at(2 * i * N);
+    o.pos[i] = reinterpret_cast<int32_t*>(at((2 * i + 1) * N));
   }
-  o.rows = w + 4 * N;
+  o.rows = at(4 * N);
   o.bytes = N > 0 ? (size_t)(4 * N + (V + 31) / 32) * 4 : 0;
   return o;
 }

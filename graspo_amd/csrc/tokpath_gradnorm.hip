@@ -294,8 +294,8 @@ int plan_of(const void* const* p, const int64_t* n, const int32_t* dtype, int64_
     if (dtype[i] < GTP_DTYPE_F32 || dtype[i] > GTP_DTYPE_F16 || n[i] < 0 || (n[i] > 0 && !p[i]) ||
         (reinterpret_cast<uintptr_t>(p[i]) & (size_of(dtype[i]) - 1)))
       return GTP_ERR_INVALID_ARGUMENT;
-    if (n[i] >= kLongest) return GTP_ERR_UNSUPPORTED;
-    bytes += n[i] * size_of(dtype[i]);
+    bytes += n[i] < kLongest ? n[i] * size_of(dtype[i]) : 0;
+    if (n[i] >= kLongest || bytes > (int64_t)1 << 60) return GTP_ERR_UNSUPPORTED;
   }
   plan.chunk = 4096;
   while (bytes / 16 / plan.chunk > 8192) plan.chunk *= 2;

@@ -31,6 +31,102 @@ static int logprob_capi(const void* a, int b, int64_t c, int64_t d, int64_t e, c
   return gtp_logprob_entropy_rows(a, b, c, d, e, f, g, h, i, j, NULL);
 }
 
+/* Token losses from hidden states, the embedding and the clipping: one field
+ * after another out of range, sizes whose products would overflow. */
+static void training_step_cases(void) {
+  const int I = GTP_ERR_INVALID_ARGUMENT, X = GTP_ERR_UNSUPPORTED, OK = GTP_OK;
+  const char* w = "training step";
+  const int64_t M = INT64_MAX;
+  void* p = PH(void*);
+  float* f = PH(float*);
+  int64_t* c = PH(int64_t*);
+  const gtp_linear_rows good = {p, p, p, GTP_DTYPE_BF16, 1, 0, 0, 2, 8, 8, 64, 1000,
+                                512, 64, 64, 8, 1};
+  const size_t fwd = gtp_linear_logprob_workspace_bytes(&good);
+  const size_t bwd = gtp_linear_logprob_backward_workspace_bytes(&good);
+  EXPECT_RC(w, fwd > 0 && bwd > 0, 1);
+  EXPECT_RC(w, gtp_linear_logprob_rows(NULL, f, f, NULL, NULL, NULL, p, fwd, NULL), I);
+  EXPECT_RC(w, gtp_linear_logprob_rows(&good, NULL, f, NULL, NULL, NULL, p, fwd, NULL), I);
+  EXPECT_RC(w, gtp_linear_logprob_rows(&good, f, f, f, NULL, NULL, p, fwd, NULL), I);
+  EXPECT_RC(w, gtp_linear_logprob_rows(&good, f, f, NULL, NULL, NULL, NULL, fwd, NULL), I);
+  EXPECT_RC(w, gtp_linear_logprob_rows(&good, f, f, NULL, NULL, NULL, p, fwd - 1, NULL), I);
+  EXPECT_RC(w, gtp_linear_logprob_backward(&good, NULL, f, NULL, p, p, p, bwd, NULL), I);
+  EXPECT_RC(w, gtp_linear_logprob_backward(&good, f, NULL, c, p, p, p, bwd, NULL), I);
+  EXPECT_RC(w, gtp_linear_logprob_backward(&good, f, f, NULL, p, p, p, bwd - 1, NULL), I);
+#define LINEAR(field, value, rc)                                                          \
+  do {                                                                                    \
+    gtp_linear_rows r_ = good;                                                            \
+    r_.field = value;                                                                     \
+    EXPECT_RC(w, gtp_linear_logprob_rows(&r_, f, f, NULL, NULL, NULL, p, SIZE_MAX, NULL), rc); \
+    EXPECT_RC(w, gtp_linear_logprob_backward(&r_, f, f, NULL, p, p, p, SIZE_MAX, NULL), rc);   \
+    EXPECT_RC(w, gtp_linear_logprob_workspace_bytes(&r_) == 0, 1);                        \
+    EXPECT_RC(w, gtp_linear_logprob_backward_workspace_bytes(&r_) == 0, 1);               \
+  } while (0)
+  LINEAR(hidden, NULL, I);
+  LINEAR(weight, NULL, I);
+  LINEAR(targets, NULL, I);
+  LINEAR(B, -1, I);
+  LINEAR(S, -1, I);
+  LINEAR(T, 9, I);
+  LINEAR(K, 0, I);
+  LINEAR(V, 0, I);
+  LINEAR(hidden_batch_stride, -1, I);
+  LINEAR(target_row_stride, -1, I);
+  LINEAR(weight_stride, 63, I);
+  LINEAR(dtype, GTP_DTYPE_F32, X);
+  LINEAR(weight_stride, 68, X);
+  LINEAR(weight_stride, M - 7, X);
+  LINEAR(weight, (void*)(uintptr_t)0x18, X);
+  LINEAR(B, M, X);
+  LINEAR(S, M, X);
+  LINEAR(V, M, X);
+  LINEAR(V, 0x7FFFFFFF, X);
+#undef LINEAR
+
+  EXPECT_RC(w, gtp_embedding_rows(p, 1, 4, M, p, 1, 10, 8, 8, 1.0f, NULL, NULL), I);
+  EXPECT_RC(w, gtp_embedding_rows(p, 1, 4, -1, p, 1, 10, 8, 8, 1.0f, p, NULL), I);
+  EXPECT_RC(w, gtp_embedding_rows(p, 1, 4, 1, p, 1, 10, 8, 7, 1.0f, p, NULL), I);
+  EXPECT_RC(w, gtp_embedding_rows(p, 1, 4, 1, p, 1, 10, 8, M, 1.0f, p, NULL), X);
+  EXPECT_RC(w, gtp_embedding_rows(p, 1, M, 1, p, 1, 10, 8, 8, 1.0f, p, NULL), X);
+  EXPECT_RC(w, gtp_embedding_rows(p, 1, 4, 1, p, 1, M, 8, 8, 1.0f, p, NULL), X);
+  EXPECT_RC(w, gtp_embedding_rows(p, 1, 4, 1, p, 1, 10, M, M, 1.0f, p, NULL), X);
+  EXPECT_RC(w, gtp_embedding_rows(NULL, 1, 0, 1, NULL, 1, 10, 8, 8, 1.0f, NULL, NULL), OK);
+  EXPECT_RC(w, gtp_embedding_order_bytes(M, 10) == 0, 1);
+  EXPECT_RC(w, gtp_embedding_order_bytes(4, M) == 0, 1);
+  EXPECT_RC(w, gtp_embedding_backward_workspace_bytes(1, M, 10, 8) == 0, 1);
+  EXPECT_RC(w, gtp_embedding_backward_workspace_bytes(1, 4, M, M) == 0, 1);
+  EXPECT_RC(w, gtp_embedding_backward_ordered_workspace_bytes(1, 4, M) == 0, 1);
+  EXPECT_RC(w, gtp_embedding_rows_ordered(p, 1, 4, 1, p, 1, 10, 8, 8, 1.0f, p, -1, p, 3, NULL), I);
+  EXPECT_RC(w, gtp_embedding_rows_ordered(p, 1, 4, 1, p, 1, 10, 8, 8, 1.0f, p, -1, NULL, SIZE_MAX,
+                                          NULL), I);
+  EXPECT_RC(w, gtp_embedding_backward(p, 1, 4, 1, p, 1, 8, 10, 8, 1.0f, -1, 0, p, p, 3, NULL), I);
+  EXPECT_RC(w, gtp_embedding_backward(p, 1, 4, 1, p, 1, M, 10, 8, 1.0f, -1, 0, p, p, SIZE_MAX,
+                                      NULL), X);
+  EXPECT_RC(w, gtp_embedding_backward(p, 1, 4, 1, p, 1, 8, M, M, 1.0f, -1, 0, p, p, SIZE_MAX,
+                                      NULL), X);
+  EXPECT_RC(w, gtp_embedding_backward_ordered(p, 3, 4, p, 1, 8, 10, 8, 1.0f, 0, p, p, SIZE_MAX,
+                                              NULL), I);
+  EXPECT_RC(w, gtp_embedding_backward_ordered(p, SIZE_MAX, 4, p, 1, M, 10, 8, 1.0f, 0, p, p,
+                                              SIZE_MAX, NULL), X);
+
+  void* t[2] = {p, PH(void*)};
+  int64_t n[2] = {8, 8};
+  int32_t d[2] = {GTP_DTYPE_F32, GTP_DTYPE_BF16};
+  EXPECT_RC(w, gtp_grad_norm((const void* const*)t, n, d, 2, 2, f, p, 8, NULL), I);
+  EXPECT_RC(w, gtp_grad_norm((const void* const*)t, n, d, -1, 2, f, p, 64, NULL), I);
+  EXPECT_RC(w, gtp_grad_norm(NULL, n, d, 2, 2, f, p, 64, NULL), I);
+  EXPECT_RC(w, gtp_clip_grads(t, n, d, 2, NULL, 1.0f, NULL), I);
+  n[1] = -1;
+  EXPECT_RC(w, gtp_grad_norm((const void* const*)t, n, d, 2, 2, f, p, 64, NULL), I);
+  n[1] = M;
+  EXPECT_RC(w, gtp_grad_norm((const void* const*)t, n, d, 2, 2, f, p, 64, NULL), X);
+  EXPECT_RC(w, gtp_clip_grads(t, n, d, 2, f, 1.0f, NULL), X);
+  EXPECT_RC(w, gtp_grad_norm_workspace_bytes((const void* const*)t, n, d, 2) == 0, 1);
+  n[1] = 8;
+  d[1] = 7;
+  EXPECT_RC(w, gtp_clip_grads(t, n, d, 2, f, 1.0f, NULL), I);
+}
+
 int main(void) {
   const int I = GTP_ERR_INVALID_ARGUMENT, X = GTP_ERR_UNSUPPORTED, OK = GTP_OK;
   const char* w = "capi";
@@ -239,6 +335,8 @@ int main(void) {
   EXPECT_RC(w, gtp_softmax_grad_bf16_cols(F, 10, 4, 4, F, F, NULL, 0, h, 9, NULL), I);
   EXPECT_RC(w, gtp_softmax_grad_bf16_cols(F, 10, 4, 4, F, F, h, 4, h, 9, NULL), I);
   EXPECT_RC(w, gtp_softmax_grad_bf16_cols(F, 10, 4, 4, F, F, NULL, 0, h, INT64_MAX, NULL), X);
+
+  training_step_cases();
 
   EXPECT_RC(w, strstr(gtp_version(), "gfx950") != NULL, 1);
 
