@@ -1168,6 +1168,8 @@ struct GradList {
     n.reserve(tensors.size());
     dtype.reserve(tensors.size());
     for (const at::Tensor& t : tensors) {
+      TORCH_CHECK_VALUE(!t.is_sparse(), "graspo_tokpath.", what,
+                        ": sparse gradients are not supported");
       TORCH_CHECK(t.is_cuda(), "graspo_tokpath.", what, ": tensors must be on a GPU");
       check_same_device(tensors[0], t, "every tensor");
       const at::ScalarType s = t.scalar_type();
@@ -1191,11 +1193,14 @@ void check_apart(at::TensorList tensors) {
   bool sorted = true;
   for (const at::Tensor& t : tensors) {
     if (t.numel() == 0) continue;
-    int64_t span = 1;
-    for (int64_t d = 0; d < t.dim(); ++d) {
-      TORCH_CHECK(t.size(d) <= 1 || t.stride(d) != 0,
-                  "graspo_tokpath.clip_grads_: a tensor overlaps itself");
-      span += (t.size(d) - 1) * t.stride(d);
+    int64_t span = t.numel();
+    if (!t.is_contiguous()) {
+      span = 1;
+      for (int64_t d = 0; d < t.dim(); ++d) {
+        TORCH_CHECK(t.size(d) <= 1 || t.stride(d) != 0,
+                    "graspo_tokpath.clip_grads_: a tensor overlaps itself");
+        span += (t.size(d) - 1) * t.stride(d);
+      }
     }
     const uintptr_t a = reinterpret_cast<uintptr_t>(t.data_ptr());
     sorted = sorted && (at.empty() || at.back().first <= a);

@@ -249,6 +249,13 @@ def test_refused_types():
         get_total_norm([torch.zeros(3, device="cuda"), torch.zeros(3)])
 
 
+def test_sparse_gradients_are_refused():
+    dense = torch.ones(4, 4, device="cuda")
+    for tensors in ([dense.to_sparse()], [dense, dense.to_sparse()]):
+        with pytest.raises(ValueError, match="sparse"):
+            get_total_norm(tensors)
+
+
 def test_captured_and_replayed():
     shapes = [(300, 70), (5,), (33, 33)] * 70
     grads = [torch.zeros(s, device="cuda") for s in shapes]
