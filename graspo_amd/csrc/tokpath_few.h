@@ -10,9 +10,9 @@
 //
 // 61 rows of 4096, 151936 of the vocabulary, bf16 (1.24 GB; a plain read of it
 // in this pattern takes 225 us, a fill 190): the lse 411 us with the tiles and
-// 320 so (50 of them the write-back of what ran before), D 381 and 291, dw 385
-// and 269; forward and backward 1.39 and 1.14 ms.  At 127 rows 1.39 ms; the
-// tiles take 1.52 at 129.  (With D in one part 1.11 and 1.28 ms, and gradients
+// 320 so (50 of them the write-back of what ran before), D 381 and 286, dw 385
+// and 262; forward and backward 1.39 and 1.12 ms.  At 127 rows 1.37 ms; the
+// tiles take 1.50 at 129.  (With D in one part 1.11 and 1.28 ms, and gradients
 // off by 0.0024 instead of 0.0017: see few_grad_logits_kernel.)
 #pragma once
 #include "tokpath_gemm.h"
@@ -41,9 +41,8 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer(const uint16_t* p, int6
                                            (int)min(max(2 * count, (int64_t)0), (int64_t)0x7FFFFFF0),
                                            0x00020000);
 }
-template <int kAux>
 __device__ __forceinline__ uint4 load16(__amdgpu_buffer_rsrc_t b, uint32_t at) {
-  return __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(b, at, 0, kAux));
+  return __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(b, at, 0, 0));
 }
 
 // The workgroups begin at different stages and go round: all at the same one
@@ -84,13 +83,13 @@ struct Product {
       for (int s = 0; s < kS; ++s)
 #pragma unroll
         for (int x = 0; x < 2; ++x)
-          to[x][s] = load16<0>(w_buf, k0 + 32 * s + 8 * q < K ? w_at[x] + 2 * (k0 + 32 * s) : kNowhere);
+          to[x][s] = load16(w_buf, k0 + 32 * s + 8 * q < K ? w_at[x] + 2 * (k0 + 32 * s) : kNowhere);
     };
     auto load_h = [&](int k0) {
 #pragma unroll
       for (int i = 0; i < kLoads; ++i) {
         const int at = tid + i * kThreads, k = k0 + 8 * (at % kC);
-        hr[i] = load16<0>(h_buf, k < h.ld ? 2 * (uint32_t)(at / kC * h.ld + k) : kNowhere);
+        hr[i] = load16(h_buf, k < h.ld ? 2 * (uint32_t)(at / kC * h.ld + k) : kNowhere);
       }
     };
     auto store_h = [&](uint4* to) {

@@ -380,7 +380,7 @@ __global__ __launch_bounds__(few::kThreads, 2) void few_lse_kernel(LseArgs a) {
   __shared__ float2 s_ms[few::kWaves][kTok];
   const int n = a.meta->n;
   if (n == 0) return;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t first = (int64_t)blockIdx.x * few::kRows + wave * few::kWaveRows;
   few::Product<E, kNB, false> x;
   x.run(a.w, first, a.h, n, a.K, s_h);
@@ -605,7 +605,8 @@ __global__ __launch_bounds__(few::kThreads, 2) void few_grad_logits_kernel(GradA
   __shared__ __attribute__((aligned(16))) uint4 s_h[2][kTok * few::kChunks<kNB>];
   __shared__ __attribute__((aligned(16))) float s_lse[kTok], s_g[kTok];
   __shared__ __attribute__((aligned(16))) int s_t[kTok];
-  const int n = a.meta->n, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int n = a.meta->n, lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   if (threadIdx.x < kTok) {  // (the product's barriers publish them)
     const int k = threadIdx.x;
     s_lse[k] = k < n ? a.rows.lse[k] : kPosInf;

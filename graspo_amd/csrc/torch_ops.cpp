@@ -5,8 +5,8 @@
 // verdict_end, logprob_backward, graspo_loss_*, lse_partial, lse_finalize,
 // decode_update, to_bf16_exact, logprob_backward_split, time_next_launch,
 // lm_head_logprob, lm_head_logprob_save, softmax_grad_bf16, linear_logprob,
-// linear_logprob_backward, embedding, embedding_backward, grad_norm,
-// clip_grads_, clip_grad_norm_}.  Each op validates
+// linear_logprob_backward, linear_loss, embedding, embedding_backward,
+// token_embedding, grad_norm, clip_grads_, clip_grad_norm_}.  Each op validates
 // its tensors (TORCH_CHECK surfaces as a Python RuntimeError), allocates the
 // outputs on the logits' device, and enqueues the HIP kernels on the stream handle passed in from Python
 // (torch.cuda.current_stream().cuda_stream), so work orders with the

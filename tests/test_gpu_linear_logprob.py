@@ -223,6 +223,34 @@ def test_mean_loss_skips_ignored(dtype):
     within(b.cpu(), gw, gw_e, "weight's gradient")
 
 
+@pytest.mark.parametrize("dtype", [BF, HF], ids=["bf16", "fp16"])
+@pytest.mark.parametrize("B,S,drop", [(2, 41, 30), (1, 129, 5), (4, 2, 0), (3, 30, 86)])
+def test_mean_loss_of_few_rows(B, S, drop, dtype):
+    """`drop` of the B x (S - 1) positions ignored, at random."""
+    V, K = 700, 72
+    h, w, t, _ = inputs(B * (S - 1), V, K, dtype, seed=B + S)
+    keep = torch.ones(B * (S - 1), dtype=torch.bool)
+    keep[torch.randperm(B * (S - 1), generator=torch.Generator().manual_seed(1))[:drop]] = False
+    labels = torch.zeros(B, S, dtype=torch.int64)
+    labels[:, 1:] = torch.where(keep, t, -100).view(B, S - 1)
+    g = torch.where(keep, -1.0 / keep.sum(), 0.0)
+    lp, lp_e, gh, gh_e, gw, gw_e = expect(h, w, t, g, dtype, parts=2)
+    hd = torch.full((B, S, K), float("nan"), dtype=dtype)
+    hd[:, :-1] = torch.where(keep[:, None], h, torch.full_like(h, float("nan"))).view(B, S - 1, K)
+    hd, wd = hd.cuda().requires_grad_(), w.cuda().requires_grad_()
+    loss = sft_cross_entropy_loss_from_hidden(hd, wd, labels.cuda())
+    want = -(lp[keep].sum() / keep.sum())
+    assert abs(float(loss.detach()) - float(want)) <= float(lp_e[keep].mean()) + 2 * W * abs(float(want))
+    a, b = torch.autograd.grad(loss, [hd, wd])
+    assert bool((a[:, -1] == 0).all())
+    a = a[:, :-1].reshape(-1, K).cpu()
+    assert bool((a[~keep] == 0).all())
+    # (the mean's gradient is divided and multiplied in fp32: 2 w more)
+    more = 2 * W
+    within(a[keep], gh[keep], (gh_e + more * gh.abs())[keep], "hidden's gradient")
+    within(b.cpu(), gw, gw_e + more * gw.abs(), "weight's gradient")
+
+
 def test_scaled_loss_gradient():
     """The loss's own gradient scales both gradients."""
     h, w, t, _ = inputs(50, 300, 64, BF, seed=9)
