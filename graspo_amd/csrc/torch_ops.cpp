@@ -932,8 +932,9 @@ at::Tensor once_only(at::Tensor grad, const at::Tensor& from, const char* what) 
 }
 
 // In a graph capture: the accumulator of a leaf's gradient runs on the stream
-// that it was made on, so while an eager graph of the leaf lives a captured
-// backward would leave the capture there, which ends the process.
+// that it was made on, so while an eager graph of the leaf lives that was made
+// on the default stream, which cannot join a capture, a captured backward ends
+// the process.  (Another stream joins it.)
 void check_leaf(const at::Tensor& leaf, const char* what, int64_t stream) {
   if (!leaf.requires_grad() || !leaf.is_leaf() ||
       !gtp_stream_capturing(reinterpret_cast<void*>(stream)))
@@ -941,10 +942,9 @@ void check_leaf(const at::Tensor& leaf, const char* what, int64_t stream) {
   const auto node = torch::autograd::impl::try_get_grad_accumulator(leaf);
   if (!node) return;
   const auto made_on = node->stream();
-  const c10::Stream now =
-      c10::impl::VirtualGuardImpl(leaf.device().type()).getStream(leaf.device());
-  TORCH_CHECK(!made_on.has_value() || *made_on == now, what,
-              ": an eager graph of the same parameter is alive on another stream; a backward "
+  const c10::impl::VirtualGuardImpl streams(leaf.device().type());
+  TORCH_CHECK(!made_on.has_value() || *made_on != streams.getDefaultStream(leaf.device()), what,
+              ": an eager graph of the same parameter is alive on the default stream; a backward "
               "cannot be captured beside it (drop the graph first)");
 }
 

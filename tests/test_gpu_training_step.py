@@ -223,6 +223,11 @@ def test_captures_beside_an_eager_graph_are_refused():
                 seen.append(str(e))
         assert len(seen) == 1 and "eager graph" in seen[0]
         del eager
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):  # one that a capture may join
+            beside = call()
+        torch.cuda.synchronize()
         graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(graph):
             out = call()
@@ -233,7 +238,7 @@ def test_captures_beside_an_eager_graph_are_refused():
         want_out = call()
         (want,) = torch.autograd.grad(want_out, [w], torch.ones_like(want_out))
         assert torch.equal(out.detach(), want_out.detach()) and torch.equal(g, want)
-        del out, want_out, kept
+        del out, want_out, kept, beside
 
 
 def test_second_derivatives_are_refused():
