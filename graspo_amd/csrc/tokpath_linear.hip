@@ -186,7 +186,8 @@ __global__ __launch_bounds__(kListBlock) void list_rows_kernel(
   float scale = 1.0f, inv = 1.0f;
   if (mean_count) {
     scale = scaled ? 16384.0f : 1.0f;
-    inv = gm / scale;
+    // (without a row gm is -g / 0, and both gradients are zeros times this)
+    inv = all ? gm / scale : 0.0f;
   } else if (scaled && top > 0.0f && top < kPosInf) {
     int e;
     frexpf(top, &e);

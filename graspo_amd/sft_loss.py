@@ -71,9 +71,10 @@ def sft_cross_entropy_loss_from_hidden(
     positions 0 .. S - 2 against ``labels[:, 1:]``, skipping ``ignore_index``
     (such positions take no part in any product).  ``hidden_states`` [B, S, K]
     and ``lm_head_weight`` [V, K] in bf16 or fp16; the loss is an fp32 scalar,
-    differentiable in both.  A label outside [0, V) raises ``RuntimeError``
-    (in a graph capture, where nothing waits for the labels, it makes the loss
-    NaN)."""
+    differentiable in both; with every position ignored it is NaN and its
+    gradients are zeros, as ``F.cross_entropy``'s.  A label outside [0, V)
+    raises ``RuntimeError`` (in a graph capture, where nothing waits for the
+    labels, it makes the loss NaN)."""
     what = "sft_cross_entropy_loss_from_hidden"
     check_operands(what, hidden_states, lm_head_weight)
     if hidden_states.dim() != 3 or labels.shape != hidden_states.shape[:2]:

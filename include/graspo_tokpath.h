@@ -652,6 +652,7 @@ int gtp_linear_logprob_rows(const gtp_linear_rows* rows, float* out_logprob, flo
  * (grad fp32 [B * T]; with mean_count, as the forward wrote it, grad[0] times
  * the mean loss): grad_hidden [B, S, K] and grad_weight [V, K], contiguous,
  * of the operands' type, either NULL.  lse: the forward's.  Needs B * T > 0.
+ * A mean over no row has gradients of zeros.
  */
 size_t gtp_linear_logprob_backward_workspace_bytes(const gtp_linear_rows* rows);
 int gtp_linear_logprob_backward(const gtp_linear_rows* rows, const float* lse, const float* grad,
