@@ -750,7 +750,8 @@ __global__ __launch_bounds__(256) void grad_hidden_rows_kernel(const float* __re
   }
 #pragma unroll
   for (int i = 0; i < 4; ++i)
-    if (c0 + i * 256 < width) to[c0 + i * 256] = E::from(v[i] * inv);
+    // (inv is the mean's gradient, which may be infinite or NaN)
+    if (c0 + i * 256 < width) to[c0 + i * 256] = E::from(k >= 0 ? v[i] * inv : 0.0f);
 }
 
 struct WeightArgs {

@@ -7,7 +7,7 @@ from __future__ import annotations
 import pytest
 import torch
 
-from graspo_amd.sft_loss import sft_cross_entropy_loss_from_hidden
+from graspo_amd.sft_loss import sft_cross_entropy_loss, sft_cross_entropy_loss_from_hidden
 
 pytestmark = pytest.mark.gpu
 
@@ -39,3 +39,22 @@ def test_a_mean_without_a_row_has_zero_gradients(B, S, dtype):
     w.grad = held.clone()
     sft_cross_entropy_loss_from_hidden(h, w, labels).backward()
     assert torch.equal(w.grad, held)
+
+
+@pytest.mark.parametrize("dtype", [BF, HF], ids=["bf16", "fp16"])
+@pytest.mark.parametrize("B,S", SHAPES)
+def test_ignored_positions_stay_zero_beside_a_gradient_that_is_not_finite(B, S, dtype):
+    """A loss scale that overflows spoils the rows that take part, not the
+    hidden states of those that do not: as the loss from logits has it."""
+    h, w, labels = step(B, S, dtype)
+    labels[:, S // 2:] = -100
+    live = torch.zeros(B, S, dtype=torch.bool, device="cuda")
+    live[:, :-1] = labels[:, 1:] != -100
+    for v in (float("inf"), float("-inf"), float("nan")):
+        g = torch.tensor(v, device="cuda")
+        gh, gw = torch.autograd.grad(sft_cross_entropy_loss_from_hidden(h, w, labels), [h, w], g)
+        assert bool((gh[~live] == 0).all())
+        assert not bool(gh[live].isfinite().any()) and not bool(gw.isfinite().any())
+        logits = (h.float() @ w.float().t()).detach().requires_grad_()
+        (gx,) = torch.autograd.grad(sft_cross_entropy_loss(logits, labels), [logits], g)
+        assert bool((gx[~live] == 0).all()) and not bool(gx[live].isfinite().any())
