@@ -479,11 +479,20 @@ __global__ __launch_bounds__(1024) void mean_kernel(const Meta* __restrict__ met
 // in a row per x by `value(x, e)`, written to `out` (row stride ld) in whole
 // 256-byte runs: through 4 KB of LDS of the wave's own, whose 16-byte chunks
 // are XOR-swizzled by the row.  `rows` and `cols` bound what is written; vec:
-// 16-byte stores (else 2-byte ones).
+// 16-byte stores (else 2-byte ones).  kLive: columns from `live` on get zeros,
+// whatever value() made of them.
 constexpr int kStoreLds = 256;  // chunks per wave
-template <typename Value>
+// the first n of 8 values, zeros behind
+__device__ __forceinline__ uint4 first_of(uint4 v, int64_t n) {
+  uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) w[i] = n >= 2 * i + 2 ? w[i] : n == 2 * i + 1 ? w[i] & 0xFFFFu : 0u;
+  return uint4{w[0], w[1], w[2], w[3]};
+}
+template <bool kLive, typename Value>
 __device__ __forceinline__ void store_block(uint4* mine, int lane, uint16_t* out, int64_t ld,
-                                            int64_t rows, int64_t cols, bool vec, Value value) {
+                                            int64_t rows, int64_t cols, int64_t live, bool vec,
+                                            Value value) {
   const int row = lane & 15;
   uint2* half = reinterpret_cast<uint2*>(mine);
 #pragma unroll
@@ -499,9 +508,10 @@ __device__ __forceinline__ void store_block(uint4* mine, int lane, uint16_t* out
 #pragma unroll
   for (int q = 0; q < 4; ++q) {
     const int r = q * 4 + (lane >> 4);
-    const uint4 v = mine[r * 16 + (c ^ r)];
+    uint4 v = mine[r * 16 + (c ^ r)];
     if (r < rows && col < cols) {
       uint16_t* to = out + r * ld + col;
+      if (kLive && col + 8 > live) v = first_of(v, live - col);
       if (vec) {
         *reinterpret_cast<uint4*>(to) = v;
       } else {
@@ -526,7 +536,10 @@ struct GradArgs {
 };
 
 // The piece's D: tokens x vocabulary, lane l of a block holding vocabulary row
-// l & 15 and 4 tokens, whose lse, g and targets are in LDS.
+// l & 15 and 4 tokens, whose lse, g and targets are in LDS.  Past the last
+// listed row D is 0, also where the weight holds an infinity (0 * inf is a NaN
+// logit there): dw reads D in chunks of 8 and multiplies what lies past the
+// last row by zeros.
 template <typename E>
 __global__ __launch_bounds__(kThreads, 1) void grad_logits_kernel(GradArgs a) {
   GTP_LOOP_LDS;
@@ -562,7 +575,7 @@ __global__ __launch_bounds__(kThreads, 1) void grad_logits_kernel(GradArgs a) {
     {
       const int64_t k = (int64_t)tt * kTile + threadIdx.x;
       const bool in = k < n_listed;
-      // a row past the last: exp(x - inf) = 0, times 0
+      // a row past the last: any value (its column is written as zeros)
       s_lse[odd][threadIdx.x] = in ? a.rows.lse[k] : kPosInf;
       s_g[odd][threadIdx.x] = in ? a.rows.g[k] : 0.0f;
       s_t[odd][threadIdx.x] = in ? (int)(a.rows.target[k] - a.v_first) : -1;
@@ -572,8 +585,9 @@ __global__ __launch_bounds__(kThreads, 1) void grad_logits_kernel(GradArgs a) {
     for (int y = 0; y < kB; ++y) {
         const int row0 = vt * kTile + wv * 128 + y * 16, v = row0 + (lane & 15);
         const int64_t col0 = (int64_t)tt * kTile + wt * 128;
-        store_block(s_out + wave * kStoreLds, lane, a.d + row0 * a.ldn + col0, a.ldn,
-                    a.w.outer - row0, a.ldn - col0, true, [&](int x, uint16_t (&e)[4]) {
+        store_block<true>(s_out + wave * kStoreLds, lane, a.d + row0 * a.ldn + col0, a.ldn,
+                          a.w.outer - row0, a.ldn - col0, n_listed - col0, true,
+                    [&](int x, uint16_t (&e)[4]) {
                       const int t0 = wt * 128 + x * 16 + 4 * (lane >> 4);
                       const float4 l = *reinterpret_cast<const float4*>(&s_lse[odd][t0]);
                       const float4 g = *reinterpret_cast<const float4*>(&s_g[odd][t0]);
@@ -797,8 +811,9 @@ __global__ __launch_bounds__(kThreads, 1) void grad_weight_kernel(WeightArgs a) 
     for (int y = 0; y < kB; ++y) {
         const int64_t row0 = (int64_t)vt * kTile + wv * 128 + y * 16;
         const int64_t col0 = (int64_t)ct * kTile + wc * 128;
-        store_block(s_out + wave * kStoreLds, lane, a.out + row0 * a.ld + col0, a.ld,
-                    a.d.outer - row0, a.width - col0, a.vec, [&](int x, uint16_t (&e)[4]) {
+        store_block<false>(s_out + wave * kStoreLds, lane, a.out + row0 * a.ld + col0, a.ld,
+                           a.d.outer - row0, a.width - col0, 0, a.vec,
+                    [&](int x, uint16_t (&e)[4]) {
 #pragma unroll
                       for (int i = 0; i < 4; ++i)
                         e[i] = E::from(acc_read(loop.acc[x][y][i]) * inv);
