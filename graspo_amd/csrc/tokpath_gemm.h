@@ -18,9 +18,9 @@
 //   16-byte chunks are XOR-swizzled by 4 (row & 3) + 2 (row / 8 & 1), so that
 //   the 8 rows x 32 bytes that half a wave reads take all 64 banks.
 //
-// Nothing past an operand's rows or its K is read: the buffer resource ends
-// with the last valid row, a chunk past K gets an offset past that end, and a
-// load out of range writes zeros to LDS.
+// Nothing past an operand's rows or its K (in whole chunks) is read: the buffer
+// resource ends with the last valid row's K, a chunk past K gets an offset past
+// that end, and a load out of range writes zeros to LDS.
 //
 // What bounds it: the part's power (the library's product keeps the matrix
 // cores busy 93% of the cycles, at 1.58 GHz).  At 8192 x 4096 x 131072 the four
@@ -132,12 +132,18 @@ struct Cursor {
 // Of the tile whose first row (kAlongK) or column (kAcrossK) is `first`, for K
 // values of K from k_first (a multiple of 8) on.
 template <Layout L>
-__device__ __forceinline__ Cursor cursor_of(const Operand& o, int64_t first, int64_t k_first,
-                                            int64_t K) {
-  const int64_t ld = o.ld * 2, outer = max((int64_t)0, o.outer - first);
+__host__ __device__ __forceinline__ Cursor cursor_of(const Operand& o, int64_t first,
+                                                     int64_t k_first, int64_t K) {
+  // (HIP's min and max are those of int on the host)
+  const int64_t ld = o.ld * 2, outer = o.outer > first ? o.outer - first : 0;
   if constexpr (L == kAlongK)
+    // (the last row ends with its K's last chunk: a wider row's gap behind it
+    // may lie past the end of the memory)
     return Cursor{reinterpret_cast<const char*>(o.p) + first * ld + k_first * 2,
-                  min((int64_t)kTile, outer) * ld - k_first * 2, (int)K};
+                  outer > 0 && K > 0
+                      ? ((outer < kTile ? outer : kTile) - 1) * ld + (K + 7) / 8 * 16
+                      : 0,
+                  (int)K};
   else
     return Cursor{reinterpret_cast<const char*>(o.p + first) + k_first * ld,
                   outer > 0 && K > 0 ? (K - 1) * ld + outer * 2 : 0, (int)K};
@@ -155,7 +161,7 @@ struct Source {
   int64_t advance;   // bytes from step to step
 
   // part of parts: this workgroup's share of the lines
-  __device__ __forceinline__ Source(int64_t ld_elements, int parts, int part, int wave, int lane)
+  __host__ __device__ __forceinline__ Source(int64_t ld_elements, int parts, int part, int wave, int lane)
       : c{nullptr, 0, 0} {
     const int64_t ld = ld_elements * 2;
     if constexpr (L == kAlongK) {
@@ -192,11 +198,11 @@ struct Source {
     int bytes;
     uint32_t v[2][2];
   };
-  __device__ __forceinline__ int bytes_left() const {
-    return (int)max((int64_t)0, min(c.left, (int64_t)kPast));
+  __host__ __device__ __forceinline__ int bytes_left() const {
+    return (int)(uint32_t)(c.left < 0 ? 0 : c.left < (int64_t)kPast ? c.left : (int64_t)kPast);
   }
   // The next step; past the last one all its loads are out of range.
-  __device__ __forceinline__ Step next() {
+  __host__ __device__ __forceinline__ Step next() {
     Step s{c.at, bytes_left(), {{v[0][0], v[0][1]}, {v[1][0], v[1][1]}}};
     if constexpr (L == kAlongK) {
       s.v[0][0] = s.v[0][1] = c0 < c.k_left ? v[0][0] : kPast;
@@ -207,18 +213,25 @@ struct Source {
     c.left -= advance;
     return s;
   }
+  __host__ __device__ __forceinline__ uint32_t offset(const Step& s, int q) const {
+    return s.v[q & 1][q >> 2] + (uint32_t)q * qstep;
+  }
   // the whole offset goes in the VGPR operand: the range check covers it
   __device__ __forceinline__ void issue(const Step& s, int q, uint4* stage, int wave) const {
     const __amdgpu_buffer_rsrc_t r =
         __builtin_amdgcn_make_buffer_rsrc((void*)s.base, (short)0, s.bytes, kRsrcWord3);
     __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_void*)(stage + (wave * kQ + q) * 64), 16,
-                                             s.v[q & 1][q >> 2] + (uint32_t)q * qstep, 0, 0, 0);
+                                             offset(s, q), 0, 0, 0);
+  }
+  // (a tile's last step may begin past K: the number of steps is even)
+  __host__ __device__ __forceinline__ int ahead_bytes() const {
+    return L == kAlongK && c.k_left <= 0 ? 0 : bytes_left();
   }
   // The lines of the step that next() will give, into L2 (4 bytes of each go
   // to LDS that nothing reads: a load without a register).
   __device__ __forceinline__ void ahead(uint32_t* unread, int wave) const {
     const __amdgpu_buffer_rsrc_t r =
-        __builtin_amdgcn_make_buffer_rsrc((void*)c.at, (short)0, bytes_left(), kRsrcWord3);
+        __builtin_amdgcn_make_buffer_rsrc((void*)c.at, (short)0, ahead_bytes(), kRsrcWord3);
     __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_void*)(unread + wave * 64), 4, line, 0, 0, 0);
   }
 };
