@@ -13,6 +13,7 @@
 // caller's other torch work exactly as the reference's ATen ops did.
 #include <ATen/ATen.h>
 #include <ATen/EmptyTensor.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/impl/VirtualGuardImpl.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
@@ -931,6 +932,13 @@ at::Tensor once_only(at::Tensor grad, const at::Tensor& from, const char* what) 
       std::string(what) + " is differentiable once only", 1))({grad})[0];
 }
 
+// The nodes have no forward-mode derivative: an operand with a tangent is
+// refused, which a call that needs no backward would drop without a word.
+void check_no_tangent(const at::Tensor& t, const char* what) {
+  TORCH_CHECK(!c10::AutogradState::get_tls_state().get_fw_grad_mode() || !t._fw_grad(0).defined(),
+              what, ": forward-mode derivatives are not supported");
+}
+
 // In a graph capture: the accumulator of a leaf's gradient runs on the stream
 // that it was made on, so while an eager graph of the leaf lives that was made
 // on the default stream, which cannot join a capture, a captured backward ends
@@ -968,6 +976,8 @@ struct LinearLoss : torch::autograd::Function<LinearLoss> {
   }
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
                                                  torch::autograd::variable_list grads) {
+    const char* what = "a token loss from hidden states";
+    check_no_tangent(grads[0], what);
     const auto saved = ctx->get_saved_variables();
     c10::optional<int64_t> ignore_index;
     if (ctx->saved_data["has_ignore"].toBool()) ignore_index = ctx->saved_data["ignore_index"].toInt();
@@ -979,7 +989,6 @@ struct LinearLoss : torch::autograd::Function<LinearLoss> {
         saved[0].detach(), saved[1].detach(), saved[2], saved[3],
         grads[0].detach().to(at::kFloat).contiguous(), count, ignore_index, need_hidden,
         need_weight, ctx->saved_data["stream"].toInt());
-    const char* what = "a token loss from hidden states";
     return {need_hidden ? once_only(gh, grads[0], what) : at::Tensor(),
             need_weight ? once_only(gw, grads[0], what) : at::Tensor(),
             at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()};
@@ -990,6 +999,7 @@ struct LinearLoss : torch::autograd::Function<LinearLoss> {
 at::Tensor linear_loss(const at::Tensor& hidden, const at::Tensor& weight,
                        const at::Tensor& targets, c10::optional<int64_t> ignore_index, bool mean,
                        std::string what, int64_t stream) {
+  for (const at::Tensor* t : {&hidden, &weight}) check_no_tangent(*t, what.c_str());
   if (at::GradMode::is_enabled() && (hidden.requires_grad() || weight.requires_grad())) {
     for (const at::Tensor* t : {&hidden, &weight}) check_leaf(*t, what.c_str(), stream);
     return LinearLoss::apply(hidden, weight, targets, ignore_index, mean, what, stream);
@@ -1132,6 +1142,7 @@ struct TokenEmbedding : torch::autograd::Function<TokenEmbedding> {
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
                                                  torch::autograd::variable_list grads) {
     const at::Tensor& grad = grads[0];
+    check_no_tangent(grad, "token_embedding");
     // (the engine runs a node on its forward's stream)
     at::Tensor out = embedding_backward(
         c10::nullopt, grad.detach(), ctx->saved_data["vocab"].toInt(),
@@ -1144,6 +1155,7 @@ struct TokenEmbedding : torch::autograd::Function<TokenEmbedding> {
 
 at::Tensor token_embedding(const at::Tensor& ids, const at::Tensor& weight, double scale,
                            int64_t padding_idx, bool check, int64_t stream) {
+  check_no_tangent(weight, "token_embedding");
   if (at::GradMode::is_enabled() && weight.requires_grad()) {
     check_leaf(weight, "token_embedding", stream);
     return TokenEmbedding::apply(ids, weight, scale, padding_idx, check, stream);

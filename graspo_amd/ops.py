@@ -357,7 +357,7 @@ def linear_loss(hidden: torch.Tensor, weight: torch.Tensor, targets: torch.Tenso
                 ignore_index: int | None = None, mean: bool = False,
                 what: str = "linear_loss") -> torch.Tensor:
     """:func:`linear_logprob`'s logprobs, or their mean loss, differentiable
-    (once) in both operands.  A bad target raises ``RuntimeError`` (in a graph
+    (once, backwards) in both operands.  A bad target raises ``RuntimeError`` (in a graph
     capture its logprob, and the mean, is NaN)."""
     return load().linear_loss(hidden, weight, _targets(targets), ignore_index, mean, what,
                               _stream(hidden))
@@ -393,8 +393,8 @@ def embedding_ordered(ids: torch.Tensor, weight: torch.Tensor, *, scale: float =
 
 def token_embedding(ids: torch.Tensor, weight: torch.Tensor, *, scale: float = 1.0,
                     padding_idx: int | None = None, check: bool = True) -> torch.Tensor:
-    """:func:`embedding`'s rows, differentiable (once) in ``weight``; a bad id
-    that ``check`` finds raises ``RuntimeError``."""
+    """:func:`embedding`'s rows, differentiable (once, backwards) in
+    ``weight``; a bad id that ``check`` finds raises ``RuntimeError``."""
     pad = _padding("token_embedding", padding_idx, weight.shape[0])
     return load().token_embedding(_targets(ids), weight, float(scale), pad, check,
                                   _stream(weight))
