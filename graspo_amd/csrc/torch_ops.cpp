@@ -1035,7 +1035,11 @@ std::tuple<at::Tensor, bool, at::Tensor> embedding(const at::Tensor& ids_, const
   void* st = reinterpret_cast<void*>(stream);
   auto shape = ids_.sizes().vec();
   shape.push_back(H);
+  // (what may raise comes before the look's launch: see verdict_wait)
+  const int dt = dtype_code(w);
   at::Tensor out = at::empty(shape, weight.options());
+  const size_t order_bytes = ordered ? gtp_embedding_order_bytes(N, V) : 0;
+  at::Tensor order = at::empty({(int64_t)order_bytes / 4}, weight.options().dtype(at::kInt));
   const int ids64 = ids.scalar_type() == at::kLong;
   const int64_t ids_stride = N > 1 ? ids.stride(0) : 1;
   at::Tensor words;
@@ -1048,14 +1052,12 @@ std::tuple<at::Tensor, bool, at::Tensor> embedding(const at::Tensor& ids_, const
     check_rc(rc, "gtp_targets_verdict");
   }
   const int64_t ld = V > 1 ? w.stride(0) : H;
-  const size_t order_bytes = ordered ? gtp_embedding_order_bytes(N, V) : 0;
-  at::Tensor order = at::empty({(int64_t)order_bytes / 4}, weight.options().dtype(at::kInt));
   const int rc =
       ordered ? gtp_embedding_rows_ordered(ids.data_ptr(), ids64, N, ids_stride, w.data_ptr(),
-                                           dtype_code(w), V, H, ld, (float)scale, out.data_ptr(),
+                                           dt, V, H, ld, (float)scale, out.data_ptr(),
                                            padding_idx, order.data_ptr(), order_bytes, st)
               : gtp_embedding_rows(ids.data_ptr(), ids64, N, ids_stride, w.data_ptr(),
-                                   dtype_code(w), V, H, ld, (float)scale, out.data_ptr(), st);
+                                   dt, V, H, ld, (float)scale, out.data_ptr(), st);
   int bad = 0, wait_rc = GTP_OK;
   if (words.defined()) wait_rc = verdict_wait(words, &bad, st);
   check_rc(rc, "gtp_embedding_rows");
