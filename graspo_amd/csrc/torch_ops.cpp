@@ -1065,6 +1065,12 @@ std::tuple<at::Tensor, bool, at::Tensor> embedding(const at::Tensor& ids_, const
   return {out, (bad & 1) != 0, order};
 }
 
+// A tensor written through its pointer counts as written: a graph that saved
+// it raises then.  (One made in inference mode has no counter.)
+void count_write(const at::Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 // The gradient of the table from that of embedding()'s rows; out: added to.
 // order: embedding()'s, in the ids' place.
 at::Tensor embedding_backward(const c10::optional<at::Tensor>& ids_, const at::Tensor& grad_,
@@ -1121,6 +1127,7 @@ at::Tensor embedding_backward(const c10::optional<at::Tensor>& ids_, const at::T
                                    (float)scale, padding_idx, out.has_value(), to.data_ptr(),
                                    ws.data_ptr(), (size_t)ws.numel(), st);
   check_rc(rc, "gtp_embedding_backward");
+  if (out.has_value()) count_write(to);
   return to;
 }
 
@@ -1240,10 +1247,11 @@ at::Tensor norm_of(const GradList& l, const at::Tensor& like, double norm_type, 
   return out;
 }
 
-void clip_by(GradList& l, const at::Tensor& norm, double max_norm, void* st) {
+void clip_by(at::TensorList tensors, GradList& l, const at::Tensor& norm, double max_norm, void* st) {
   check_rc(gtp_clip_grads(l.p.data(), l.n.data(), l.dtype.data(), l.size(), norm.data_ptr<float>(),
                           (float)max_norm, st),
            "gtp_clip_grads");
+  for (const at::Tensor& t : tensors) count_write(t);
   for (auto& c : l.copies) c.first.copy_(c.second);
 }
 
@@ -1260,7 +1268,7 @@ void clip_grads_(at::TensorList tensors, const at::Tensor& norm, double max_norm
   TORCH_CHECK(norm.scalar_type() == at::kFloat && norm.numel() == 1,
               "graspo_tokpath.clip_grads_: norm must be one float32");
   const c10::DeviceGuard guard(tensors[0].device());
-  clip_by(l, norm, max_norm, reinterpret_cast<void*>(stream));
+  clip_by(tensors, l, norm, max_norm, reinterpret_cast<void*>(stream));
 }
 
 // Both, from one look at the list.
@@ -1271,7 +1279,7 @@ at::Tensor clip_grad_norm_(at::TensorList tensors, double max_norm, double norm_
   const c10::DeviceGuard guard(tensors[0].device());
   void* st = reinterpret_cast<void*>(stream);
   const at::Tensor norm = norm_of(l, tensors[0], norm_type, st);
-  clip_by(l, norm, max_norm, st);
+  clip_by(tensors, l, norm, max_norm, st);
   return norm;
 }
 
