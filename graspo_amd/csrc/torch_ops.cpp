@@ -1207,9 +1207,39 @@ struct GradList {
   int64_t size() const { return (int64_t)p.size(); }
 };
 
+// Whether a and b, whose spans in memory overlap, are known to share no byte:
+// columns of one buffer, say.  At some stride P of theirs, the dims that step
+// by multiples of P aside, each fills less than P bytes, and modulo P these do
+// not meet.
+bool apart(const at::Tensor& a, const at::Tensor& b) {
+  const int64_t sa = a.element_size(), sb = b.element_size();
+  auto extent = [](const at::Tensor& t, int64_t es, int64_t P) {
+    int64_t bytes = es;
+    for (int64_t d = 0; d < t.dim(); ++d)
+      if (t.stride(d) * es % P != 0) bytes += (t.size(d) - 1) * t.stride(d) * es;
+    return bytes;
+  };
+  auto apart_at = [&](int64_t P) {
+    const int64_t ea = extent(a, sa, P), eb = extent(b, sb, P);
+    int64_t off = (reinterpret_cast<intptr_t>(b.data_ptr()) - reinterpret_cast<intptr_t>(a.data_ptr())) % P;
+    if (off < 0) off += P;
+    return ea <= off && off + eb <= P;
+  };
+  for (int64_t d = 0; d < a.dim(); ++d)
+    if (a.size(d) > 1 && apart_at(a.stride(d) * sa)) return true;
+  for (int64_t d = 0; d < b.dim(); ++d)
+    if (b.size(d) > 1 && apart_at(b.stride(d) * sb)) return true;
+  return false;
+}
+
 // In-place products of overlapping tensors would race (and scale twice).
 void check_apart(at::TensorList tensors) {
-  std::vector<std::pair<uintptr_t, uintptr_t>> at;
+  struct Span {
+    uintptr_t from, to;
+    const at::Tensor* t;
+    bool operator<(const Span& o) const { return from < o.from; }
+  };
+  std::vector<Span> at;
   at.reserve(tensors.size());
   bool sorted = true;
   for (const at::Tensor& t : tensors) {
@@ -1224,13 +1254,17 @@ void check_apart(at::TensorList tensors) {
       }
     }
     const uintptr_t a = reinterpret_cast<uintptr_t>(t.data_ptr());
-    sorted = sorted && (at.empty() || at.back().first <= a);
-    at.emplace_back(a, a + span * t.element_size());
+    sorted = sorted && (at.empty() || at.back().from <= a);
+    at.push_back({a, a + span * t.element_size(), &t});
   }
   if (!sorted) std::sort(at.begin(), at.end());
-  for (size_t i = 1; i < at.size(); ++i)
-    TORCH_CHECK(at[i].first >= at[i - 1].second,
-                "graspo_tokpath.clip_grads_: tensors overlap in memory (the same one twice?)");
+  uintptr_t reach = 0;
+  for (size_t i = 0; i < at.size(); ++i) {
+    for (size_t j = 0; at[i].from < reach && j < i; ++j)
+      TORCH_CHECK(at[j].to <= at[i].from || apart(*at[j].t, *at[i].t),
+                  "graspo_tokpath.clip_grads_: tensors overlap in memory (the same one twice?)");
+    reach = std::max(reach, at[i].to);
+  }
 }
 
 at::Tensor norm_of(const GradList& l, const at::Tensor& like, double norm_type, void* st) {
