@@ -1031,7 +1031,9 @@ std::tuple<at::Tensor, bool, at::Tensor> embedding(const at::Tensor& ids_, const
   const at::Tensor ids = flat_ids(ids_, weight, "embedding");
   const c10::DeviceGuard guard(weight.device());
   const int64_t N = ids.size(0), V = weight.size(0), H = weight.size(1);
-  const at::Tensor w = H == 1 || weight.stride(1) == 1 ? weight : weight.contiguous();
+  // (rows that overlap, as an expanded one's do, are copied too)
+  const bool in_place = (H == 1 || weight.stride(1) == 1) && (V == 1 || weight.stride(0) >= H);
+  const at::Tensor w = in_place ? weight : weight.contiguous();
   void* st = reinterpret_cast<void*>(stream);
   auto shape = ids_.sizes().vec();
   shape.push_back(H);
