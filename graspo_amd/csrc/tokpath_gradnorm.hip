@@ -361,6 +361,7 @@ extern "C" int gtp_grad_norm(const void* const* tensors, const int64_t* sizes,
   const int rc = norm::plan_of(tensors, sizes, dtypes, count, plan);
   if (rc != GTP_OK) return rc;
   if (!out_norm || !workspace || workspace_bytes < (size_t)plan.chunks * sizeof(double) ||
+      (reinterpret_cast<uintptr_t>(workspace) & 7u) ||
       norm_type < norm::kOne || norm_type > norm::kMax)
     return GTP_ERR_INVALID_ARGUMENT;
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);

@@ -841,6 +841,11 @@ struct Carve {
   }
 };
 
+// Its parts are read in 16-byte chunks.
+inline bool usable(const void* workspace) {
+  return (reinterpret_cast<uintptr_t>(workspace) & 15u) == 0;
+}
+
 // The sizes that a call's kernels share.
 struct Shape {
   int64_t N, K8, ldh, ldn;  // rows with a target; K to a multiple of 8; row strides
@@ -1112,7 +1117,7 @@ extern "C" int gtp_linear_logprob_rows(const gtp_linear_rows* rows, float* out_l
   if ((s.N > 0 && (!out_logprob || !out_lse)) || !workspace || (!mean_loss != !mean_count))
     return GTP_ERR_INVALID_ARGUMENT;
   const lin::Forward f = lin::forward_space(s, workspace);
-  if (workspace_bytes < f.bytes) return GTP_ERR_INVALID_ARGUMENT;
+  if (workspace_bytes < f.bytes || !lin::usable(workspace)) return GTP_ERR_INVALID_ARGUMENT;
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   for (int i = 1; verdict && i < GTP_VERDICT_WORDS; ++i) verdict[i] = GTP_VERDICT_GOOD;
   hipLaunchKernelGGL(lin::list_rows_kernel, dim3(1), dim3(lin::kListBlock), 0, st, a,
@@ -1159,7 +1164,7 @@ extern "C" int gtp_linear_logprob_backward(const gtp_linear_rows* rows, const fl
   if (!lse || !grad || !workspace) return GTP_ERR_INVALID_ARGUMENT;
   const lin::Pieces p = lin::pieces_of(s, rows->V, rows->K);
   const lin::Backward b = lin::backward_space(rows, s, p, workspace);
-  if (workspace_bytes < b.bytes) return GTP_ERR_INVALID_ARGUMENT;
+  if (workspace_bytes < b.bytes || !lin::usable(workspace)) return GTP_ERR_INVALID_ARGUMENT;
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   hipLaunchKernelGGL(lin::list_rows_kernel, dim3(1), dim3(lin::kListBlock), 0, st, a, b.rows,
                      b.meta, nullptr, nullptr, nullptr, grad, mean_count, lse, b.slot,

@@ -640,7 +640,8 @@ typedef struct gtp_linear_rows {
  * rows that are not ignored (NaN without one, or with a bad target) and that
  * count.  verdict: GTP_VERDICT_WORDS pinned words, each GTP_VERDICT_PENDING,
  * answered ahead of the products (gtp_verdict_wait), or NULL.  The workspace
- * (gtp_linear_logprob_workspace_bytes) carries nothing between calls.
+ * (gtp_linear_logprob_workspace_bytes, 16-byte aligned, here and in the
+ * backward) carries nothing between calls.
  */
 size_t gtp_linear_logprob_workspace_bytes(const gtp_linear_rows* rows);
 int gtp_linear_logprob_rows(const gtp_linear_rows* rows, float* out_logprob, float* out_lse,
@@ -683,8 +684,8 @@ int gtp_embedding_rows(const void* ids, int ids_int64, int64_t N, int64_t ids_st
  *   grad_weight  [V, H] contiguous of `dtype`; accumulate: added to what the
  *                rows hold, and rows without a token are neither read nor
  *                written
- * The workspace (gtp_embedding_backward_workspace_bytes) carries nothing
- * between calls.
+ * The workspace (gtp_embedding_backward_workspace_bytes, 4-byte aligned, here
+ * and below) carries nothing between calls.
  */
 size_t gtp_embedding_backward_workspace_bytes(int dtype, int64_t N, int64_t V, int64_t H);
 int gtp_embedding_backward(const void* ids, int ids_int64, int64_t N, int64_t ids_stride,
@@ -717,7 +718,8 @@ int gtp_embedding_backward_ordered(const void* order, size_t order_bytes, int64_
  * gtp_clip_grads -- multiplies them, in place, by min(1, max_norm / (*norm +
  * 1e-6)) (one fp32 product, one rounding; NaN where the norm is NaN); nothing
  * is read or written where that is 1.  The tensors must not overlap.
- * The workspace (gtp_grad_norm_workspace_bytes) carries nothing between calls.
+ * The workspace (gtp_grad_norm_workspace_bytes, 8-byte aligned) carries nothing
+ * between calls.
  */
 size_t gtp_grad_norm_workspace_bytes(const void* const* tensors, const int64_t* sizes,
                                      const int32_t* dtypes, int64_t count);
