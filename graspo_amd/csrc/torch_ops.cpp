@@ -1288,6 +1288,7 @@ void clip_by(at::TensorList tensors, GradList& l, const at::Tensor& norm, double
                           (float)max_norm, st),
            "gtp_clip_grads");
   for (const at::Tensor& t : tensors) count_write(t);
+  const at::NoGradGuard untracked;  // (gradients may be of a graph)
   for (auto& c : l.copies) c.first.copy_(c.second);
 }
 
