@@ -1,13 +1,6 @@
-"""Token logprobs and losses from hidden states and the lm_head weight.
-
-What their two public forms, ``graspo_loss.sequence_log_probs_from_hidden`` and
-``sft_loss.sft_cross_entropy_loss_from_hidden``, check alike.  Both are
-:func:`graspo_amd.ops.linear_loss`: nothing of the size of the logits is kept
-between forward and backward, which computes them again a piece of the
-vocabulary at a time.  Against ``_selected_token_log_probs_from_hidden``
-(tensor_utils.py), which keeps the fp32 logits: one product more, and 4 N V
-bytes less (8.1 GB at 8192 tokens of 248320).
-"""
+"""What the two public forms of the losses from hidden states,
+``graspo_loss.sequence_log_probs_from_hidden`` and
+``sft_loss.sft_cross_entropy_loss_from_hidden``, check alike."""
 
 from __future__ import annotations
 
