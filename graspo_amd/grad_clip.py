@@ -2,7 +2,8 @@
 
 The names and arguments of ``torch.nn.utils``: one launch per 192 tensors for
 the norm and one for the clipping, whatever their sizes and types, the norm
-summed in 64 bits and the gradients rounded once.  The reference's training
+summed in 64 bits and the gradients rounded once (``foreach`` is torch's choice
+between its own two ways, and says nothing here).  The reference's training
 step clips between backward and optimizer
 (``models/qwen35_36/training.py:427-441``).
 """
@@ -43,7 +44,8 @@ def _raise_if_nonfinite(what: str, norm: torch.Tensor, norm_type: float) -> None
                            f"gradients cannot be clipped")
 
 
-def get_total_norm(tensors, norm_type: float = 2.0, error_if_nonfinite: bool = False) -> torch.Tensor:
+def get_total_norm(tensors, norm_type: float = 2.0, error_if_nonfinite: bool = False,
+                   foreach: bool | None = None) -> torch.Tensor:
     """The norm (``norm_type`` 1, 2 or inf) over all elements of ``tensors``
     (fp32, bf16, fp16, mixed, of one GPU) as an fp32 scalar on the device; 0
     without a tensor."""
@@ -58,7 +60,8 @@ def get_total_norm(tensors, norm_type: float = 2.0, error_if_nonfinite: bool = F
     return norm
 
 
-def clip_grads_with_norm_(parameters, max_norm: float, total_norm: torch.Tensor) -> None:
+def clip_grads_with_norm_(parameters, max_norm: float, total_norm: torch.Tensor,
+                          foreach: bool | None = None) -> None:
     """Multiplies the parameters' gradients, in place, by min(1, ``max_norm``
     / (``total_norm`` + 1e-6)): ``total_norm`` as :func:`get_total_norm` gives
     it, or combined over ranks.  Gradients that overlap in memory (a parameter
@@ -71,7 +74,7 @@ def clip_grads_with_norm_(parameters, max_norm: float, total_norm: torch.Tensor)
 
 
 def clip_grad_norm_(parameters, max_norm: float, norm_type: float = 2.0,
-                    error_if_nonfinite: bool = False) -> torch.Tensor:
+                    error_if_nonfinite: bool = False, foreach: bool | None = None) -> torch.Tensor:
     """Clips the parameters' gradients, in place, to a total norm of
     ``max_norm`` and returns the norm that they had (an fp32 scalar on the
     device).  Without ``error_if_nonfinite`` nothing waits for the GPU; with
