@@ -1,0 +1,295 @@
+// tokpath_states.hip -- the models' states follow the beams (gfx950).
+//
+// A state is a tensor whose first dimension counts the beams' rows (a layer's
+// keys or values [R, heads, length, dim], a recurrent state), read and written
+// as bytes.
+//
+// - reorder_kernel, in place: row g K + k becomes row parent[g K + k], of the
+//   same group.  A thread holds the same few bytes of all K rows: it loads those
+//   that go elsewhere, then stores, so any map of a group onto itself (swaps,
+//   cycles) needs no second buffer; where every source stays, as the parents of
+//   a beam step do, rows that stay are neither read nor written.
+// - expand_kernel: row g of a prompt's state to the K rows of its beams, each
+//   byte read once.
+// Bound by memory: the bytes of the rows that change, read and written.
+#include "tokpath_common.h"
+
+namespace gtp {
+namespace states {
+
+constexpr int kBlock = 256;
+constexpr int kMost = 192;   // tensors per launch, addresses in the arguments
+constexpr int kMaxBeams = 64;
+constexpr int kDims = GTP_STATE_DIMS;
+
+// A row's bytes as units of kBytes: `run` of them in a run without gaps, runs
+// in up to kDims dimensions (the innermost first).
+struct Shape {
+  uint32_t units;          // per row
+  uint32_t run;            // units per run
+  uint32_t size[kDims];    // runs along each dimension
+  int64_t stride[kDims];   // bytes
+  int64_t row_stride;      // bytes
+};
+
+struct List {
+  void* p[kMost];
+};
+struct Pairs {
+  const void* from[kMost];
+  void* to[kMost];
+};
+
+__device__ __forceinline__ int64_t offset_of(const Shape& s, uint32_t u, int bytes) {
+  uint32_t r = u / s.run;
+  int64_t at = (int64_t)(u - r * s.run) * bytes;
+#pragma unroll
+  for (int d = 0; d < kDims; ++d) {
+    if (s.size[d] == 1) continue;
+    const uint32_t q = r / s.size[d];
+    at += (int64_t)(r - q * s.size[d]) * s.stride[d];
+    r = q;
+  }
+  return at;
+}
+
+template <int kBytes>
+struct Unit;
+template <>
+struct Unit<16> { typedef uint32_t type __attribute__((ext_vector_type(4))); };
+template <>
+struct Unit<8> { typedef uint32_t type __attribute__((ext_vector_type(2))); };
+template <>
+struct Unit<4> { typedef uint32_t type; };
+template <>
+struct Unit<2> { typedef uint16_t type; };
+template <>
+struct Unit<1> { typedef uint8_t type; };
+
+// tiles: workgroups per (tensor, group).  kMany: more than 16 beams.
+template <int kBytes, bool kMany>
+__global__ __launch_bounds__(kBlock) void reorder_kernel(List l, Shape s, const int32_t* parents,
+                                                         uint32_t groups, int K, uint32_t tiles,
+                                                         int32_t* bad) {
+  using U = typename Unit<kBytes>::type;
+  const uint32_t tile = blockIdx.x % tiles, rest = blockIdx.x / tiles;
+  const uint32_t g = rest % groups, t = rest / groups;
+  const int64_t base = (int64_t)g * K;
+  // lane k: where row k comes from
+  const int lane = threadIdx.x & (kWave - 1);
+  const int64_t p = lane < K ? (int64_t)parents[base + lane] - base : lane;
+  const bool wrong = lane < K && (p < 0 || p >= K);
+  const int from = wrong ? lane : (int)p;
+  // a parent outside the group leaves its row as it is
+  if (bad && __ballot(wrong) && t == 0 && tile == 0 && threadIdx.x == 0) *bad = 1;
+  uint64_t moving = __ballot(from != lane);
+  // A wave stays whole (lanes past the row's end repeat its last unit: loaded
+  // and stored by the same instructions as that one, the same values).
+  uint32_t u = tile * kBlock + threadIdx.x;
+  if (moving == 0 || __builtin_amdgcn_readfirstlane(u) >= s.units) return;
+  if (u >= s.units) u = s.units - 1;
+  const bool apart = __ballot(from != lane && ((moving >> from) & 1)) == 0;
+  char* at = reinterpret_cast<char*>(l.p[t]) + base * s.row_stride + offset_of(s, u, kBytes);
+  auto row = [&](int k) { return at + (int64_t)k * s.row_stride; };
+  if (apart) {
+    // every source stays, as a beam step's do: four rows at a time
+    while (moving) {
+      U v[4];
+      int to[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        to[i] = moving ? __ffsll((unsigned long long)moving) - 1 : -1;
+        moving &= moving - 1;
+        if (to[i] >= 0)
+          v[i] = *reinterpret_cast<const U*>(row(__builtin_amdgcn_readlane(from, to[i])));
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (to[i] >= 0) *reinterpret_cast<U*>(row(to[i])) = v[i];
+    }
+    return;
+  }
+  // all loads ahead of all stores
+  if constexpr (!kMany) {
+    U v[16];
+#pragma unroll
+    for (int k = 0; k < 16; ++k)
+      v[k] = *reinterpret_cast<const U*>(row(__builtin_amdgcn_readlane(from, k < K ? k : K - 1)));
+#pragma unroll
+    for (int k = 0; k < 16; ++k)
+      if ((moving >> k) & 1) *reinterpret_cast<U*>(row(k)) = v[k];
+  } else {
+    // 4 bytes at a time: 64 rows of them fit the registers
+    constexpr int kPart = kBytes < 4 ? kBytes : 4;
+    using P = typename Unit<kPart>::type;
+#pragma unroll 1
+    for (int o = 0; o < kBytes; o += kPart) {
+      P v[kMaxBeams];
+#pragma unroll
+      for (int k = 0; k < kMaxBeams; ++k)
+        v[k] = *reinterpret_cast<const P*>(
+            row(__builtin_amdgcn_readlane(from, k < K ? k : K - 1)) + o);
+#pragma unroll
+      for (int k = 0; k < kMaxBeams; ++k)
+        if ((moving >> k) & 1) *reinterpret_cast<P*>(row(k) + o) = v[k];
+    }
+  }
+}
+
+// The copies are contiguous: row_units units of kBytes each.
+template <int kBytes>
+__global__ __launch_bounds__(kBlock) void expand_kernel(Pairs l, Shape s, uint32_t groups, int K,
+                                                        uint32_t tiles) {
+  using U = typename Unit<kBytes>::type;
+  const uint32_t tile = blockIdx.x % tiles, rest = blockIdx.x / tiles;
+  const uint32_t g = rest % groups, t = rest / groups;
+  const uint32_t u = tile * kBlock + threadIdx.x;
+  if (u >= s.units) return;
+  const U v = *reinterpret_cast<const U*>(reinterpret_cast<const char*>(l.from[t]) +
+                                          (int64_t)g * s.row_stride + offset_of(s, u, kBytes));
+  U* to = reinterpret_cast<U*>(l.to[t]) + (int64_t)g * K * s.units + u;
+  for (int k = 0; k < K; ++k) to[(int64_t)k * s.units] = v;
+}
+
+// ------------------------------------------------------------------- host
+
+// The unit (16 bytes or the largest power of two that divides every address
+// and stride) and the row's shape in it.
+int shape_of(const gtp_state_shape* q, uintptr_t addresses, Shape& s, int& bytes) {
+  uint64_t all = addresses | (uint64_t)q->run_bytes;
+  int64_t runs = 1;
+  for (int d = 0; d < kDims; ++d) {
+    if (q->sizes[d] < 1) return GTP_ERR_INVALID_ARGUMENT;
+    if (q->sizes[d] > 0x7FFFFFFF || runs * q->sizes[d] > 0x7FFFFFFF) return GTP_ERR_UNSUPPORTED;
+    runs *= q->sizes[d];
+    if (q->sizes[d] > 1) all |= (uint64_t)q->strides[d];
+    s.size[d] = (uint32_t)q->sizes[d];
+    s.stride[d] = q->strides[d];
+  }
+  all |= (uint64_t)q->row_stride;
+  bytes = 16;
+  while (bytes > 1 && all % bytes) bytes /= 2;
+  if (q->run_bytes / bytes > 0x7FFFFFFF || q->run_bytes / bytes * runs > 0x7FFFFFFF)
+    return GTP_ERR_UNSUPPORTED;
+  s.run = (uint32_t)(q->run_bytes / bytes);
+  s.units = (uint32_t)(s.run * runs);
+  s.row_stride = q->row_stride;
+  return GTP_OK;
+}
+
+int check(const gtp_state_shape* q, int64_t count, int64_t groups, int32_t beams) {
+  if (!q || count < 0 || groups < 0 || beams < 1 || q->run_bytes < 0)
+    return GTP_ERR_INVALID_ARGUMENT;
+  if (beams > kMaxBeams || groups * beams > 0x7FFFFFFF) return GTP_ERR_UNSUPPORTED;
+  return GTP_OK;
+}
+
+template <int kBytes>
+void reorder(const List& l, const Shape& s, const int32_t* parents, int64_t n, int64_t groups,
+             int K, int32_t* bad, hipStream_t st) {
+  const uint32_t tiles = (s.units + kBlock - 1) / kBlock;
+  const dim3 grid((uint32_t)(tiles * groups * n));
+  if (K <= 16)
+    hipLaunchKernelGGL((reorder_kernel<kBytes, false>), grid, dim3(kBlock), 0, st, l, s, parents,
+                       (uint32_t)groups, K, tiles, bad);
+  else
+    hipLaunchKernelGGL((reorder_kernel<kBytes, true>), grid, dim3(kBlock), 0, st, l, s, parents,
+                       (uint32_t)groups, K, tiles, bad);
+}
+
+// tensors per launch: their workgroups fit a grid
+int64_t per_launch(const Shape& s, int64_t groups, int64_t count) {
+  const int64_t each = ((int64_t)s.units + kBlock - 1) / kBlock * groups;
+  int64_t n = 0x7FFFFFFFll / (each > 0 ? each : 1);
+  if (n > kMost) n = kMost;
+  return n < count ? n : count;
+}
+
+}  // namespace states
+}  // namespace gtp
+
+using namespace gtp;
+
+extern "C" int gtp_reorder_states(void* const* tensors, int64_t count,
+                                  const gtp_state_shape* shape, const int32_t* parents,
+                                  int64_t groups, int32_t beams, int32_t* bad, void* stream) {
+  int rc = states::check(shape, count, groups, beams);
+  if (rc != GTP_OK) return rc;
+  if (count == 0 || groups == 0 || shape->run_bytes == 0) return GTP_OK;
+  if (!tensors || !parents) return GTP_ERR_INVALID_ARGUMENT;
+  uintptr_t all = 0;
+  for (int64_t i = 0; i < count; ++i) {
+    if (!tensors[i]) return GTP_ERR_INVALID_ARGUMENT;
+    all |= reinterpret_cast<uintptr_t>(tensors[i]);
+  }
+  states::Shape s;
+  int bytes;
+  rc = states::shape_of(shape, all, s, bytes);
+  if (rc != GTP_OK) return rc;
+  const int64_t most = states::per_launch(s, groups, count);
+  if (most < 1) return GTP_ERR_UNSUPPORTED;
+  hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  for (int64_t first = 0; first < count; first += most) {
+    const int64_t n = count - first < most ? count - first : most;
+    states::List l;
+    for (int64_t i = 0; i < n; ++i) l.p[i] = tensors[first + i];
+    switch (bytes) {
+      case 16: states::reorder<16>(l, s, parents, n, groups, beams, bad, st); break;
+      case 8: states::reorder<8>(l, s, parents, n, groups, beams, bad, st); break;
+      case 4: states::reorder<4>(l, s, parents, n, groups, beams, bad, st); break;
+      case 2: states::reorder<2>(l, s, parents, n, groups, beams, bad, st); break;
+      default: states::reorder<1>(l, s, parents, n, groups, beams, bad, st); break;
+    }
+  }
+  return hipGetLastError() == hipSuccess ? GTP_OK : GTP_ERR_LAUNCH;
+}
+
+extern "C" int gtp_expand_states(const void* const* tensors, void* const* outs, int64_t count,
+                                 const gtp_state_shape* shape, int64_t groups, int32_t beams,
+                                 void* stream) {
+  int rc = states::check(shape, count, groups, beams);
+  if (rc != GTP_OK) return rc;
+  if (count == 0 || groups == 0 || shape->run_bytes == 0) return GTP_OK;
+  if (!tensors || !outs) return GTP_ERR_INVALID_ARGUMENT;
+  uintptr_t all = 0;
+  for (int64_t i = 0; i < count; ++i) {
+    if (!tensors[i] || !outs[i]) return GTP_ERR_INVALID_ARGUMENT;
+    all |= reinterpret_cast<uintptr_t>(tensors[i]) | reinterpret_cast<uintptr_t>(outs[i]);
+  }
+  states::Shape s;
+  int bytes;
+  rc = states::shape_of(shape, all, s, bytes);
+  if (rc != GTP_OK) return rc;
+  const int64_t most = states::per_launch(s, groups, count);
+  if (most < 1) return GTP_ERR_UNSUPPORTED;
+  hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  const uint32_t tiles = (s.units + states::kBlock - 1) / states::kBlock;
+  for (int64_t first = 0; first < count; first += most) {
+    const int64_t n = count - first < most ? count - first : most;
+    states::Pairs l;
+    for (int64_t i = 0; i < n; ++i) {
+      l.from[i] = tensors[first + i];
+      l.to[i] = outs[first + i];
+    }
+    const dim3 grid((uint32_t)(tiles * groups * n)), block(states::kBlock);
+    const uint32_t G = (uint32_t)groups;
+    switch (bytes) {
+      case 16:
+        hipLaunchKernelGGL(states::expand_kernel<16>, grid, block, 0, st, l, s, G, beams, tiles);
+        break;
+      case 8:
+        hipLaunchKernelGGL(states::expand_kernel<8>, grid, block, 0, st, l, s, G, beams, tiles);
+        break;
+      case 4:
+        hipLaunchKernelGGL(states::expand_kernel<4>, grid, block, 0, st, l, s, G, beams, tiles);
+        break;
+      case 2:
+        hipLaunchKernelGGL(states::expand_kernel<2>, grid, block, 0, st, l, s, G, beams, tiles);
+        break;
+      default:
+        hipLaunchKernelGGL(states::expand_kernel<1>, grid, block, 0, st, l, s, G, beams, tiles);
+        break;
+    }
+  }
+  return hipGetLastError() == hipSuccess ? GTP_OK : GTP_ERR_LAUNCH;
+}

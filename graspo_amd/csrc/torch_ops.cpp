@@ -6,7 +6,8 @@
 // decode_update, to_bf16_exact, logprob_backward_split, time_next_launch,
 // lm_head_logprob, lm_head_logprob_save, softmax_grad_bf16, linear_logprob,
 // linear_logprob_backward, linear_loss, embedding, embedding_backward,
-// token_embedding, grad_norm, clip_grads_, clip_grad_norm_}.  Each op validates
+// token_embedding, grad_norm, clip_grads_, clip_grad_norm_, beam_candidates,
+// beam_advance, beam_step, beam_finish, reorder_states_, expand_states}.  Each op validates
 // its tensors (TORCH_CHECK surfaces as a Python RuntimeError), allocates the
 // outputs on the logits' device, and enqueues the HIP kernels on the stream handle passed in from Python
 // (torch.cuda.current_stream().cuda_stream), so work orders with the
@@ -1235,7 +1236,7 @@ bool apart(const at::Tensor& a, const at::Tensor& b) {
 }
 
 // In-place products of overlapping tensors would race (and scale twice).
-void check_apart(at::TensorList tensors) {
+void check_apart(at::TensorList tensors, const char* what = "clip_grads_") {
   struct Span {
     uintptr_t from, to;
     const at::Tensor* t;
@@ -1251,7 +1252,7 @@ void check_apart(at::TensorList tensors) {
       span = 1;
       for (int64_t d = 0; d < t.dim(); ++d) {
         TORCH_CHECK(t.size(d) <= 1 || t.stride(d) != 0,
-                    "graspo_tokpath.clip_grads_: a tensor overlaps itself");
+                    "graspo_tokpath.", what, ": a tensor overlaps itself");
         span += (t.size(d) - 1) * t.stride(d);
       }
     }
@@ -1264,7 +1265,7 @@ void check_apart(at::TensorList tensors) {
   for (size_t i = 0; i < at.size(); ++i) {
     for (size_t j = 0; at[i].from < reach && j < i; ++j)
       TORCH_CHECK(at[j].to <= at[i].from || apart(*at[j].t, *at[i].t),
-                  "graspo_tokpath.clip_grads_: tensors overlap in memory (the same one twice?)");
+                  "graspo_tokpath.", what, ": tensors overlap in memory (the same one twice?)");
     reach = std::max(reach, at[i].to);
   }
 }
@@ -1320,7 +1321,412 @@ at::Tensor clip_grad_norm_(at::TensorList tensors, double max_norm, double norm_
   return norm;
 }
 
+// ------------------------------------------------- beam search
+
+// logits [G * K, V] or [G, K, V], any strides but of the columns; scores [G, K]
+gtp_beam_rows beam_rows(const at::Tensor& logits, const at::Tensor& scores, int64_t candidates,
+                        const c10::optional<at::Tensor>& allow_mask,
+                        const c10::optional<at::Tensor>& done, const char* what) {
+  TORCH_CHECK(logits.is_cuda(), "graspo_tokpath.", what, ": logits must be a GPU tensor");
+  check_same_device(logits, scores, "scores");
+  TORCH_CHECK(scores.scalar_type() == at::kFloat && scores.dim() == 2 && scores.is_contiguous() &&
+                  scores.size(1) > 0,
+              "graspo_tokpath.", what, ": scores must be contiguous float32 [groups, beams]");
+  const int64_t G = scores.size(0), K = scores.size(1), V = logits.size(-1);
+  TORCH_CHECK((logits.dim() == 2 && logits.size(0) == G * K) ||
+                  (logits.dim() == 3 && logits.size(0) == G && logits.size(1) == K),
+              "graspo_tokpath.", what, ": logits must be [groups * beams, V] or [groups, beams, V]");
+  TORCH_CHECK(V > 0 && (V == 1 || logits.stride(-1) == 1), "graspo_tokpath.", what,
+              ": logits rows must be contiguous and not empty");
+  TORCH_CHECK(K <= 32 && candidates >= 1 && candidates <= 64, "graspo_tokpath.", what,
+              ": at most 32 beams and 64 candidates, got ", K, " and ", candidates);
+  gtp_beam_rows r{};
+  r.logits = logits.data_ptr();
+  r.scores = scores.data_ptr<float>();
+  r.groups = G;
+  r.vocab = V;
+  const bool two = logits.dim() == 2;
+  r.beam_stride = two ? logits.stride(0) : logits.stride(1);
+  r.group_stride = two ? K * logits.stride(0) : logits.stride(0);
+  r.dtype = dtype_code(logits);
+  r.beams = (int32_t)K;
+  r.candidates = (int32_t)candidates;
+  if (allow_mask.has_value()) {
+    const auto& m = *allow_mask;
+    check_same_device(logits, m, "allow_mask");
+    TORCH_CHECK((m.scalar_type() == at::kInt || m.scalar_type() == at::kUInt32) && m.dim() == 2 &&
+                    m.size(0) == G * K && m.size(1) >= (V + 31) / 32 &&
+                    (m.size(1) == 1 || m.stride(1) == 1),
+                "graspo_tokpath.", what,
+                ": allow_mask must be int32/uint32 [groups * beams, >= ceil(V/32)]");
+    // (rows that share a mask are copied)
+    TORCH_CHECK(m.size(0) <= 1 || m.stride(0) >= (V + 31) / 32, "graspo_tokpath.", what,
+                ": allow_mask rows overlap");
+    r.allow_mask = static_cast<const uint32_t*>(m.data_ptr());
+    r.mask_stride = G * K > 1 ? m.stride(0) : m.size(1);
+  }
+  if (done.has_value()) {
+    check_same_device(logits, *done, "done");
+    TORCH_CHECK(done->scalar_type() == at::kBool && done->dim() == 1 && done->size(0) == G &&
+                    done->is_contiguous(),
+                "graspo_tokpath.", what, ": done must be contiguous bool [groups]");
+    r.done = static_cast<const uint8_t*>(done->data_ptr());
+  }
+  return r;
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> beam_candidates(
+    const at::Tensor& logits, const at::Tensor& scores, int64_t candidates,
+    const c10::optional<at::Tensor>& allow_mask, const c10::optional<at::Tensor>& done,
+    int64_t stream) {
+  const gtp_beam_rows r = beam_rows(logits, scores, candidates, allow_mask, done, "beam_candidates");
+  const c10::DeviceGuard guard(logits.device());
+  const auto i32 = scores.options().dtype(at::kInt);
+  at::Tensor out = at::empty({r.groups, candidates}, scores.options());
+  at::Tensor beams = at::empty({r.groups, candidates}, i32);
+  at::Tensor tokens = at::empty({r.groups, candidates}, i32.dtype(at::kLong));
+  at::Tensor status = at::empty({r.groups * r.beams}, i32);
+  at::Tensor ws = at::empty({(int64_t)gtp_beam_workspace_bytes(&r)}, i32.dtype(at::kByte));
+  check_rc(gtp_beam_candidates(&r, out.data_ptr<float>(), beams.data_ptr<int32_t>(),
+                               tokens.data_ptr<int64_t>(), status.data_ptr<int32_t>(),
+                               ws.data_ptr(), (size_t)ws.numel(), reinterpret_cast<void*>(stream)),
+           "gtp_beam_candidates");
+  return {out, beams, tokens, status};
+}
+
+using BeamOut = std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor,
+                           at::Tensor>;
+
+// A step's state, with new tensors for what it becomes.
+struct BeamStep {
+  gtp_beam_state s{};
+  BeamOut out;
+  BeamStep(const at::Tensor& scores, const at::Tensor& pool_scores, const at::Tensor& pool_rows,
+           const at::Tensor& pool_steps, const at::Tensor& done, int64_t eos, int64_t pad,
+           double length, int64_t step, bool early, const c10::optional<at::Tensor>& tokens_out,
+           const c10::optional<at::Tensor>& parents_out, const char* what) {
+    const int64_t G = scores.size(0), K = scores.size(1);
+    auto check = [&](const at::Tensor& t, at::ScalarType dt, const char* name) {
+      check_same_device(scores, t, name);
+      TORCH_CHECK(t.scalar_type() == dt && t.dim() == 2 && t.size(0) == G && t.size(1) == K &&
+                      t.is_contiguous(),
+                  "graspo_tokpath.", what, ": ", name, " must be contiguous ", dt,
+                  " [groups, beams]");
+    };
+    check(pool_scores, at::kFloat, "pool_scores");
+    check(pool_rows, at::kInt, "pool_rows");
+    check(pool_steps, at::kInt, "pool_steps");
+    check_same_device(scores, done, "done");
+    TORCH_CHECK(done.scalar_type() == at::kBool && done.dim() == 1 && done.size(0) == G &&
+                    done.is_contiguous(),
+                "graspo_tokpath.", what, ": done must be contiguous bool [groups]");
+    TORCH_CHECK(step >= 0 && step < INT32_MAX, "graspo_tokpath.", what, ": step must be >= 0");
+    TORCH_CHECK(length > 0.0 && length <= std::numeric_limits<double>::max(), "graspo_tokpath.",
+                what, ": (step + 1)^length_penalty must be positive and finite");
+    auto to = [&](const c10::optional<at::Tensor>& t, at::ScalarType dt, const char* name) {
+      if (!t.has_value()) return at::empty({G * K}, scores.options().dtype(dt));
+      check_same_device(scores, *t, name);
+      TORCH_CHECK(t->scalar_type() == dt && t->dim() == 1 && t->size(0) == G * K &&
+                      t->is_contiguous(),
+                  "graspo_tokpath.", what, ": ", name, " must be contiguous ", dt,
+                  " [groups * beams]");
+      return *t;
+    };
+    at::Tensor tokens = to(tokens_out, at::kLong, "tokens_out");
+    at::Tensor parents = to(parents_out, at::kInt, "parents_out");
+    at::Tensor n_scores = at::empty({G, K}, scores.options());
+    at::Tensor n_pool = at::empty({G, K}, scores.options());
+    at::Tensor n_rows = at::empty({G, K}, pool_rows.options());
+    at::Tensor n_steps = at::empty({G, K}, pool_rows.options());
+    at::Tensor n_done = at::empty({G}, done.options());
+    s.scores = scores.data_ptr<float>();
+    s.pool_scores = pool_scores.data_ptr<float>();
+    s.pool_rows = pool_rows.data_ptr<int32_t>();
+    s.pool_steps = pool_steps.data_ptr<int32_t>();
+    s.done = static_cast<const uint8_t*>(done.data_ptr());
+    s.out_tokens = tokens.data_ptr<int64_t>();
+    s.out_parents = parents.data_ptr<int32_t>();
+    s.out_scores = n_scores.data_ptr<float>();
+    s.out_pool_scores = n_pool.data_ptr<float>();
+    s.out_pool_rows = n_rows.data_ptr<int32_t>();
+    s.out_pool_steps = n_steps.data_ptr<int32_t>();
+    s.out_done = static_cast<uint8_t*>(n_done.data_ptr());
+    s.eos_token_id = eos;
+    s.pad_token_id = pad;
+    s.length = length;
+    s.step = (int32_t)step;
+    s.early_stopping = early;
+    out = {tokens, parents, n_scores, n_pool, n_rows, n_steps, n_done};
+  }
+  // tensors of the caller's that were written
+  void written(const c10::optional<at::Tensor>& tokens_out,
+               const c10::optional<at::Tensor>& parents_out) const {
+    for (const auto* t : {&tokens_out, &parents_out})
+      if (t->has_value() && !(*t)->is_inference()) (*t)->unsafeGetTensorImpl()->bump_version();
+  }
+};
+
+BeamOut beam_advance(const at::Tensor& c_scores, const at::Tensor& c_beams,
+                     const at::Tensor& c_tokens, const at::Tensor& scores,
+                     const at::Tensor& pool_scores, const at::Tensor& pool_rows,
+                     const at::Tensor& pool_steps, const at::Tensor& done, int64_t eos, int64_t pad,
+                     double length, int64_t step, bool early,
+                     const c10::optional<at::Tensor>& tokens_out,
+                     const c10::optional<at::Tensor>& parents_out, int64_t stream) {
+  TORCH_CHECK(scores.is_cuda() && scores.scalar_type() == at::kFloat && scores.dim() == 2 &&
+                  scores.is_contiguous() && scores.size(1) > 0 && scores.size(1) <= 32,
+              "graspo_tokpath.beam_advance: scores must be a contiguous float32 GPU tensor "
+              "[groups, beams], at most 32 beams");
+  const int64_t G = scores.size(0), n = c_scores.dim() == 2 ? c_scores.size(1) : 0;
+  TORCH_CHECK(n >= 1 && n <= 64, "graspo_tokpath.beam_advance: 1 to 64 candidates, got ", n);
+  auto check = [&](const at::Tensor& t, at::ScalarType dt, const char* name) {
+    check_same_device(scores, t, name);
+    TORCH_CHECK(t.scalar_type() == dt && t.dim() == 2 && t.size(0) == G && t.size(1) == n &&
+                    t.is_contiguous(),
+                "graspo_tokpath.beam_advance: ", name, " must be contiguous ", dt,
+                " [groups, candidates]");
+  };
+  check(c_scores, at::kFloat, "candidates' scores");
+  check(c_beams, at::kInt, "candidates' beams");
+  check(c_tokens, at::kLong, "candidates' tokens");
+  const c10::DeviceGuard guard(scores.device());
+  BeamStep b(scores, pool_scores, pool_rows, pool_steps, done, eos, pad, length, step, early,
+             tokens_out, parents_out, "beam_advance");
+  check_rc(gtp_beam_advance(c_scores.data_ptr<float>(), c_beams.data_ptr<int32_t>(),
+                            c_tokens.data_ptr<int64_t>(), G, (int32_t)scores.size(1), (int32_t)n,
+                            &b.s, reinterpret_cast<void*>(stream)),
+           "gtp_beam_advance");
+  b.written(tokens_out, parents_out);
+  return b.out;
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor,
+           at::Tensor>
+beam_step(const at::Tensor& logits, const at::Tensor& scores, const at::Tensor& pool_scores,
+          const at::Tensor& pool_rows, const at::Tensor& pool_steps, const at::Tensor& done,
+          int64_t candidates, int64_t eos, int64_t pad, double length, int64_t step, bool early,
+          const c10::optional<at::Tensor>& allow_mask, const c10::optional<at::Tensor>& tokens_out,
+          const c10::optional<at::Tensor>& parents_out, int64_t stream) {
+  const gtp_beam_rows r = beam_rows(logits, scores, candidates, allow_mask, done, "beam_step");
+  const c10::DeviceGuard guard(logits.device());
+  BeamStep b(scores, pool_scores, pool_rows, pool_steps, done, eos, pad, length, step, early,
+             tokens_out, parents_out, "beam_step");
+  at::Tensor status = at::empty({r.groups * r.beams}, pool_rows.options());
+  at::Tensor ws = at::empty({(int64_t)gtp_beam_workspace_bytes(&r)}, scores.options().dtype(at::kByte));
+  check_rc(gtp_beam_step(&r, &b.s, status.data_ptr<int32_t>(), ws.data_ptr(), (size_t)ws.numel(),
+                         reinterpret_cast<void*>(stream)),
+           "gtp_beam_step");
+  b.written(tokens_out, parents_out);
+  return std::tuple_cat(b.out, std::make_tuple(status));
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor> beam_finish(
+    const at::Tensor& scores, const at::Tensor& pool_scores, const at::Tensor& pool_rows,
+    const at::Tensor& pool_steps, const at::Tensor& done, const at::Tensor& tokens,
+    const at::Tensor& parents, double length, int64_t eos, int64_t pad, int64_t give,
+    int64_t stream) {
+  TORCH_CHECK(scores.is_cuda() && scores.dim() == 2 && scores.size(1) > 0 && scores.size(1) <= 32,
+              "graspo_tokpath.beam_finish: scores must be a GPU tensor [groups, beams], at most 32 "
+              "beams");
+  const int64_t G = scores.size(0), K = scores.size(1);
+  auto check = [&](const at::Tensor& t, at::ScalarType dt, at::IntArrayRef shape, const char* name) {
+    check_same_device(scores, t, name);
+    TORCH_CHECK(t.scalar_type() == dt && t.sizes() == shape && t.is_contiguous(),
+                "graspo_tokpath.beam_finish: ", name, " must be contiguous ", dt, " ", shape);
+  };
+  const int64_t T = tokens.dim() == 2 ? tokens.size(0) : -1;
+  check(scores, at::kFloat, {G, K}, "scores");
+  check(pool_scores, at::kFloat, {G, K}, "pool_scores");
+  check(pool_rows, at::kInt, {G, K}, "pool_rows");
+  check(pool_steps, at::kInt, {G, K}, "pool_steps");
+  check(done, at::kBool, {G}, "done");
+  check(tokens, at::kLong, {T, G * K}, "tokens");
+  check(parents, at::kInt, {T, G * K}, "parents");
+  TORCH_CHECK(give >= 1 && give <= K && T < INT32_MAX,
+              "graspo_tokpath.beam_finish: 1 to ", K, " hypotheses of a group, got ", give);
+  TORCH_CHECK(length > 0.0, "graspo_tokpath.beam_finish: the length must be positive");
+  const c10::DeviceGuard guard(scores.device());
+  at::Tensor out = at::empty({G, give}, scores.options());
+  at::Tensor lengths = at::empty({G, give}, pool_rows.options());
+  at::Tensor seq = at::empty({G, give, T}, tokens.options());
+  check_rc(gtp_beam_finish(scores.data_ptr<float>(), pool_scores.data_ptr<float>(),
+                           pool_rows.data_ptr<int32_t>(), pool_steps.data_ptr<int32_t>(),
+                           static_cast<const uint8_t*>(done.data_ptr()), tokens.data_ptr<int64_t>(),
+                           parents.data_ptr<int32_t>(), G, (int32_t)K, (int32_t)T, length, eos, pad,
+                           (int32_t)give, out.data_ptr<float>(), lengths.data_ptr<int32_t>(),
+                           seq.data_ptr<int64_t>(), T, reinterpret_cast<void*>(stream)),
+           "gtp_beam_finish");
+  return {out, lengths, seq};
+}
+
+// ------------------------------------------------- states of the beams
+
+// A state's rows as runs of bytes.  in_memory_order: dimensions by stride, as
+// suits a copy onto itself; else in the tensor's own order.
+gtp_state_shape state_shape(const at::Tensor& t, bool in_memory_order, const char* what) {
+  const int64_t es = t.element_size();
+  std::vector<std::pair<int64_t, int64_t>> dims;  // (stride, size), innermost first
+  for (int64_t d = t.dim() - 1; d >= 1; --d)
+    if (t.size(d) != 1) dims.emplace_back(t.stride(d) * es, t.size(d));
+  if (in_memory_order) {
+    std::stable_sort(dims.begin(), dims.end(),
+                     [](const auto& a, const auto& b) { return a.first < b.first; });
+    // (each dimension steps over all that lies within it, the rows' own too)
+    std::vector<std::pair<int64_t, int64_t>> all = dims;
+    if (t.size(0) > 1) all.emplace_back(t.stride(0) * es, t.size(0));
+    std::sort(all.begin(), all.end());
+    int64_t span = es;
+    for (const auto& d : all) {
+      TORCH_CHECK(d.first >= span || t.numel() == 0, "graspo_tokpath.", what,
+                  ": a state overlaps itself");
+      span += (d.second - 1) * d.first;
+    }
+  }
+  gtp_state_shape s;
+  s.run_bytes = t.numel() == 0 ? 0 : es;
+  s.row_stride = t.size(0) > 1 ? t.stride(0) * es : 0;
+  for (int d = 0; d < GTP_STATE_DIMS; ++d) {
+    s.sizes[d] = 1;
+    s.strides[d] = 0;
+  }
+  int at = -1;  // the last dimension of runs
+  for (const auto& d : dims) {
+    if (at < 0 && d.first == s.run_bytes) {
+      s.run_bytes *= d.second;
+    } else if (at >= 0 && d.first == s.strides[at] * s.sizes[at]) {
+      s.sizes[at] *= d.second;
+    } else {
+      ++at;
+      TORCH_CHECK(at < GTP_STATE_DIMS, "graspo_tokpath.", what,
+                  ": a state of more strided dimensions than are supported");
+      s.sizes[at] = d.second;
+      s.strides[at] = d.first;
+    }
+  }
+  return s;
+}
+
+bool same_shape(const gtp_state_shape& a, const gtp_state_shape& b) {
+  bool same = a.run_bytes == b.run_bytes && a.row_stride == b.row_stride;
+  for (int d = 0; d < GTP_STATE_DIMS; ++d)
+    same = same && a.sizes[d] == b.sizes[d] && a.strides[d] == b.strides[d];
+  return same;
+}
+
+void check_states(at::TensorList states, int64_t rows, const char* what) {
+  for (const at::Tensor& t : states) {
+    TORCH_CHECK(t.is_cuda() && t.layout() == at::kStrided, "graspo_tokpath.", what,
+                ": states must be dense GPU tensors");
+    check_same_device(states[0], t, "every state");
+    TORCH_CHECK(t.dim() >= 1 && (rows < 0 || t.size(0) == rows), "graspo_tokpath.", what,
+                ": a state's first dimension must count the rows (", rows, "), got ", t.sizes());
+  }
+}
+
+void reorder_states_(at::TensorList states, const at::Tensor& parents, int64_t beams, bool check,
+                     int64_t stream) {
+  if (states.empty()) return;
+  TORCH_CHECK(beams >= 1 && beams <= 64, "graspo_tokpath.reorder_states_: 1 to 64 beams, got ",
+              beams);
+  TORCH_CHECK(parents.scalar_type() == at::kInt && parents.dim() == 1 && parents.is_contiguous() &&
+                  parents.size(0) % beams == 0,
+              "graspo_tokpath.reorder_states_: parents must be contiguous int32 [groups * beams]");
+  const int64_t R = parents.size(0);
+  check_states(states, R, "reorder_states_");
+  check_same_device(states[0], parents, "parents");
+  for (const at::Tensor& t : states)
+    TORCH_CHECK(!t.requires_grad() || !at::GradMode::is_enabled(),
+                "graspo_tokpath.reorder_states_: a state that requires a gradient");
+  const c10::DeviceGuard guard(states[0].device());
+  std::vector<gtp_state_shape> shapes;
+  shapes.reserve(states.size());
+  for (const at::Tensor& t : states) shapes.push_back(state_shape(t, true, "reorder_states_"));
+  check_apart(states, "reorder_states_");
+  void* st = reinterpret_cast<void*>(stream);
+  at::Tensor bad;
+  check = check && R > 0 && !gtp_stream_capturing(st);
+  if (check) bad = at::zeros({1}, parents.options());
+  std::vector<void*> p;
+  p.reserve(states.size());
+  for (size_t i = 0; i < states.size();) {
+    p.clear();
+    size_t j = i;
+    for (; j < states.size() && same_shape(shapes[i], shapes[j]); ++j) p.push_back(states[j].data_ptr());
+    check_rc(gtp_reorder_states(p.data(), (int64_t)p.size(), &shapes[i], parents.data_ptr<int32_t>(),
+                                R / beams, (int32_t)beams,
+                                check ? bad.data_ptr<int32_t>() : nullptr, st),
+             "gtp_reorder_states");
+    i = j;
+  }
+  for (const at::Tensor& t : states)
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+  TORCH_CHECK(!check || bad.item<int32_t>() == 0,
+              "graspo_tokpath.reorder_states_: a parent lies outside its row's group (such rows "
+              "stay as they were)");
+}
+
+std::vector<at::Tensor> expand_states(at::TensorList states, int64_t beams, int64_t stream) {
+  TORCH_CHECK(beams >= 1 && beams <= 64, "graspo_tokpath.expand_states: 1 to 64 beams, got ", beams);
+  std::vector<at::Tensor> outs;
+  if (states.empty()) return outs;
+  check_states(states, states[0].dim() >= 1 ? states[0].size(0) : -1, "expand_states");
+  for (const at::Tensor& t : states)
+    TORCH_CHECK(!t.requires_grad() || !at::GradMode::is_enabled(),
+                "graspo_tokpath.expand_states: a state that requires a gradient");
+  const c10::DeviceGuard guard(states[0].device());
+  std::vector<gtp_state_shape> shapes;
+  shapes.reserve(states.size());
+  outs.reserve(states.size());
+  for (const at::Tensor& t : states) {
+    auto size = t.sizes().vec();
+    size[0] *= beams;
+    outs.push_back(at::empty(size, t.options()));
+    shapes.push_back(state_shape(t, false, "expand_states"));
+  }
+  std::vector<const void*> from;
+  std::vector<void*> to;
+  for (size_t i = 0; i < states.size();) {
+    from.clear();
+    to.clear();
+    size_t j = i;
+    for (; j < states.size() && same_shape(shapes[i], shapes[j]); ++j) {
+      from.push_back(states[j].data_ptr());
+      to.push_back(outs[j].data_ptr());
+    }
+    check_rc(gtp_expand_states(from.data(), to.data(), (int64_t)from.size(), &shapes[i],
+                               states[i].size(0), (int32_t)beams, reinterpret_cast<void*>(stream)),
+             "gtp_expand_states");
+    i = j;
+  }
+  return outs;
+}
+
 TORCH_LIBRARY(graspo_tokpath, m) {
+  m.def(
+      "beam_candidates(Tensor logits, Tensor scores, int candidates, Tensor? allow_mask, "
+      "Tensor? done, int stream) -> (Tensor, Tensor, Tensor, Tensor)",
+      &beam_candidates);
+  m.def(
+      "beam_advance(Tensor c_scores, Tensor c_beams, Tensor c_tokens, Tensor scores, "
+      "Tensor pool_scores, Tensor pool_rows, Tensor pool_steps, Tensor done, int eos, int pad, "
+      "float length, int step, bool early, Tensor(a!)? tokens_out, Tensor(b!)? parents_out, "
+      "int stream) -> (Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor)",
+      &beam_advance);
+  m.def(
+      "beam_step(Tensor logits, Tensor scores, Tensor pool_scores, Tensor pool_rows, "
+      "Tensor pool_steps, Tensor done, int candidates, int eos, int pad, float length, int step, "
+      "bool early, Tensor? allow_mask, Tensor(a!)? tokens_out, Tensor(b!)? parents_out, "
+      "int stream) -> (Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor)",
+      &beam_step);
+  m.def(
+      "beam_finish(Tensor scores, Tensor pool_scores, Tensor pool_rows, Tensor pool_steps, "
+      "Tensor done, Tensor tokens, Tensor parents, float length, int eos, int pad, int give, "
+      "int stream) -> (Tensor, Tensor, Tensor)",
+      &beam_finish);
+  m.def("reorder_states_(Tensor(a!)[] states, Tensor parents, int beams, bool check, int stream) "
+        "-> ()",
+        &reorder_states_);
+  m.def("expand_states(Tensor[] states, int beams, int stream) -> Tensor[]", &expand_states);
   m.def("embedding(Tensor ids, Tensor weight, float scale, bool check, bool ordered, int padding_idx, "
         "int stream) -> (Tensor, bool, Tensor)",
         &embedding);

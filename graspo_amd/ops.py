@@ -482,3 +482,93 @@ def raise_on_bad_status(status: torch.Tensor, what: str) -> None:
         rows = bad.nonzero().flatten()[:8].tolist()
         names = ", ".join(STATUS_NAMES.get(c, str(c)) for c in codes)
         raise RuntimeError(f"{what}: invalid rows {rows} ({names})")
+
+
+class BeamCandidates(NamedTuple):
+    scores: torch.Tensor  # fp32 [G, n], best first; -inf where there is none
+    beams: torch.Tensor   # int32 [G, n], in [0, beams); -1
+    tokens: torch.Tensor  # int64 [G, n]; -1
+    status: torch.Tensor  # int32 [G * beams], 0 = ok
+
+
+def beam_candidates(logits: torch.Tensor, scores: torch.Tensor, *, candidates: int | None = None,
+                    allow_mask: torch.Tensor | None = None,
+                    done: torch.Tensor | None = None) -> BeamCandidates:
+    """The best of ``scores[g, k] + log_softmax(logits[g, k])[v]`` over the
+    beams k and tokens v of each group g, in one read of the logits ([G * K, V]
+    or [G, K, V] bf16 / fp16 / fp32, any strides but the columns'; ``scores``
+    fp32 [G, K]; as many as ``candidates``, by default 2 K, at most 64).  They
+    are ordered in 64 bits; equal ones by beam, then by token.  A beam whose
+    score is -inf, and the beams of a group that is ``done`` (bool [G]), are not
+    read.  ``allow_mask``: packed rows [G * K, >= ceil(V / 32)], as
+    :func:`sample`'s; the softmax is over all tokens."""
+    n = 2 * scores.shape[-1] if candidates is None else int(candidates)
+    return BeamCandidates(*load().beam_candidates(logits, scores, n, allow_mask, done,
+                                                  _stream(logits)))
+
+
+class BeamAdvance(NamedTuple):
+    tokens: torch.Tensor       # int64 [G * K], what each slot goes on with
+    parents: torch.Tensor      # int32 [G * K], the row that each slot continues
+    scores: torch.Tensor       # fp32 [G, K]; -inf: a dead beam
+    pool_scores: torch.Tensor  # fp32 [G, K], finished ones' score / length, best first
+    pool_rows: torch.Tensor    # int32 [G, K], the row that ended; -1: empty
+    pool_steps: torch.Tensor   # int32 [G, K], at which step; -1: empty
+    done: torch.Tensor         # bool [G]
+
+
+def beam_advance(candidates: BeamCandidates, scores: torch.Tensor, pool_scores: torch.Tensor,
+                 pool_rows: torch.Tensor, pool_steps: torch.Tensor, done: torch.Tensor, *,
+                 eos_token_id: int, pad_token_id: int, length: float, step: int,
+                 early_stopping: bool = False, tokens_out: torch.Tensor | None = None,
+                 parents_out: torch.Tensor | None = None) -> BeamAdvance:
+    """Moves every group on by its candidates (include/graspo_tokpath.h has the
+    rules), into new tensors; ``length`` is what finished scores are divided
+    by.  ``tokens_out`` and ``parents_out``: written in the new ones' place."""
+    c = candidates
+    return BeamAdvance(*load().beam_advance(
+        c.scores, c.beams, c.tokens, scores, pool_scores, pool_rows, pool_steps, done,
+        int(eos_token_id), int(pad_token_id), float(length), int(step), bool(early_stopping),
+        tokens_out, parents_out, _stream(scores)))
+
+
+def beam_step(logits: torch.Tensor, scores: torch.Tensor, pool_scores: torch.Tensor,
+              pool_rows: torch.Tensor, pool_steps: torch.Tensor, done: torch.Tensor, *,
+              eos_token_id: int, pad_token_id: int, length: float, step: int,
+              early_stopping: bool = False, allow_mask: torch.Tensor | None = None,
+              tokens_out: torch.Tensor | None = None, parents_out: torch.Tensor | None = None
+              ) -> tuple[BeamAdvance, torch.Tensor]:
+    """:func:`beam_candidates` (2 K of them) and :func:`beam_advance` in two
+    launches; also the rows' status."""
+    out = load().beam_step(
+        logits, scores, pool_scores, pool_rows, pool_steps, done, 2 * scores.shape[-1],
+        int(eos_token_id), int(pad_token_id), float(length), int(step), bool(early_stopping),
+        allow_mask, tokens_out, parents_out, _stream(logits))
+    return BeamAdvance(*out[:7]), out[7]
+
+
+def beam_finish(scores: torch.Tensor, pool_scores: torch.Tensor, pool_rows: torch.Tensor,
+                pool_steps: torch.Tensor, done: torch.Tensor, tokens: torch.Tensor,
+                parents: torch.Tensor, *, length: float, eos_token_id: int, pad_token_id: int,
+                give: int):
+    """The ``give`` best hypotheses of each group after the steps whose tokens
+    (int64 [T, G * K]) and parents (int32) are given, beams that still go on
+    among them at score / ``length``: (scores fp32 [G, give], lengths int32, -inf
+    and 0 where there is none, tokens int64 [G, give, T] padded behind)."""
+    return load().beam_finish(scores, pool_scores, pool_rows, pool_steps, done, tokens, parents,
+                              float(length), int(eos_token_id), int(pad_token_id), int(give),
+                              _stream(scores))
+
+
+def reorder_states_(states, parents: torch.Tensor, beams: int, *, check: bool = True) -> None:
+    """Row r of every tensor of ``states`` becomes, in place, what row
+    ``parents[r]`` was (int32 [G * beams], within r's group of ``beams`` rows,
+    at most 64).  ``check`` waits for the GPU and raises where one is not; such
+    a row stays as it was."""
+    if states:
+        load().reorder_states_(states, parents, int(beams), check, _stream(states[0]))
+
+
+def expand_states(states, beams: int) -> list[torch.Tensor]:
+    """``t.repeat_interleave(beams, 0)`` of every tensor, each read once."""
+    return load().expand_states(states, int(beams), _stream(states[0])) if states else []

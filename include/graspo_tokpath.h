@@ -729,6 +729,138 @@ int gtp_grad_norm(const void* const* tensors, const int64_t* sizes, const int32_
 int gtp_clip_grads(void* const* tensors, const int64_t* sizes, const int32_t* dtypes,
                    int64_t count, const float* norm, float max_norm, void* stream);
 
+/*
+ * One step of a beam search over vocabulary-wide logits.  The reference's
+ * generation loops sample only (models/qwen3/adapter.py:259-318): these have
+ * no counterpart there.  With logits x [G, K, V] and the beams' running scores
+ * [G, K], the candidates of a group are
+ *
+ *   c[k, v] = scores[k] + x[k, v] - log sum_w exp x[k, w]
+ *
+ * for every token v that the row's mask allows, x[k, v] > -inf, beams with a
+ * finite score, groups that are not done; the rows of the others are not read.
+ * Candidates are ordered by c (in 64 bits, from a sum of fp32 exponentials),
+ * then by beam, then by token; scores are given rounded to fp32.
+ *
+ *   logits      group_stride and beam_stride apart (elements; 0 where beams
+ *               share a row), unit column stride, any alignment of whole
+ *               elements
+ *   allow_mask  packed as gtp_sample_rows' is, [G * K] rows of mask_stride
+ *               32-bit words, or NULL
+ *   done        [G], or NULL: no group is
+ * beams <= 32, candidates <= 64 (2 * beams leave `beams` live ones).
+ */
+typedef struct gtp_beam_rows {
+  const void* logits;
+  const uint32_t* allow_mask;
+  const float* scores;
+  const uint8_t* done;
+  int64_t groups, vocab;
+  int64_t group_stride, beam_stride, mask_stride;
+  int32_t dtype, beams, candidates;
+} gtp_beam_rows;
+
+/*
+ * gtp_beam_candidates -- the `candidates` best of each group: out_scores fp32,
+ * out_beams int32 (in [0, beams)) and out_tokens int64, [G, candidates], best
+ * first; where there are fewer: -inf, -1, -1.  out_status [G * K] (or NULL):
+ * GTP_ROW_NONFINITE for a live row with a NaN or +inf (it has no candidate) or
+ * a score that is NaN or +inf, GTP_ROW_EMPTY for one without an allowed token.
+ * The workspace (gtp_beam_workspace_bytes, 8-byte aligned, here and in
+ * gtp_beam_step) carries nothing between calls.
+ */
+size_t gtp_beam_workspace_bytes(const gtp_beam_rows* rows);
+int gtp_beam_candidates(const gtp_beam_rows* rows, float* out_scores, int32_t* out_beams,
+                        int64_t* out_tokens, int32_t* out_status, void* workspace,
+                        size_t workspace_bytes, void* stream);
+
+/*
+ * What a group is moved on from, and to (all device pointers, [G, K] but done
+ * [G]; outputs must not overlap inputs).  The pool holds the finished
+ * hypotheses, best first: score / length, the row (g K + k) whose end-of-
+ * sequence token finished it, and at which step; -inf, -1, -1 where empty.
+ *
+ * In the candidates' order, of the first K those whose token is eos_token_id
+ * join the pool at score / length (the K best are kept; of equal ones the
+ * earlier), and the first K others become the beams.  A beam's best child keeps
+ * its slot, the rest take the free slots in order: out_parents (rows) maps a
+ * group onto itself with parents[parents[r]] = parents[r].  Slots without a
+ * candidate are dead: pad_token_id, their own row, -inf.  A group is done when
+ * its pool is full and early_stopping is set or no live beam's score / length
+ * is above the pool's last, and when no beam is left; one that was done before
+ * gets pad_token_id, its own rows, and all else as it was.
+ */
+typedef struct gtp_beam_state {
+  const float* scores;
+  const float* pool_scores;
+  const int32_t* pool_rows;
+  const int32_t* pool_steps;
+  const uint8_t* done;
+  int64_t* out_tokens;
+  int32_t* out_parents;
+  float* out_scores;
+  float* out_pool_scores;
+  int32_t* out_pool_rows;
+  int32_t* out_pool_steps;
+  uint8_t* out_done;
+  int64_t eos_token_id, pad_token_id;
+  double length;          /* (step + 1)^length_penalty, > 0 and finite */
+  int32_t step;           /* tokens generated before */
+  int32_t early_stopping;
+} gtp_beam_state;
+
+/* gtp_beam_advance -- by the candidates that gtp_beam_candidates gave. */
+int gtp_beam_advance(const float* scores, const int32_t* beams, const int64_t* tokens,
+                     int64_t groups, int32_t num_beams, int32_t candidates,
+                     const gtp_beam_state* state, void* stream);
+
+/* gtp_beam_step -- both in two launches; rows' scores and done are the state's. */
+int gtp_beam_step(const gtp_beam_rows* rows, const gtp_beam_state* state, int32_t* out_status,
+                  void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * gtp_beam_finish -- the `give` <= K best hypotheses of each group after `steps`
+ * steps: the pool's, and of groups that are not done the live beams' at
+ * score / length.  tokens and parents [steps, G * K] are what the steps gave.
+ * out_scores and out_lengths [G, give] (-inf and 0 where there is none),
+ * out_tokens [G * give] rows of `steps` tokens out_stride apart, the
+ * end-of-sequence token last and pad_token_id behind it.
+ */
+int gtp_beam_finish(const float* scores, const float* pool_scores, const int32_t* pool_rows,
+                    const int32_t* pool_steps, const uint8_t* done, const int64_t* tokens,
+                    const int32_t* parents, int64_t groups, int32_t num_beams, int32_t steps,
+                    double length, int64_t eos_token_id, int64_t pad_token_id, int32_t give,
+                    float* out_scores, int32_t* out_lengths, int64_t* out_tokens,
+                    int64_t out_stride, void* stream);
+
+/*
+ * The states of a model (a layer's keys and values, recurrent states), whose
+ * first dimension counts rows, as bytes: a row is sizes[3] x .. x sizes[0] runs
+ * of run_bytes each, strides bytes apart (sizes of 1 where there are fewer
+ * dimensions; strides may be in any order, runs must not overlap).
+ */
+#define GTP_STATE_DIMS 4
+typedef struct gtp_state_shape {
+  int64_t run_bytes;
+  int64_t row_stride;
+  int64_t sizes[GTP_STATE_DIMS], strides[GTP_STATE_DIMS];
+} gtp_state_shape;
+
+/*
+ * gtp_reorder_states -- in place: row r of each of `count` tensors of one shape
+ * (`tensors` is a HOST array, read during the call) becomes row parents[r], for
+ * the groups * beams rows r, all at once.  parents[r] lies in r's group of
+ * `beams` rows; where it does not, the row stays and *bad (or NULL; the caller
+ * zeroes it) is set to 1.  The tensors must not overlap.  beams <= 64.
+ * gtp_expand_states -- outs[i] [groups * beams] contiguous rows: row
+ * g * beams + k is row g of tensors[i].
+ */
+int gtp_reorder_states(void* const* tensors, int64_t count, const gtp_state_shape* shape,
+                       const int32_t* parents, int64_t groups, int32_t beams, int32_t* bad,
+                       void* stream);
+int gtp_expand_states(const void* const* tensors, void* const* outs, int64_t count,
+                      const gtp_state_shape* shape, int64_t groups, int32_t beams, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
