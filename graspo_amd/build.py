@@ -27,7 +27,7 @@ HIP_SOURCES = ["tokpath_logprob.hip", "tokpath_sampler.hip", "tokpath_sampler_fa
                "tokpath_loss.hip", "tokpath_decode.hip",
                "tokpath_narrow.hip", "tokpath_lmhead.hip", "tokpath_linear.hip",
                "tokpath_embedding.hip", "tokpath_gradnorm.hip", "tokpath_beam.hip",
-               "tokpath_states.hip"]
+               "tokpath_states.hip", "tokpath_lora.hip"]
 HIP_FLAGS = [
     "--offload-arch=gfx950",
     "-O3",

@@ -1,0 +1,898 @@
+// tokpath_lora.hip -- low-rank adapters of many requests beside a shared projection (gfx950).
+//
+// Row n with adapter e = id[n] and scale s_e:
+//   u = s_e x A_e^T            [N, r]       out = base + u B_e^T     [N, O]
+// and, with g the gradient of out,
+//   v = s_e g B_e              [N, r]       dx  = v A_e              [N, K]
+//   dA_e = sum_n v_n^T x_n     [r, K]       dB_e = sum_n g_n^T u_n   [O, r]
+// (base's gradient is g).  r is small: every product reads or writes one long
+// matrix once and is bound by that, so there are three kernels, each on the
+// matrix cores (16x16x32 for 16-bit types, 16x16x4 for fp32):
+//
+// - shrink_kernel: rows x long axis -> [rows, r], the long axis split over
+//   waves and workgroups, fp32 partial sums.
+// - expand_kernel: [rows, r] -> rows x long axis, added to base.
+// - outer_kernel: two tall matrices -> [r, long], rows split over workgroups.
+//
+// Rows are sorted by adapter on the device (plan_kernel: a stable counting sort
+// of the requests), each adapter's run padded to whole tiles, so a tile has one
+// adapter and every sum an order that the ids fix.
+//
+// u and v are fp32 sums.  As 16-bit operands they are two parts, hi + lo (16
+// bits or more of them): rounded once, u alone would cost as much as the
+// output's own rounding where base is small.
+#include "tokpath_gemm.h"
+
+namespace gtp {
+namespace lora {
+
+using gemm::f32x4;
+using gemm::s16x8;
+
+constexpr int kWaves = 4;
+constexpr int kBlock = kWaves * kWave;
+constexpr int kMaxAdapters = 1024;
+constexpr int kMaxRank = 256;
+constexpr int kRankStep = 64;   // of shrink and outer
+
+template <typename T>
+struct Mat;
+template <>
+struct Mat<uint16_t> {
+  static constexpr int kE = 8;       // values per 16 bytes
+  static constexpr int kParts = 2;   // of a low-rank operand
+  __device__ static __forceinline__ f32x4 mma(u32x4 a, u32x4 b, f32x4 c) {
+    return gemm::Bf16::mul(__builtin_bit_cast(s16x8, a), __builtin_bit_cast(s16x8, b), c);
+  }
+  __device__ static __forceinline__ float to(uint16_t v) { return gemm::Bf16::to(v); }
+  __device__ static __forceinline__ uint16_t from(float v) { return gemm::Bf16::from(v); }
+};
+template <>
+struct Mat<_Float16> {
+  static constexpr int kE = 8;
+  static constexpr int kParts = 2;
+  __device__ static __forceinline__ f32x4 mma(u32x4 a, u32x4 b, f32x4 c) {
+    return gemm::F16::mul(__builtin_bit_cast(s16x8, a), __builtin_bit_cast(s16x8, b), c);
+  }
+  __device__ static __forceinline__ float to(_Float16 v) { return (float)v; }
+  __device__ static __forceinline__ _Float16 from(float v) { return (_Float16)v; }
+};
+template <>
+struct Mat<float> {
+  static constexpr int kE = 4;
+  static constexpr int kParts = 1;
+  __device__ static __forceinline__ f32x4 mma(u32x4 a, u32x4 b, f32x4 c) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      c = __builtin_amdgcn_mfma_f32_16x16x4f32(u2f(a[j]), u2f(b[j]), c, 0, 0, 0);
+    return c;
+  }
+  __device__ static __forceinline__ float to(float v) { return v; }
+  __device__ static __forceinline__ float from(float v) { return v; }
+};
+
+template <typename T>
+struct __attribute__((packed, aligned(sizeof(T)))) Any16 {
+  u32x4 v;
+};
+
+// kE values from p, of which `left` are there; the others are zeros.
+template <typename T>
+__device__ __forceinline__ u32x4 load16(const T* p, int64_t left) {
+  constexpr int E = Mat<T>::kE;
+  if (left >= E) return reinterpret_cast<const Any16<T>*>(p)->v;
+  u32x4 v = {0u, 0u, 0u, 0u};
+#pragma unroll
+  for (int j = 0; j < E; ++j) {
+    if (j >= left) break;
+    if constexpr (E == 4)
+      v[j] = __builtin_bit_cast(uint32_t, p[j]);
+    else
+      v[j / 2] |= (uint32_t)__builtin_bit_cast(uint16_t, p[j]) << (16 * (j & 1));
+  }
+  return v;
+}
+template <typename T>
+__device__ __forceinline__ void store16(T* p, u32x4 v, int64_t left) {
+  constexpr int E = Mat<T>::kE;
+  if (left >= E) {
+    reinterpret_cast<Any16<T>*>(p)->v = v;
+    return;
+  }
+#pragma unroll
+  for (int j = 0; j < E; ++j) {
+    if (j >= left) break;
+    if constexpr (E == 4)
+      p[j] = u2f(v[j]);
+    else
+      p[j] = __builtin_bit_cast(T, (uint16_t)(v[j / 2] >> (16 * (j & 1))));
+  }
+}
+
+// ------------------------------------------------------------------- plan
+// Where the rows are in the order of adapters: position p in [0, tiles * T).
+// Classes: adapters 0 .. E-1, E: rows without one, E + 1: bad ids.
+// In memory (int32): start[E + 3] (an adapter's first position; the last: the
+// end), rows[E + 2], first[E + 2] (its first request in `order`), order[B],
+// adapter[tiles] (-1: no tile).
+
+// Each adapter's scale, or one for all, and where the forward puts them: what
+// reads them later, the backward too, has them from there.
+struct Scale {
+  const float* each;
+  float all;
+  float* to;
+};
+
+struct Plan {
+  const int32_t* mem;  // null: all rows in order, adapter 0
+  int32_t N, B, S, T, E, tiles;
+
+  __host__ __device__ static int64_t words(int64_t B, int64_t E, int64_t tiles) {
+    return 3 * (E + 3) + B + tiles;
+  }
+  __device__ __forceinline__ const int32_t* start() const { return mem; }
+  __device__ __forceinline__ const int32_t* rows() const { return mem + E + 3; }
+  __device__ __forceinline__ const int32_t* first() const { return mem + 2 * (E + 3); }
+  __device__ __forceinline__ const int32_t* order() const { return mem + 3 * (E + 3); }
+  __device__ __forceinline__ const int32_t* adapter() const { return order() + B; }
+  // tile t's class, -1 where there is no such tile
+  __device__ __forceinline__ int tile(int t) const { return mem ? adapter()[t] : 0; }
+  // the row at position p of class e, -1 behind its last
+  __device__ __forceinline__ int row(int p, int e) const {
+    if (!mem) return p < N ? p : -1;
+    const int j = p - start()[e];
+    if (j >= rows()[e]) return -1;
+    const int b = j / S;
+    return order()[first()[e] + b] * S + (j - b * S);
+  }
+};
+
+constexpr int kPlanBlock = 1024;
+constexpr int kPlanWaves = kPlanBlock / kWave;
+
+// Wave w sorts requests [w B/16, (w + 1) B/16): it counts them by class, the
+// counts are summed class by class, and it puts them down in order.
+__global__ __launch_bounds__(kPlanBlock) void plan_kernel(const void* ids, int ids64, int B, int S,
+                                                          int T, int E, int tiles, int32_t* mem) {
+  extern __shared__ int32_t count[];  // [classes][waves]
+  __shared__ int32_t begin[kMaxAdapters + 2];
+  const int classes = E + 2, lane = threadIdx.x & (kWave - 1), w = threadIdx.x / kWave;
+  int32_t* start = mem;
+  int32_t* rows = mem + E + 3;
+  int32_t* first = mem + 2 * (E + 3);
+  int32_t* order = mem + 3 * (E + 3);
+  int32_t* adapter = order + B;
+  for (int i = threadIdx.x; i < classes * kPlanWaves; i += kPlanBlock) count[i] = 0;
+  for (int i = threadIdx.x; i < tiles; i += kPlanBlock) adapter[i] = -1;
+  __syncthreads();
+  const int share = (B + kPlanWaves - 1) / kPlanWaves;
+  const int from = w * share < B ? w * share : B, to = from + share < B ? from + share : B;
+  auto class_of = [&](int i) {
+    const int64_t id = ids64 ? reinterpret_cast<const int64_t*>(ids)[i]
+                             : (int64_t)reinterpret_cast<const int32_t*>(ids)[i];
+    return id >= 0 && id < E ? (int)id : id == -1 ? E : E + 1;
+  };
+  // lanes with this lane's class
+  auto alike = [&](int c, bool in) {
+    uint64_t m = __ballot(in);
+    for (int b = 0; (1 << b) < classes; ++b) {
+      const uint64_t on = __ballot((c >> b) & 1);
+      m &= (c >> b) & 1 ? on : ~on;
+    }
+    return m;
+  };
+  const uint64_t below = (1ull << lane) - 1;
+  for (int i = from; i < to; i += kWave) {
+    const bool in = i + lane < to;
+    const int c = in ? class_of(i + lane) : 0;
+    const uint64_t m = alike(c, in);
+    if (in && (m & below) == 0) count[c * kPlanWaves + w] += __popcll(m);
+    wave_lds_sync();
+  }
+  __syncthreads();
+  // exclusive sums: of the requests, and of the positions
+  int base = 0;
+  int64_t pos = 0;
+  if (threadIdx.x < kWave) {
+    for (int c0 = 0; c0 < classes; c0 += kWave) {
+      const int c = c0 + lane;
+      int n = 0;
+      if (c < classes)
+        for (int k = 0; k < kPlanWaves; ++k) n += count[c * kPlanWaves + k];
+      const int padded = (int)(((int64_t)n * S + T - 1) / T * T);
+      int a = n, p = padded;
+      for (int o = 1; o < kWave; o <<= 1) {
+        const int x = __shfl_up(a, o, kWave), y = __shfl_up(p, o, kWave);
+        if (lane >= o) {
+          a += x;
+          p += y;
+        }
+      }
+      if (c < classes) {
+        begin[c] = base + a - n;
+        first[c] = base + a - n;
+        rows[c] = n * S;
+        start[c] = (int)pos + p - padded;
+        if (c == classes - 1) start[classes] = (int)pos + p;
+        for (int t = 0; t < padded / T; ++t) adapter[((int)pos + p - padded) / T + t] = c;
+      }
+      base += __shfl(a, kWave - 1, kWave);
+      pos += __shfl(p, kWave - 1, kWave);
+    }
+  }
+  __syncthreads();
+  for (int c = threadIdx.x; c < classes; c += kPlanBlock) {
+    int at = begin[c];
+    for (int k = 0; k < kPlanWaves; ++k) {
+      const int n = count[c * kPlanWaves + k];
+      count[c * kPlanWaves + k] = at;
+      at += n;
+    }
+  }
+  __syncthreads();
+  for (int i = from; i < to; i += kWave) {
+    const bool in = i + lane < to;
+    const int c = in ? class_of(i + lane) : 0;
+    const uint64_t m = alike(c, in);
+    if (in) order[count[c * kPlanWaves + w] + __popcll(m & below)] = i + lane;
+    wave_lds_sync();
+    if (in && (m & below) == 0) count[c * kPlanWaves + w] += __popcll(m);
+    wave_lds_sync();
+  }
+}
+
+// ----------------------------------------------------------------- shrink
+
+// low[split][position][r] = rows . W_e[r]: x [N, C] against W [E, r, C], both
+// along C.  A step is 128 bytes of each row: quad q of the wave takes 32 of
+// them, as two 16-byte operands, so that a row's four lanes read a whole line.
+template <typename T, int RB, int NB>
+__global__ __launch_bounds__(kBlock) void shrink_kernel(Plan plan, const T* x, int64_t ld,
+                                                        const T* W, int C, int r, int splits,
+                                                        float* low, Scale scale) {
+  constexpr int E = Mat<T>::kE;
+  constexpr int kSteps = RB == 1 ? 4 : 1;  // loaded at a time
+  constexpr int kRows = RB * 16;
+  __shared__ int rows[kRows];
+  __shared__ float sum[kRows][NB * 16 + 1];
+  const int lane = threadIdx.x & (kWave - 1), w = threadIdx.x / kWave;
+  const int split = blockIdx.x % splits, tile = blockIdx.x / splits;
+  const int r0 = blockIdx.y * kRankStep;
+  if (scale.to && blockIdx.x == 0 && blockIdx.y == 0)
+    for (int i = threadIdx.x; i < plan.E; i += kBlock)
+      scale.to[i] = scale.each ? scale.each[i] : scale.all;
+  const int e = plan.tile(tile);
+  if (e < 0 || e >= plan.E) return;
+  if (threadIdx.x < kRows) rows[threadIdx.x] = plan.row(tile * kRows + threadIdx.x, e);
+  __syncthreads();
+  const int m = lane & 15, q = lane >> 4;
+  const T* px[RB];
+#pragma unroll
+  for (int b = 0; b < RB; ++b) {
+    // (a tile's first row is there; rows that are not repeat it)
+    const int row = rows[b * 16 + m] < 0 ? rows[0] : rows[b * 16 + m];
+    px[b] = x + row * ld + q * 2 * E;
+  }
+  const T* pw[NB];
+#pragma unroll
+  for (int b = 0; b < NB; ++b) {
+    const int i = r0 + b * 16 + m < r ? r0 + b * 16 + m : r - 1;
+    pw[b] = W + ((int64_t)e * r + i) * C + q * 2 * E;
+  }
+  const int steps = (C + 8 * E - 1) / (8 * E), shares = splits * kWaves;
+  const int share = (steps + shares - 1) / shares;
+  const int from = (split * kWaves + w) * share;
+  const int to = from + share < steps ? from + share : steps;
+  f32x4 acc[RB][NB];
+#pragma unroll
+  for (int a = 0; a < RB; ++a)
+#pragma unroll
+    for (int b = 0; b < NB; ++b) acc[a][b] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  for (int s0 = from; s0 < to; s0 += kSteps) {
+    u32x4 vx[kSteps][RB][2], vw[kSteps][NB][2];
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i) {
+      const int64_t c = (int64_t)(s0 + i) * 8 * E;
+      const int64_t left = s0 + i < to ? C - c - q * 2 * E : 0;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+#pragma unroll
+        for (int b = 0; b < RB; ++b) vx[i][b][h] = load16(px[b] + c + h * E, left - h * E);
+#pragma unroll
+        for (int b = 0; b < NB; ++b) vw[i][b][h] = load16(pw[b] + c + h * E, left - h * E);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int a = 0; a < RB; ++a)
+#pragma unroll
+          for (int b = 0; b < NB; ++b)
+            acc[a][b] = Mat<T>::mma(vx[i][a][h], vw[i][b][h], acc[a][b]);
+  }
+  // acc[a][b][i]: row 16 a + 4 q + i, rank 16 b + m; the waves' sums in order
+  for (int k = 0; k < kWaves; ++k) {
+    if (w == k) {
+#pragma unroll
+      for (int a = 0; a < RB; ++a)
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            float& s = sum[a * 16 + 4 * q + i][b * 16 + m];
+            s = k == 0 ? acc[a][b][i] : s + acc[a][b][i];
+          }
+    }
+    __syncthreads();
+  }
+  const int n = r - r0 < kRankStep ? r - r0 : kRankStep;
+  float* to_low = low + ((int64_t)split * plan.tiles + tile) * kRows * r + r0;
+  for (int i = threadIdx.x; i < kRows * n; i += kBlock)
+    to_low[(int64_t)(i / n) * r + i % n] = sum[i / n][i % n];
+}
+
+// a low-rank value: the splits' sum, scaled
+__device__ __forceinline__ float low_at(const float* low, int64_t split_stride, int splits,
+                                        int64_t at, float scale) {
+  float s = low[at];
+  for (int k = 1; k < splits; ++k) s += low[at + k * split_stride];
+  return s * scale;
+}
+
+// ----------------------------------------------------------------- expand
+
+// out[row] = base[row] + low[position] W_e^T: W [E, C, r].  The long axis is
+// the product's M: lane (m, q) of a strip of 64 bytes holds 16 consecutive
+// bytes of row m.  Contraction units of 16 bytes: the hi part's, then the lo
+// part's (which meet the same W).
+template <typename T, int RB>
+__global__ __launch_bounds__(kBlock) void expand_kernel(Plan plan, const float* low, int splits,
+                                                        const float* scales, const T* W, int C,
+                                                        int r, const T* base, int64_t ld_base,
+                                                        T* out, int strips, int blocks) {
+  constexpr int E = Mat<T>::kE, P = Mat<T>::kParts, MB = E / 4;
+  constexpr int kRows = RB * 16;
+  constexpr int kStrip = 4 * E;  // columns
+  extern __shared__ u32x4 frags[];  // [kRows][units + 1]
+  __shared__ int rows[kRows];
+  const int lane = threadIdx.x & (kWave - 1), w = threadIdx.x / kWave;
+  const int block = blockIdx.x % blocks, tile = blockIdx.x / blocks;
+  const int e = plan.tile(tile);
+  if (e < 0) return;
+  if (threadIdx.x < kRows) rows[threadIdx.x] = plan.row(tile * kRows + threadIdx.x, e);
+  const int chunks = (r + E - 1) / E, units = P * chunks, ld = units + 1;
+  const bool adapted = e < plan.E;
+  if (adapted) {
+    const float scale = scales[e];
+    const int64_t split_stride = (int64_t)plan.tiles * kRows * r;
+    T* f = reinterpret_cast<T*>(frags);
+    for (int i = threadIdx.x; i < kRows * chunks * E; i += kBlock) {
+      const int n = i / (chunks * E), k = i % (chunks * E);
+      const float v = k < r ? low_at(low, split_stride, splits,
+                                     ((int64_t)tile * kRows + n) * r + k, scale)
+                            : 0.0f;
+      const T hi = Mat<T>::from(v);
+      f[(int64_t)n * ld * E + k] = hi;
+      if constexpr (P == 2)
+        f[(int64_t)n * ld * E + chunks * E + k] = Mat<T>::from(v - Mat<T>::to(hi));
+    }
+  }
+  __syncthreads();
+  const int m = lane & 15, q = lane >> 4;
+  int row[RB];
+#pragma unroll
+  for (int b = 0; b < RB; ++b) row[b] = rows[b * 16 + m];
+  const int last = (block + 1) * strips * kWaves;
+  for (int strip = block * strips * kWaves + w; strip < last; strip += kWaves) {
+    const int64_t c0 = (int64_t)strip * kStrip;
+    if (c0 >= C) break;
+    const int64_t c = c0 + q * E, left = C - c;
+    u32x4 vb[RB];
+    if (base) {
+#pragma unroll
+      for (int b = 0; b < RB; ++b)
+        vb[b] = row[b] >= 0 ? load16(base + row[b] * ld_base + c, left) : u32x4{0u, 0u, 0u, 0u};
+    }
+    f32x4 acc[RB][MB];
+#pragma unroll
+    for (int a = 0; a < RB; ++a)
+#pragma unroll
+      for (int b = 0; b < MB; ++b) acc[a][b] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    if (adapted) {
+      const T* pw[MB];
+#pragma unroll
+      for (int b = 0; b < MB; ++b) {
+        // M index m of block b is column E (m / 4) + 4 b + m % 4 of the strip
+        int64_t o = c0 + E * (m >> 2) + 4 * b + (m & 3);
+        if (o >= C) o = C - 1;
+        pw[b] = W + ((int64_t)e * C + o) * r;
+      }
+      for (int u0 = 0; u0 < units; u0 += 4) {
+        const int u = u0 + q, k = u >= chunks ? u - chunks : u;
+        const bool in = u < units;
+        u32x4 vw[MB], vl[RB];
+#pragma unroll
+        for (int b = 0; b < MB; ++b) vw[b] = load16(pw[b] + k * E, in ? r - k * E : 0);
+#pragma unroll
+        for (int a = 0; a < RB; ++a)
+          vl[a] = in ? frags[(a * 16 + m) * ld + u] : u32x4{0u, 0u, 0u, 0u};
+#pragma unroll
+        for (int a = 0; a < RB; ++a)
+#pragma unroll
+          for (int b = 0; b < MB; ++b) acc[a][b] = Mat<T>::mma(vw[b], vl[a], acc[a][b]);
+      }
+    }
+    if (left <= 0) continue;
+    const float bad = e > plan.E ? __builtin_nanf("") : 0.0f;
+#pragma unroll
+    for (int a = 0; a < RB; ++a) {
+      if (row[a] < 0) continue;
+      u32x4 v;
+#pragma unroll
+      for (int j = 0; j < E; j += (E == 4 ? 1 : 2)) {
+        if constexpr (E == 4) {
+          v[j] = f2u(acc[a][0][j] + (base ? u2f(vb[a][j]) : 0.0f) + bad);
+        } else {
+          float y[2];
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const float old = base ? Mat<T>::to(__builtin_bit_cast(
+                                         T, (uint16_t)(vb[a][j / 2] >> (16 * h))))
+                                   : 0.0f;
+            y[h] = acc[a][(j + h) / 4][(j + h) % 4] + old + bad;
+          }
+          v[j / 2] = (uint32_t)__builtin_bit_cast(uint16_t, Mat<T>::from(y[0])) |
+                     (uint32_t)__builtin_bit_cast(uint16_t, Mat<T>::from(y[1])) << 16;
+        }
+      }
+      store16(out + (int64_t)row[a] * C + c, v, left);
+    }
+  }
+}
+
+// --------------------------------------------- small pieces of the backward
+
+// out [E][b][a] from in [E][a][b]
+template <typename T>
+__global__ __launch_bounds__(kBlock) void turn_kernel(const T* in, T* out, int64_t n, int a, int b) {
+  const int64_t i = (int64_t)blockIdx.x * kBlock + threadIdx.x;
+  if (i >= n) return;
+  const int64_t e = i / ((int64_t)a * b), k = i - e * a * b;
+  const int64_t y = k / a, x = k - y * a;
+  out[i] = in[e * a * b + x * b + y];
+}
+
+// The low-rank rows along the positions, as outer_kernel reads them: to
+// [parts][r][positions], zeros where there is no row of an adapter.
+template <typename T>
+__global__ __launch_bounds__(kBlock) void turn_low_kernel(Plan plan, const float* low, int splits,
+                                                          const float* scales, int r, T* to) {
+  constexpr int P = Mat<T>::kParts;
+  const int64_t n = (int64_t)plan.tiles * plan.T;
+  const int64_t i = (int64_t)blockIdx.x * kBlock + threadIdx.x;
+  if (i >= n * r) return;
+  const int64_t k = i / n, p = i - k * n;
+  const int e = plan.tile((int)(p / plan.T));
+  float v = 0.0f;
+  if (e >= 0 && e < plan.E && plan.row((int)p, e) >= 0)
+    v = low_at(low, n * r, splits, p * r + k, scales[e]);
+  const T hi = Mat<T>::from(v);
+  to[i] = hi;
+  if constexpr (P == 2) to[n * r + i] = Mat<T>::from(v - Mat<T>::to(hi));
+}
+
+// ------------------------------------------------------------------ outer
+
+// One of a backward's two: y [N, C] and low [parts][r][positions].
+struct Side {
+  const void* y;
+  const void* low;
+  float* part;  // [slots][r][C]
+  int64_t ld;
+  int32_t C, blocks;  // workgroups along C
+};
+
+// part[slot][k][c] = sum over a chunk's rows of one adapter of low[k] y[c].
+// Chunk i and adapter e have slot i + e: the next one in the order of positions
+// has one of the two raised.  A step is 32 rows: lane (m, q) loads 16 bytes of
+// rows 8 q .. 8 q + 7, which turned around are the rows' axis of kE operands.
+template <typename T, int NB>
+__global__ __launch_bounds__(kBlock) void outer_kernel(Plan plan, Side one, Side two, int r,
+                                                       int chunk) {
+  constexpr int E = Mat<T>::kE, P = Mat<T>::kParts;
+  constexpr int kCols = 16 * E;
+  __shared__ float sum[16][kCols + 4];
+  const int lane = threadIdx.x & (kWave - 1), w = threadIdx.x / kWave;
+  const int all = one.blocks + two.blocks;
+  const int i = blockIdx.x / all, at = blockIdx.x % all;
+  const Side s = at < one.blocks ? one : two;
+  const int c0 = (at < one.blocks ? at : at - one.blocks) * kCols;
+  const int r0 = blockIdx.y * kRankStep;
+  const int64_t n = (int64_t)plan.tiles * plan.T;
+  const int m = lane & 15, q = lane >> 4;
+  const T* y = reinterpret_cast<const T*>(s.y) + c0 + m * E;
+  const T* low = reinterpret_cast<const T*>(s.low);
+  const int64_t left = s.C - c0 - m * E;
+  const int begin = i * chunk;
+  const int end = plan.mem ? plan.start()[plan.E] : plan.N;  // of the adapters' rows
+  int stop = begin + chunk < end ? begin + chunk : end;
+  for (int p = begin; p < stop;) {
+    const int e = plan.tile(p / plan.T);
+    int to = plan.mem ? plan.start()[e] + plan.rows()[e] : end;  // the adapter's last row
+    const int next = plan.mem ? plan.start()[e + 1] : end;
+    if (to > stop) to = stop;
+    f32x4 acc[E][NB];
+#pragma unroll
+    for (int a = 0; a < E; ++a)
+#pragma unroll
+      for (int b = 0; b < NB; ++b) acc[a][b] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    const int share = ((to - p + kWaves - 1) / kWaves + 31) / 32 * 32;
+    const int mine = p + w * share, until = mine + share < to ? mine + share : to;
+    for (int s0 = mine; s0 < until; s0 += 32) {
+      u32x4 v[8], vl[NB][P][2];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const int at_p = s0 + q * 8 + k;
+        const int row = at_p < until ? plan.row(at_p, e) : -1;
+        v[k] = row >= 0 ? load16(y + row * s.ld, left) : u32x4{0u, 0u, 0u, 0u};
+      }
+#pragma unroll
+      for (int b = 0; b < NB; ++b) {
+        const int k = r0 + b * 16 + m;
+        // (positions behind the last tile's end are none of the wave's rows)
+        const bool in = k < r && s0 + q * 8 < until;
+        const T* pl = low + (int64_t)(in ? k : 0) * n + s0 + q * 8;
+#pragma unroll
+        for (int h = 0; h < P; ++h)
+          vl[b][h][0] = load16(pl + h * n * r, in ? E : 0);
+        if constexpr (E == 4) vl[b][0][1] = load16(pl + 4, in ? E : 0);
+      }
+      if constexpr (E == 8) {
+        // 8 x 8 values turned: operand j has column 8 m + j of the 8 rows
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          u32x4 o;
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            o[k] = __builtin_amdgcn_perm(v[2 * k + 1][j / 2], v[2 * k][j / 2],
+                                         j & 1 ? 0x07060302u : 0x05040100u);
+#pragma unroll
+          for (int b = 0; b < NB; ++b)
+#pragma unroll
+            for (int h = 0; h < P; ++h) acc[j][b] = Mat<T>::mma(o, vl[b][h][0], acc[j][b]);
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const u32x4 o = {v[4 * h][j], v[4 * h + 1][j], v[4 * h + 2][j], v[4 * h + 3][j]};
+#pragma unroll
+            for (int b = 0; b < NB; ++b) acc[j][b] = Mat<T>::mma(o, vl[b][0][h], acc[j][b]);
+          }
+      }
+    }
+    // acc[j][b][k]: rank 16 b + m, column E (4 q + k) + j; the waves' in order
+    float* part = s.part + (int64_t)(i + e) * r * s.C;
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+      for (int wave = 0; wave < kWaves; ++wave) {
+        if (w == wave) {
+#pragma unroll
+          for (int j = 0; j < E; ++j)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              float& t = sum[m][E * (4 * q + k) + j];
+              t = wave == 0 ? acc[j][b][k] : t + acc[j][b][k];
+            }
+        }
+        __syncthreads();
+      }
+      for (int t = threadIdx.x; t < 16 * kCols; t += kBlock) {
+        const int k = r0 + b * 16 + t / kCols, c = c0 + t % kCols;
+        if (k < r && c < s.C) part[(int64_t)k * s.C + c] = sum[t / kCols][t % kCols];
+      }
+      __syncthreads();
+    }
+    p = next;
+  }
+}
+
+// grad [E][r][C] (turned: [E][C][r]) from the slots' sums, in order
+template <typename T>
+__global__ __launch_bounds__(kBlock) void outer_sum_kernel(Plan plan, const float* part, int r,
+                                                           int C, int chunk, int turned, T* grad) {
+  const int64_t each = (int64_t)r * C, t = (int64_t)blockIdx.x * kBlock + threadIdx.x;
+  if (t >= each * plan.E) return;
+  const int e = (int)(t / each);
+  int64_t k = t - e * each;
+  const int64_t at = k;
+  if (turned) k = (at % r) * C + at / r;
+  const int from = plan.mem ? plan.start()[e] : 0;
+  const int n = plan.mem ? plan.rows()[e] : plan.N;
+  float s = 0.0f;
+  if (n > 0)
+    for (int i = from / chunk; i <= (from + n - 1) / chunk; ++i) s += part[(i + e) * each + k];
+  grad[e * each + at] = Mat<T>::from(s);
+}
+
+// ------------------------------------------------------------------- host
+
+// Sizes that the launches and the workspaces go by.
+struct Sizes {
+  int32_t T, tiles, splits_x, splits_g;
+  int64_t plan_bytes, scale_bytes, low_bytes;  // low: the forward's partial sums
+};
+
+int64_t round_up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
+
+// Workgroups for the chip, of at least 4 steps of 128 bytes for each wave.
+int32_t splits_of(int64_t tiles, int64_t C, int64_t size) {
+  const int64_t steps = (C * size + 127) / 128;
+  int64_t s = (768 + tiles - 1) / tiles, most = (steps + 4 * kWaves - 1) / (4 * kWaves);
+  if (s > most) s = most;
+  return (int32_t)(s < 1 ? 1 : s);
+}
+
+Sizes sizes_of(const gtp_lora* q) {
+  Sizes z;
+  const int64_t N = q->requests * q->rows, size = q->dtype == GTP_DTYPE_F32 ? 4 : 2;
+  // (and what a tile's low-rank rows take of LDS: 33 KB at a rank of 128)
+  z.T = N <= 1024 || q->rank > 128 ? 16 : 64;
+  int64_t runs = q->adapters + 2 < q->requests ? q->adapters + 2 : q->requests;
+  z.tiles = (int32_t)((N + z.T - 1) / z.T + (q->ids ? runs : 0));
+  z.splits_x = splits_of(z.tiles, q->in, size);
+  z.splits_g = splits_of(z.tiles, q->out, size);
+  z.plan_bytes = q->ids ? round_up(Plan::words(q->requests, q->adapters, z.tiles) * 4, 256) : 0;
+  z.scale_bytes = round_up((int64_t)q->adapters * 4, 256);
+  z.low_bytes = round_up((int64_t)z.splits_x * z.tiles * z.T * q->rank * 4, 256);
+  return z;
+}
+
+int check(const gtp_lora* q) {
+  if (!q || q->requests < 0 || q->rows < 0 || q->in < 1 || q->out < 1 || q->rank < 1 ||
+      q->adapters < 1)
+    return GTP_ERR_INVALID_ARGUMENT;
+  if (q->dtype != GTP_DTYPE_F32 && q->dtype != GTP_DTYPE_BF16 && q->dtype != GTP_DTYPE_F16)
+    return GTP_ERR_INVALID_ARGUMENT;
+  if (!q->ids && q->adapters != 1 && q->requests > 0 && q->rows > 0) return GTP_ERR_INVALID_ARGUMENT;
+  if (q->rank > kMaxRank || q->adapters > kMaxAdapters || q->in > (1 << 24) ||
+      q->out > (1 << 24) || q->requests > (1 << 24) || q->rows > (1 << 24) ||
+      q->requests * q->rows > (1 << 24) - 131072 ||
+      (int64_t)q->adapters * q->rank * (q->in > q->out ? q->in : q->out) > (1ll << 38))
+    return GTP_ERR_UNSUPPORTED;
+  return GTP_OK;
+}
+
+bool aligned(const void* p, uintptr_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; }
+
+Plan plan_of(const gtp_lora* q, const Sizes& z, const void* state) {
+  Plan p;
+  p.mem = q->ids ? reinterpret_cast<const int32_t*>(state) : nullptr;
+  p.B = (int32_t)q->requests;
+  p.S = (int32_t)q->rows;
+  p.N = p.B * p.S;
+  p.T = z.T;
+  p.E = q->adapters;
+  p.tiles = z.tiles;
+  return p;
+}
+
+template <typename T, int RB>
+void shrink(const Plan& p, const T* x, int64_t ld, const T* W, int64_t C, int r, int splits,
+            float* low, Scale scale, hipStream_t s) {
+  const dim3 grid((uint32_t)((int64_t)p.tiles * splits), (uint32_t)((r + kRankStep - 1) / kRankStep));
+  if (r <= 16)
+    hipLaunchKernelGGL((shrink_kernel<T, RB, 1>), grid, dim3(kBlock), 0, s, p, x, ld, W, (int)C, r,
+                       splits, low, scale);
+  else if (r <= 32)
+    hipLaunchKernelGGL((shrink_kernel<T, RB, 2>), grid, dim3(kBlock), 0, s, p, x, ld, W, (int)C, r,
+                       splits, low, scale);
+  else
+    hipLaunchKernelGGL((shrink_kernel<T, RB, 4>), grid, dim3(kBlock), 0, s, p, x, ld, W, (int)C, r,
+                       splits, low, scale);
+}
+template <typename T>
+void shrink(const Plan& p, const T* x, int64_t ld, const T* W, int64_t C, int r, int splits,
+            float* low, Scale scale, hipStream_t s) {
+  if (p.T == 16) shrink<T, 1>(p, x, ld, W, C, r, splits, low, scale, s);
+  else shrink<T, 4>(p, x, ld, W, C, r, splits, low, scale, s);
+}
+
+template <typename T>
+void expand(const Plan& p, const float* low, int splits, const float* scales, const T* W, int64_t C, int r,
+            const T* base, int64_t ld_base, T* out, hipStream_t s) {
+  constexpr int E = Mat<T>::kE, P = Mat<T>::kParts;
+  const int64_t wave_strips = (C + 4 * E * kWaves - 1) / (4 * E * kWaves);
+  // strips per wave: fewer where there are few tiles
+  int64_t blocks = (2048 + p.tiles - 1) / p.tiles;
+  if (blocks > wave_strips) blocks = wave_strips;
+  const int strips = (int)((wave_strips + blocks - 1) / blocks);
+  blocks = (wave_strips + strips - 1) / strips;
+  const size_t lds = (size_t)p.T * (P * ((r + E - 1) / E) + 1) * 16;
+  const dim3 grid((uint32_t)(p.tiles * blocks));
+  if (p.T == 16)
+    hipLaunchKernelGGL((expand_kernel<T, 1>), grid, dim3(kBlock), lds, s, p, low, splits, scales, W,
+                       (int)C, r, base, ld_base, out, strips, (int)blocks);
+  else
+    hipLaunchKernelGGL((expand_kernel<T, 4>), grid, dim3(kBlock), lds, s, p, low, splits, scales, W,
+                       (int)C, r, base, ld_base, out, strips, (int)blocks);
+}
+
+template <typename T>
+void forward(const gtp_lora* q, const Sizes& z, char* state, hipStream_t s) {
+  const Plan p = plan_of(q, z, state);
+  if (q->ids)
+    hipLaunchKernelGGL(plan_kernel, dim3(1), dim3(kPlanBlock),
+                       (size_t)(q->adapters + 2) * kPlanWaves * 4, s, q->ids, (int)q->ids_int64,
+                       p.B, p.S, p.T, p.E, p.tiles, reinterpret_cast<int32_t*>(state));
+  float* scales = reinterpret_cast<float*>(state + z.plan_bytes);
+  float* low = reinterpret_cast<float*>(state + z.plan_bytes + z.scale_bytes);
+  shrink<T>(p, reinterpret_cast<const T*>(q->x), q->x_stride, reinterpret_cast<const T*>(q->a),
+            q->in, q->rank, z.splits_x, low, Scale{q->scales, q->scale, scales}, s);
+  expand<T>(p, low, z.splits_x, scales, reinterpret_cast<const T*>(q->b), q->out, q->rank,
+            reinterpret_cast<const T*>(q->base), q->base_stride, reinterpret_cast<T*>(q->y), s);
+}
+
+// The backward's workspace.
+struct Work {
+  int64_t turned_a, turned_b, low_v, low_tu, low_tv, part_a, part_b, bytes;
+  int chunk, chunks;
+};
+
+Work work_of(const gtp_lora* q, const Sizes& z) {
+  Work k;
+  const int64_t size = q->dtype == GTP_DTYPE_F32 ? 4 : 2, parts = size == 4 ? 1 : 2;
+  const int64_t n = (int64_t)z.tiles * z.T, r = q->rank, E = q->adapters;
+  int64_t at = 0;
+  auto take = [&](int64_t bytes) {
+    const int64_t here = at;
+    at += round_up(bytes, 256);
+    return here;
+  };
+  k.turned_a = take(E * r * q->in * size);
+  k.turned_b = take(E * r * q->out * size);
+  k.low_v = take((int64_t)z.splits_g * n * r * 4);
+  k.low_tu = take(n * r * size * parts);
+  k.low_tv = take(n * r * size * parts);
+  // chunks of rows: workgroups for the chip, of at least 128 rows
+  const int64_t cols = 16 * (16 / size), blocks = (q->in + cols - 1) / cols + (q->out + cols - 1) / cols;
+  int64_t chunks = (1024 + blocks - 1) / blocks;
+  if (chunks > (n + 127) / 128) chunks = (n + 127) / 128;
+  if (chunks < 1) chunks = 1;
+  k.chunk = (int)round_up((n + chunks - 1) / chunks, z.T < 64 ? 64 : z.T);
+  k.chunks = (int)((n + k.chunk - 1) / k.chunk);
+  k.part_a = take((k.chunks + E) * r * q->in * 4);
+  k.part_b = take((k.chunks + E) * r * q->out * 4);
+  k.bytes = at;
+  return k;
+}
+
+template <typename T>
+void backward(const gtp_lora* q, const gtp_lora_grads* d, const Sizes& z, const char* state,
+              char* ws, hipStream_t s) {
+  constexpr int E = Mat<T>::kE;
+  const Plan p = plan_of(q, z, state);
+  const Work k = work_of(q, z);
+  const float* scales = reinterpret_cast<const float*>(state + z.plan_bytes);
+  const float* low_u = reinterpret_cast<const float*>(state + z.plan_bytes + z.scale_bytes);
+  float* low_v = reinterpret_cast<float*>(ws + k.low_v);
+  T* turned_b = reinterpret_cast<T*>(ws + k.turned_b);
+  const int r = q->rank;
+  const int64_t na = (int64_t)p.E * r * q->in, nb = (int64_t)p.E * r * q->out;
+  const int64_t nl = (int64_t)p.tiles * p.T * r;
+  auto blocks_of = [](int64_t n) { return dim3((uint32_t)((n + kBlock - 1) / kBlock)); };
+  if (d->grad_x || d->grad_a) {
+    hipLaunchKernelGGL(turn_kernel<T>, blocks_of(nb), dim3(kBlock), 0, s,
+                       reinterpret_cast<const T*>(q->b), turned_b, nb, (int)q->out, r);
+    shrink<T>(p, reinterpret_cast<const T*>(d->grad), d->grad_stride, turned_b, q->out, r,
+              z.splits_g, low_v, Scale{nullptr, 0.0f, nullptr}, s);
+  }
+  if (d->grad_x) {
+    T* turned_a = reinterpret_cast<T*>(ws + k.turned_a);
+    hipLaunchKernelGGL(turn_kernel<T>, blocks_of(na), dim3(kBlock), 0, s,
+                       reinterpret_cast<const T*>(q->a), turned_a, na, r, (int)q->in);
+    expand<T>(p, low_v, z.splits_g, scales, turned_a, q->in, r, static_cast<const T*>(nullptr),
+              0, reinterpret_cast<T*>(d->grad_x), s);
+  }
+  if (!d->grad_a && !d->grad_b) return;
+  T* tu = reinterpret_cast<T*>(ws + k.low_tu);
+  T* tv = reinterpret_cast<T*>(ws + k.low_tv);
+  float* part_a = reinterpret_cast<float*>(ws + k.part_a);
+  float* part_b = reinterpret_cast<float*>(ws + k.part_b);
+  const int64_t cols = 16 * E;
+  Side a{q->x, tv, part_a, q->x_stride, (int32_t)q->in, 0};
+  Side b{d->grad, tu, part_b, d->grad_stride, (int32_t)q->out, 0};
+  if (d->grad_a) {
+    a.blocks = (int32_t)((q->in + cols - 1) / cols);
+    hipLaunchKernelGGL(turn_low_kernel<T>, blocks_of(nl), dim3(kBlock), 0, s, p, low_v, z.splits_g,
+                       scales, r, tv);
+  }
+  if (d->grad_b) {
+    b.blocks = (int32_t)((q->out + cols - 1) / cols);
+    hipLaunchKernelGGL(turn_low_kernel<T>, blocks_of(nl), dim3(kBlock), 0, s, p, low_u, z.splits_x,
+                       scales, r, tu);
+  }
+  const dim3 grid((uint32_t)((int64_t)k.chunks * (a.blocks + b.blocks)),
+                  (uint32_t)((r + kRankStep - 1) / kRankStep));
+  if (r <= 16)
+    hipLaunchKernelGGL((outer_kernel<T, 1>), grid, dim3(kBlock), 0, s, p, a, b, r, k.chunk);
+  else if (r <= 32)
+    hipLaunchKernelGGL((outer_kernel<T, 2>), grid, dim3(kBlock), 0, s, p, a, b, r, k.chunk);
+  else
+    hipLaunchKernelGGL((outer_kernel<T, 4>), grid, dim3(kBlock), 0, s, p, a, b, r, k.chunk);
+  if (d->grad_a)
+    hipLaunchKernelGGL(outer_sum_kernel<T>, blocks_of(na), dim3(kBlock), 0, s, p, part_a, r,
+                       (int)q->in, k.chunk, 0, reinterpret_cast<T*>(d->grad_a));
+  if (d->grad_b)
+    hipLaunchKernelGGL(outer_sum_kernel<T>, blocks_of(nb), dim3(kBlock), 0, s, p, part_b, r,
+                       (int)q->out, k.chunk, 1, reinterpret_cast<T*>(d->grad_b));
+}
+
+}  // namespace lora
+}  // namespace gtp
+
+using namespace gtp;
+
+extern "C" size_t gtp_lora_state_bytes(const gtp_lora* q) {
+  if (lora::check(q) != GTP_OK) return 0;
+  if (q->requests * q->rows == 0) return 256;
+  const lora::Sizes z = lora::sizes_of(q);
+  return (size_t)(z.plan_bytes + z.scale_bytes + z.low_bytes);
+}
+
+extern "C" int gtp_lora_add(const gtp_lora* q, void* state, size_t state_bytes, void* stream) {
+  const int rc = lora::check(q);
+  if (rc != GTP_OK) return rc;
+  const int64_t N = q->requests * q->rows;
+  if (N == 0) return GTP_OK;
+  const uintptr_t size = q->dtype == GTP_DTYPE_F32 ? 4 : 2;
+  if (!q->x || !q->a || !q->b || !q->base || !q->y || !state ||
+      q->x_stride < 0 || q->base_stride < 0 || state_bytes < gtp_lora_state_bytes(q) ||
+      !lora::aligned(state, 16) || !lora::aligned(q->scales, 4) || !lora::aligned(q->x, size) ||
+      !lora::aligned(q->a, size) || !lora::aligned(q->b, size) || !lora::aligned(q->base, size) ||
+      !lora::aligned(q->y, size) || (q->ids && !lora::aligned(q->ids, q->ids_int64 ? 8 : 4)))
+    return GTP_ERR_INVALID_ARGUMENT;
+  const lora::Sizes z = lora::sizes_of(q);
+  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  char* mem = reinterpret_cast<char*>(state);
+  if (q->dtype == GTP_DTYPE_BF16) lora::forward<uint16_t>(q, z, mem, s);
+  else if (q->dtype == GTP_DTYPE_F16) lora::forward<_Float16>(q, z, mem, s);
+  else lora::forward<float>(q, z, mem, s);
+  return hipGetLastError() == hipSuccess ? GTP_OK : GTP_ERR_LAUNCH;
+}
+
+extern "C" size_t gtp_lora_backward_workspace_bytes(const gtp_lora* q) {
+  if (lora::check(q) != GTP_OK) return 0;
+  if (q->requests * q->rows == 0) return 256;
+  return (size_t)lora::work_of(q, lora::sizes_of(q)).bytes;
+}
+
+extern "C" int gtp_lora_backward(const gtp_lora* q, const gtp_lora_grads* d, const void* state,
+                                 size_t state_bytes, void* workspace, size_t workspace_bytes,
+                                 void* stream) {
+  const int rc = lora::check(q);
+  if (rc != GTP_OK) return rc;
+  if (!d) return GTP_ERR_INVALID_ARGUMENT;
+  if (q->requests * q->rows == 0) return GTP_ERR_UNSUPPORTED;
+  const uintptr_t size = q->dtype == GTP_DTYPE_F32 ? 4 : 2;
+  if (!q->x || !q->a || !q->b || !d->grad || !state || !workspace ||
+      q->x_stride < 0 || d->grad_stride < 0 || state_bytes < gtp_lora_state_bytes(q) ||
+      workspace_bytes < gtp_lora_backward_workspace_bytes(q) || !lora::aligned(state, 16) ||
+      !lora::aligned(workspace, 256) || !lora::aligned(q->x, size) || !lora::aligned(q->a, size) || !lora::aligned(q->b, size) ||
+      !lora::aligned(d->grad, size) || (d->grad_x && !lora::aligned(d->grad_x, size)) ||
+      (d->grad_a && !lora::aligned(d->grad_a, size)) ||
+      (d->grad_b && !lora::aligned(d->grad_b, size)))
+    return GTP_ERR_INVALID_ARGUMENT;
+  const lora::Sizes z = lora::sizes_of(q);
+  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  const char* mem = reinterpret_cast<const char*>(state);
+  char* ws = reinterpret_cast<char*>(workspace);
+  if (q->dtype == GTP_DTYPE_BF16) lora::backward<uint16_t>(q, d, z, mem, ws, s);
+  else if (q->dtype == GTP_DTYPE_F16) lora::backward<_Float16>(q, d, z, mem, ws, s);
+  else lora::backward<float>(q, d, z, mem, ws, s);
+  return hipGetLastError() == hipSuccess ? GTP_OK : GTP_ERR_LAUNCH;
+}

@@ -7,7 +7,8 @@
 // lm_head_logprob, lm_head_logprob_save, softmax_grad_bf16, linear_logprob,
 // linear_logprob_backward, linear_loss, embedding, embedding_backward,
 // token_embedding, grad_norm, clip_grads_, clip_grad_norm_, beam_candidates,
-// beam_advance, beam_step, beam_finish, reorder_states_, expand_states}.  Each op validates
+// beam_advance, beam_step, beam_finish, reorder_states_, expand_states,
+// lora_add_state, lora_backward, lora_add}.  Each op validates
 // its tensors (TORCH_CHECK surfaces as a Python RuntimeError), allocates the
 // outputs on the logits' device, and enqueues the HIP kernels on the stream handle passed in from Python
 // (torch.cuda.current_stream().cuda_stream), so work orders with the
@@ -1701,7 +1702,222 @@ std::vector<at::Tensor> expand_states(at::TensorList states, int64_t beams, int6
   return outs;
 }
 
+// ------------------------------------------------- low-rank adapters
+
+// [..., n] as rows with unit column stride: their distance, or a copy
+at::Tensor as_rows(const at::Tensor& t, int64_t n, int64_t& stride) {
+  at::Tensor rows = t.reshape({-1, n});
+  if ((n > 1 && rows.stride(1) != 1) || (rows.size(0) > 1 && rows.stride(0) < 0)) rows = rows.contiguous();
+  stride = rows.size(0) > 1 ? rows.stride(0) : n;
+  return rows;
+}
+
+// x [..., K], a [E, r, K], b [E, N, r]; requests of as many rows each (none:
+// all rows have adapter 0 of 1)
+gtp_lora lora_of(const at::Tensor& x, const at::Tensor& a, const at::Tensor& b,
+                 c10::optional<int64_t> requests, const char* what) {
+  TORCH_CHECK(x.is_cuda() && x.dim() >= 1 && x.size(-1) > 0, "graspo_tokpath.", what,
+              ": x must be a [..., K] GPU tensor");
+  const int64_t K = x.size(-1);
+  for (const auto* t : {&a, &b}) {
+    check_same_device(x, *t, "the adapters");
+    TORCH_CHECK(t->scalar_type() == x.scalar_type() && t->dim() == 3 && t->is_contiguous(),
+                "graspo_tokpath.", what, ": adapters must be contiguous [E, r, K] and [E, N, r] of "
+                "x's dtype");
+  }
+  const int64_t E = a.size(0), r = a.size(1), N = b.size(1);
+  TORCH_CHECK(a.size(2) == K && b.size(0) == E && b.size(2) == r && E > 0 && r > 0 && N > 0,
+              "graspo_tokpath.", what, ": adapters ", a.sizes(), " and ", b.sizes(),
+              " do not go with x ", x.sizes());
+  TORCH_CHECK(r <= 256 && E <= 1024, "graspo_tokpath.", what,
+              ": at most 1024 adapters of rank 256, got ", E, " of ", r);
+  gtp_lora q{};
+  q.a = a.data_ptr();
+  q.b = b.data_ptr();
+  q.in = K;
+  q.out = N;
+  q.rank = (int32_t)r;
+  q.adapters = (int32_t)E;
+  q.dtype = dtype_code(x);
+  const int64_t rows = x.numel() / K;
+  if (requests.has_value()) {
+    TORCH_CHECK(*requests > 0 ? rows % *requests == 0 : rows == 0, "graspo_tokpath.", what, ": ",
+                rows, " rows are not those of ", *requests, " requests");
+    q.ids = &q;  // (there; the forward says where)
+    q.requests = *requests;
+    q.rows = q.requests > 0 ? rows / q.requests : 0;
+  } else {
+    TORCH_CHECK(E == 1, "graspo_tokpath.", what, ": ", E, " adapters and no adapter_ids");
+    q.requests = 1;
+    q.rows = rows;
+  }
+  return q;
+}
+
+// (base + s x a^T b^T, what the backward takes of it)
+std::tuple<at::Tensor, at::Tensor> lora_add_state(const at::Tensor& base, const at::Tensor& x,
+                                                  const at::Tensor& a, const at::Tensor& b,
+                                                  const c10::optional<at::Tensor>& ids,
+                                                  const c10::optional<at::Tensor>& scales,
+                                                  double scale, bool check, int64_t stream) {
+  c10::optional<int64_t> requests;
+  if (ids.has_value()) {
+    check_same_device(x, *ids, "adapter_ids");
+    TORCH_CHECK((ids->scalar_type() == at::kInt || ids->scalar_type() == at::kLong) &&
+                    ids->dim() == 1 && ids->is_contiguous(),
+                "graspo_tokpath.lora_add: adapter_ids must be contiguous int32 or int64 [requests]");
+    requests = ids->size(0);
+  }
+  gtp_lora q = lora_of(x, a, b, requests, "lora_add");
+  if (ids.has_value()) {
+    q.ids = ids->data_ptr();
+    q.ids_int64 = ids->scalar_type() == at::kLong;
+  }
+  q.scale = (float)scale;
+  if (scales.has_value()) {
+    check_same_device(x, *scales, "scaling");
+    TORCH_CHECK(scales->scalar_type() == at::kFloat && scales->dim() == 1 &&
+                    scales->size(0) == q.adapters && scales->is_contiguous(),
+                "graspo_tokpath.lora_add: scaling must be contiguous float32 [E]");
+    q.scales = scales->data_ptr<float>();
+  }
+  check_same_device(x, base, "base");
+  TORCH_CHECK(base.scalar_type() == x.scalar_type() && base.dim() == x.dim() &&
+                  base.sizes().slice(0, base.dim() - 1) == x.sizes().slice(0, x.dim() - 1) &&
+                  base.size(-1) == q.out,
+              "graspo_tokpath.lora_add: base must be [..., N] beside x [..., K], of its dtype; got ",
+              base.sizes(), " and ", x.sizes());
+  const c10::DeviceGuard guard(x.device());
+  const at::Tensor xr = as_rows(x, q.in, q.x_stride), br = as_rows(base, q.out, q.base_stride);
+  at::Tensor out = at::empty(base.sizes(), base.options());
+  q.x = xr.data_ptr();
+  q.base = br.data_ptr();
+  q.y = out.data_ptr();
+  at::Tensor state = at::empty({(int64_t)gtp_lora_state_bytes(&q)}, x.options().dtype(at::kByte));
+  void* st = reinterpret_cast<void*>(stream);
+  at::Tensor words, shifted;
+  check = check && ids.has_value() && q.requests * q.rows > 0 && !gtp_stream_capturing(st);
+  if (check) {
+    // (-1, no adapter, is one of the good ones)
+    shifted = at::add(*ids, 1);
+    words = verdict_words();
+    const int rc = gtp_targets_verdict(shifted.data_ptr(), q.ids_int64, q.requests, 1,
+                                       q.adapters + 1, nullptr, nullptr, verdict_ptr(words), st);
+    int found = 0;
+    if (rc == GTP_ERR_LAUNCH) verdict_wait(words, &found, st);
+    check_rc(rc, "gtp_targets_verdict");
+  }
+  const int rc = gtp_lora_add(&q, state.data_ptr(), (size_t)state.numel(), st);
+  int bad = 0, wait_rc = GTP_OK;
+  if (check) wait_rc = verdict_wait(words, &bad, st);
+  check_rc(rc, "gtp_lora_add");
+  check_rc(wait_rc, "gtp_verdict_wait");
+  TORCH_CHECK(!(bad & 1), "lora_add: an adapter id is outside [-1, ", q.adapters, ")");
+  return {out, state};
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor> lora_backward(
+    const at::Tensor& grad, const at::Tensor& x, const at::Tensor& a, const at::Tensor& b,
+    const at::Tensor& state, c10::optional<int64_t> requests, bool need_x, bool need_a, bool need_b,
+    int64_t stream) {
+  gtp_lora q = lora_of(x, a, b, requests, "lora_backward");
+  if (requests.has_value()) q.ids = state.data_ptr();
+  check_same_device(x, grad, "grad");
+  check_same_device(x, state, "state");
+  TORCH_CHECK(grad.scalar_type() == x.scalar_type() && grad.dim() >= 1 && grad.size(-1) == q.out &&
+                  grad.numel() == q.requests * q.rows * q.out,
+              "graspo_tokpath.lora_backward: grad must be the output's shape and dtype");
+  TORCH_CHECK(state.scalar_type() == at::kByte && state.is_contiguous() &&
+                  (size_t)state.numel() == gtp_lora_state_bytes(&q),
+              "graspo_tokpath.lora_backward: the state is not one of these sizes");
+  const c10::DeviceGuard guard(x.device());
+  const at::Tensor xr = as_rows(x, q.in, q.x_stride);
+  q.x = xr.data_ptr();
+  gtp_lora_grads d{};
+  const at::Tensor gr = as_rows(grad, q.out, d.grad_stride);
+  d.grad = gr.data_ptr();
+  at::Tensor gx, ga, gb;
+  const bool none = q.requests * q.rows == 0;
+  if (need_x) gx = at::empty(x.sizes(), x.options());
+  if (need_a) ga = none ? at::zeros(a.sizes(), a.options()) : at::empty(a.sizes(), a.options());
+  if (need_b) gb = none ? at::zeros(b.sizes(), b.options()) : at::empty(b.sizes(), b.options());
+  if (none || !(need_x || need_a || need_b)) return {gx, ga, gb};
+  d.grad_x = need_x ? gx.data_ptr() : nullptr;
+  d.grad_a = need_a ? ga.data_ptr() : nullptr;
+  d.grad_b = need_b ? gb.data_ptr() : nullptr;
+  at::Tensor ws = at::empty({(int64_t)gtp_lora_backward_workspace_bytes(&q)},
+                            x.options().dtype(at::kByte));
+  check_rc(gtp_lora_backward(&q, &d, state.data_ptr(), (size_t)state.numel(), ws.data_ptr(),
+                             (size_t)ws.numel(), reinterpret_cast<void*>(stream)),
+           "gtp_lora_backward");
+  return {gx, ga, gb};
+}
+
+struct LoraAdd : torch::autograd::Function<LoraAdd> {
+  static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& base,
+                            const at::Tensor& x, const at::Tensor& a, const at::Tensor& b,
+                            const c10::optional<at::Tensor>& ids,
+                            const c10::optional<at::Tensor>& scales, double scale, bool check,
+                            int64_t stream) {
+    auto [out, state] = lora_add_state(base, x, a, b, ids, scales, scale, check, stream);
+    // (the state holds the ids' order and the scales, which the caller may refill
+    // before the backward)
+    ctx->save_for_backward({x, a, b, state});
+    ctx->saved_data["requests"] = ids.has_value() ? ids->size(0) : -1;
+    ctx->saved_data["stream"] = stream;
+    return out;
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                 torch::autograd::variable_list grads) {
+    const char* what = "lora_add";
+    check_no_tangent(grads[0], what);
+    const auto saved = ctx->get_saved_variables();
+    c10::optional<int64_t> requests = ctx->saved_data["requests"].toInt();
+    if (*requests < 0) requests = c10::nullopt;
+    const bool nx = ctx->needs_input_grad(1), na = ctx->needs_input_grad(2),
+               nb = ctx->needs_input_grad(3);
+    // (the engine runs a node on its forward's stream)
+    auto [gx, ga, gb] = lora_backward(grads[0].detach(), saved[0].detach(), saved[1].detach(),
+                                      saved[2].detach(), saved[3], requests, nx, na, nb,
+                                      ctx->saved_data["stream"].toInt());
+    return {ctx->needs_input_grad(0) ? grads[0] : at::Tensor(),
+            once_only(gx, grads[0], what), once_only(ga, grads[0], what),
+            once_only(gb, grads[0], what), at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor(),
+            at::Tensor()};
+  }
+};
+
+at::Tensor lora_add(const at::Tensor& base, const at::Tensor& x, const at::Tensor& a,
+                    const at::Tensor& b, const c10::optional<at::Tensor>& ids,
+                    const c10::optional<at::Tensor>& scales, double scale, bool check,
+                    int64_t stream) {
+  bool grad = false;
+  for (const at::Tensor* t : {&base, &x, &a, &b}) {
+    check_no_tangent(*t, "lora_add");
+    grad = grad || t->requires_grad();
+  }
+  TORCH_CHECK(!scales.has_value() || !scales->requires_grad(),
+              "lora_add: the scaling has no gradient");
+  grad = grad && at::GradMode::is_enabled();
+  if (grad)
+    for (const at::Tensor* t : {&base, &x, &a, &b}) check_leaf(*t, "lora_add", stream);
+  // a single adapter without its dimension, and views of a larger tensor
+  const at::Tensor a3 = (a.dim() == 2 ? a.unsqueeze(0) : a).contiguous();
+  const at::Tensor b3 = (b.dim() == 2 ? b.unsqueeze(0) : b).contiguous();
+  if (grad) return LoraAdd::apply(base, x, a3, b3, ids, scales, scale, check, stream);
+  return std::get<0>(lora_add_state(base, x, a3, b3, ids, scales, scale, check, stream));
+}
+
 TORCH_LIBRARY(graspo_tokpath, m) {
+  m.def("lora_add_state(Tensor base, Tensor x, Tensor a, Tensor b, Tensor? ids, Tensor? scales, "
+        "float scale, bool check, int stream) -> (Tensor, Tensor)",
+        &lora_add_state);
+  m.def("lora_backward(Tensor grad, Tensor x, Tensor a, Tensor b, Tensor state, int? requests, "
+        "bool need_x, bool need_a, bool need_b, int stream) -> (Tensor, Tensor, Tensor)",
+        &lora_backward);
+  m.def("lora_add(Tensor base, Tensor x, Tensor a, Tensor b, Tensor? ids, Tensor? scales, "
+        "float scale, bool check, int stream) -> Tensor",
+        &lora_add);
   m.def(
       "beam_candidates(Tensor logits, Tensor scores, int candidates, Tensor? allow_mask, "
       "Tensor? done, int stream) -> (Tensor, Tensor, Tensor, Tensor)",

@@ -572,3 +572,38 @@ def reorder_states_(states, parents: torch.Tensor, beams: int, *, check: bool = 
 def expand_states(states, beams: int) -> list[torch.Tensor]:
     """``t.repeat_interleave(beams, 0)`` of every tensor, each read once."""
     return load().expand_states(states, int(beams), _stream(states[0])) if states else []
+
+
+def lora_add_state(base: torch.Tensor, x: torch.Tensor, lora_a: torch.Tensor,
+                   lora_b: torch.Tensor, *, adapter_ids: torch.Tensor | None = None,
+                   scales: torch.Tensor | None = None, scale: float = 1.0, check: bool = True):
+    """(``base + s_e (x a_e^T) b_e^T``, the state that :func:`lora_backward`
+    takes): x [..., K], base [..., N], ``lora_a`` [E, r, K], ``lora_b`` [E, N,
+    r] of one dtype; ``adapter_ids`` [requests], whose rows follow one another,
+    -1 for none (None: adapter 0 of 1); ``scales`` fp32 [E], else ``scale``.
+    ``check`` waits for a look at the ids and raises on one outside [-1, E);
+    without it, and in a graph capture, its rows are NaN."""
+    return load().lora_add_state(base, x, lora_a, lora_b, adapter_ids, scales, float(scale), check,
+                                 _stream(x))
+
+
+def lora_backward(grad: torch.Tensor, x: torch.Tensor, lora_a: torch.Tensor,
+                  lora_b: torch.Tensor, state: torch.Tensor, *, requests: int | None = None,
+                  need_x: bool = True, need_a: bool = True, need_b: bool = True):
+    """The gradients (x's, ``lora_a``'s, ``lora_b``'s; None for one not asked
+    for) of :func:`lora_add_state` from its state and output's ``grad``
+    (base's is ``grad`` itself); sums in fp32 in an order that the ids fix.
+    ``requests``: how many ids the forward had (None: it had none)."""
+    gx, ga, gb = load().lora_backward(grad, x, lora_a, lora_b, state, requests, need_x, need_a,
+                                      need_b, _stream(x))
+    return (gx if need_x else None), (ga if need_a else None), (gb if need_b else None)
+
+
+def lora_add(base: torch.Tensor, x: torch.Tensor, lora_a: torch.Tensor, lora_b: torch.Tensor, *,
+             adapter_ids: torch.Tensor | None = None, scales: torch.Tensor | None = None,
+             scale: float = 1.0, check: bool = True) -> torch.Tensor:
+    """:func:`lora_add_state`'s output, differentiable (once, backwards) in
+    base, x and the adapters (any strides; [r, K] and [N, r] of a single
+    one)."""
+    return load().lora_add(base, x, lora_a, lora_b, adapter_ids, scales, float(scale), check,
+                           _stream(x))

@@ -861,6 +861,67 @@ int gtp_reorder_states(void* const* tensors, int64_t count, const gtp_state_shap
 int gtp_expand_states(const void* const* tensors, void* const* outs, int64_t count,
                       const gtp_state_shape* shape, int64_t groups, int32_t beams, void* stream);
 
+/*
+ * Low-rank adapters of many requests beside a shared projection, as the
+ * reference's LoRALinear adds one (backends/graspoflow/lora.py:76): `requests`
+ * of `rows` rows each, request b with adapter e = ids[b] (-1: none),
+ *
+ *   y = base + scales[e] (x a_e^T) b_e^T
+ *
+ *   x     [requests * rows, in]   rows x_stride apart
+ *   base  [requests * rows, out]  rows base_stride apart: what the projection gave
+ *   y     [requests * rows, out]  contiguous; may be base where base is contiguous
+ *   a     [adapters, rank, in], b [adapters, out, rank], contiguous
+ *   scales [adapters] fp32, or NULL: `scale` for all
+ *   ids   [requests] int32 / int64, or NULL: all rows have adapter 0 of 1
+ * all of `dtype` but scales and ids, any alignment of whole elements.  Rows
+ * without an adapter are base's; an id outside [-1, adapters) gives rows of NaN.
+ * Sums in fp32; the rank-sized ones meet 16-bit operands as two 16-bit parts.
+ * rank <= 256, adapters <= 1024, in and out <= 2^24, requests * rows <= 2^24 -
+ * 2^17: others return GTP_ERR_UNSUPPORTED.
+ */
+typedef struct gtp_lora {
+  const void* x;
+  const void* base;
+  void* y;
+  const void* a;
+  const void* b;
+  const float* scales;
+  const void* ids;
+  int64_t requests, rows, in, out;
+  int64_t x_stride, base_stride;
+  int32_t dtype, ids_int64, rank, adapters;
+  float scale;
+} gtp_lora;
+
+/*
+ * gtp_lora_add -- y.  state (gtp_lora_state_bytes, 16-byte aligned) receives the
+ * rows' order by adapter, the scales and x a_e^T, which the backward takes;
+ * without one it is a workspace.
+ */
+size_t gtp_lora_state_bytes(const gtp_lora* lora);
+int gtp_lora_add(const gtp_lora* lora, void* state, size_t state_bytes, void* stream);
+
+/*
+ * gtp_lora_backward -- from grad, that of y ([requests * rows, out], rows
+ * grad_stride apart), the gradients of x [requests * rows, in], a and b,
+ * contiguous, each or NULL (base's is grad).  `lora` and `state` are the
+ * forward's (base, y and scales are not read, ids only for being there); rows without
+ * an adapter and those of a bad id have no part in a's and b's.  Every sum has
+ * an order that the ids fix.  The workspace (256-byte aligned) carries nothing
+ * between calls.  Without a row: GTP_ERR_UNSUPPORTED.
+ */
+typedef struct gtp_lora_grads {
+  const void* grad;
+  int64_t grad_stride;
+  void* grad_x;
+  void* grad_a;
+  void* grad_b;
+} gtp_lora_grads;
+size_t gtp_lora_backward_workspace_bytes(const gtp_lora* lora);
+int gtp_lora_backward(const gtp_lora* lora, const gtp_lora_grads* grads, const void* state,
+                      size_t state_bytes, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
