@@ -7,10 +7,12 @@
 //
 // - beam_slices_kernel: each wave streams a slice of one row once.  A chunk of
 //   2048 16-bit (1024 fp32) logits is folded into a running sum of exponentials
-//   (one reference for the wave, in base 2), and whatever lies above the slice's
-//   running threshold is appended to a list in LDS by ballots; past 96 entries
-//   the list is cut to its n best and the threshold rises to the last of them.
-//   Within a row the order by logit is the order by score, so n per slice do.
+//   (one reference for the wave, in base 2).  Of what lies above the slice's
+//   running threshold only the vector of 8 (4) is noted, by a ballot; 64 of them
+//   are read again at a time, a lane each, and their values above the threshold
+//   listed; the list is cut to about its n best and the threshold rises to the
+//   last of them.  Within a row the order by logit is the order by score, so n
+//   per slice do.
 // - beam_merge_kernel: a workgroup per group turns the slices' sums into each
 //   row's log-sum-exp in 64 bits (scores of different beams are compared, and
 //   a sum rounded to 32 bits would decide near-ties), takes the n best of
@@ -26,12 +28,12 @@ namespace beam {
 constexpr int kWaves = 4;
 constexpr int kBlock = kWaves * kWave;
 constexpr int kU = 4;           // 16-byte vectors per lane and chunk
-constexpr int kCap = 640;       // list entries per wave: kCut and the 512 of an append
-constexpr int kCut = 96;        // entries from which on the list is cut
+constexpr int kNoted = 320;     // vectors noted per wave: 63 and a chunk's 256
+constexpr int kCap = 640;       // list entries per wave: kMaxSlots and a batch's 512
 constexpr int kMaxN = 64;       // candidates: one lane each
 constexpr int kMaxK = 32;
-constexpr int kMaxKeys = 8192;  // K S n: at most 32 per thread of the merge
-constexpr uint32_t kOrdNegInf = 0x007FFFFFu;  // ord32(-inf)
+constexpr int kMaxSlots = 80;   // keys that a slice gives: n and up to a quarter or half more
+constexpr int kMaxKeys = 8192;  // K S slots: what the merge holds in registers
 
 struct Rows {
   const void* x;
@@ -39,9 +41,9 @@ struct Rows {
   const float* score;    // [G, K]
   const uint8_t* done;   // [G] or null
   int64_t V, group_stride, beam_stride, mask_stride;  // mask_stride in bytes
-  int32_t G, K, n, S;
+  int32_t G, K, n, S, slots;
   int64_t L;             // a slice's logits, a multiple of 512
-  uint64_t* keys;        // [G K S n]
+  uint64_t* keys;        // [G K S slots], 0: none
   float2* sums;          // [G K S]: maximum, sum
 };
 
@@ -53,84 +55,76 @@ __device__ __forceinline__ float residual(float m) {
   return by_fma(m) ? __builtin_fmaf(m, kLog2e, -(m * kLog2e)) : 0.0f;
 }
 
+// How many of the mask's lanes lie below this one.
+__device__ __forceinline__ int lanes_below(uint64_t mask) {
+  return __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32),
+                                   __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0u));
+}
+
 // A beam that goes on: a finite score in a group that is not done.
 __device__ __forceinline__ bool live(const Rows& r, int row) {
   return !(r.done && r.done[row / r.K]) && __builtin_fabsf(r.score[row]) < kPosInf;
 }
 
-// The n best of a wave's list, in no order, and the threshold that they set.
-// count, tau and the list are the same for all lanes.
+// A wave's list of what lay above its threshold: cut to the best, in no order,
+// when it grows.  count, tau and the list are the same for all lanes.
 struct Top {
   uint64_t* list;
   int count;
   float tau;
 
-  // the largest T with at least n keys >= T; n keys exactly stop the search
-  template <typename Count>
-  __device__ __forceinline__ static uint64_t cut_at(int n, Count count_from) {
-    uint64_t T = 0;
-    for (int b = 63; b >= 0; --b) {
-      const uint64_t t = T | (1ull << b);
-      const int c = count_from(t);
-      if (c >= n) T = t;
-      if (c == n) break;
-    }
-    return T;
-  }
-
-  __device__ __forceinline__ void cut(int n, int lane) {
-    if (count <= n) return;
+  // Keeps the best, n to slots of them (count > slots).  most: no value lies
+  // above it.  Which of the others stay makes no difference to the n best, and
+  // few halvings end between n and slots.
+  __device__ __forceinline__ void cut(int n, int slots, float most, int lane) {
     wave_lds_sync();
-    uint64_t T;
-    if (count <= 2 * kWave) {
-      const uint64_t a = lane < count ? list[lane] : 0;
-      const uint64_t b = lane + kWave < count ? list[lane + kWave] : 0;
-      T = cut_at(n, [&](uint64_t t) {
-        return __popcll(__ballot(a >= t)) + __popcll(__ballot(b >= t));
-      });
-      wave_lds_sync();
-      const uint64_t ka = __ballot(a >= T), kb = __ballot(b >= T);
-      const uint64_t below = (1ull << lane) - 1;
-      if (a >= T) list[__popcll(ka & below)] = a;
-      if (b >= T) list[__popcll(ka) + __popcll(kb & below)] = b;
-      count = __popcll(ka) + __popcll(kb);
-    } else {
-      // rows of many equal logits
-      const int m = count;
-      T = cut_at(n, [&](uint64_t t) {
-        int c = 0;
-        for (int i = 0; i < m; i += kWave)
-          c += __popcll(__ballot(i + lane < m && list[i + lane] >= t));
-        return c;
-      });
-      int kept = 0;
-      for (int i = 0; i < m; i += kWave) {
-        const uint64_t a = i + lane < m ? list[i + lane] : 0;
-        const uint64_t ka = __ballot(a >= T);
-        wave_lds_sync();
-        if (a >= T) list[kept + __popcll(ka & ((1ull << lane) - 1))] = a;
-        wave_lds_sync();
-        kept += __popcll(ka);
+    // up to 128 entries two per lane; more are read again for each count
+    const bool few = count <= 2 * kWave;
+    const uint64_t a = lane < count ? list[lane] : 0;
+    const uint64_t b = lane + kWave < count ? list[lane + kWave] : 0;
+    auto at_least = [&](uint64_t t) {
+      int c = __popcll(__ballot(a >= t)) + __popcll(__ballot(b >= t));
+      if (!few)
+        for (int i = 2 * kWave; i < count; i += kWave)
+          c += __popcll(__ballot(i + lane < count && list[i + lane] >= t));
+      return __builtin_amdgcn_readfirstlane(c);
+    };
+    // between the threshold and the largest, by the first 32 bits
+    uint32_t lo = __builtin_amdgcn_readfirstlane(ord32(tau));
+    uint32_t hi = __builtin_amdgcn_readfirstlane(ord32(most + 0.0f));
+    int c = count;
+    while (lo < hi && c > slots) {
+      const uint32_t mid = lo + (hi - lo + 1) / 2;
+      const int m = at_least((uint64_t)mid << 32);
+      if (m >= n) {
+        lo = mid;
+        c = m;
+      } else {
+        hi = mid - 1;
       }
-      count = kept;
     }
-    // what comes later has a larger token id: only more than the last counts
-    const uint32_t hi = (uint32_t)(T >> 32);
-    tau = hi <= kOrdNegInf ? kNegInf : unord32(hi);
-  }
-
-  // Appends y[j] (token id0 + j) where it lies above the threshold.
-  template <int E>
-  __device__ __forceinline__ void append(const float (&y)[E], int32_t id0, int n, int lane) {
-#pragma unroll
-    for (int j = 0; j < E; ++j) {
-      const bool in = y[j] > tau;
-      const uint64_t at = __ballot(in);
-      if (at == 0) continue;
-      if (in) list[count + __popcll(at & ((1ull << lane) - 1))] = rank_key(y[j] + 0.0f, id0 + j);
-      count += __popcll(at);
+    uint64_t T = (uint64_t)lo << 32;
+    // many equal ones: the lowest tokens of them
+    for (int i = 31; i >= 0 && c > slots; --i) {
+      const uint64_t t = T | (1ull << i);
+      const int m = at_least(t);
+      if (m >= n) {
+        T = t;
+        c = m;
+      }
     }
-    if (count > kCut) cut(n, lane);
+    int kept = 0;
+    for (int i = 0; i < count; i += kWave) {
+      const uint64_t x = i + lane < count ? list[i + lane] : 0;
+      wave_lds_sync();
+      const uint64_t k = __ballot(x >= T);
+      if (x >= T) list[kept + lanes_below(k)] = x;
+      wave_lds_sync();
+      kept += __popcll(k);
+    }
+    count = kept;
+    // (n entries lie at lo or above, and what comes later has a larger token)
+    tau = unord32(lo);
   }
 };
 
@@ -139,79 +133,159 @@ struct __attribute__((packed, aligned(sizeof(T)))) Unaligned {
   u32x4 v;
 };
 
-// The slice's vector at element e (E elements); what lies past `end` is -inf.
+// The vector at element i of a row, as far as `end`; what lies past it is -inf.
 template <typename T>
-__device__ __forceinline__ u32x4 load_vec(const T* row, int64_t e, int64_t end) {
-  constexpr int E = Vec<T>::kE;
-  if (e + E <= end) return reinterpret_cast<const Unaligned<T>*>(row + e)->v;
+__device__ __forceinline__ u32x4 load_vec(const T* row, int64_t i, int64_t end) {
+  constexpr int E = Vec<T>::kE, kBits = 8 * sizeof(T);
   constexpr uint32_t kNone = sizeof(T) == 4 ? 0xFF800000u
-                             : __is_same(T, _Float16) ? 0xFC00u : 0xFF80u;
-  u32x4 v;
-#pragma unroll
-  for (int w = 0; w < 4; ++w) {
-    if constexpr (sizeof(T) == 4) {
-      v[w] = e + w < end ? __builtin_bit_cast(uint32_t, row[e + w]) : kNone;
-    } else {
-      const uint32_t lo = e + 2 * w < end ? __builtin_bit_cast(uint16_t, row[e + 2 * w]) : kNone;
-      const uint32_t hi = e + 2 * w + 1 < end ? __builtin_bit_cast(uint16_t, row[e + 2 * w + 1]) : kNone;
-      v[w] = lo | hi << 16;
+                             : __is_same(T, _Float16) ? 0xFC00FC00u : 0xFF80FF80u;
+  u32x4 v = {kNone, kNone, kNone, kNone};
+  if (i + E <= end) return reinterpret_cast<const Unaligned<T>*>(row + i)->v;
+  if (i >= end) return v;
+  // one element on: towards the first, or the last
+  auto down = [](u32x4 x, uint32_t in) {
+    if constexpr (kBits == 32) return u32x4{x[1], x[2], x[3], in};
+    else
+      return u32x4{x[0] >> 16 | x[1] << 16, x[1] >> 16 | x[2] << 16, x[2] >> 16 | x[3] << 16,
+                   x[3] >> 16 | in << 16};
+  };
+  if (end >= E) {
+    // the row's last E, moved down to begin with element i
+    v = reinterpret_cast<const Unaligned<T>*>(row + end - E)->v;
+#pragma unroll 1
+    for (int64_t k = i + E - end; k > 0; --k) v = down(v, kNone);
+  } else {
+    // (a row of fewer than E)
+#pragma unroll 1
+    for (int j = 0; j < E; ++j) {
+      uint32_t x = kNone;
+      if (j < end) {
+        if constexpr (kBits == 32) x = __builtin_bit_cast(uint32_t, row[j]);
+        else x = __builtin_bit_cast(uint16_t, row[j]);
+      }
+      v = down(v, x);
     }
   }
   return v;
 }
 
+// The float below t (not below -inf), for "more than that" in "at least t"'s place.
+__device__ __forceinline__ float below(float t) {
+  const uint32_t u = f2u(t);
+  if (t == kNegInf) return t;
+  if (t == 0.0f) return u2f(0x80000001u);
+  return u2f(u & 0x80000000u ? u + 1 : u - 1);
+}
+
+// 64 lanes in `groups` (a power of two) of neighbours: the least of their maxima.
+__device__ __forceinline__ float least_maximum(float v, int groups) {
+  const int each = kWave / groups;
+#define GTP_STEP(J)                                       \
+  {                                                       \
+    const float o = u2f(lane_xor<J>(f2u(v)));             \
+    v = J < each ? fmaxf(v, o) : fminf(v, o);             \
+  }
+  GTP_STEP(1) GTP_STEP(2) GTP_STEP(4) GTP_STEP(8) GTP_STEP(16) GTP_STEP(32)
+#undef GTP_STEP
+  return u2f(__builtin_amdgcn_readfirstlane(f2u(v)));
+}
+
+// A wave's maximum, in a scalar register.
+__device__ __forceinline__ float uniform_max(float v) {
+  v = fmaxf(v, u2f(lane_xor<1>(f2u(v))));
+  v = fmaxf(v, u2f(lane_xor<2>(f2u(v))));
+  v = fmaxf(v, u2f(lane_xor<4>(f2u(v))));
+  v = fmaxf(v, u2f(lane_xor<8>(f2u(v))));
+  v = fmaxf(v, u2f(lane_xor<16>(f2u(v))));
+  v = fmaxf(v, u2f(lane_xor<32>(f2u(v))));
+  return u2f(__builtin_amdgcn_readfirstlane(f2u(v)));
+}
+
+// A slice's state, carried from chunk to chunk.  The code is kept small: the
+// kernel runs a few microseconds, of which fetching it for the first time is a
+// part that all waves wait for.
 template <typename T, bool kMask>
-__global__ __launch_bounds__(kBlock) void beam_slices_kernel(Rows r) {
-  constexpr int E = Vec<T>::kE;
-  constexpr int64_t kChunk = (int64_t)kU * kWave * E;
-  __shared__ uint64_t lists[kWaves][kCap];
-  const int lane = threadIdx.x & (kWave - 1);
-  const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-  const int64_t at = (int64_t)blockIdx.x * kWaves + wid;
-  if (at >= (int64_t)r.G * r.K * r.S) return;
-  const int row = (int)(at / r.S), slice = (int)(at % r.S);
-  if (!live(r, row)) return;
-  const T* x = reinterpret_cast<const T*>(r.x) + (row / r.K) * r.group_stride +
-               (row % r.K) * r.beam_stride;
-  const uint8_t* mask = kMask ? r.mask + row * r.mask_stride : nullptr;
-  const int64_t begin = slice * r.L;
-  const int64_t end = begin + r.L < r.V ? begin + r.L : r.V;
+struct Slice {
+  static constexpr int E = Vec<T>::kE;
+  static constexpr int64_t kChunk = (int64_t)kU * kWave * E;
+  const T* x;
+  const uint8_t* mask;
+  uint32_t* noted;  // LDS: vectors of the slice
+  int64_t begin, end;
+  int n, slots, lane, notes;
+  Top top;
+  float top_x, s;  // the wave's maximum, the lane's sum
+  u32x4 v[kU];
+  uint32_t bits[kU];
 
-  Top top{lists[wid], 0, kNegInf};
-  float top_x = kNegInf, s = 0.0f;  // the wave's maximum, the lane's sum
-
-  u32x4 next[kU];
-  uint32_t bits_next[kU];
-  auto load = [&](int64_t e) {
+  // the kE bits of the vector at element i
+  __device__ __forceinline__ uint32_t bits_at(int64_t i) const {
+    return (uint32_t)mask[i >> 3] >> (E == 4 ? i & 7 : 0);
+  }
+  __device__ __forceinline__ void load(int64_t e) {
+    const int64_t i0 = e + (int64_t)lane * E;
+    if (e + kChunk <= end) {
 #pragma unroll
-    for (int u = 0; u < kU; ++u) {
-      const int64_t i = e + ((int64_t)u * kWave + lane) * E;
-      if (i < end) {
-        next[u] = load_vec(x, i, end);
-        if constexpr (kMask) bits_next[u] = (uint32_t)mask[i >> 3] >> (i & 7);
+      for (int u = 0; u < kU; ++u) {
+        v[u] = reinterpret_cast<const Unaligned<T>*>(x + i0 + u * kWave * E)->v;
+        if constexpr (kMask) bits[u] = bits_at(i0 + u * kWave * E);
+      }
+    } else if (e < end) {
+#pragma unroll
+      for (int u = 0; u < kU; ++u) {
+        const int64_t i = i0 + u * kWave * E;
+        v[u] = load_vec(x, i, end);
+        if constexpr (kMask) bits[u] = i < end ? bits_at(i) : 0u;
       }
     }
-  };
-  load(begin);
-  bool first = true;
-  for (int64_t e = begin; e < end; e += kChunk) {
-    float y[kU][E];
-    uint32_t bits[kU];
+  }
+
+  // Lists what lies above the threshold in 64 of the noted vectors from `first`
+  // on, or the fewer that there are: in the order of their tokens, for of equal
+  // logits the first count.
+  __device__ __forceinline__ void take(int first) {
+    float y[E];
+    int64_t i = 0;
+    uint32_t hits = 0;
+    if (first + lane < notes) {
+      i = begin + (int64_t)noted[first + lane] * E;
+      Vec<T>::cvt(load_vec(x, i, end), y);
+#pragma unroll
+      for (int j = 0; j < E; ++j) hits |= y[j] > top.tau ? 1u << j : 0u;
+      if constexpr (kMask) hits &= bits_at(i);
+    }
+    const uint32_t mine = __popc(hits), upto = wave_scan_u32(mine);
+    int to = top.count + (int)(upto - mine);
+#pragma unroll
+    for (int j = 0; j < E; ++j)
+      if (hits >> j & 1u) top.list[to++] = rank_key(y[j] + 0.0f, (int32_t)i + j);
+    top.count += __builtin_amdgcn_readlane(upto, kWave - 1);
+    if (top.count > slots) top.cut(n, slots, top_x, lane);
+  }
+
+  // Folds the chunk at e, with the next one's loads on their way (ahead of the
+  // first one: only those).
+  __device__ __forceinline__ void fold(int64_t e) {
+    u32x4 now[kU];
+    uint32_t allowed[kU];
 #pragma unroll
     for (int u = 0; u < kU; ++u) {
-      const int64_t i = e + ((int64_t)u * kWave + lane) * E;
-      if (i < end) {
-        Vec<T>::cvt(next[u], y[u]);
-      } else {
-#pragma unroll
-        for (int j = 0; j < E; ++j) y[u][j] = kNegInf;
-      }
-      if constexpr (kMask) bits[u] = bits_next[u];
+      now[u] = v[u];
+      if constexpr (kMask) allowed[u] = bits[u];
     }
     load(e + kChunk);
-    const float m = block_max_raw<kU, E>(y);
-    if (__ballot(m > top_x)) {
-      const float up = wave_max(fmaxf(m, top_x));
+    if (e < begin) return;
+
+    float y[kU][E], m[kU];
+#pragma unroll
+    for (int u = 0; u < kU; ++u) {
+      Vec<T>::cvt(now[u], y[u]);
+      m[u] = vec_max<E>(y[u]);
+    }
+    const float most = max3raw(max3raw(m[0], m[1], m[2]), m[3], m[3]);
+    static_assert(kU == 4, "");
+    if (__ballot(most > top_x)) {
+      const float up = uniform_max(fmaxf(most, top_x));
       if (top_x > kNegInf)
         s *= __builtin_amdgcn_exp2f((top_x - up) * kLog2e + (residual(up) - residual(top_x)));
       top_x = up;
@@ -234,53 +308,86 @@ __global__ __launch_bounds__(kBlock) void beam_slices_kernel(Rows r) {
     }
     s += (part[0] + part[1]) + (part[2] + part[3]);
 
-    auto masked = [&](int u, float (&z)[E]) {
-#pragma unroll
-      for (int j = 0; j < E; ++j)
-        z[j] = !kMask || ((bits[u] >> j) & 1u) ? y[u][j] : kNegInf;
-    };
-    float best = m;
-    if (first) {
-      // n lanes hold a logit at least as large as the n-th largest of the
-      // lanes' maxima: a threshold before anything is in the list
-      if constexpr (kMask) {
-        best = kNegInf;
-#pragma unroll
-        for (int u = 0; u < kU; ++u) {
-          float z[E];
-          masked(u, z);
-          best = max3raw(best, vec_max<E>(z), best);
-        }
-      }
-      const uint32_t o = best == best ? ord32(best + 0.0f) : kOrdNegInf;
-      uint32_t t0 = 0;
-      for (int b = 31; b >= 0; --b) {
-        const uint32_t t = t0 | (1u << b);
-        const int c = __popcll(__ballot(o >= t));
-        if (c >= r.n) t0 = t;
-        if (c == r.n) break;
-      }
-      // (the float below it; there is none between the two zeros)
-      t0 = t0 == 0x80000000u ? 0x7FFFFFFEu : t0 > 0u ? t0 - 1u : 0u;
-      top.tau = t0 <= kOrdNegInf ? kNegInf : unord32(t0);
-      first = false;
-    }
-    if (__ballot(best > top.tau)) {
+    if constexpr (kMask) {
 #pragma unroll
       for (int u = 0; u < kU; ++u) {
-        float z[E];
-        masked(u, z);
-        if (__ballot(vec_max<E>(z) > top.tau))
-          top.append<E>(z, (int32_t)(e + ((int64_t)u * kWave + lane) * E), r.n, lane);
+        m[u] = kNegInf;
+#pragma unroll
+        for (int j = 0; j < E; ++j)
+          m[u] = max3raw(m[u], (allowed[u] >> j) & 1u ? y[u][j] : kNegInf, m[u]);
       }
     }
+    if (e == begin) {
+      // as many groups of lanes as candidates: each one's maximum is at least
+      // the least of them, a threshold before anything is in the list
+      float best = max3raw(max3raw(m[0], m[1], m[2]), m[3], m[3]);
+      if (!(best == best)) best = kNegInf;
+      const int groups = n <= 1 ? 1 : 1 << (32 - __builtin_clz(n - 1));
+      top.tau = below(least_maximum(best, groups));
+    }
+    const uint32_t id = (uint32_t)((e - begin) / E) + lane;
+#pragma unroll
+    for (int u = 0; u < kU; ++u) {
+      const uint64_t k = __ballot(m[u] > top.tau);
+      if (k == 0) continue;
+      if (m[u] > top.tau) noted[notes + lanes_below(k)] = id + u * kWave;
+      notes += __popcll(k);
+    }
+    const bool last = e + kChunk >= end;
+    int taken = 0;
+    if (notes >= (last ? 1 : kWave)) {
+      wave_lds_sync();
+      for (; notes - taken >= (last ? 1 : kWave); taken += kWave) take(taken);
+      // fewer than 64 are left
+      const int left = notes > taken ? notes - taken : 0;
+      const uint32_t id_left = lane < left ? noted[taken + lane] : 0u;
+      wave_lds_sync();
+      if (lane < left) noted[lane] = id_left;
+      notes = left;
+    }
   }
-  top.cut(r.n, lane);
+};
+
+template <typename T, bool kMask>
+__global__ __launch_bounds__(kBlock) void beam_slices_kernel(Rows r) {
+  using S = Slice<T, kMask>;
+  __shared__ uint64_t lists[kWaves][kCap];
+  __shared__ uint32_t noted[kWaves][kNoted];
+  const int lane = threadIdx.x & (kWave - 1);
+  const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int64_t at = (int64_t)blockIdx.x * kWaves + wid;
+  if (at >= (int64_t)r.G * r.K * r.S) return;
+  const int row = (int)(at / r.S), slice = (int)(at % r.S);
+  if (!live(r, row)) return;
+  S w;
+  w.x = reinterpret_cast<const T*>(r.x) + (row / r.K) * r.group_stride +
+        (row % r.K) * r.beam_stride;
+  w.mask = kMask ? r.mask + row * r.mask_stride : nullptr;
+  w.noted = noted[wid];
+  w.begin = slice * r.L;
+  w.end = w.begin + r.L < r.V ? w.begin + r.L : r.V;
+  w.n = r.n;
+  w.slots = r.slots;
+  w.lane = lane;
+  w.notes = 0;
+  w.top = Top{lists[wid], 0, kNegInf};
+  w.top_x = kNegInf;
+  w.s = 0.0f;
+#pragma unroll
+  for (int u = 0; u < kU; ++u) {
+    w.v[u] = u32x4{0u, 0u, 0u, 0u};
+    w.bits[u] = 0u;
+  }
+#pragma unroll 1
+  for (int64_t e = w.begin - S::kChunk; e < w.end; e += S::kChunk) w.fold(e);
+
   wave_lds_sync();
-  if (lane < r.n) r.keys[at * r.n + lane] = lane < top.count ? top.list[lane] : 0ull;
+  for (int i = lane; i < r.slots; i += kWave)
+    r.keys[at * r.slots + i] = i < w.top.count ? w.top.list[i] : 0ull;
+  float s = w.s;
 #pragma unroll
   for (int o = kWave / 2; o > 0; o >>= 1) s += __shfl_xor(s, o, kWave);
-  if (lane == 0) r.sums[at] = make_float2(top_x, s);
+  if (lane == 0) r.sums[at] = make_float2(w.top_x, s);
 }
 
 // ------------------------------------------------------------------ a step
@@ -309,108 +416,115 @@ struct Candidates {
   int64_t token[kMaxN];
 };
 
-struct Scratch {
-  float score[2 * kMaxK];
-  int32_t row[2 * kMaxK], step[2 * kMaxK];
-  int32_t beam[kMaxK];
+// Lane k's beam and pool entry, read ahead of the candidates.
+struct Before {
+  float score, pool_score;
+  int32_t pool_row, pool_step;
+  bool done;
 };
+__device__ __forceinline__ Before before(const State& st, int g, int K, int lane) {
+  Before b;
+  const int64_t i = (int64_t)g * K + (lane < K ? lane : 0);
+  b.score = st.score[i];
+  b.pool_score = st.pool_score[i];
+  b.pool_row = st.pool_row[i];
+  b.pool_step = st.pool_step[i];
+  b.done = st.done[g] != 0;
+  return b;
+}
+
+__device__ __forceinline__ float lane_float(float v, int from) {
+  return u2f(__builtin_amdgcn_readlane(f2u(v), from));
+}
 
 // Moves group g on, by one wave; c: its n candidates, best first.
-__device__ __forceinline__ void advance(const State& st, const Candidates& c, Scratch& w, int g,
-                                        int K, int n, int lane) {
+__device__ __forceinline__ void advance(const State& st, const Before& old, const Candidates& c,
+                                        int g, int K, int n, int lane) {
   const int64_t base = (int64_t)g * K;
-  const uint64_t below = (1ull << lane) - 1;
-  if (st.done[g]) {
+  const uint64_t below_lane = (1ull << lane) - 1;
+  if (old.done) {
     if (lane < K) {
       st.token[base + lane] = st.pad;
       st.parent[base + lane] = (int32_t)base + lane;
-      st.new_score[base + lane] = st.score[base + lane];
-      st.new_pool_score[base + lane] = st.pool_score[base + lane];
-      st.new_pool_row[base + lane] = st.pool_row[base + lane];
-      st.new_pool_step[base + lane] = st.pool_step[base + lane];
+      st.new_score[base + lane] = old.score;
+      st.new_pool_score[base + lane] = old.pool_score;
+      st.new_pool_row[base + lane] = old.pool_row;
+      st.new_pool_step[base + lane] = old.pool_step;
     }
     if (lane == 0) st.new_done[g] = 1;
     return;
   }
   const bool mine = lane < n;
-  const bool valid = mine && c.beam[lane] >= 0;
-  const bool ended = valid && c.token[lane] == st.eos;
-  // the pool: what it held, then the finished ones among the first K; of equal
-  // scores the earlier stays ahead
-  if (lane < K) {
-    w.score[lane] = st.pool_score[base + lane];
-    w.row[lane] = st.pool_row[base + lane];
-    w.step[lane] = st.pool_step[base + lane];
-    w.score[K + lane] = ended ? (float)((double)c.score[lane] / st.length) : kNegInf;
-    w.row[K + lane] = ended ? (int32_t)base + c.beam[lane] : -1;
-    w.step[K + lane] = ended ? st.step : -1;
+  const int beam = mine ? c.beam[lane] : -1;
+  const float score = mine ? c.score[lane] : kNegInf;
+  const int64_t token = mine ? c.token[lane] : -1;
+  const bool valid = beam >= 0;
+  const bool ended = valid && token == st.eos;
+  // The pool: what it held (lane k's), then the finished ones among the first K
+  // candidates; of equal scores the earlier stays ahead.
+  const float held = lane < K ? old.pool_score : kNegInf;
+  const float fresh = lane < K && ended ? (float)((double)score / st.length) : kNegInf;
+  int rank_held = 0, rank_fresh = 0;
+  for (int i = 0; i < K; ++i) {
+    const float h = lane_float(held, i), f = lane_float(fresh, i);
+    rank_held += (h > held || (h == held && i < lane)) + (f > held);
+    rank_fresh += (h >= fresh) + (f > fresh || (f == fresh && i < lane));
   }
-  wave_lds_sync();
-  float last = kNegInf;  // the pool's K-th score
-  {
-    const bool in = lane < 2 * K;
-    const float v = in ? w.score[lane] : 0.0f;
-    int rank = 0;
-    for (int i = 0; i < 2 * K; ++i) {
-      const float o = w.score[i];
-      rank += o > v || (o == v && i < lane) ? 1 : 0;
-    }
-    if (in && rank < K) {
-      st.new_pool_score[base + rank] = v;
-      st.new_pool_row[base + rank] = v == kNegInf ? -1 : w.row[lane];
-      st.new_pool_step[base + rank] = v == kNegInf ? -1 : w.step[lane];
-    }
-    const uint64_t at = __ballot(in && rank == K - 1);
-    if (at) last = __shfl(v, __ffsll((unsigned long long)at) - 1, kWave);
+  if (lane < K && rank_held < K) {
+    st.new_pool_score[base + rank_held] = held;
+    st.new_pool_row[base + rank_held] = held == kNegInf ? -1 : old.pool_row;
+    st.new_pool_step[base + rank_held] = held == kNegInf ? -1 : old.pool_step;
   }
-  // the first K others go on
+  if (lane < K && rank_fresh < K) {
+    st.new_pool_score[base + rank_fresh] = fresh;
+    st.new_pool_row[base + rank_fresh] = fresh == kNegInf ? -1 : (int32_t)base + beam;
+    st.new_pool_step[base + rank_fresh] = fresh == kNegInf ? -1 : st.step;
+  }
+  const uint64_t last_held = __ballot(lane < K && rank_held == K - 1);
+  const uint64_t last_fresh = __ballot(lane < K && rank_fresh == K - 1);
+  const float last = last_held ? lane_float(held, __ffsll((unsigned long long)last_held) - 1)
+                     : last_fresh ? lane_float(fresh, __ffsll((unsigned long long)last_fresh) - 1)
+                                  : kNegInf;
+  // The first K others go on: a beam's best one stays in its slot, the rest
+  // take the free slots in order; slots beyond the candidates' are dead.
   const uint64_t others = __ballot(mine && !ended);
-  const int j = __popcll(others & below);
+  const int j = __popcll(others & below_lane);
   const bool goes = mine && !ended && j < K;
   const uint64_t going = __ballot(goes && valid);
-  if (lane < K) w.beam[lane] = -1;
-  wave_lds_sync();
-  if (goes && valid) w.beam[j] = c.beam[lane];
-  wave_lds_sync();
-  // a beam's best one stays in its slot, the rest take the free slots in order
   uint32_t taken = 0;
-  bool again = false;
-  for (int i = 0; i < K; ++i) {
-    const int p = w.beam[i];
-    if (p < 0) continue;
-    taken |= 1u << p;
-    again |= goes && valid && i < j && p == c.beam[lane];
+  uint64_t staying = 0;
+  for (uint64_t left = going; left; left &= left - 1) {
+    const int i = __ffsll((unsigned long long)left) - 1;
+    const uint32_t slot = 1u << __builtin_amdgcn_readlane(beam, i);
+    if (!(taken & slot)) staying |= 1ull << i;
+    taken |= slot;
   }
-  const bool moves = goes && (!valid || again);
-  const uint64_t moving = __ballot(moves);
+  const bool stays = (staying >> lane) & 1;
+  const uint64_t moving = __ballot(goes && !stays);
+  uint32_t free = ~taken;
   if (goes) {
-    int slot;
-    if (!moves) {
-      slot = c.beam[lane];
-    } else {
-      uint32_t free = ~taken;
-      for (int i = __popcll(moving & below); i > 0; --i) free &= free - 1;
+    int slot = beam;
+    if (!stays) {
+      for (int i = __popcll(moving & below_lane); i > 0; --i) free &= free - 1;
       slot = __ffs((int)free) - 1;
     }
-    st.token[base + slot] = valid ? c.token[lane] : st.pad;
-    st.parent[base + slot] = (int32_t)base + (valid ? c.beam[lane] : slot);
-    st.new_score[base + slot] = valid ? c.score[lane] : kNegInf;
+    st.token[base + slot] = valid ? token : st.pad;
+    st.parent[base + slot] = (int32_t)base + (valid ? beam : slot);
+    st.new_score[base + slot] = valid ? score : kNegInf;
   }
-  // Every slot has one of the first n - (ended) >= K candidates when n >= 2 K;
-  // a shorter list leaves slots without: dead ones.
-  const int given = __popcll(__ballot(goes));
-  if (given < K) {
-    uint32_t free = ~taken;
+  if (__popcll(__ballot(goes)) < K) {
+    free = ~taken;
     for (int i = __popcll(moving); i > 0; --i) free &= free - 1;
-    if (lane < K && (free >> lane) & 1u) {
+    if (lane < K && ((free >> lane) & 1u)) {
       st.token[base + lane] = st.pad;
       st.parent[base + lane] = (int32_t)base + lane;
       st.new_score[base + lane] = kNegInf;
     }
   }
   // the best that a live beam's score reaches at this length
-  const int best_at = going ? __ffsll((unsigned long long)going) - 1 : 0;
-  const float best = going ? (float)((double)c.score[best_at] / st.length) : kNegInf;
+  const float best = going ? (float)((double)lane_float(score, __ffsll((unsigned long long)going) - 1) /
+                                     st.length)
+                           : kNegInf;
   if (lane == 0)
     st.new_done[g] = (last > kNegInf && (st.early || last >= best)) || !going ? 1 : 0;
 }
@@ -430,55 +544,70 @@ struct Out {
   int32_t* status;  // [G K] or null
 };
 
+constexpr int kMergeBlock = 1024;
+constexpr int kMergeWaves = kMergeBlock / kWave;
+constexpr int kHold = kMaxKeys / kMergeBlock;  // candidates per thread, in registers
+constexpr int kList = 1024;                    // candidates that are compared with each other
+
+__device__ __forceinline__ double lane_xor_double(double v, int o) {
+  const uint64_t u = shfl_xor_u64(__builtin_bit_cast(uint64_t, v), o);
+  return __builtin_bit_cast(double, u);
+}
+
 template <bool kStep>
-__global__ __launch_bounds__(kBlock) void beam_merge_kernel(Rows r, Out out, State st) {
-  extern __shared__ uint64_t dyn[];  // 2 x entries
-  __shared__ double offset[kMaxK];  // score - log sum 2^{(x - m) c}
+__global__ __launch_bounds__(kMergeBlock) void beam_merge_kernel(Rows r, Out out, State st) {
+  __shared__ double offset[kMaxK];  // score - log sum 2^{(x - m) c}; -inf: no candidates
   __shared__ float row_top[kMaxK];  // m
-  __shared__ uint64_t best[kBlock], best_at[kBlock];
+  __shared__ uint32_t best[kMergeWaves][kWave];
+  __shared__ uint64_t list_o[kList], list_at[kList];
   __shared__ Candidates c;
-  __shared__ Scratch scratch;
   __shared__ int entries;
-  __shared__ uint64_t cut, cut_at;
-  const int g = blockIdx.x, tid = threadIdx.x, lane = tid & (kWave - 1), wid = tid / kWave;
-  const int per_row = r.S * r.n, total = r.K * per_row;
+  const int g = blockIdx.x, tid = threadIdx.x, lane = tid & (kWave - 1);
+  const int wid = __builtin_amdgcn_readfirstlane(tid / kWave);
+  const int per_row = r.S * r.slots, total = r.K * per_row;
   const int64_t base = (int64_t)g * r.K;
   const bool done = r.done && r.done[g];
-  if (tid == 0) {
-    entries = 0;
+  // all that is read from memory, ahead of what it is for
+  uint64_t key[kHold];
+#pragma unroll
+  for (int j = 0; j < kHold; ++j) {
+    key[j] = 0;
+    const int i = j * kMergeBlock + tid;
+    if (j * kMergeBlock < total && i < total && !done) key[j] = r.keys[base * per_row + i];
   }
+  Before old;
+  if constexpr (kStep) {
+    if (wid == 0) old = before(st, g, r.K, lane);
+  }
+  if (tid == 0) entries = 0;
   if (tid < r.n) {
     c.score[tid] = kNegInf;
     c.beam[tid] = -1;
     c.token[tid] = -1;
   }
-  // each row's log-sum-exp
-  for (int k = wid; k < r.K; k += kWaves) {
+  // each row's log-sum-exp (S <= 64: a slice per lane)
+  for (int k = wid; k < r.K; k += kMergeWaves) {
     int status = GTP_ROW_OK;
     double off = -__builtin_huge_val();
     const float score = r.score[base + k];
     float top = kNegInf;
     if (live(r, (int)base + k)) {
-      const float2* p = r.sums + (base + k) * r.S;
-      for (int i = lane; i < r.S; i += kWave) top = fmaxf(top, p[i].x);
-      top = wave_max(top);
-      double s = 0.0;
-      for (int i = lane; i < r.S; i += kWave) {
-        const float2 v = p[i];
-        // (a NaN stays, also where nothing finite was seen)
-        if (v.y != v.y) s += (double)v.y;
-        else if (v.x > kNegInf)
-          s += (double)v.y *
-               exp2(((double)v.x - (double)top) * (double)kLog2e - (double)residual(v.x));
-      }
-#pragma unroll
-      for (int o = kWave / 2; o > 0; o >>= 1) s += __shfl_xor(s, o, kWave);
-      // (the exponents are multiples of the fp32 log2(e))
+      float2 v = make_float2(kNegInf, 0.0f);
       bool any = false;  // (a slice's first key is there where any is)
-      for (int i = lane; i < r.S; i += kWave) any |= r.keys[((base + k) * r.S + i) * r.n] != 0;
-      const bool some = __ballot(any) != 0;
+      if (lane < r.S) {
+        v = r.sums[(base + k) * r.S + lane];
+        any = r.keys[((base + k) * r.S + lane) * r.slots] != 0;
+      }
+      top = wave_max(v.x);
+      // (a NaN stays, also where nothing finite was seen)
+      double s = (double)v.y;
+      if (v.x > kNegInf && v.x < kPosInf)
+        s *= exp2(((double)v.x - (double)top) * (double)kLog2e - (double)residual(v.x));
+#pragma unroll
+      for (int o = kWave / 2; o > 0; o >>= 1) s += lane_xor_double(s, o);
+      // (the exponents are multiples of the fp32 log2(e))
       if (s != s) status = GTP_ROW_NONFINITE;
-      else if (!some) status = GTP_ROW_EMPTY;
+      else if (!__ballot(any)) status = GTP_ROW_EMPTY;
       else off = (double)score - log2(s) / (double)kLog2e;
     } else if (!done && !(score == kNegInf)) {
       status = GTP_ROW_NONFINITE;
@@ -490,87 +619,127 @@ __global__ __launch_bounds__(kBlock) void beam_merge_kernel(Rows r, Out out, Sta
     }
   }
   __syncthreads();
-  // Candidate i: its score in an order of integers (0: none) and its place.
-  auto candidate = [&](int i, uint64_t& at) {
-    const int k = i / per_row;
-    at = ~0ull;
-    if (offset[k] == -__builtin_huge_val()) return (uint64_t)0;
-    const uint64_t key = r.keys[base * per_row + i];
-    if (key == 0) return (uint64_t)0;
-    at = (uint64_t)k << 32 | (uint32_t)rank_key_id(key);
-    return ord64(((double)rank_key_y(key) - (double)row_top[k]) + offset[k]);
-  };
-  auto better = [](uint64_t o, uint64_t at, uint64_t than_o, uint64_t than_at) {
-    return o > than_o || (o == than_o && at < than_at);
-  };
   if (!done) {
-    // n threads hold a candidate at least as good as the n-th best of the
-    // threads' best ones; what is worse than that is out, so that no more than
-    // these threads' candidates are left
-    uint64_t mine = 0, mine_at = ~0ull;
-    for (int i = tid; i < total; i += kBlock) {
-      uint64_t at;
-      const uint64_t o = candidate(i, at);
-      if (better(o, at, mine, mine_at)) {
-        mine = o;
-        mine_at = at;
-      }
+    // a candidate's score in an order of integers (0: none) and its place
+    uint64_t o[kHold];
+    uint32_t top = 0;
+#pragma unroll
+    for (int j = 0; j < kHold; ++j) {
+      o[j] = 0;
+      if (j * kMergeBlock >= total) continue;
+      const int k = (j * kMergeBlock + tid) / per_row;
+      if (key[j] == 0 || offset[k] == -__builtin_huge_val()) continue;
+      o[j] = ord64(((double)rank_key_y(key[j]) - (double)row_top[k]) + offset[k]);
+      const uint32_t h = (uint32_t)(o[j] >> 32);
+      top = h > top ? h : top;
     }
-    best[tid] = mine;
-    best_at[tid] = mine_at;
+    auto place = [&](int j) {
+      return (uint64_t)((j * kMergeBlock + tid) / per_row) << 32 | (uint32_t)rank_key_id(key[j]);
+    };
+    best[wid][lane] = top;
     __syncthreads();
-    int rank = 0;
-    for (int i = 0; i < kBlock; ++i) {
-      const uint64_t o = best[i];
-      // (threads without any are equal: their number decides)
-      if (o >= mine)
-        rank += better(o, best_at[i], mine, mine_at) || (mine == 0 && o == 0 && i < tid) ? 1 : 0;
-    }
-    if (rank == r.n - 1) {
-      cut = mine;
-      cut_at = mine_at;
-    }
-    __syncthreads();
-    const uint64_t from = cut, from_at = cut_at;
-    for (int i = tid; i < total; i += kBlock) {
-      uint64_t at;
-      const uint64_t o = candidate(i, at);
-      if (o == 0 || better(from, from_at, o, at)) continue;
-      const int e = atomicAdd(&entries, 1);
-      dyn[2 * e] = o;
-      dyn[2 * e + 1] = at;
-    }
-    __syncthreads();
-    const int m = entries;
-    for (int e = tid; e < m; e += kBlock) {
-      const uint64_t o = dyn[2 * e], at = dyn[2 * e + 1];
-      int rank = 0;
-      for (int i = 0; i < m; ++i) {
-        const uint64_t p = dyn[2 * i];
-        rank += better(p, dyn[2 * i + 1], o, at) ? 1 : 0;
-      }
-      if (rank < r.n) {
-        c.score[rank] = (float)unord64(o);
-        c.beam[rank] = (int32_t)(at >> 32);
-        c.token[rank] = (int64_t)(uint32_t)at;
-      }
-    }
+    // groups of lanes, as many as candidates are wanted or more: the least of
+    // their maxima is a threshold that enough of them reach
+    uint32_t m = 0;
+#pragma unroll
+    for (int w = 0; w < kMergeWaves; ++w) m = best[w][lane] > m ? best[w][lane] : m;
+    const int groups = r.n <= 1 ? 1 : 1 << (32 - __builtin_clz(r.n - 1));
+    const int each = kWave / groups;
+#define GTP_STEP(J)                                          \
+  {                                                          \
+    const uint32_t x = lane_xor<J>(m);                       \
+    m = J < each ? (x > m ? x : m) : (x < m ? x : m);        \
   }
-  __syncthreads();
+    GTP_STEP(1) GTP_STEP(2) GTP_STEP(4) GTP_STEP(8) GTP_STEP(16) GTP_STEP(32)
+#undef GTP_STEP
+    const uint64_t at_least = m > 0 ? (uint64_t)m << 32 : 1ull;
+    int mine = 0;
+#pragma unroll
+    for (int j = 0; j < kHold; ++j) mine += o[j] >= at_least ? 1 : 0;
+    int to = mine > 0 ? atomicAdd(&entries, mine) : 0;
+#pragma unroll
+    for (int j = 0; j < kHold; ++j) {
+      if (o[j] < at_least) continue;
+      if (to < kList) {
+        list_o[to] = o[j];
+        list_at[to] = place(j);
+      }
+      ++to;
+    }
+    __syncthreads();
+    auto better = [](uint64_t o, uint64_t at, uint64_t than_o, uint64_t than_at) {
+      return o > than_o || (o == than_o && at < than_at);
+    };
+    auto take = [&](int rank, uint64_t o, uint64_t at) {
+      c.score[rank] = (float)unord64(o);
+      c.beam[rank] = (int32_t)(at >> 32);
+      c.token[rank] = (int64_t)(uint32_t)at;
+    };
+    const int n = entries;
+    if (n <= kList) {
+      for (int e = tid; e < n; e += kMergeBlock) {
+        const uint64_t mo = list_o[e], ma = list_at[e];
+        int rank = 0;
+#pragma unroll 4
+        for (int i = 0; i < n; ++i) rank += better(list_o[i], list_at[i], mo, ma) ? 1 : 0;
+        if (rank < r.n) take(rank, mo, ma);
+      }
+    } else {
+      // (many equal scores) one after the other: the best behind the last
+      uint64_t last_o = ~0ull, last_at = 0;
+      for (int rank = 0; rank < r.n; ++rank) {
+        uint64_t mo = 0, ma = ~0ull;
+#pragma unroll
+        for (int j = 0; j < kHold; ++j) {
+          if (o[j] == 0) continue;
+          const uint64_t at = place(j);
+          if (better(last_o, last_at, o[j], at) && better(o[j], at, mo, ma)) {
+            mo = o[j];
+            ma = at;
+          }
+        }
+        for (int x = kWave / 2; x > 0; x >>= 1) {
+          const uint64_t oo = shfl_xor_u64(mo, x), oa = shfl_xor_u64(ma, x);
+          if (better(oo, oa, mo, ma)) {
+            mo = oo;
+            ma = oa;
+          }
+        }
+        __syncthreads();
+        if (lane == 0) {
+          list_o[wid] = mo;
+          list_at[wid] = ma;
+        }
+        __syncthreads();
+        for (int w = 0; w < kMergeWaves; ++w)
+          if (better(list_o[w], list_at[w], mo, ma)) {
+            mo = list_o[w];
+            ma = list_at[w];
+          }
+        if (mo == 0) break;
+        last_o = mo;
+        last_at = ma;
+        if (tid == 0) take(rank, mo, ma);
+      }
+    }
+    __syncthreads();
+  }
   if (out.score && tid < r.n) {
     out.score[(int64_t)g * r.n + tid] = c.score[tid];
     out.beam[(int64_t)g * r.n + tid] = c.beam[tid];
     out.token[(int64_t)g * r.n + tid] = c.token[tid];
   }
-  if (kStep && wid == 0) advance(st, c, scratch, g, r.K, r.n, lane);
+  if constexpr (kStep) {
+    if (wid == 0) advance(st, old, c, g, r.K, r.n, lane);
+  }
 }
 
 __global__ __launch_bounds__(kWave) void beam_advance_kernel(State st, const float* score,
                                                              const int32_t* beam,
                                                              const int64_t* token, int K, int n) {
   __shared__ Candidates c;
-  __shared__ Scratch scratch;
   const int g = blockIdx.x, lane = threadIdx.x;
+  const Before old = before(st, g, K, lane);
   if (lane < n) {
     const int64_t i = (int64_t)g * n + lane;
     const int b = beam[i];
@@ -580,7 +749,7 @@ __global__ __launch_bounds__(kWave) void beam_advance_kernel(State st, const flo
     c.token[lane] = token[i];
   }
   wave_lds_sync();
-  advance(st, c, scratch, g, K, n, lane);
+  advance(st, old, c, g, K, n, lane);
 }
 
 // The best hypotheses of each group behind its last step, and their tokens,
@@ -637,11 +806,14 @@ __global__ __launch_bounds__(kWave) void beam_finish_kernel(
 
 // ------------------------------------------------------------------ launches
 
-// Slices per row: waves enough for the chip (2048: 2 per SIMD) of at least two
-// chunks each, and what the merge can hold.
+// Keys that a slice gives, and slices per row: waves enough for the chip (2048:
+// 2 per SIMD) of at least a chunk each, and what the merge can hold.  [4, 151936]
+// by chunks of 2048 8.2 us, by two of them 11.4; [256, 248320] with 4096 waves
+// 32.3 us for 31.1.
+int64_t slots_of(int64_t n) { return n <= 4 ? n + 2 : n <= 16 ? n + n / 2 : n + n / 4; }
 void slices_of(int64_t G, int64_t K, int64_t n, int64_t V, int64_t& S, int64_t& L) {
   int64_t want = (2048 + G * K - 1) / (G * K);
-  const int64_t most = kMaxKeys / (K * n), full = (V + 4095) / 4096;
+  const int64_t most = kMaxKeys / (K * slots_of(n)), full = (V + 2047) / 2048;
   if (want > most) want = most;
   if (want > full) want = full;
   if (want > kWave) want = kWave;
@@ -725,20 +897,19 @@ int run(const gtp_beam_rows* q, const Out& out, const gtp_beam_state* step, void
   int64_t S, L;
   slices_of(r.G, r.K, r.n, r.V, S, L);
   r.S = (int32_t)S;
+  r.slots = (int32_t)slots_of(r.n);
   r.L = L;
   const int64_t slices = (int64_t)r.G * r.K * S;
   r.keys = reinterpret_cast<uint64_t*>(workspace);
-  r.sums = reinterpret_cast<float2*>(r.keys + slices * r.n);
+  r.sums = reinterpret_cast<float2*>(r.keys + slices * r.slots);
   if (q->dtype == GTP_DTYPE_BF16) launch_slices<uint16_t>(r, s);
   else if (q->dtype == GTP_DTYPE_F16) launch_slices<_Float16>(r, s);
   else launch_slices<float>(r, s);
-  const int64_t keys = (int64_t)r.K * S * r.n;
-  const size_t lds = (size_t)((keys + kBlock - 1) / kBlock * r.n) * 16;
   const State st = step ? state_of(step) : State{};
   if (step)
-    hipLaunchKernelGGL(beam_merge_kernel<true>, dim3(r.G), dim3(kBlock), lds, s, r, out, st);
+    hipLaunchKernelGGL(beam_merge_kernel<true>, dim3(r.G), dim3(kMergeBlock), 0, s, r, out, st);
   else
-    hipLaunchKernelGGL(beam_merge_kernel<false>, dim3(r.G), dim3(kBlock), lds, s, r, out, st);
+    hipLaunchKernelGGL(beam_merge_kernel<false>, dim3(r.G), dim3(kMergeBlock), 0, s, r, out, st);
   return hipGetLastError() == hipSuccess ? GTP_OK : GTP_ERR_LAUNCH;
 }
 
@@ -752,7 +923,7 @@ extern "C" size_t gtp_beam_workspace_bytes(const gtp_beam_rows* rows) {
   if (rows->groups == 0) return 8;
   int64_t S, L;
   beam::slices_of(rows->groups, rows->beams, rows->candidates, rows->vocab, S, L);
-  return (size_t)(rows->groups * rows->beams * S) * (size_t)(rows->candidates + 1) * 8;
+  return (size_t)(rows->groups * rows->beams * S) * (size_t)(beam::slots_of(rows->candidates) + 1) * 8;
 }
 
 extern "C" int gtp_beam_candidates(const gtp_beam_rows* rows, float* out_scores,
