@@ -112,9 +112,9 @@ __device__ __forceinline__ void store16(T* p, u32x4 v, int64_t left) {
 // ------------------------------------------------------------------- plan
 // Where the rows are in the order of adapters: position p in [0, tiles * T).
 // Classes: adapters 0 .. E-1, E: rows without one, E + 1: bad ids.
-// In memory (int32): start[E + 3] (an adapter's first position; the last: the
-// end), rows[E + 2], first[E + 2] (its first request in `order`), order[B],
-// adapter[tiles] (-1: no tile).
+// In memory (int32): start[E + 3] (a class's first position; the last: the
+// end), rows[E + 3], tile[tiles][4] (its class or -1, the class's first request
+// in `order` and its rows, the tile's first row among them), order[B].
 
 // Each adapter's scale, or one for all, and where the forward puts them: what
 // reads them later, the backward too, has them from there.
@@ -124,27 +124,32 @@ struct Scale {
   float* to;
 };
 
+struct Tile {
+  int e, first, rows, at;
+};
+
 struct Plan {
   const int32_t* mem;  // null: all rows in order, adapter 0
   int32_t N, B, S, T, E, tiles;
 
+  __host__ __device__ static int64_t head(int64_t E) { return (2 * (E + 3) + 3) / 4 * 4; }
   __host__ __device__ static int64_t words(int64_t B, int64_t E, int64_t tiles) {
-    return 3 * (E + 3) + B + tiles;
+    return head(E) + 4 * tiles + B;
   }
-  __device__ __forceinline__ const int32_t* start() const { return mem; }
-  __device__ __forceinline__ const int32_t* rows() const { return mem + E + 3; }
-  __device__ __forceinline__ const int32_t* first() const { return mem + 2 * (E + 3); }
-  __device__ __forceinline__ const int32_t* order() const { return mem + 3 * (E + 3); }
-  __device__ __forceinline__ const int32_t* adapter() const { return order() + B; }
-  // tile t's class, -1 where there is no such tile
-  __device__ __forceinline__ int tile(int t) const { return mem ? adapter()[t] : 0; }
-  // the row at position p of class e, -1 behind its last
-  __device__ __forceinline__ int row(int p, int e) const {
-    if (!mem) return p < N ? p : -1;
-    const int j = p - start()[e];
-    if (j >= rows()[e]) return -1;
+  __device__ __forceinline__ int start(int e) const { return mem ? mem[e] : e ? tiles * T : 0; }
+  __device__ __forceinline__ int rows(int e) const { return mem ? mem[E + 3 + e] : N; }
+  __device__ __forceinline__ Tile tile(int t) const {
+    if (!mem) return Tile{0, 0, N, t * T};
+    const int4 v = reinterpret_cast<const int4*>(mem + head(E))[t];
+    return Tile{v.x, v.y, v.z, v.w};
+  }
+  // row n of tile t, -1 behind the class's last
+  __device__ __forceinline__ int row(const Tile& t, int n) const {
+    const int j = t.at + n;
+    if (j >= t.rows) return -1;
+    if (!mem) return j;
     const int b = j / S;
-    return order()[first()[e] + b] * S + (j - b * S);
+    return mem[head(E) + 4 * tiles + t.first + b] * S + (j - b * S);
   }
 };
 
@@ -156,15 +161,11 @@ constexpr int kPlanWaves = kPlanBlock / kWave;
 __global__ __launch_bounds__(kPlanBlock) void plan_kernel(const void* ids, int ids64, int B, int S,
                                                           int T, int E, int tiles, int32_t* mem) {
   extern __shared__ int32_t count[];  // [classes][waves]
-  __shared__ int32_t begin[kMaxAdapters + 2];
+  __shared__ int32_t first[kMaxAdapters + 2], rows[kMaxAdapters + 2], start[kMaxAdapters + 3];
   const int classes = E + 2, lane = threadIdx.x & (kWave - 1), w = threadIdx.x / kWave;
-  int32_t* start = mem;
-  int32_t* rows = mem + E + 3;
-  int32_t* first = mem + 2 * (E + 3);
-  int32_t* order = mem + 3 * (E + 3);
-  int32_t* adapter = order + B;
+  int4* tile = reinterpret_cast<int4*>(mem + Plan::head(E));
+  int32_t* order = mem + Plan::head(E) + 4 * tiles;
   for (int i = threadIdx.x; i < classes * kPlanWaves; i += kPlanBlock) count[i] = 0;
-  for (int i = threadIdx.x; i < tiles; i += kPlanBlock) adapter[i] = -1;
   __syncthreads();
   const int share = (B + kPlanWaves - 1) / kPlanWaves;
   const int from = w * share < B ? w * share : B, to = from + share < B ? from + share : B;
@@ -192,15 +193,16 @@ __global__ __launch_bounds__(kPlanBlock) void plan_kernel(const void* ids, int i
   }
   __syncthreads();
   // exclusive sums: of the requests, and of the positions
-  int base = 0;
-  int64_t pos = 0;
   if (threadIdx.x < kWave) {
+    int base = 0, pos = 0;
     for (int c0 = 0; c0 < classes; c0 += kWave) {
       const int c = c0 + lane;
       int n = 0;
-      if (c < classes)
+      if (c < classes) {
+#pragma unroll
         for (int k = 0; k < kPlanWaves; ++k) n += count[c * kPlanWaves + k];
-      const int padded = (int)(((int64_t)n * S + T - 1) / T * T);
+      }
+      const int padded = (n * S + T - 1) / T * T;
       int a = n, p = padded;
       for (int o = 1; o < kWave; o <<= 1) {
         const int x = __shfl_up(a, o, kWave), y = __shfl_up(p, o, kWave);
@@ -210,12 +212,10 @@ __global__ __launch_bounds__(kPlanBlock) void plan_kernel(const void* ids, int i
         }
       }
       if (c < classes) {
-        begin[c] = base + a - n;
         first[c] = base + a - n;
         rows[c] = n * S;
-        start[c] = (int)pos + p - padded;
-        if (c == classes - 1) start[classes] = (int)pos + p;
-        for (int t = 0; t < padded / T; ++t) adapter[((int)pos + p - padded) / T + t] = c;
+        start[c] = pos + p - padded;
+        if (c == classes - 1) start[classes] = pos + p;
       }
       base += __shfl(a, kWave - 1, kWave);
       pos += __shfl(p, kWave - 1, kWave);
@@ -223,12 +223,27 @@ __global__ __launch_bounds__(kPlanBlock) void plan_kernel(const void* ids, int i
   }
   __syncthreads();
   for (int c = threadIdx.x; c < classes; c += kPlanBlock) {
-    int at = begin[c];
+    int at = first[c];
+    mem[c] = start[c];
+    mem[E + 3 + c] = rows[c];
+    if (c == classes - 1) mem[classes] = start[classes];
     for (int k = 0; k < kPlanWaves; ++k) {
       const int n = count[c * kPlanWaves + k];
       count[c * kPlanWaves + k] = at;
       at += n;
     }
+  }
+  for (int t = threadIdx.x; t < tiles; t += kPlanBlock) {
+    // the last class that begins at or before the tile (empty ones begin where
+    // the next one does)
+    int lo = 0, hi = classes;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) / 2;
+      if (start[mid] <= t * T) lo = mid;
+      else hi = mid;
+    }
+    tile[t] = t * T < start[classes] ? make_int4(lo, first[lo], rows[lo], t * T - start[lo])
+                                     : make_int4(-1, 0, 0, 0);
   }
   __syncthreads();
   for (int i = from; i < to; i += kWave) {
@@ -252,7 +267,7 @@ __global__ __launch_bounds__(kBlock) void shrink_kernel(Plan plan, const T* x, i
                                                         const T* W, int C, int r, int splits,
                                                         float* low, Scale scale) {
   constexpr int E = Mat<T>::kE;
-  constexpr int kSteps = RB == 1 ? 4 : 1;  // loaded at a time
+  constexpr int kSteps = RB == 1 ? 4 : NB == 4 ? 1 : 2;  // loaded at a time
   constexpr int kRows = RB * 16;
   __shared__ int rows[kRows];
   __shared__ float sum[kRows][NB * 16 + 1];
@@ -262,9 +277,10 @@ __global__ __launch_bounds__(kBlock) void shrink_kernel(Plan plan, const T* x, i
   if (scale.to && blockIdx.x == 0 && blockIdx.y == 0)
     for (int i = threadIdx.x; i < plan.E; i += kBlock)
       scale.to[i] = scale.each ? scale.each[i] : scale.all;
-  const int e = plan.tile(tile);
+  const Tile at = plan.tile(tile);
+  const int e = at.e;
   if (e < 0 || e >= plan.E) return;
-  if (threadIdx.x < kRows) rows[threadIdx.x] = plan.row(tile * kRows + threadIdx.x, e);
+  if (threadIdx.x < kRows) rows[threadIdx.x] = plan.row(at, threadIdx.x);
   __syncthreads();
   const int m = lane & 15, q = lane >> 4;
   const T* px[RB];
@@ -347,12 +363,14 @@ __device__ __forceinline__ float low_at(const float* low, int64_t split_stride, 
 // out[row] = base[row] + low[position] W_e^T: W [E, C, r].  The long axis is
 // the product's M: lane (m, q) of a strip of 64 bytes holds 16 consecutive
 // bytes of row m.  Contraction units of 16 bytes: the hi part's, then the lo
-// part's (which meet the same W).
+// part's (which meet the same W).  A strip's base is loaded a strip ahead.
+// turned: also [parts][r][positions], for outer_kernel, zeros where there is no
+// row.
 template <typename T, int RB>
 __global__ __launch_bounds__(kBlock) void expand_kernel(Plan plan, const float* low, int splits,
                                                         const float* scales, const T* W, int C,
                                                         int r, const T* base, int64_t ld_base,
-                                                        T* out, int strips, int blocks) {
+                                                        T* out, int strips, int blocks, T* turned) {
   constexpr int E = Mat<T>::kE, P = Mat<T>::kParts, MB = E / 4;
   constexpr int kRows = RB * 16;
   constexpr int kStrip = 4 * E;  // columns
@@ -360,17 +378,35 @@ __global__ __launch_bounds__(kBlock) void expand_kernel(Plan plan, const float* 
   __shared__ int rows[kRows];
   const int lane = threadIdx.x & (kWave - 1), w = threadIdx.x / kWave;
   const int block = blockIdx.x % blocks, tile = blockIdx.x / blocks;
-  const int e = plan.tile(tile);
+  const Tile at = plan.tile(tile);
+  const int e = at.e;
   if (e < 0) return;
-  if (threadIdx.x < kRows) rows[threadIdx.x] = plan.row(tile * kRows + threadIdx.x, e);
+  const int m = lane & 15, q = lane >> 4;
+  int row[RB];
+#pragma unroll
+  for (int b = 0; b < RB; ++b) row[b] = plan.row(at, b * 16 + m);
+  const int first = block * strips * kWaves + w, last = (block + 1) * strips * kWaves;
+  u32x4 vb[RB];
+  auto load_base = [&](int strip) {
+    const int64_t c = (int64_t)strip * kStrip + q * E;
+#pragma unroll
+    for (int b = 0; b < RB; ++b)
+      vb[b] = row[b] >= 0 ? load16(base + row[b] * ld_base + c, C - c) : u32x4{0u, 0u, 0u, 0u};
+  };
+  if (base) load_base(first);
   const int chunks = (r + E - 1) / E, units = P * chunks, ld = units + 1;
   const bool adapted = e < plan.E;
   if (adapted) {
+    if (w == 0) {
+#pragma unroll
+      for (int b = 0; b < RB; ++b)
+        if (q == 0) rows[b * 16 + m] = row[b];
+    }
     const float scale = scales[e];
     const int64_t split_stride = (int64_t)plan.tiles * kRows * r;
     T* f = reinterpret_cast<T*>(frags);
     for (int i = threadIdx.x; i < kRows * chunks * E; i += kBlock) {
-      const int n = i / (chunks * E), k = i % (chunks * E);
+      const int n = i / (chunks * E), k = i - n * (chunks * E);
       const float v = k < r ? low_at(low, split_stride, splits,
                                      ((int64_t)tile * kRows + n) * r + k, scale)
                             : 0.0f;
@@ -379,22 +415,25 @@ __global__ __launch_bounds__(kBlock) void expand_kernel(Plan plan, const float* 
       if constexpr (P == 2)
         f[(int64_t)n * ld * E + chunks * E + k] = Mat<T>::from(v - Mat<T>::to(hi));
     }
+    __syncthreads();
+    if (turned && block == 0) {
+      const int64_t n_all = (int64_t)plan.tiles * kRows;
+      for (int i = threadIdx.x; i < P * r * kRows; i += kBlock) {
+        const int n = i % kRows, k = i / kRows, part = k >= r ? 1 : 0;
+        turned[k * n_all + tile * kRows + n] =
+            rows[n] >= 0 ? f[(int64_t)n * ld * E + part * chunks * E + k - part * r] : T{};
+      }
+    }
   }
-  __syncthreads();
-  const int m = lane & 15, q = lane >> 4;
-  int row[RB];
-#pragma unroll
-  for (int b = 0; b < RB; ++b) row[b] = rows[b * 16 + m];
-  const int last = (block + 1) * strips * kWaves;
-  for (int strip = block * strips * kWaves + w; strip < last; strip += kWaves) {
+  for (int strip = first; strip < last; strip += kWaves) {
     const int64_t c0 = (int64_t)strip * kStrip;
     if (c0 >= C) break;
     const int64_t c = c0 + q * E, left = C - c;
-    u32x4 vb[RB];
+    u32x4 old[RB];
     if (base) {
 #pragma unroll
-      for (int b = 0; b < RB; ++b)
-        vb[b] = row[b] >= 0 ? load16(base + row[b] * ld_base + c, left) : u32x4{0u, 0u, 0u, 0u};
+      for (int b = 0; b < RB; ++b) old[b] = vb[b];
+      if (strip + kWaves < last) load_base(strip + kWaves);
     }
     f32x4 acc[RB][MB];
 #pragma unroll
@@ -425,24 +464,23 @@ __global__ __launch_bounds__(kBlock) void expand_kernel(Plan plan, const float* 
           for (int b = 0; b < MB; ++b) acc[a][b] = Mat<T>::mma(vw[b], vl[a], acc[a][b]);
       }
     }
-    if (left <= 0) continue;
     const float bad = e > plan.E ? __builtin_nanf("") : 0.0f;
 #pragma unroll
     for (int a = 0; a < RB; ++a) {
-      if (row[a] < 0) continue;
+      if (row[a] < 0 || left <= 0) continue;
       u32x4 v;
 #pragma unroll
       for (int j = 0; j < E; j += (E == 4 ? 1 : 2)) {
         if constexpr (E == 4) {
-          v[j] = f2u(acc[a][0][j] + (base ? u2f(vb[a][j]) : 0.0f) + bad);
+          v[j] = f2u(acc[a][0][j] + (base ? u2f(old[a][j]) : 0.0f) + bad);
         } else {
           float y[2];
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            const float old = base ? Mat<T>::to(__builtin_bit_cast(
-                                         T, (uint16_t)(vb[a][j / 2] >> (16 * h))))
+            const float was = base ? Mat<T>::to(__builtin_bit_cast(
+                                         T, (uint16_t)(old[a][j / 2] >> (16 * h))))
                                    : 0.0f;
-            y[h] = acc[a][(j + h) / 4][(j + h) % 4] + old + bad;
+            y[h] = acc[a][(j + h) / 4][(j + h) % 4] + was + bad;
           }
           v[j / 2] = (uint32_t)__builtin_bit_cast(uint16_t, Mat<T>::from(y[0])) |
                      (uint32_t)__builtin_bit_cast(uint16_t, Mat<T>::from(y[1])) << 16;
@@ -455,30 +493,41 @@ __global__ __launch_bounds__(kBlock) void expand_kernel(Plan plan, const float* 
 
 // --------------------------------------------- small pieces of the backward
 
-// out [E][b][a] from in [E][a][b]
-template <typename T>
-__global__ __launch_bounds__(kBlock) void turn_kernel(const T* in, T* out, int64_t n, int a, int b) {
-  const int64_t i = (int64_t)blockIdx.x * kBlock + threadIdx.x;
-  if (i >= n) return;
-  const int64_t e = i / ((int64_t)a * b), k = i - e * a * b;
-  const int64_t y = k / a, x = k - y * a;
-  out[i] = in[e * a * b + x * b + y];
-}
+// A matrix [E][a][b] turned to [E][b][a].
+struct Turn {
+  const void* in;
+  void* out;
+  int64_t n;  // values, 0: none
+  int a, b;
+};
 
-// The low-rank rows along the positions, as outer_kernel reads them: to
-// [parts][r][positions], zeros where there is no row of an adapter.
+// Ahead of the backward's products, in one launch: a turned, b turned, and the
+// low-rank rows `low` along the positions as outer_kernel reads them, [parts][r]
+// [positions], zeros where there is no row of an adapter.
 template <typename T>
-__global__ __launch_bounds__(kBlock) void turn_low_kernel(Plan plan, const float* low, int splits,
-                                                          const float* scales, int r, T* to) {
+__global__ __launch_bounds__(kBlock) void turn_kernel(Turn one, Turn two, int blocks_one,
+                                                      int blocks_two, Plan plan, const float* low,
+                                                      int splits, const float* scales, int r,
+                                                      T* to) {
+  const int64_t block = blockIdx.x;
+  if (block < blocks_one + blocks_two) {
+    const Turn t = block < blocks_one ? one : two;
+    const int64_t i = (block < blocks_one ? block : block - blocks_one) * kBlock + threadIdx.x;
+    if (i >= t.n) return;
+    const int64_t each = (int64_t)t.a * t.b, e = i / each;
+    const int k = (int)(i - e * each), y = k / t.a, x = k - y * t.a;
+    reinterpret_cast<T*>(t.out)[i] = reinterpret_cast<const T*>(t.in)[e * each + (int64_t)x * t.b + y];
+    return;
+  }
   constexpr int P = Mat<T>::kParts;
   const int64_t n = (int64_t)plan.tiles * plan.T;
-  const int64_t i = (int64_t)blockIdx.x * kBlock + threadIdx.x;
+  const int64_t i = (block - blocks_one - blocks_two) * kBlock + threadIdx.x;
   if (i >= n * r) return;
   const int64_t k = i / n, p = i - k * n;
-  const int e = plan.tile((int)(p / plan.T));
+  const Tile t = plan.tile((int)(p / plan.T));
   float v = 0.0f;
-  if (e >= 0 && e < plan.E && plan.row((int)p, e) >= 0)
-    v = low_at(low, n * r, splits, p * r + k, scales[e]);
+  if (t.e >= 0 && t.e < plan.E && t.at + (int)(p % plan.T) < t.rows)
+    v = low_at(low, n * r, splits, p * r + k, scales[t.e]);
   const T hi = Mat<T>::from(v);
   to[i] = hi;
   if constexpr (P == 2) to[n * r + i] = Mat<T>::from(v - Mat<T>::to(hi));
@@ -486,13 +535,16 @@ __global__ __launch_bounds__(kBlock) void turn_low_kernel(Plan plan, const float
 
 // ------------------------------------------------------------------ outer
 
+constexpr int kMaxChunk = 1024;  // rows of a chunk, their numbers in LDS
+
 // One of a backward's two: y [N, C] and low [parts][r][positions].
 struct Side {
   const void* y;
   const void* low;
-  float* part;  // [slots][r][C]
+  float* part;  // [slots][r][C] (turned: [slots][C][r])
   int64_t ld;
   int32_t C, blocks;  // workgroups along C
+  int32_t turned;
 };
 
 // part[slot][k][c] = sum over a chunk's rows of one adapter of low[k] y[c].
@@ -505,6 +557,7 @@ __global__ __launch_bounds__(kBlock) void outer_kernel(Plan plan, Side one, Side
   constexpr int E = Mat<T>::kE, P = Mat<T>::kParts;
   constexpr int kCols = 16 * E;
   __shared__ float sum[16][kCols + 4];
+  __shared__ int rows[kMaxChunk];
   const int lane = threadIdx.x & (kWave - 1), w = threadIdx.x / kWave;
   const int all = one.blocks + two.blocks;
   const int i = blockIdx.x / all, at = blockIdx.x % all;
@@ -517,13 +570,16 @@ __global__ __launch_bounds__(kBlock) void outer_kernel(Plan plan, Side one, Side
   const T* low = reinterpret_cast<const T*>(s.low);
   const int64_t left = s.C - c0 - m * E;
   const int begin = i * chunk;
-  const int end = plan.mem ? plan.start()[plan.E] : plan.N;  // of the adapters' rows
-  int stop = begin + chunk < end ? begin + chunk : end;
+  const int end = plan.start(plan.E);  // of the adapters' positions
+  const int stop = begin + chunk < end ? begin + chunk : end;
+  for (int p = begin + threadIdx.x; p < stop; p += kBlock) {
+    const Tile t = plan.tile(p / plan.T);
+    rows[p - begin] = plan.row(t, p % plan.T);
+  }
+  __syncthreads();
   for (int p = begin; p < stop;) {
-    const int e = plan.tile(p / plan.T);
-    int to = plan.mem ? plan.start()[e] + plan.rows()[e] : end;  // the adapter's last row
-    const int next = plan.mem ? plan.start()[e + 1] : end;
-    if (to > stop) to = stop;
+    const int e = plan.tile(p / plan.T).e;
+    const int next = plan.start(e + 1), to = next < stop ? next : stop;
     f32x4 acc[E][NB];
 #pragma unroll
     for (int a = 0; a < E; ++a)
@@ -531,18 +587,25 @@ __global__ __launch_bounds__(kBlock) void outer_kernel(Plan plan, Side one, Side
       for (int b = 0; b < NB; ++b) acc[a][b] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     const int share = ((to - p + kWaves - 1) / kWaves + 31) / 32 * 32;
     const int mine = p + w * share, until = mine + share < to ? mine + share : to;
+    u32x4 next_v[8];
+    auto load = [&](int s0) {
+      // (positions are whole tiles of 16 or 64: 8 of them are there or not)
+      const bool in = s0 + q * 8 < until;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const int row = in ? rows[s0 + q * 8 + k - begin] : -1;
+        next_v[k] = row >= 0 ? load16(y + row * s.ld, left) : u32x4{0u, 0u, 0u, 0u};
+      }
+    };
+    load(mine);
     for (int s0 = mine; s0 < until; s0 += 32) {
       u32x4 v[8], vl[NB][P][2];
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const int at_p = s0 + q * 8 + k;
-        const int row = at_p < until ? plan.row(at_p, e) : -1;
-        v[k] = row >= 0 ? load16(y + row * s.ld, left) : u32x4{0u, 0u, 0u, 0u};
-      }
+      for (int k = 0; k < 8; ++k) v[k] = next_v[k];
+      load(s0 + 32);
 #pragma unroll
       for (int b = 0; b < NB; ++b) {
         const int k = r0 + b * 16 + m;
-        // (positions behind the last tile's end are none of the wave's rows)
         const bool in = k < r && s0 + q * 8 < until;
         const T* pl = low + (int64_t)(in ? k : 0) * n + s0 + q * 8;
 #pragma unroll
@@ -592,8 +655,10 @@ __global__ __launch_bounds__(kBlock) void outer_kernel(Plan plan, Side one, Side
         __syncthreads();
       }
       for (int t = threadIdx.x; t < 16 * kCols; t += kBlock) {
-        const int k = r0 + b * 16 + t / kCols, c = c0 + t % kCols;
-        if (k < r && c < s.C) part[(int64_t)k * s.C + c] = sum[t / kCols][t % kCols];
+        const int x = s.turned ? t % 16 : t / kCols, z = s.turned ? t / 16 : t % kCols;
+        const int k = r0 + b * 16 + x, c = c0 + z;
+        if (k < r && c < s.C)
+          part[s.turned ? (int64_t)c * r + k : (int64_t)k * s.C + c] = sum[x][z];
       }
       __syncthreads();
     }
@@ -601,22 +666,29 @@ __global__ __launch_bounds__(kBlock) void outer_kernel(Plan plan, Side one, Side
   }
 }
 
-// grad [E][r][C] (turned: [E][C][r]) from the slots' sums, in order
+// grad [E][each] from the slots' sums, in order, both sides in one launch
+struct Sum {
+  const float* part;
+  void* grad;
+  int64_t each;   // values of an adapter
+  int64_t blocks;
+};
 template <typename T>
-__global__ __launch_bounds__(kBlock) void outer_sum_kernel(Plan plan, const float* part, int r,
-                                                           int C, int chunk, int turned, T* grad) {
-  const int64_t each = (int64_t)r * C, t = (int64_t)blockIdx.x * kBlock + threadIdx.x;
-  if (t >= each * plan.E) return;
-  const int e = (int)(t / each);
-  int64_t k = t - e * each;
-  const int64_t at = k;
-  if (turned) k = (at % r) * C + at / r;
-  const int from = plan.mem ? plan.start()[e] : 0;
-  const int n = plan.mem ? plan.rows()[e] : plan.N;
-  float s = 0.0f;
-  if (n > 0)
-    for (int i = from / chunk; i <= (from + n - 1) / chunk; ++i) s += part[(i + e) * each + k];
-  grad[e * each + at] = Mat<T>::from(s);
+__global__ __launch_bounds__(kBlock) void outer_sum_kernel(Plan plan, Sum one, Sum two, int chunk) {
+  const int64_t block = blockIdx.x;
+  const Sum s = block < one.blocks ? one : two;
+  const int64_t t = (block < one.blocks ? block : block - one.blocks) * kBlock + threadIdx.x;
+  if (t >= s.each * plan.E) return;
+  const int e = (int)(t / s.each);
+  const int n = plan.rows(e);
+  float v = 0.0f;
+  if (n > 0) {
+    const int from = plan.start(e) / chunk, to = (plan.start(e) + n - 1) / chunk;
+    const float* p = s.part + (int64_t)(from + e) * s.each + (t - e * s.each);
+#pragma unroll 8
+    for (int i = from; i <= to; ++i, p += s.each) v += *p;
+  }
+  reinterpret_cast<T*>(s.grad)[t] = Mat<T>::from(v);
 }
 
 // ------------------------------------------------------------------- host
@@ -632,7 +704,7 @@ int64_t round_up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
 // Workgroups for the chip, of at least 4 steps of 128 bytes for each wave.
 int32_t splits_of(int64_t tiles, int64_t C, int64_t size) {
   const int64_t steps = (C * size + 127) / 128;
-  int64_t s = (768 + tiles - 1) / tiles, most = (steps + 4 * kWaves - 1) / (4 * kWaves);
+  int64_t s = (512 + tiles - 1) / tiles, most = (steps + 4 * kWaves - 1) / (4 * kWaves);
   if (s > most) s = most;
   return (int32_t)(s < 1 ? 1 : s);
 }
@@ -662,6 +734,7 @@ int check(const gtp_lora* q) {
   if (q->rank > kMaxRank || q->adapters > kMaxAdapters || q->in > (1 << 24) ||
       q->out > (1 << 24) || q->requests > (1 << 24) || q->rows > (1 << 24) ||
       q->requests * q->rows > (1 << 24) - 131072 ||
+      q->rank * (q->in > q->out ? q->in : q->out) > 0x7FFFFFFF ||
       (int64_t)q->adapters * q->rank * (q->in > q->out ? q->in : q->out) > (1ll << 38))
     return GTP_ERR_UNSUPPORTED;
   return GTP_OK;
@@ -704,11 +777,11 @@ void shrink(const Plan& p, const T* x, int64_t ld, const T* W, int64_t C, int r,
 
 template <typename T>
 void expand(const Plan& p, const float* low, int splits, const float* scales, const T* W, int64_t C, int r,
-            const T* base, int64_t ld_base, T* out, hipStream_t s) {
+            const T* base, int64_t ld_base, T* out, T* turned, hipStream_t s) {
   constexpr int E = Mat<T>::kE, P = Mat<T>::kParts;
   const int64_t wave_strips = (C + 4 * E * kWaves - 1) / (4 * E * kWaves);
   // strips per wave: fewer where there are few tiles
-  int64_t blocks = (2048 + p.tiles - 1) / p.tiles;
+  int64_t blocks = (1024 + p.tiles - 1) / p.tiles;
   if (blocks > wave_strips) blocks = wave_strips;
   const int strips = (int)((wave_strips + blocks - 1) / blocks);
   blocks = (wave_strips + strips - 1) / strips;
@@ -716,10 +789,10 @@ void expand(const Plan& p, const float* low, int splits, const float* scales, co
   const dim3 grid((uint32_t)(p.tiles * blocks));
   if (p.T == 16)
     hipLaunchKernelGGL((expand_kernel<T, 1>), grid, dim3(kBlock), lds, s, p, low, splits, scales, W,
-                       (int)C, r, base, ld_base, out, strips, (int)blocks);
+                       (int)C, r, base, ld_base, out, strips, (int)blocks, turned);
   else
     hipLaunchKernelGGL((expand_kernel<T, 4>), grid, dim3(kBlock), lds, s, p, low, splits, scales, W,
-                       (int)C, r, base, ld_base, out, strips, (int)blocks);
+                       (int)C, r, base, ld_base, out, strips, (int)blocks, turned);
 }
 
 template <typename T>
@@ -734,7 +807,8 @@ void forward(const gtp_lora* q, const Sizes& z, char* state, hipStream_t s) {
   shrink<T>(p, reinterpret_cast<const T*>(q->x), q->x_stride, reinterpret_cast<const T*>(q->a),
             q->in, q->rank, z.splits_x, low, Scale{q->scales, q->scale, scales}, s);
   expand<T>(p, low, z.splits_x, scales, reinterpret_cast<const T*>(q->b), q->out, q->rank,
-            reinterpret_cast<const T*>(q->base), q->base_stride, reinterpret_cast<T*>(q->y), s);
+            reinterpret_cast<const T*>(q->base), q->base_stride, reinterpret_cast<T*>(q->y),
+            static_cast<T*>(nullptr), s);
 }
 
 // The backward's workspace.
@@ -763,7 +837,8 @@ Work work_of(const gtp_lora* q, const Sizes& z) {
   int64_t chunks = (1024 + blocks - 1) / blocks;
   if (chunks > (n + 127) / 128) chunks = (n + 127) / 128;
   if (chunks < 1) chunks = 1;
-  k.chunk = (int)round_up((n + chunks - 1) / chunks, z.T < 64 ? 64 : z.T);
+  k.chunk = (int)round_up((n + chunks - 1) / chunks, 64);
+  if (k.chunk > kMaxChunk) k.chunk = kMaxChunk;
   k.chunks = (int)((n + k.chunk - 1) / k.chunk);
   k.part_a = take((k.chunks + E) * r * q->in * 4);
   k.part_b = take((k.chunks + E) * r * q->out * 4);
@@ -780,42 +855,39 @@ void backward(const gtp_lora* q, const gtp_lora_grads* d, const Sizes& z, const 
   const float* scales = reinterpret_cast<const float*>(state + z.plan_bytes);
   const float* low_u = reinterpret_cast<const float*>(state + z.plan_bytes + z.scale_bytes);
   float* low_v = reinterpret_cast<float*>(ws + k.low_v);
+  T* turned_a = reinterpret_cast<T*>(ws + k.turned_a);
   T* turned_b = reinterpret_cast<T*>(ws + k.turned_b);
+  T* tu = reinterpret_cast<T*>(ws + k.low_tu);
+  T* tv = reinterpret_cast<T*>(ws + k.low_tv);
   const int r = q->rank;
   const int64_t na = (int64_t)p.E * r * q->in, nb = (int64_t)p.E * r * q->out;
   const int64_t nl = (int64_t)p.tiles * p.T * r;
-  auto blocks_of = [](int64_t n) { return dim3((uint32_t)((n + kBlock - 1) / kBlock)); };
-  if (d->grad_x || d->grad_a) {
-    hipLaunchKernelGGL(turn_kernel<T>, blocks_of(nb), dim3(kBlock), 0, s,
-                       reinterpret_cast<const T*>(q->b), turned_b, nb, (int)q->out, r);
+  const bool need_v = d->grad_x || d->grad_a;
+  auto blocks_of = [](int64_t n) { return (n + kBlock - 1) / kBlock; };
+  const Turn ta{q->a, turned_a, d->grad_x ? na : 0, r, (int)q->in};
+  const Turn tb{q->b, turned_b, need_v ? nb : 0, (int)q->out, r};
+  const int64_t turns = blocks_of(ta.n) + blocks_of(tb.n) + (d->grad_b ? blocks_of(nl) : 0);
+  if (turns > 0)
+    hipLaunchKernelGGL(turn_kernel<T>, dim3((uint32_t)turns), dim3(kBlock), 0, s, ta, tb,
+                       (int)blocks_of(ta.n), (int)blocks_of(tb.n), p, low_u, z.splits_x, scales, r,
+                       tu);
+  if (need_v)
     shrink<T>(p, reinterpret_cast<const T*>(d->grad), d->grad_stride, turned_b, q->out, r,
               z.splits_g, low_v, Scale{nullptr, 0.0f, nullptr}, s);
-  }
-  if (d->grad_x) {
-    T* turned_a = reinterpret_cast<T*>(ws + k.turned_a);
-    hipLaunchKernelGGL(turn_kernel<T>, blocks_of(na), dim3(kBlock), 0, s,
-                       reinterpret_cast<const T*>(q->a), turned_a, na, r, (int)q->in);
-    expand<T>(p, low_v, z.splits_g, scales, turned_a, q->in, r, static_cast<const T*>(nullptr),
-              0, reinterpret_cast<T*>(d->grad_x), s);
-  }
+  if (d->grad_x)
+    expand<T>(p, low_v, z.splits_g, scales, turned_a, q->in, r, static_cast<const T*>(nullptr), 0,
+              reinterpret_cast<T*>(d->grad_x), d->grad_a ? tv : static_cast<T*>(nullptr), s);
+  else if (d->grad_a)
+    hipLaunchKernelGGL(turn_kernel<T>, dim3((uint32_t)blocks_of(nl)), dim3(kBlock), 0, s, Turn{},
+                       Turn{}, 0, 0, p, low_v, z.splits_g, scales, r, tv);
   if (!d->grad_a && !d->grad_b) return;
-  T* tu = reinterpret_cast<T*>(ws + k.low_tu);
-  T* tv = reinterpret_cast<T*>(ws + k.low_tv);
   float* part_a = reinterpret_cast<float*>(ws + k.part_a);
   float* part_b = reinterpret_cast<float*>(ws + k.part_b);
   const int64_t cols = 16 * E;
-  Side a{q->x, tv, part_a, q->x_stride, (int32_t)q->in, 0};
-  Side b{d->grad, tu, part_b, d->grad_stride, (int32_t)q->out, 0};
-  if (d->grad_a) {
-    a.blocks = (int32_t)((q->in + cols - 1) / cols);
-    hipLaunchKernelGGL(turn_low_kernel<T>, blocks_of(nl), dim3(kBlock), 0, s, p, low_v, z.splits_g,
-                       scales, r, tv);
-  }
-  if (d->grad_b) {
-    b.blocks = (int32_t)((q->out + cols - 1) / cols);
-    hipLaunchKernelGGL(turn_low_kernel<T>, blocks_of(nl), dim3(kBlock), 0, s, p, low_u, z.splits_x,
-                       scales, r, tu);
-  }
+  const Side a{q->x, tv, part_a, q->x_stride, (int32_t)q->in,
+               d->grad_a ? (int32_t)((q->in + cols - 1) / cols) : 0, 0};
+  const Side b{d->grad, tu, part_b, d->grad_stride, (int32_t)q->out,
+               d->grad_b ? (int32_t)((q->out + cols - 1) / cols) : 0, 1};
   const dim3 grid((uint32_t)((int64_t)k.chunks * (a.blocks + b.blocks)),
                   (uint32_t)((r + kRankStep - 1) / kRankStep));
   if (r <= 16)
@@ -824,12 +896,10 @@ void backward(const gtp_lora* q, const gtp_lora_grads* d, const Sizes& z, const 
     hipLaunchKernelGGL((outer_kernel<T, 2>), grid, dim3(kBlock), 0, s, p, a, b, r, k.chunk);
   else
     hipLaunchKernelGGL((outer_kernel<T, 4>), grid, dim3(kBlock), 0, s, p, a, b, r, k.chunk);
-  if (d->grad_a)
-    hipLaunchKernelGGL(outer_sum_kernel<T>, blocks_of(na), dim3(kBlock), 0, s, p, part_a, r,
-                       (int)q->in, k.chunk, 0, reinterpret_cast<T*>(d->grad_a));
-  if (d->grad_b)
-    hipLaunchKernelGGL(outer_sum_kernel<T>, blocks_of(nb), dim3(kBlock), 0, s, p, part_b, r,
-                       (int)q->out, k.chunk, 1, reinterpret_cast<T*>(d->grad_b));
+  const Sum sa{part_a, d->grad_a, (int64_t)r * q->in, d->grad_a ? blocks_of(na) : 0};
+  const Sum sb{part_b, d->grad_b, (int64_t)r * q->out, d->grad_b ? blocks_of(nb) : 0};
+  hipLaunchKernelGGL(outer_sum_kernel<T>, dim3((uint32_t)(sa.blocks + sb.blocks)), dim3(kBlock), 0,
+                     s, p, sa, sb, k.chunk);
 }
 
 }  // namespace lora
