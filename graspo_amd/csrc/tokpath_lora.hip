@@ -350,12 +350,88 @@ __global__ __launch_bounds__(kBlock) void shrink_kernel(Plan plan, const T* x, i
     to_low[(int64_t)(i / n) * r + i % n] = sum[i / n][i % n];
 }
 
-// a low-rank value: the splits' sum, scaled
-__device__ __forceinline__ float low_at(const float* low, int64_t split_stride, int splits,
-                                        int64_t at, float scale) {
-  float s = low[at];
-  for (int k = 1; k < splits; ++k) s += low[at + k * split_stride];
-  return s * scale;
+// kE low-rank values of a position from k on: the splits' sums, scaled, as the
+// parts' operands; zeros past the rank.
+template <typename T>
+__device__ __forceinline__ void low_units(const float* low, int64_t split_stride, int splits,
+                                          int r, int k, float scale, u32x4 (&unit)[Mat<T>::kParts]) {
+  constexpr int E = Mat<T>::kE, P = Mat<T>::kParts;
+  float v[E];
+#pragma unroll
+  for (int j = 0; j < E; ++j) v[j] = 0.0f;
+  if (k + E <= r) {
+#pragma unroll 4
+    for (int i = 0; i < splits; ++i) {
+      const float* p = low + i * split_stride + k;
+#pragma unroll
+      for (int j = 0; j < E; ++j) v[j] += p[j];
+    }
+  } else {
+    for (int i = 0; i < splits; ++i)
+#pragma unroll
+      for (int j = 0; j < E; ++j)
+        if (k + j < r) v[j] += low[i * split_stride + k + j];
+  }
+#pragma unroll
+  for (int h = 0; h < P; ++h) unit[h] = u32x4{0u, 0u, 0u, 0u};
+#pragma unroll
+  for (int j = 0; j < E; ++j) {
+    const float x = v[j] * scale;
+    if constexpr (E == 4) {
+      unit[0][j] = f2u(x);
+    } else {
+      const T hi = Mat<T>::from(x), lo = Mat<T>::from(x - Mat<T>::to(hi));
+      unit[0][j / 2] |= (uint32_t)__builtin_bit_cast(uint16_t, hi) << (16 * (j & 1));
+      unit[1][j / 2] |= (uint32_t)__builtin_bit_cast(uint16_t, lo) << (16 * (j & 1));
+    }
+  }
+}
+
+// The low-rank rows as the products' operands, from the splits' sums, a thread
+// for a position's kE values: `units` [positions][parts][chunks] for
+// expand_kernel, `turned` [parts][r][positions] for outer_kernel (zeros where
+// there is no row of an adapter), either null.
+template <typename T>
+__device__ __forceinline__ void low_operands(const Plan& plan, const float* low, int splits,
+                                             const float* scales, int r, int64_t i, u32x4* units,
+                                             T* turned) {
+  constexpr int E = Mat<T>::kE, P = Mat<T>::kParts;
+  const int64_t n = (int64_t)plan.tiles * plan.T;
+  const int chunks = (r + E - 1) / E;
+  if (i >= n * chunks) return;
+  const int c = (int)(i / n);
+  const int64_t p = i - c * n;
+  const Tile t = plan.tile((int)(p / plan.T));
+  const bool in = t.e >= 0 && t.e < plan.E;
+  u32x4 u[P];
+  if (in && t.at + (int)(p % plan.T) < t.rows) {
+    low_units<T>(low + p * r, n * r, splits, r, c * E, scales[t.e], u);
+  } else {
+#pragma unroll
+    for (int h = 0; h < P; ++h) u[h] = u32x4{0u, 0u, 0u, 0u};
+  }
+#pragma unroll
+  for (int h = 0; h < P; ++h) {
+    if (units && in) units[(p * P + h) * chunks + c] = u[h];
+    if (turned) {
+#pragma unroll
+      for (int j = 0; j < E; ++j)
+        if (c * E + j < r) {
+          T x;
+          if constexpr (E == 4) x = u2f(u[h][j]);
+          else x = __builtin_bit_cast(T, (uint16_t)(u[h][j / 2] >> (16 * (j & 1))));
+          turned[((int64_t)h * r + c * E + j) * n + p] = x;
+        }
+    }
+  }
+}
+
+template <typename T>
+__global__ __launch_bounds__(kBlock) void low_kernel(Plan plan, const float* low, int splits,
+                                                     const float* scales, int r, u32x4* units,
+                                                     T* turned) {
+  low_operands<T>(plan, low, splits, scales, r, (int64_t)blockIdx.x * kBlock + threadIdx.x, units,
+                  turned);
 }
 
 // ----------------------------------------------------------------- expand
@@ -364,18 +440,18 @@ __device__ __forceinline__ float low_at(const float* low, int64_t split_stride, 
 // the product's M: lane (m, q) of a strip of 64 bytes holds 16 consecutive
 // bytes of row m.  Contraction units of 16 bytes: the hi part's, then the lo
 // part's (which meet the same W).  A strip's base is loaded a strip ahead.
-// turned: also [parts][r][positions], for outer_kernel, zeros where there is no
-// row.
+// ready: low_kernel's units; null: summed here, which is less than a launch for
+// tiles of 16 rows.
 template <typename T, int RB>
 __global__ __launch_bounds__(kBlock) void expand_kernel(Plan plan, const float* low, int splits,
                                                         const float* scales, const T* W, int C,
                                                         int r, const T* base, int64_t ld_base,
-                                                        T* out, int strips, int blocks, T* turned) {
+                                                        T* out, int strips, int blocks,
+                                                        const u32x4* ready) {
   constexpr int E = Mat<T>::kE, P = Mat<T>::kParts, MB = E / 4;
   constexpr int kRows = RB * 16;
   constexpr int kStrip = 4 * E;  // columns
   extern __shared__ u32x4 frags[];  // [kRows][units + 1]
-  __shared__ int rows[kRows];
   const int lane = threadIdx.x & (kWave - 1), w = threadIdx.x / kWave;
   const int block = blockIdx.x % blocks, tile = blockIdx.x / blocks;
   const Tile at = plan.tile(tile);
@@ -397,33 +473,22 @@ __global__ __launch_bounds__(kBlock) void expand_kernel(Plan plan, const float* 
   const int chunks = (r + E - 1) / E, units = P * chunks, ld = units + 1;
   const bool adapted = e < plan.E;
   if (adapted) {
-    if (w == 0) {
+    if (ready) {
+      const u32x4* from = ready + (int64_t)tile * kRows * units;
+      for (int i = threadIdx.x; i < kRows * units; i += kBlock)
+        frags[i / units * ld + i % units] = from[i];
+    } else {
+      const float scale = scales[e];
+      const int64_t split_stride = (int64_t)plan.tiles * kRows * r;
+      for (int i = threadIdx.x; i < kRows * chunks; i += kBlock) {
+        const int n = i / chunks, c = i - n * chunks;
+        u32x4 u[P];
+        low_units<T>(low + ((int64_t)tile * kRows + n) * r, split_stride, splits, r, c * E, scale, u);
 #pragma unroll
-      for (int b = 0; b < RB; ++b)
-        if (q == 0) rows[b * 16 + m] = row[b];
-    }
-    const float scale = scales[e];
-    const int64_t split_stride = (int64_t)plan.tiles * kRows * r;
-    T* f = reinterpret_cast<T*>(frags);
-    for (int i = threadIdx.x; i < kRows * chunks * E; i += kBlock) {
-      const int n = i / (chunks * E), k = i - n * (chunks * E);
-      const float v = k < r ? low_at(low, split_stride, splits,
-                                     ((int64_t)tile * kRows + n) * r + k, scale)
-                            : 0.0f;
-      const T hi = Mat<T>::from(v);
-      f[(int64_t)n * ld * E + k] = hi;
-      if constexpr (P == 2)
-        f[(int64_t)n * ld * E + chunks * E + k] = Mat<T>::from(v - Mat<T>::to(hi));
-    }
-    __syncthreads();
-    if (turned && block == 0) {
-      const int64_t n_all = (int64_t)plan.tiles * kRows;
-      for (int i = threadIdx.x; i < P * r * kRows; i += kBlock) {
-        const int n = i % kRows, k = i / kRows, part = k >= r ? 1 : 0;
-        turned[k * n_all + tile * kRows + n] =
-            rows[n] >= 0 ? f[(int64_t)n * ld * E + part * chunks * E + k - part * r] : T{};
+        for (int h = 0; h < P; ++h) frags[n * ld + h * chunks + c] = u[h];
       }
     }
+    __syncthreads();
   }
   for (int strip = first; strip < last; strip += kWaves) {
     const int64_t c0 = (int64_t)strip * kStrip;
@@ -501,36 +566,25 @@ struct Turn {
   int a, b;
 };
 
-// Ahead of the backward's products, in one launch: a turned, b turned, and the
-// low-rank rows `low` along the positions as outer_kernel reads them, [parts][r]
-// [positions], zeros where there is no row of an adapter.
+// Ahead of the backward's products, in one launch: a turned, b turned, and
+// low_kernel's `turned` of the forward's sums.
 template <typename T>
-__global__ __launch_bounds__(kBlock) void turn_kernel(Turn one, Turn two, int blocks_one,
-                                                      int blocks_two, Plan plan, const float* low,
-                                                      int splits, const float* scales, int r,
-                                                      T* to) {
+__global__ __launch_bounds__(kBlock) void turn_kernel(Turn one, Turn two, int64_t blocks_one,
+                                                      int64_t blocks_two, Plan plan,
+                                                      const float* low, int splits,
+                                                      const float* scales, int r, T* to) {
   const int64_t block = blockIdx.x;
-  if (block < blocks_one + blocks_two) {
-    const Turn t = block < blocks_one ? one : two;
-    const int64_t i = (block < blocks_one ? block : block - blocks_one) * kBlock + threadIdx.x;
-    if (i >= t.n) return;
-    const int64_t each = (int64_t)t.a * t.b, e = i / each;
-    const int k = (int)(i - e * each), y = k / t.a, x = k - y * t.a;
-    reinterpret_cast<T*>(t.out)[i] = reinterpret_cast<const T*>(t.in)[e * each + (int64_t)x * t.b + y];
+  if (block >= blocks_one + blocks_two) {
+    low_operands<T>(plan, low, splits, scales, r,
+                    (block - blocks_one - blocks_two) * kBlock + threadIdx.x, nullptr, to);
     return;
   }
-  constexpr int P = Mat<T>::kParts;
-  const int64_t n = (int64_t)plan.tiles * plan.T;
-  const int64_t i = (block - blocks_one - blocks_two) * kBlock + threadIdx.x;
-  if (i >= n * r) return;
-  const int64_t k = i / n, p = i - k * n;
-  const Tile t = plan.tile((int)(p / plan.T));
-  float v = 0.0f;
-  if (t.e >= 0 && t.e < plan.E && t.at + (int)(p % plan.T) < t.rows)
-    v = low_at(low, n * r, splits, p * r + k, scales[t.e]);
-  const T hi = Mat<T>::from(v);
-  to[i] = hi;
-  if constexpr (P == 2) to[n * r + i] = Mat<T>::from(v - Mat<T>::to(hi));
+  const Turn t = block < blocks_one ? one : two;
+  const int64_t i = (block < blocks_one ? block : block - blocks_one) * kBlock + threadIdx.x;
+  if (i >= t.n) return;
+  const int64_t each = (int64_t)t.a * t.b, e = i / each;
+  const int k = (int)(i - e * each), y = k / t.a, x = k - y * t.a;
+  reinterpret_cast<T*>(t.out)[i] = reinterpret_cast<const T*>(t.in)[e * each + (int64_t)x * t.b + y];
 }
 
 // ------------------------------------------------------------------ outer
@@ -696,7 +750,7 @@ __global__ __launch_bounds__(kBlock) void outer_sum_kernel(Plan plan, Sum one, S
 // Sizes that the launches and the workspaces go by.
 struct Sizes {
   int32_t T, tiles, splits_x, splits_g;
-  int64_t plan_bytes, scale_bytes, low_bytes;  // low: the forward's partial sums
+  int64_t plan_bytes, scale_bytes, low_bytes, units_bytes;  // low: the forward's partial sums
 };
 
 int64_t round_up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
@@ -721,6 +775,9 @@ Sizes sizes_of(const gtp_lora* q) {
   z.plan_bytes = q->ids ? round_up(Plan::words(q->requests, q->adapters, z.tiles) * 4, 256) : 0;
   z.scale_bytes = round_up((int64_t)q->adapters * 4, 256);
   z.low_bytes = round_up((int64_t)z.splits_x * z.tiles * z.T * q->rank * 4, 256);
+  // low_kernel's operands; tiles of 16 rows do without
+  const int64_t E = 16 / size, units = (size == 4 ? 1 : 2) * ((q->rank + E - 1) / E);
+  z.units_bytes = (int64_t)z.tiles * z.T * units * 16;
   return z;
 }
 
@@ -777,7 +834,7 @@ void shrink(const Plan& p, const T* x, int64_t ld, const T* W, int64_t C, int r,
 
 template <typename T>
 void expand(const Plan& p, const float* low, int splits, const float* scales, const T* W, int64_t C, int r,
-            const T* base, int64_t ld_base, T* out, T* turned, hipStream_t s) {
+            const T* base, int64_t ld_base, T* out, const u32x4* ready, hipStream_t s) {
   constexpr int E = Mat<T>::kE, P = Mat<T>::kParts;
   const int64_t wave_strips = (C + 4 * E * kWaves - 1) / (4 * E * kWaves);
   // strips per wave: fewer where there are few tiles
@@ -789,10 +846,18 @@ void expand(const Plan& p, const float* low, int splits, const float* scales, co
   const dim3 grid((uint32_t)(p.tiles * blocks));
   if (p.T == 16)
     hipLaunchKernelGGL((expand_kernel<T, 1>), grid, dim3(kBlock), lds, s, p, low, splits, scales, W,
-                       (int)C, r, base, ld_base, out, strips, (int)blocks, turned);
+                       (int)C, r, base, ld_base, out, strips, (int)blocks, ready);
   else
     hipLaunchKernelGGL((expand_kernel<T, 4>), grid, dim3(kBlock), lds, s, p, low, splits, scales, W,
-                       (int)C, r, base, ld_base, out, strips, (int)blocks, turned);
+                       (int)C, r, base, ld_base, out, strips, (int)blocks, ready);
+}
+
+template <typename T>
+void low_launch(const Plan& p, const float* low, int splits, const float* scales, int r,
+                u32x4* units, T* turned, hipStream_t s) {
+  const int64_t n = (int64_t)p.tiles * p.T * ((r + Mat<T>::kE - 1) / Mat<T>::kE);
+  hipLaunchKernelGGL(low_kernel<T>, dim3((uint32_t)((n + kBlock - 1) / kBlock)), dim3(kBlock), 0, s,
+                     p, low, splits, scales, r, units, turned);
 }
 
 template <typename T>
@@ -806,14 +871,19 @@ void forward(const gtp_lora* q, const Sizes& z, char* state, hipStream_t s) {
   float* low = reinterpret_cast<float*>(state + z.plan_bytes + z.scale_bytes);
   shrink<T>(p, reinterpret_cast<const T*>(q->x), q->x_stride, reinterpret_cast<const T*>(q->a),
             q->in, q->rank, z.splits_x, low, Scale{q->scales, q->scale, scales}, s);
+  u32x4* units = nullptr;
+  if (z.T != 16) {
+    units = reinterpret_cast<u32x4*>(state + z.plan_bytes + z.scale_bytes + z.low_bytes);
+    low_launch<T>(p, low, z.splits_x, scales, q->rank, units, static_cast<T*>(nullptr), s);
+  }
   expand<T>(p, low, z.splits_x, scales, reinterpret_cast<const T*>(q->b), q->out, q->rank,
             reinterpret_cast<const T*>(q->base), q->base_stride, reinterpret_cast<T*>(q->y),
-            static_cast<T*>(nullptr), s);
+            units, s);
 }
 
 // The backward's workspace.
 struct Work {
-  int64_t turned_a, turned_b, low_v, low_tu, low_tv, part_a, part_b, bytes;
+  int64_t turned_a, turned_b, low_v, units_v, low_tu, low_tv, part_a, part_b, bytes;
   int chunk, chunks;
 };
 
@@ -830,6 +900,7 @@ Work work_of(const gtp_lora* q, const Sizes& z) {
   k.turned_a = take(E * r * q->in * size);
   k.turned_b = take(E * r * q->out * size);
   k.low_v = take((int64_t)z.splits_g * n * r * 4);
+  k.units_v = take(z.units_bytes);
   k.low_tu = take(n * r * size * parts);
   k.low_tv = take(n * r * size * parts);
   // chunks of rows: workgroups for the chip, of at least 128 rows
@@ -861,7 +932,7 @@ void backward(const gtp_lora* q, const gtp_lora_grads* d, const Sizes& z, const 
   T* tv = reinterpret_cast<T*>(ws + k.low_tv);
   const int r = q->rank;
   const int64_t na = (int64_t)p.E * r * q->in, nb = (int64_t)p.E * r * q->out;
-  const int64_t nl = (int64_t)p.tiles * p.T * r;
+  const int64_t nl = (int64_t)p.tiles * p.T * ((r + E - 1) / E);
   const bool need_v = d->grad_x || d->grad_a;
   auto blocks_of = [](int64_t n) { return (n + kBlock - 1) / kBlock; };
   const Turn ta{q->a, turned_a, d->grad_x ? na : 0, r, (int)q->in};
@@ -869,17 +940,17 @@ void backward(const gtp_lora* q, const gtp_lora_grads* d, const Sizes& z, const 
   const int64_t turns = blocks_of(ta.n) + blocks_of(tb.n) + (d->grad_b ? blocks_of(nl) : 0);
   if (turns > 0)
     hipLaunchKernelGGL(turn_kernel<T>, dim3((uint32_t)turns), dim3(kBlock), 0, s, ta, tb,
-                       (int)blocks_of(ta.n), (int)blocks_of(tb.n), p, low_u, z.splits_x, scales, r,
-                       tu);
-  if (need_v)
+                       blocks_of(ta.n), blocks_of(tb.n), p, low_u, z.splits_x, scales, r, tu);
+  if (need_v) {
+    u32x4* units = reinterpret_cast<u32x4*>(ws + k.units_v);
     shrink<T>(p, reinterpret_cast<const T*>(d->grad), d->grad_stride, turned_b, q->out, r,
               z.splits_g, low_v, Scale{nullptr, 0.0f, nullptr}, s);
-  if (d->grad_x)
-    expand<T>(p, low_v, z.splits_g, scales, turned_a, q->in, r, static_cast<const T*>(nullptr), 0,
-              reinterpret_cast<T*>(d->grad_x), d->grad_a ? tv : static_cast<T*>(nullptr), s);
-  else if (d->grad_a)
-    hipLaunchKernelGGL(turn_kernel<T>, dim3((uint32_t)blocks_of(nl)), dim3(kBlock), 0, s, Turn{},
-                       Turn{}, 0, 0, p, low_v, z.splits_g, scales, r, tv);
+    low_launch<T>(p, low_v, z.splits_g, scales, r, d->grad_x ? units : nullptr,
+                  d->grad_a ? tv : static_cast<T*>(nullptr), s);
+    if (d->grad_x)
+      expand<T>(p, low_v, z.splits_g, scales, turned_a, q->in, r, static_cast<const T*>(nullptr), 0,
+                reinterpret_cast<T*>(d->grad_x), units, s);
+  }
   if (!d->grad_a && !d->grad_b) return;
   float* part_a = reinterpret_cast<float*>(ws + k.part_a);
   float* part_b = reinterpret_cast<float*>(ws + k.part_b);
@@ -911,7 +982,7 @@ extern "C" size_t gtp_lora_state_bytes(const gtp_lora* q) {
   if (lora::check(q) != GTP_OK) return 0;
   if (q->requests * q->rows == 0) return 256;
   const lora::Sizes z = lora::sizes_of(q);
-  return (size_t)(z.plan_bytes + z.scale_bytes + z.low_bytes);
+  return (size_t)(z.plan_bytes + z.scale_bytes + z.low_bytes + (z.T == 16 ? 0 : z.units_bytes));
 }
 
 extern "C" int gtp_lora_add(const gtp_lora* q, void* state, size_t state_bytes, void* stream) {
