@@ -128,9 +128,57 @@ struct Tile {
   int e, first, rows, at;
 };
 
+__device__ __forceinline__ int class_at(const void* ids, int ids64, int i, int E) {
+  const int64_t id = ids64 ? reinterpret_cast<const int64_t*>(ids)[i]
+                           : (int64_t)reinterpret_cast<const int32_t*>(ids)[i];
+  return id >= 0 && id < E ? (int)id : id == -1 ? E : E + 1;
+}
+
+// The plan of at most 64 requests, by every wave that needs it, in registers:
+// lane i's request, and lane p's request in their order.
+struct Few {
+  int c;             // the request's class
+  int before, same;  // requests of lower classes, of this one
+  int place;         // among those of its class
+  int tiles_before, tiles;
+  int order;
+
+  __device__ __forceinline__ void make(const void* ids, int ids64, int B, int S, int T, int E,
+                                       int lane) {
+    c = lane < B ? class_at(ids, ids64, lane, E) : E + 2;
+    before = same = place = 0;
+    for (int j = 0; j < B; ++j) {
+      const int o = __builtin_amdgcn_readlane(c, j);
+      before += o < c;
+      same += o == c;
+      place += o == c && j < lane;
+    }
+    tiles = lane < B ? (same * S + T - 1) / T : 0;
+    tiles_before = 0;
+    for (uint64_t m = __ballot(lane < B && place == 0); m; m &= m - 1) {
+      const int j = __ffsll((unsigned long long)m) - 1;
+      tiles_before += __builtin_amdgcn_readlane(c, j) < c ? __builtin_amdgcn_readlane(tiles, j) : 0;
+    }
+    // (lanes without a request keep out of the requests' places)
+    order = __builtin_amdgcn_ds_permute(4 * (lane < B ? before + place : lane), lane);
+  }
+  // tile t
+  __device__ __forceinline__ Tile find(int t, int S, int T, int lane) const {
+    const uint64_t m = __ballot(tiles > 0 && place == 0 && t >= tiles_before &&
+                                t < tiles_before + tiles);
+    if (m == 0) return Tile{-1, 0, 0, 0};
+    const int j = __ffsll((unsigned long long)m) - 1;
+    return Tile{__builtin_amdgcn_readlane(c, j), __builtin_amdgcn_readlane(before, j),
+                __builtin_amdgcn_readlane(same, j) * S,
+                (t - __builtin_amdgcn_readlane(tiles_before, j)) * T};
+  }
+};
+
 struct Plan {
   const int32_t* mem;  // null: all rows in order, adapter 0
   int32_t N, B, S, T, E, tiles;
+  const void* ids;     // 64 requests at most, not yet in mem: Few's
+  int32_t ids64;
 
   __host__ __device__ static int64_t head(int64_t E) { return (2 * (E + 3) + 3) / 4 * 4; }
   __host__ __device__ static int64_t words(int64_t B, int64_t E, int64_t tiles) {
@@ -153,6 +201,65 @@ struct Plan {
   }
 };
 
+// A tile and its rows, for a whole wave.
+struct Where {
+  Tile tile;
+  int order;  // of Few
+
+  __device__ __forceinline__ Where(const Plan& p, int t, int lane) {
+    if (p.ids) {
+      Few f;
+      f.make(p.ids, p.ids64, p.B, p.S, p.T, p.E, lane);
+      tile = f.find(t, p.S, p.T, lane);
+      order = f.order;
+    } else {
+      tile = p.tile(t);
+      order = 0;
+    }
+  }
+  // row n of the tile, -1 behind the class's last (all lanes call)
+  __device__ __forceinline__ int row(const Plan& p, int n) const {
+    if (!p.ids) return p.row(tile, n);
+    const int j = tile.at + n, b = j / p.S;
+    const int request = __shfl(order, (tile.first + b) & (kWave - 1), kWave);
+    return j < tile.rows ? request * p.S + (j - b * p.S) : -1;
+  }
+};
+
+// Few's plan put into memory, by one wave.
+__device__ __forceinline__ void keep(const Plan& p, int32_t* mem, int lane) {
+  Few f;
+  f.make(p.ids, p.ids64, p.B, p.S, p.T, p.E, lane);
+  for (int c0 = 0; c0 <= p.E + 2; c0 += kWave) {
+    const int c = c0 + lane;
+    int start = 0, rows = 0;
+    for (uint64_t m = __ballot(lane < p.B && f.place == 0); m; m &= m - 1) {
+      const int j = __ffsll((unsigned long long)m) - 1;
+      const int o = __builtin_amdgcn_readlane(f.c, j);
+      start += o < c ? __builtin_amdgcn_readlane(f.tiles, j) * p.T : 0;
+      rows = o == c ? __builtin_amdgcn_readlane(f.same, j) * p.S : rows;
+    }
+    if (c <= p.E + 2) {
+      mem[c] = start;
+      mem[p.E + 3 + c] = rows;
+    }
+  }
+  int4* tile = reinterpret_cast<int4*>(mem + Plan::head(p.E));
+  for (int t0 = 0; t0 < p.tiles; t0 += kWave) {
+    const int t = t0 + lane;
+    int4 v = make_int4(-1, 0, 0, 0);
+    for (uint64_t m = __ballot(lane < p.B && f.place == 0); m; m &= m - 1) {
+      const int j = __ffsll((unsigned long long)m) - 1;
+      const int from = __builtin_amdgcn_readlane(f.tiles_before, j);
+      if (t >= from && t < from + __builtin_amdgcn_readlane(f.tiles, j))
+        v = make_int4(__builtin_amdgcn_readlane(f.c, j), __builtin_amdgcn_readlane(f.before, j),
+                      __builtin_amdgcn_readlane(f.same, j) * p.S, (t - from) * p.T);
+    }
+    if (t < p.tiles) tile[t] = v;
+  }
+  if (lane < p.B) mem[Plan::head(p.E) + 4 * p.tiles + lane] = f.order;
+}
+
 constexpr int kPlanBlock = 1024;
 constexpr int kPlanWaves = kPlanBlock / kWave;
 
@@ -169,11 +276,7 @@ __global__ __launch_bounds__(kPlanBlock) void plan_kernel(const void* ids, int i
   __syncthreads();
   const int share = (B + kPlanWaves - 1) / kPlanWaves;
   const int from = w * share < B ? w * share : B, to = from + share < B ? from + share : B;
-  auto class_of = [&](int i) {
-    const int64_t id = ids64 ? reinterpret_cast<const int64_t*>(ids)[i]
-                             : (int64_t)reinterpret_cast<const int32_t*>(ids)[i];
-    return id >= 0 && id < E ? (int)id : id == -1 ? E : E + 1;
-  };
+  auto class_of = [&](int i) { return class_at(ids, ids64, i, E); };
   // lanes with this lane's class
   auto alike = [&](int c, bool in) {
     uint64_t m = __ballot(in);
@@ -265,22 +368,33 @@ __global__ __launch_bounds__(kPlanBlock) void plan_kernel(const void* ids, int i
 template <typename T, int RB, int NB>
 __global__ __launch_bounds__(kBlock) void shrink_kernel(Plan plan, const T* x, int64_t ld,
                                                         const T* W, int C, int r, int splits,
-                                                        float* low, Scale scale) {
+                                                        float* low, Scale scale,
+                                                        int32_t* kept) {
   constexpr int E = Mat<T>::kE;
-  constexpr int kSteps = RB == 1 ? 4 : NB == 4 ? 1 : 2;  // loaded at a time
+  constexpr int kSteps = RB == 1 ? 4 : 1;  // loaded at a time
   constexpr int kRows = RB * 16;
   __shared__ int rows[kRows];
-  __shared__ float sum[kRows][NB * 16 + 1];
+  constexpr int kHalf = NB == 4 && RB == 4 ? 2 : RB;  // blocks of rows summed at a time
+  __shared__ float sum[kWaves][kHalf * 16][NB * 16 + 1];
   const int lane = threadIdx.x & (kWave - 1), w = threadIdx.x / kWave;
   const int split = blockIdx.x % splits, tile = blockIdx.x / splits;
   const int r0 = blockIdx.y * kRankStep;
-  if (scale.to && blockIdx.x == 0 && blockIdx.y == 0)
-    for (int i = threadIdx.x; i < plan.E; i += kBlock)
-      scale.to[i] = scale.each ? scale.each[i] : scale.all;
-  const Tile at = plan.tile(tile);
-  const int e = at.e;
+  if (blockIdx.x == plan.tiles * splits) {
+    // a workgroup more: what the others' kernels find in memory
+    if (blockIdx.y == 0) {
+      for (int i = threadIdx.x; i < plan.E; i += kBlock)
+        scale.to[i] = scale.each ? scale.each[i] : scale.all;
+      if (kept && w == 0) keep(plan, kept, lane);
+    }
+    return;
+  }
+  const Where at(plan, tile, lane);
+  const int e = at.tile.e;
   if (e < 0 || e >= plan.E) return;
-  if (threadIdx.x < kRows) rows[threadIdx.x] = plan.row(at, threadIdx.x);
+  if (w == 0) {
+    const int row = at.row(plan, lane);
+    if (lane < kRows) rows[lane] = row;
+  }
   __syncthreads();
   const int m = lane & 15, q = lane >> 4;
   const T* px[RB];
@@ -296,17 +410,20 @@ __global__ __launch_bounds__(kBlock) void shrink_kernel(Plan plan, const T* x, i
     const int i = r0 + b * 16 + m < r ? r0 + b * 16 + m : r - 1;
     pw[b] = W + ((int64_t)e * r + i) * C + q * 2 * E;
   }
-  const int steps = (C + 8 * E - 1) / (8 * E), shares = splits * kWaves;
-  const int share = (steps + shares - 1) / shares;
-  const int from = (split * kWaves + w) * share;
+  // the workgroup's steps, its waves by turns
+  const int steps = (C + 8 * E - 1) / (8 * E);
+  const int share = (steps + splits * kWaves * kSteps - 1) / (splits * kWaves * kSteps) * kWaves * kSteps;
+  const int from = split * share;
   const int to = from + share < steps ? from + share : steps;
   f32x4 acc[RB][NB];
 #pragma unroll
   for (int a = 0; a < RB; ++a)
 #pragma unroll
     for (int b = 0; b < NB; ++b) acc[a][b] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-  for (int s0 = from; s0 < to; s0 += kSteps) {
-    u32x4 vx[kSteps][RB][2], vw[kSteps][NB][2];
+  // tiles of 64 rows load a turn ahead; those of 16 mostly have one turn
+  constexpr bool kAhead = RB > 1;
+  u32x4 nx[kSteps][RB][2], nw[kSteps][NB][2];
+  auto load = [&](int s0) {
 #pragma unroll
     for (int i = 0; i < kSteps; ++i) {
       const int64_t c = (int64_t)(s0 + i) * 8 * E;
@@ -314,11 +431,26 @@ __global__ __launch_bounds__(kBlock) void shrink_kernel(Plan plan, const T* x, i
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
 #pragma unroll
-        for (int b = 0; b < RB; ++b) vx[i][b][h] = load16(px[b] + c + h * E, left - h * E);
+        for (int b = 0; b < RB; ++b) nx[i][b][h] = load16(px[b] + c + h * E, left - h * E);
 #pragma unroll
-        for (int b = 0; b < NB; ++b) vw[i][b][h] = load16(pw[b] + c + h * E, left - h * E);
+        for (int b = 0; b < NB; ++b) nw[i][b][h] = load16(pw[b] + c + h * E, left - h * E);
       }
     }
+  };
+  if (kAhead) load(from + w * kSteps);
+  for (int s0 = from + w * kSteps; s0 < to; s0 += kWaves * kSteps) {
+    if (!kAhead) load(s0);
+    u32x4 vx[kSteps][RB][2], vw[kSteps][NB][2];
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+#pragma unroll
+        for (int b = 0; b < RB; ++b) vx[i][b][h] = nx[i][b][h];
+#pragma unroll
+        for (int b = 0; b < NB; ++b) vw[i][b][h] = nw[i][b][h];
+      }
+    if (kAhead && s0 + kWaves * kSteps < to) load(s0 + kWaves * kSteps);
 #pragma unroll
     for (int i = 0; i < kSteps; ++i)
 #pragma unroll
@@ -330,24 +462,26 @@ __global__ __launch_bounds__(kBlock) void shrink_kernel(Plan plan, const T* x, i
             acc[a][b] = Mat<T>::mma(vx[i][a][h], vw[i][b][h], acc[a][b]);
   }
   // acc[a][b][i]: row 16 a + 4 q + i, rank 16 b + m; the waves' sums in order
-  for (int k = 0; k < kWaves; ++k) {
-    if (w == k) {
-#pragma unroll
-      for (int a = 0; a < RB; ++a)
-#pragma unroll
-        for (int b = 0; b < NB; ++b)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            float& s = sum[a * 16 + 4 * q + i][b * 16 + m];
-            s = k == 0 ? acc[a][b][i] : s + acc[a][b][i];
-          }
-    }
-    __syncthreads();
-  }
   const int n = r - r0 < kRankStep ? r - r0 : kRankStep;
   float* to_low = low + ((int64_t)split * plan.tiles + tile) * kRows * r + r0;
-  for (int i = threadIdx.x; i < kRows * n; i += kBlock)
-    to_low[(int64_t)(i / n) * r + i % n] = sum[i / n][i % n];
+#pragma unroll
+  for (int a0 = 0; a0 < RB; a0 += kHalf) {
+#pragma unroll
+    for (int a = 0; a < kHalf; ++a)
+#pragma unroll
+      for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sum[w][a * 16 + 4 * q + i][b * 16 + m] = acc[a0 + a][b][i];
+    __syncthreads();
+    for (int i = threadIdx.x; i < kHalf * 16 * n; i += kBlock) {
+      const int y = i / n, x = i - y * n;
+      float v = sum[0][y][x];
+#pragma unroll
+      for (int k = 1; k < kWaves; ++k) v += sum[k][y][x];
+      to_low[(int64_t)(a0 * 16 + y) * r + x] = v;
+    }
+    if (a0 + kHalf < RB) __syncthreads();
+  }
 }
 
 // kE low-rank values of a position from k on: the splits' sums, scaled, as the
@@ -440,27 +574,27 @@ __global__ __launch_bounds__(kBlock) void low_kernel(Plan plan, const float* low
 // the product's M: lane (m, q) of a strip of 64 bytes holds 16 consecutive
 // bytes of row m.  Contraction units of 16 bytes: the hi part's, then the lo
 // part's (which meet the same W).  A strip's base is loaded a strip ahead.
-// ready: low_kernel's units; null: summed here, which is less than a launch for
-// tiles of 16 rows.
+// ready: low_kernel's units; null: summed here, which takes less than a launch
+// where a thread has few of them.  turned: as low_kernel's (with ready null).
 template <typename T, int RB>
 __global__ __launch_bounds__(kBlock) void expand_kernel(Plan plan, const float* low, int splits,
                                                         const float* scales, const T* W, int C,
                                                         int r, const T* base, int64_t ld_base,
                                                         T* out, int strips, int blocks,
-                                                        const u32x4* ready) {
+                                                        const u32x4* ready, T* turned) {
   constexpr int E = Mat<T>::kE, P = Mat<T>::kParts, MB = E / 4;
   constexpr int kRows = RB * 16;
   constexpr int kStrip = 4 * E;  // columns
   extern __shared__ u32x4 frags[];  // [kRows][units + 1]
   const int lane = threadIdx.x & (kWave - 1), w = threadIdx.x / kWave;
   const int block = blockIdx.x % blocks, tile = blockIdx.x / blocks;
-  const Tile at = plan.tile(tile);
-  const int e = at.e;
+  const Where at(plan, tile, lane);
+  const int e = at.tile.e;
   if (e < 0) return;
   const int m = lane & 15, q = lane >> 4;
   int row[RB];
 #pragma unroll
-  for (int b = 0; b < RB; ++b) row[b] = plan.row(at, b * 16 + m);
+  for (int b = 0; b < RB; ++b) row[b] = at.row(plan, b * 16 + m);
   const int first = block * strips * kWaves + w, last = (block + 1) * strips * kWaves;
   u32x4 vb[RB];
   auto load_base = [&](int strip) {
@@ -489,6 +623,17 @@ __global__ __launch_bounds__(kBlock) void expand_kernel(Plan plan, const float* 
       }
     }
     __syncthreads();
+    if (turned && block == 0 && w == 0) {
+      // (a lane for a row)
+      const int64_t n_all = (int64_t)plan.tiles * kRows;
+      const bool in = at.row(plan, lane) >= 0;
+      if (lane < kRows)
+        for (int k = 0; k < P * r; ++k) {
+          const int part = k >= r ? 1 : 0, i = k - part * r;
+          const T* f = reinterpret_cast<const T*>(&frags[lane * ld + part * chunks + i / E]);
+          turned[k * n_all + tile * kRows + lane] = in ? f[i % E] : T{};
+        }
+    }
   }
   for (int strip = first; strip < last; strip += kWaves) {
     const int64_t c0 = (int64_t)strip * kStrip;
@@ -558,33 +703,42 @@ __global__ __launch_bounds__(kBlock) void expand_kernel(Plan plan, const float* 
 
 // --------------------------------------------- small pieces of the backward
 
-// A matrix [E][a][b] turned to [E][b][a].
+// A matrix [E][a][b] turned to [E][b][a], in tiles of 32 x 32.
 struct Turn {
   const void* in;
   void* out;
-  int64_t n;  // values, 0: none
+  int64_t tiles;  // of all, 0: none
   int a, b;
 };
 
 // Ahead of the backward's products, in one launch: a turned, b turned, and
 // low_kernel's `turned` of the forward's sums.
 template <typename T>
-__global__ __launch_bounds__(kBlock) void turn_kernel(Turn one, Turn two, int64_t blocks_one,
-                                                      int64_t blocks_two, Plan plan,
+__global__ __launch_bounds__(kBlock) void turn_kernel(Turn one, Turn two, Plan plan,
                                                       const float* low, int splits,
                                                       const float* scales, int r, T* to) {
+  __shared__ T tile[32][33];
   const int64_t block = blockIdx.x;
-  if (block >= blocks_one + blocks_two) {
+  if (block >= one.tiles + two.tiles) {
     low_operands<T>(plan, low, splits, scales, r,
-                    (block - blocks_one - blocks_two) * kBlock + threadIdx.x, nullptr, to);
+                    (block - one.tiles - two.tiles) * kBlock + threadIdx.x, nullptr, to);
     return;
   }
-  const Turn t = block < blocks_one ? one : two;
-  const int64_t i = (block < blocks_one ? block : block - blocks_one) * kBlock + threadIdx.x;
-  if (i >= t.n) return;
-  const int64_t each = (int64_t)t.a * t.b, e = i / each;
-  const int k = (int)(i - e * each), y = k / t.a, x = k - y * t.a;
-  reinterpret_cast<T*>(t.out)[i] = reinterpret_cast<const T*>(t.in)[e * each + (int64_t)x * t.b + y];
+  const Turn t = block < one.tiles ? one : two;
+  const int64_t i = block < one.tiles ? block : block - one.tiles;
+  const int across = (t.b + 31) / 32, each = (t.a + 31) / 32 * across;
+  const int64_t e = i / each, at = e * t.a * t.b;
+  const int k = (int)(i - e * each), x0 = k / across * 32, y0 = k % across * 32;
+  const T* in = reinterpret_cast<const T*>(t.in) + at;
+  T* out = reinterpret_cast<T*>(t.out) + at;
+  const int lane = threadIdx.x & 31, row = threadIdx.x / 32;
+#pragma unroll
+  for (int j = row; j < 32; j += kBlock / 32)
+    if (x0 + j < t.a && y0 + lane < t.b) tile[j][lane] = in[(int64_t)(x0 + j) * t.b + y0 + lane];
+  __syncthreads();
+#pragma unroll
+  for (int j = row; j < 32; j += kBlock / 32)
+    if (y0 + j < t.b && x0 + lane < t.a) out[(int64_t)(y0 + j) * t.a + x0 + lane] = tile[lane][j];
 }
 
 // ------------------------------------------------------------------ outer
@@ -610,7 +764,7 @@ __global__ __launch_bounds__(kBlock) void outer_kernel(Plan plan, Side one, Side
                                                        int chunk) {
   constexpr int E = Mat<T>::kE, P = Mat<T>::kParts;
   constexpr int kCols = 16 * E;
-  __shared__ float sum[16][kCols + 4];
+  __shared__ float sum[kWaves][16][kCols + 4];
   __shared__ int rows[kMaxChunk];
   const int lane = threadIdx.x & (kWave - 1), w = threadIdx.x / kWave;
   const int all = one.blocks + two.blocks;
@@ -696,23 +850,18 @@ __global__ __launch_bounds__(kBlock) void outer_kernel(Plan plan, Side one, Side
     float* part = s.part + (int64_t)(i + e) * r * s.C;
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
-      for (int wave = 0; wave < kWaves; ++wave) {
-        if (w == wave) {
 #pragma unroll
-          for (int j = 0; j < E; ++j)
+      for (int j = 0; j < E; ++j)
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              float& t = sum[m][E * (4 * q + k) + j];
-              t = wave == 0 ? acc[j][b][k] : t + acc[j][b][k];
-            }
-        }
-        __syncthreads();
-      }
+        for (int k = 0; k < 4; ++k) sum[w][m][E * (4 * q + k) + j] = acc[j][b][k];
+      __syncthreads();
       for (int t = threadIdx.x; t < 16 * kCols; t += kBlock) {
         const int x = s.turned ? t % 16 : t / kCols, z = s.turned ? t / 16 : t % kCols;
         const int k = r0 + b * 16 + x, c = c0 + z;
-        if (k < r && c < s.C)
-          part[s.turned ? (int64_t)c * r + k : (int64_t)k * s.C + c] = sum[x][z];
+        float v = sum[0][x][z];
+#pragma unroll
+        for (int wave = 1; wave < kWaves; ++wave) v += sum[wave][x][z];
+        if (k < r && c < s.C) part[s.turned ? (int64_t)c * r + k : (int64_t)k * s.C + c] = v;
       }
       __syncthreads();
     }
@@ -755,10 +904,14 @@ struct Sizes {
 
 int64_t round_up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
 
-// Workgroups for the chip, of at least 4 steps of 128 bytes for each wave.
-int32_t splits_of(int64_t tiles, int64_t C, int64_t size) {
+// Workgroups for the chip, of at least one turn of their waves (shrink_kernel's
+// kSteps steps of 128 bytes each).
+int32_t splits_of(int64_t tiles, int64_t C, int64_t size, int T) {
+  const int64_t turn = kWaves * (T == 16 ? 4 : 1);
   const int64_t steps = (C * size + 127) / 128;
-  int64_t s = (512 + tiles - 1) / tiles, most = (steps + 4 * kWaves - 1) / (4 * kWaves);
+  int64_t s = (512 + tiles - 1) / tiles, most = (steps + turn - 1) / turn;
+  // (every split is a sum more for each low-rank value)
+  if (T != 16 && most > 8) most = 8;
   if (s > most) s = most;
   return (int32_t)(s < 1 ? 1 : s);
 }
@@ -770,12 +923,12 @@ Sizes sizes_of(const gtp_lora* q) {
   z.T = N <= 1024 || q->rank > 128 ? 16 : 64;
   int64_t runs = q->adapters + 2 < q->requests ? q->adapters + 2 : q->requests;
   z.tiles = (int32_t)((N + z.T - 1) / z.T + (q->ids ? runs : 0));
-  z.splits_x = splits_of(z.tiles, q->in, size);
-  z.splits_g = splits_of(z.tiles, q->out, size);
+  z.splits_x = splits_of(z.tiles, q->in, size, z.T);
+  z.splits_g = splits_of(z.tiles, q->out, size, z.T);
   z.plan_bytes = q->ids ? round_up(Plan::words(q->requests, q->adapters, z.tiles) * 4, 256) : 0;
   z.scale_bytes = round_up((int64_t)q->adapters * 4, 256);
   z.low_bytes = round_up((int64_t)z.splits_x * z.tiles * z.T * q->rank * 4, 256);
-  // low_kernel's operands; tiles of 16 rows do without
+  // low_kernel's operands
   const int64_t E = 16 / size, units = (size == 4 ? 1 : 2) * ((q->rank + E - 1) / E);
   z.units_bytes = (int64_t)z.tiles * z.T * units * 16;
   return z;
@@ -799,8 +952,11 @@ int check(const gtp_lora* q) {
 
 bool aligned(const void* p, uintptr_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; }
 
-Plan plan_of(const gtp_lora* q, const Sizes& z, const void* state) {
+// few: the plan is not yet in the state, and need not be
+Plan plan_of(const gtp_lora* q, const Sizes& z, const void* state, bool few) {
   Plan p;
+  p.ids = few ? q->ids : nullptr;
+  p.ids64 = q->ids_int64;
   p.mem = q->ids ? reinterpret_cast<const int32_t*>(state) : nullptr;
   p.B = (int32_t)q->requests;
   p.S = (int32_t)q->rows;
@@ -813,28 +969,28 @@ Plan plan_of(const gtp_lora* q, const Sizes& z, const void* state) {
 
 template <typename T, int RB>
 void shrink(const Plan& p, const T* x, int64_t ld, const T* W, int64_t C, int r, int splits,
-            float* low, Scale scale, hipStream_t s) {
-  const dim3 grid((uint32_t)((int64_t)p.tiles * splits), (uint32_t)((r + kRankStep - 1) / kRankStep));
+            float* low, Scale scale, int32_t* kept, hipStream_t s) {
+  const dim3 grid((uint32_t)((int64_t)p.tiles * splits + (scale.to ? 1 : 0)), (uint32_t)((r + kRankStep - 1) / kRankStep));
   if (r <= 16)
     hipLaunchKernelGGL((shrink_kernel<T, RB, 1>), grid, dim3(kBlock), 0, s, p, x, ld, W, (int)C, r,
-                       splits, low, scale);
+                       splits, low, scale, kept);
   else if (r <= 32)
     hipLaunchKernelGGL((shrink_kernel<T, RB, 2>), grid, dim3(kBlock), 0, s, p, x, ld, W, (int)C, r,
-                       splits, low, scale);
+                       splits, low, scale, kept);
   else
     hipLaunchKernelGGL((shrink_kernel<T, RB, 4>), grid, dim3(kBlock), 0, s, p, x, ld, W, (int)C, r,
-                       splits, low, scale);
+                       splits, low, scale, kept);
 }
 template <typename T>
 void shrink(const Plan& p, const T* x, int64_t ld, const T* W, int64_t C, int r, int splits,
-            float* low, Scale scale, hipStream_t s) {
-  if (p.T == 16) shrink<T, 1>(p, x, ld, W, C, r, splits, low, scale, s);
-  else shrink<T, 4>(p, x, ld, W, C, r, splits, low, scale, s);
+            float* low, Scale scale, int32_t* kept, hipStream_t s) {
+  if (p.T == 16) shrink<T, 1>(p, x, ld, W, C, r, splits, low, scale, kept, s);
+  else shrink<T, 4>(p, x, ld, W, C, r, splits, low, scale, kept, s);
 }
 
 template <typename T>
 void expand(const Plan& p, const float* low, int splits, const float* scales, const T* W, int64_t C, int r,
-            const T* base, int64_t ld_base, T* out, const u32x4* ready, hipStream_t s) {
+            const T* base, int64_t ld_base, T* out, const u32x4* ready, T* turned, hipStream_t s) {
   constexpr int E = Mat<T>::kE, P = Mat<T>::kParts;
   const int64_t wave_strips = (C + 4 * E * kWaves - 1) / (4 * E * kWaves);
   // strips per wave: fewer where there are few tiles
@@ -846,10 +1002,12 @@ void expand(const Plan& p, const float* low, int splits, const float* scales, co
   const dim3 grid((uint32_t)(p.tiles * blocks));
   if (p.T == 16)
     hipLaunchKernelGGL((expand_kernel<T, 1>), grid, dim3(kBlock), lds, s, p, low, splits, scales, W,
-                       (int)C, r, base, ld_base, out, strips, (int)blocks, ready);
+                       (int)C, r, base, ld_base, out, strips, (int)blocks, ready,
+                       turned);
   else
     hipLaunchKernelGGL((expand_kernel<T, 4>), grid, dim3(kBlock), lds, s, p, low, splits, scales, W,
-                       (int)C, r, base, ld_base, out, strips, (int)blocks, ready);
+                       (int)C, r, base, ld_base, out, strips, (int)blocks, ready,
+                       turned);
 }
 
 template <typename T>
@@ -860,25 +1018,36 @@ void low_launch(const Plan& p, const float* low, int splits, const float* scales
                      p, low, splits, scales, r, units, turned);
 }
 
+// Whether the operands are made in a launch of their own: where expand_kernel
+// would have more than 256 of them to sum for a tile (a thread each).
+bool low_apart(const gtp_lora* q, const Sizes& z) {
+  const int E = q->dtype == GTP_DTYPE_F32 ? 4 : 8;
+  return z.T * ((q->rank + E - 1) / E) > kBlock;
+}
+
 template <typename T>
 void forward(const gtp_lora* q, const Sizes& z, char* state, hipStream_t s) {
-  const Plan p = plan_of(q, z, state);
-  if (q->ids)
+  const bool few = q->ids && q->requests <= kWave;
+  const Plan p = plan_of(q, z, state, few);
+  int32_t* mem = reinterpret_cast<int32_t*>(state);
+  if (q->ids && !few)
     hipLaunchKernelGGL(plan_kernel, dim3(1), dim3(kPlanBlock),
                        (size_t)(q->adapters + 2) * kPlanWaves * 4, s, q->ids, (int)q->ids_int64,
-                       p.B, p.S, p.T, p.E, p.tiles, reinterpret_cast<int32_t*>(state));
+                       p.B, p.S, p.T, p.E, p.tiles, mem);
   float* scales = reinterpret_cast<float*>(state + z.plan_bytes);
   float* low = reinterpret_cast<float*>(state + z.plan_bytes + z.scale_bytes);
   shrink<T>(p, reinterpret_cast<const T*>(q->x), q->x_stride, reinterpret_cast<const T*>(q->a),
-            q->in, q->rank, z.splits_x, low, Scale{q->scales, q->scale, scales}, s);
+            q->in, q->rank, z.splits_x, low, Scale{q->scales, q->scale, scales},
+            few ? mem : nullptr, s);
   u32x4* units = nullptr;
-  if (z.T != 16) {
+  if (low_apart(q, z)) {
     units = reinterpret_cast<u32x4*>(state + z.plan_bytes + z.scale_bytes + z.low_bytes);
-    low_launch<T>(p, low, z.splits_x, scales, q->rank, units, static_cast<T*>(nullptr), s);
+    low_launch<T>(plan_of(q, z, state, false), low, z.splits_x, scales, q->rank, units,
+                  static_cast<T*>(nullptr), s);
   }
   expand<T>(p, low, z.splits_x, scales, reinterpret_cast<const T*>(q->b), q->out, q->rank,
-            reinterpret_cast<const T*>(q->base), q->base_stride, reinterpret_cast<T*>(q->y),
-            units, s);
+            reinterpret_cast<const T*>(q->base), q->base_stride, reinterpret_cast<T*>(q->y), units,
+            static_cast<T*>(nullptr), s);
 }
 
 // The backward's workspace.
@@ -905,7 +1074,7 @@ Work work_of(const gtp_lora* q, const Sizes& z) {
   k.low_tv = take(n * r * size * parts);
   // chunks of rows: workgroups for the chip, of at least 128 rows
   const int64_t cols = 16 * (16 / size), blocks = (q->in + cols - 1) / cols + (q->out + cols - 1) / cols;
-  int64_t chunks = (1024 + blocks - 1) / blocks;
+  int64_t chunks = (768 + blocks - 1) / blocks;
   if (chunks > (n + 127) / 128) chunks = (n + 127) / 128;
   if (chunks < 1) chunks = 1;
   k.chunk = (int)round_up((n + chunks - 1) / chunks, 64);
@@ -921,7 +1090,7 @@ template <typename T>
 void backward(const gtp_lora* q, const gtp_lora_grads* d, const Sizes& z, const char* state,
               char* ws, hipStream_t s) {
   constexpr int E = Mat<T>::kE;
-  const Plan p = plan_of(q, z, state);
+  const Plan p = plan_of(q, z, state, false);
   const Work k = work_of(q, z);
   const float* scales = reinterpret_cast<const float*>(state + z.plan_bytes);
   const float* low_u = reinterpret_cast<const float*>(state + z.plan_bytes + z.scale_bytes);
@@ -935,21 +1104,24 @@ void backward(const gtp_lora* q, const gtp_lora_grads* d, const Sizes& z, const 
   const int64_t nl = (int64_t)p.tiles * p.T * ((r + E - 1) / E);
   const bool need_v = d->grad_x || d->grad_a;
   auto blocks_of = [](int64_t n) { return (n + kBlock - 1) / kBlock; };
-  const Turn ta{q->a, turned_a, d->grad_x ? na : 0, r, (int)q->in};
-  const Turn tb{q->b, turned_b, need_v ? nb : 0, (int)q->out, r};
-  const int64_t turns = blocks_of(ta.n) + blocks_of(tb.n) + (d->grad_b ? blocks_of(nl) : 0);
+  auto tiles_of = [](int64_t a, int64_t b) { return (a + 31) / 32 * ((b + 31) / 32); };
+  const Turn ta{q->a, turned_a, d->grad_x ? p.E * tiles_of(r, q->in) : 0, r, (int)q->in};
+  const Turn tb{q->b, turned_b, need_v ? p.E * tiles_of(q->out, r) : 0, (int)q->out, r};
+  const int64_t turns = ta.tiles + tb.tiles + (d->grad_b ? blocks_of(nl) : 0);
   if (turns > 0)
-    hipLaunchKernelGGL(turn_kernel<T>, dim3((uint32_t)turns), dim3(kBlock), 0, s, ta, tb,
-                       blocks_of(ta.n), blocks_of(tb.n), p, low_u, z.splits_x, scales, r, tu);
+    hipLaunchKernelGGL(turn_kernel<T>, dim3((uint32_t)turns), dim3(kBlock), 0, s, ta, tb, p, low_u,
+                       z.splits_x, scales, r, tu);
   if (need_v) {
     u32x4* units = reinterpret_cast<u32x4*>(ws + k.units_v);
     shrink<T>(p, reinterpret_cast<const T*>(d->grad), d->grad_stride, turned_b, q->out, r,
-              z.splits_g, low_v, Scale{nullptr, 0.0f, nullptr}, s);
-    low_launch<T>(p, low_v, z.splits_g, scales, r, d->grad_x ? units : nullptr,
-                  d->grad_a ? tv : static_cast<T*>(nullptr), s);
+              z.splits_g, low_v, Scale{nullptr, 0.0f, nullptr}, nullptr, s);
+    const bool apart = low_apart(q, z) || !d->grad_x;
+    T* to = d->grad_a ? tv : nullptr;
+    if (apart)
+      low_launch<T>(p, low_v, z.splits_g, scales, r, d->grad_x ? units : nullptr, to, s);
     if (d->grad_x)
       expand<T>(p, low_v, z.splits_g, scales, turned_a, q->in, r, static_cast<const T*>(nullptr), 0,
-                reinterpret_cast<T*>(d->grad_x), units, s);
+                reinterpret_cast<T*>(d->grad_x), apart ? units : nullptr, apart ? nullptr : to, s);
   }
   if (!d->grad_a && !d->grad_b) return;
   float* part_a = reinterpret_cast<float*>(ws + k.part_a);
@@ -982,7 +1154,8 @@ extern "C" size_t gtp_lora_state_bytes(const gtp_lora* q) {
   if (lora::check(q) != GTP_OK) return 0;
   if (q->requests * q->rows == 0) return 256;
   const lora::Sizes z = lora::sizes_of(q);
-  return (size_t)(z.plan_bytes + z.scale_bytes + z.low_bytes + (z.T == 16 ? 0 : z.units_bytes));
+  return (size_t)(z.plan_bytes + z.scale_bytes + z.low_bytes +
+                  (lora::low_apart(q, z) ? z.units_bytes : 0));
 }
 
 extern "C" int gtp_lora_add(const gtp_lora* q, void* state, size_t state_bytes, void* stream) {
