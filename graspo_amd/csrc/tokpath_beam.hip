@@ -562,24 +562,28 @@ __global__ __launch_bounds__(kMergeBlock) void beam_merge_kernel(Rows r, Out out
   __shared__ uint64_t list_o[kList], list_at[kList];
   __shared__ Candidates c;
   __shared__ int entries;
+  __shared__ int row_any[kMaxK], row_status[kMaxK];
   const int g = blockIdx.x, tid = threadIdx.x, lane = tid & (kWave - 1);
   const int wid = __builtin_amdgcn_readfirstlane(tid / kWave);
   const int per_row = r.S * r.slots, total = r.K * per_row;
   const int64_t base = (int64_t)g * r.K;
-  const bool done = r.done && r.done[g];
-  // all that is read from memory, ahead of what it is for
+  // All that is read from memory first, whether it will be needed or not: each
+  // wait for it is a microsecond.  (What beams that are not live left in the
+  // workspace is any bits, and not looked at.)
   uint64_t key[kHold];
 #pragma unroll
   for (int j = 0; j < kHold; ++j) {
     key[j] = 0;
     const int i = j * kMergeBlock + tid;
-    if (j * kMergeBlock < total && i < total && !done) key[j] = r.keys[base * per_row + i];
+    if (j * kMergeBlock < total && i < total) key[j] = r.keys[base * per_row + i];
   }
   Before old;
   if constexpr (kStep) {
     if (wid == 0) old = before(st, g, r.K, lane);
   }
+  const bool done = r.done && r.done[g];
   if (tid == 0) entries = 0;
+  if (tid < kMaxK) row_any[tid] = 0;
   if (tid < r.n) {
     c.score[tid] = kNegInf;
     c.beam[tid] = -1;
@@ -587,27 +591,23 @@ __global__ __launch_bounds__(kMergeBlock) void beam_merge_kernel(Rows r, Out out
   }
   // each row's log-sum-exp (S <= 64: a slice per lane)
   for (int k = wid; k < r.K; k += kMergeWaves) {
+    const float score = r.score[base + k];
+    float2 v = r.sums[(base + k) * r.S + (lane < r.S ? lane : 0)];
     int status = GTP_ROW_OK;
     double off = -__builtin_huge_val();
-    const float score = r.score[base + k];
     float top = kNegInf;
-    if (live(r, (int)base + k)) {
-      float2 v = make_float2(kNegInf, 0.0f);
-      bool any = false;  // (a slice's first key is there where any is)
-      if (lane < r.S) {
-        v = r.sums[(base + k) * r.S + lane];
-        any = r.keys[((base + k) * r.S + lane) * r.slots] != 0;
-      }
-      top = wave_max(v.x);
+    if (!done && __builtin_fabsf(score) < kPosInf) {
+      if (lane >= r.S) v = make_float2(kNegInf, 0.0f);
+      top = uniform_max(v.x);
       // (a NaN stays, also where nothing finite was seen)
       double s = (double)v.y;
       if (v.x > kNegInf && v.x < kPosInf)
         s *= exp2(((double)v.x - (double)top) * (double)kLog2e - (double)residual(v.x));
 #pragma unroll
       for (int o = kWave / 2; o > 0; o >>= 1) s += lane_xor_double(s, o);
-      // (the exponents are multiples of the fp32 log2(e))
+      // (the exponents are multiples of the fp32 log2(e); without a sum there
+      // is no candidate either)
       if (s != s) status = GTP_ROW_NONFINITE;
-      else if (!__ballot(any)) status = GTP_ROW_EMPTY;
       else off = (double)score - log2(s) / (double)kLog2e;
     } else if (!done && !(score == kNegInf)) {
       status = GTP_ROW_NONFINITE;
@@ -615,7 +615,7 @@ __global__ __launch_bounds__(kMergeBlock) void beam_merge_kernel(Rows r, Out out
     if (lane == 0) {
       offset[k] = off;
       row_top[k] = top;
-      if (out.status) out.status[base + k] = status;
+      row_status[k] = status;
     }
   }
   __syncthreads();
@@ -629,6 +629,7 @@ __global__ __launch_bounds__(kMergeBlock) void beam_merge_kernel(Rows r, Out out
       if (j * kMergeBlock >= total) continue;
       const int k = (j * kMergeBlock + tid) / per_row;
       if (key[j] == 0 || offset[k] == -__builtin_huge_val()) continue;
+      row_any[k] = 1;
       o[j] = ord64(((double)rank_key_y(key[j]) - (double)row_top[k]) + offset[k]);
       const uint32_t h = (uint32_t)(o[j] >> 32);
       top = h > top ? h : top;
@@ -723,6 +724,13 @@ __global__ __launch_bounds__(kMergeBlock) void beam_merge_kernel(Rows r, Out out
       }
     }
     __syncthreads();
+  }
+  if (out.status && tid < r.K) {
+    // (a live row without a candidate; done groups have none)
+    const bool live_row = !done && __builtin_fabsf(r.score[base + tid]) < kPosInf;
+    out.status[base + tid] = live_row && row_status[tid] == GTP_ROW_OK && !row_any[tid]
+                                 ? GTP_ROW_EMPTY
+                                 : row_status[tid];
   }
   if (out.score && tid < r.n) {
     out.score[(int64_t)g * r.n + tid] = c.score[tid];

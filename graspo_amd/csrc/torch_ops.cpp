@@ -1324,6 +1324,28 @@ at::Tensor clip_grad_norm_(at::TensorList tensors, double max_norm, double norm_
 
 // ------------------------------------------------- beam search
 
+// Contiguous tensors cut from one allocation (an allocation each takes 0.8 us
+// of a call of 10), which lives as long as any of them.
+struct Cut {
+  at::Tensor all;
+  int64_t at = 0;
+  Cut(int64_t bytes, const at::Tensor& like)
+      : all(at::empty({bytes}, like.options().dtype(at::kByte))) {}
+  static int64_t room(int64_t bytes) { return (bytes + 255) / 256 * 256; }
+  at::Tensor take(at::IntArrayRef sizes, at::ScalarType dt) {
+    at::Tensor t = at::detail::make_tensor<c10::TensorImpl>(
+        c10::Storage(all.storage()), all.key_set(), at::scalarTypeToTypeMeta(dt));
+    const int64_t es = (int64_t)c10::elementSize(dt);
+    int64_t bytes = es;
+    for (int64_t n : sizes) bytes *= n;
+    t.unsafeGetTensorImpl()->set_storage_offset(at / es);
+    t.unsafeGetTensorImpl()->set_sizes_contiguous(sizes);
+    at += room(bytes);
+    TORCH_INTERNAL_ASSERT(at <= all.numel());
+    return t;
+  }
+};
+
 // logits [G * K, V] or [G, K, V], any strides but of the columns; scores [G, K]
 gtp_beam_rows beam_rows(const at::Tensor& logits, const at::Tensor& scores, int64_t candidates,
                         const c10::optional<at::Tensor>& allow_mask,
@@ -1402,6 +1424,7 @@ using BeamOut = std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::T
 struct BeamStep {
   gtp_beam_state s{};
   BeamOut out;
+  at::Tensor status;
   BeamStep(const at::Tensor& scores, const at::Tensor& pool_scores, const at::Tensor& pool_rows,
            const at::Tensor& pool_steps, const at::Tensor& done, int64_t eos, int64_t pad,
            double length, int64_t step, bool early, const c10::optional<at::Tensor>& tokens_out,
@@ -1424,8 +1447,10 @@ struct BeamStep {
     TORCH_CHECK(step >= 0 && step < INT32_MAX, "graspo_tokpath.", what, ": step must be >= 0");
     TORCH_CHECK(length > 0.0 && length <= std::numeric_limits<double>::max(), "graspo_tokpath.",
                 what, ": (step + 1)^length_penalty must be positive and finite");
+    const int64_t n = G * K;
+    Cut cut(Cut::room(8 * n) + 6 * Cut::room(4 * n) + Cut::room(G), scores);
     auto to = [&](const c10::optional<at::Tensor>& t, at::ScalarType dt, const char* name) {
-      if (!t.has_value()) return at::empty({G * K}, scores.options().dtype(dt));
+      if (!t.has_value()) return cut.take({n}, dt);
       check_same_device(scores, *t, name);
       TORCH_CHECK(t->scalar_type() == dt && t->dim() == 1 && t->size(0) == G * K &&
                       t->is_contiguous(),
@@ -1435,11 +1460,12 @@ struct BeamStep {
     };
     at::Tensor tokens = to(tokens_out, at::kLong, "tokens_out");
     at::Tensor parents = to(parents_out, at::kInt, "parents_out");
-    at::Tensor n_scores = at::empty({G, K}, scores.options());
-    at::Tensor n_pool = at::empty({G, K}, scores.options());
-    at::Tensor n_rows = at::empty({G, K}, pool_rows.options());
-    at::Tensor n_steps = at::empty({G, K}, pool_rows.options());
-    at::Tensor n_done = at::empty({G}, done.options());
+    at::Tensor n_scores = cut.take({G, K}, at::kFloat);
+    at::Tensor n_pool = cut.take({G, K}, at::kFloat);
+    at::Tensor n_rows = cut.take({G, K}, at::kInt);
+    at::Tensor n_steps = cut.take({G, K}, at::kInt);
+    at::Tensor n_done = cut.take({G}, at::kBool);
+    status = cut.take({n}, at::kInt);
     s.scores = scores.data_ptr<float>();
     s.pool_scores = pool_scores.data_ptr<float>();
     s.pool_rows = pool_rows.data_ptr<int32_t>();
@@ -1512,13 +1538,12 @@ beam_step(const at::Tensor& logits, const at::Tensor& scores, const at::Tensor& 
   const c10::DeviceGuard guard(logits.device());
   BeamStep b(scores, pool_scores, pool_rows, pool_steps, done, eos, pad, length, step, early,
              tokens_out, parents_out, "beam_step");
-  at::Tensor status = at::empty({r.groups * r.beams}, pool_rows.options());
   at::Tensor ws = at::empty({(int64_t)gtp_beam_workspace_bytes(&r)}, scores.options().dtype(at::kByte));
-  check_rc(gtp_beam_step(&r, &b.s, status.data_ptr<int32_t>(), ws.data_ptr(), (size_t)ws.numel(),
+  check_rc(gtp_beam_step(&r, &b.s, b.status.data_ptr<int32_t>(), ws.data_ptr(), (size_t)ws.numel(),
                          reinterpret_cast<void*>(stream)),
            "gtp_beam_step");
   b.written(tokens_out, parents_out);
-  return std::tuple_cat(b.out, std::make_tuple(status));
+  return std::tuple_cat(b.out, std::make_tuple(b.status));
 }
 
 std::tuple<at::Tensor, at::Tensor, at::Tensor> beam_finish(
@@ -1607,6 +1632,22 @@ gtp_state_shape state_shape(const at::Tensor& t, bool in_memory_order, const cha
   return s;
 }
 
+// of every state; neighbours alike are looked at once
+std::vector<gtp_state_shape> state_shapes(at::TensorList states, bool in_memory_order,
+                                          const char* what) {
+  std::vector<gtp_state_shape> shapes;
+  shapes.reserve(states.size());
+  for (size_t i = 0; i < states.size(); ++i) {
+    const at::Tensor& t = states[i];
+    if (i > 0 && t.sizes() == states[i - 1].sizes() && t.strides() == states[i - 1].strides() &&
+        t.element_size() == states[i - 1].element_size())
+      shapes.push_back(shapes.back());
+    else
+      shapes.push_back(state_shape(t, in_memory_order, what));
+  }
+  return shapes;
+}
+
 bool same_shape(const gtp_state_shape& a, const gtp_state_shape& b) {
   bool same = a.run_bytes == b.run_bytes && a.row_stride == b.row_stride;
   for (int d = 0; d < GTP_STATE_DIMS; ++d)
@@ -1639,10 +1680,19 @@ void reorder_states_(at::TensorList states, const at::Tensor& parents, int64_t b
     TORCH_CHECK(!t.requires_grad() || !at::GradMode::is_enabled(),
                 "graspo_tokpath.reorder_states_: a state that requires a gradient");
   const c10::DeviceGuard guard(states[0].device());
-  std::vector<gtp_state_shape> shapes;
-  shapes.reserve(states.size());
-  for (const at::Tensor& t : states) shapes.push_back(state_shape(t, true, "reorder_states_"));
-  check_apart(states, "reorder_states_");
+  const std::vector<gtp_state_shape> shapes = state_shapes(states, true, "reorder_states_");
+  // (one behind the other, as a cache's layers mostly are, they are apart)
+  uintptr_t reach = 0;
+  for (const at::Tensor& t : states) {
+    const uintptr_t from = reinterpret_cast<uintptr_t>(t.data_ptr());
+    if (from < reach) {
+      check_apart(states, "reorder_states_");
+      break;
+    }
+    int64_t last = 0;
+    for (int64_t d = 0; d < t.dim(); ++d) last += (t.size(d) - 1) * t.stride(d);
+    if (t.numel() > 0) reach = from + (last + 1) * t.element_size();
+  }
   void* st = reinterpret_cast<void*>(stream);
   at::Tensor bad;
   check = check && R > 0 && !gtp_stream_capturing(st);
@@ -1675,14 +1725,18 @@ std::vector<at::Tensor> expand_states(at::TensorList states, int64_t beams, int6
     TORCH_CHECK(!t.requires_grad() || !at::GradMode::is_enabled(),
                 "graspo_tokpath.expand_states: a state that requires a gradient");
   const c10::DeviceGuard guard(states[0].device());
-  std::vector<gtp_state_shape> shapes;
-  shapes.reserve(states.size());
+  const std::vector<gtp_state_shape> shapes = state_shapes(states, false, "expand_states");
   outs.reserve(states.size());
+  // small ones from one allocation: they live and go together
+  int64_t bytes = 0;
+  for (const at::Tensor& t : states) bytes += Cut::room(t.numel() * beams * t.element_size());
+  const bool small = bytes <= (32 << 20);
+  Cut cut(small ? bytes : 0, states[0]);
+  std::vector<int64_t> size;
   for (const at::Tensor& t : states) {
-    auto size = t.sizes().vec();
+    size.assign(t.sizes().begin(), t.sizes().end());
     size[0] *= beams;
-    outs.push_back(at::empty(size, t.options()));
-    shapes.push_back(state_shape(t, false, "expand_states"));
+    outs.push_back(small ? cut.take(size, t.scalar_type()) : at::empty(size, t.options()));
   }
   std::vector<const void*> from;
   std::vector<void*> to;
@@ -1706,6 +1760,10 @@ std::vector<at::Tensor> expand_states(at::TensorList states, int64_t beams, int6
 
 // [..., n] as rows with unit column stride: their distance, or a copy
 at::Tensor as_rows(const at::Tensor& t, int64_t n, int64_t& stride) {
+  if (t.is_contiguous()) {
+    stride = n;
+    return t;
+  }
   at::Tensor rows = t.reshape({-1, n});
   if ((n > 1 && rows.stride(1) != 1) || (rows.size(0) > 1 && rows.stride(0) < 0)) rows = rows.contiguous();
   stride = rows.size(0) > 1 ? rows.stride(0) : n;
@@ -1887,17 +1945,66 @@ struct LoraAdd : torch::autograd::Function<LoraAdd> {
   }
 };
 
+// What lora_add refuses whatever the device (here, and not in Python, where it
+// takes 3 us of a call of 12).
+void check_lora(const at::Tensor& base, const at::Tensor& x, const at::Tensor& a,
+                const at::Tensor& b, const c10::optional<at::Tensor>& ids,
+                const c10::optional<at::Tensor>& scales) {
+  const at::ScalarType dt = x.scalar_type();
+  TORCH_CHECK_VALUE(dt == at::kFloat || dt == at::kBFloat16 || dt == at::kHalf,
+                    "lora_add: x must be float32, bfloat16 or float16, got ", dt);
+  const std::pair<const char*, const at::Tensor*> others[] = {
+      {"base", &base}, {"lora_a", &a}, {"lora_b", &b}};
+  for (const auto& o : others)
+    TORCH_CHECK_VALUE(o.second->scalar_type() == dt, "lora_add: ", o.first, " must be ", dt,
+                      " as x, got ", o.second->scalar_type());
+  TORCH_CHECK_VALUE((a.dim() == 2 || a.dim() == 3) && b.dim() == a.dim(),
+                    "lora_add: expected adapters [E, r, K] and [E, N, r] (or [r, K] and [N, r]), "
+                    "got ", a.sizes(), " and ", b.sizes());
+  const int64_t E = a.dim() == 3 ? a.size(0) : 1, r = a.size(-2), K = a.size(-1), N = b.size(-2);
+  TORCH_CHECK_VALUE(x.dim() >= 1 && x.size(-1) == K && b.size(-1) == r &&
+                        (a.dim() == 2 || b.size(0) == E) && base.dim() == x.dim() &&
+                        base.size(-1) == N &&
+                        base.sizes().slice(0, x.dim() - 1) == x.sizes().slice(0, x.dim() - 1) &&
+                        E > 0 && r > 0 && K > 0 && N > 0,
+                    "lora_add: base ", base.sizes(), ", x ", x.sizes(), " and adapters ", a.sizes(),
+                    ", ", b.sizes(), " do not go together");
+  TORCH_CHECK_VALUE(r <= 256 && E <= 1024, "lora_add: at most 1024 adapters of rank 256, got ", E,
+                    " of ", r);
+  if (ids.has_value()) {
+    TORCH_CHECK_VALUE(ids->scalar_type() == at::kInt || ids->scalar_type() == at::kLong,
+                      "lora_add: adapter_ids must be int32 or int64, got ", ids->scalar_type());
+    TORCH_CHECK_VALUE(ids->dim() >= 1 && ids->dim() < x.dim() &&
+                          ids->sizes() == x.sizes().slice(0, ids->dim()),
+                      "lora_add: adapter_ids ", ids->sizes(),
+                      " are not of the leading dimensions of x ", x.sizes());
+  } else {
+    TORCH_CHECK_VALUE(E == 1, "lora_add: ", E, " adapters and no adapter_ids");
+  }
+  if (scales.has_value()) {
+    TORCH_CHECK_VALUE(scales->scalar_type() == at::kFloat && scales->dim() == 1 &&
+                          scales->size(0) == E,
+                      "lora_add: scaling must be a number or float32 [", E, "], got ",
+                      scales->scalar_type(), " ", scales->sizes());
+    TORCH_CHECK_VALUE(!scales->requires_grad(), "lora_add: the scaling has no gradient");
+  }
+  TORCH_CHECK(x.is_cuda(), "graspo_tokpath: tensors must be on a GPU (got ", x.device(),
+              "); there is no CPU path");
+}
+
 at::Tensor lora_add(const at::Tensor& base, const at::Tensor& x, const at::Tensor& a,
-                    const at::Tensor& b, const c10::optional<at::Tensor>& ids,
-                    const c10::optional<at::Tensor>& scales, double scale, bool check,
+                    const at::Tensor& b, const c10::optional<at::Tensor>& ids_,
+                    const c10::optional<at::Tensor>& scales_, double scale, bool check,
                     int64_t stream) {
+  check_lora(base, x, a, b, ids_, scales_);
+  c10::optional<at::Tensor> ids, scales;
+  if (ids_.has_value()) ids = ids_->dim() == 1 ? ids_->contiguous() : ids_->reshape({-1}).contiguous();
+  if (scales_.has_value()) scales = scales_->contiguous();
   bool grad = false;
   for (const at::Tensor* t : {&base, &x, &a, &b}) {
     check_no_tangent(*t, "lora_add");
     grad = grad || t->requires_grad();
   }
-  TORCH_CHECK(!scales.has_value() || !scales->requires_grad(),
-              "lora_add: the scaling has no gradient");
   grad = grad && at::GradMode::is_enabled();
   if (grad)
     for (const at::Tensor* t : {&base, &x, &a, &b}) check_leaf(*t, "lora_add", stream);

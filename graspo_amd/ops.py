@@ -604,6 +604,6 @@ def lora_add(base: torch.Tensor, x: torch.Tensor, lora_a: torch.Tensor, lora_b: 
              scale: float = 1.0, check: bool = True) -> torch.Tensor:
     """:func:`lora_add_state`'s output, differentiable (once, backwards) in
     base, x and the adapters (any strides; [r, K] and [N, r] of a single
-    one)."""
-    return load().lora_add(base, x, lora_a, lora_b, adapter_ids, scales, float(scale), check,
-                           _stream(x))
+    one; ``adapter_ids`` of x's leading dimensions).  Checks its arguments."""
+    stream = torch._C._cuda_getCurrentRawStream(x.device.index) if x.is_cuda else 0
+    return load().lora_add(base, x, lora_a, lora_b, adapter_ids, scales, scale, check, stream)

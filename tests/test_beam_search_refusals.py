@@ -82,7 +82,7 @@ def test_beam_buffers():
     L = lib()
     r = rows()
     need = L.gtp_beam_workspace_bytes(r)
-    assert need == 2 * 4 * 1 * 9 * 8  # one slice per row: 8 keys and a sum
+    assert need == 2 * 4 * 1 * 13 * 8  # one slice per row: 12 keys and a sum
     assert L.gtp_beam_workspace_bytes(rows(beams=40)) == 0
     for bad in ((None, 4096, 4096), (4096, None, 4096), (4096, 4096, None)):
         assert L.gtp_beam_candidates(r, *bad, None, 4096, need, None) == INVALID
