@@ -42,6 +42,7 @@ struct Rows {
   const uint8_t* done;   // [G] or null
   int64_t V, group_stride, beam_stride, mask_stride;  // mask_stride in bytes
   int32_t G, K, n, S, slots;
+  uint32_t row_magic;    // i / (S slots) = i row_magic >> 32, i < kMaxKeys
   int64_t L;             // a slice's logits, a multiple of 512
   uint64_t* keys;        // [G K S slots], 0: none
   float2* sums;          // [G K S]: maximum, sum
@@ -627,7 +628,7 @@ __global__ __launch_bounds__(kMergeBlock) void beam_merge_kernel(Rows r, Out out
     for (int j = 0; j < kHold; ++j) {
       o[j] = 0;
       if (j * kMergeBlock >= total) continue;
-      const int k = (j * kMergeBlock + tid) / per_row;
+      const int k = (int)__umulhi(j * kMergeBlock + tid, r.row_magic);
       if (key[j] == 0 || offset[k] == -__builtin_huge_val()) continue;
       row_any[k] = 1;
       o[j] = ord64(((double)rank_key_y(key[j]) - (double)row_top[k]) + offset[k]);
@@ -635,7 +636,8 @@ __global__ __launch_bounds__(kMergeBlock) void beam_merge_kernel(Rows r, Out out
       top = h > top ? h : top;
     }
     auto place = [&](int j) {
-      return (uint64_t)((j * kMergeBlock + tid) / per_row) << 32 | (uint32_t)rank_key_id(key[j]);
+      return (uint64_t)__umulhi(j * kMergeBlock + tid, r.row_magic) << 32 |
+             (uint32_t)rank_key_id(key[j]);
     };
     best[wid][lane] = top;
     __syncthreads();
@@ -656,16 +658,23 @@ __global__ __launch_bounds__(kMergeBlock) void beam_merge_kernel(Rows r, Out out
     const uint64_t at_least = m > 0 ? (uint64_t)m << 32 : 1ull;
     int mine = 0;
 #pragma unroll
-    for (int j = 0; j < kHold; ++j) mine += o[j] >= at_least ? 1 : 0;
-    int to = mine > 0 ? atomicAdd(&entries, mine) : 0;
+    for (int j = 0; j < kHold; ++j)
+      if (j * kMergeBlock < total) mine += __popcll(__ballot(o[j] >= at_least));
+    int to = 0;
+    if (mine > 0) {
+      if (lane == 0) to = atomicAdd(&entries, mine);
+      to = __builtin_amdgcn_readfirstlane(to);
+    }
 #pragma unroll
     for (int j = 0; j < kHold; ++j) {
-      if (o[j] < at_least) continue;
-      if (to < kList) {
-        list_o[to] = o[j];
-        list_at[to] = place(j);
+      if (mine == 0 || j * kMergeBlock >= total) continue;
+      const uint64_t k = __ballot(o[j] >= at_least);
+      const int e = to + lanes_below(k);
+      if (o[j] >= at_least && e < kList) {
+        list_o[e] = o[j];
+        list_at[e] = place(j);
       }
-      ++to;
+      to += __popcll(k);
     }
     __syncthreads();
     auto better = [](uint64_t o, uint64_t at, uint64_t than_o, uint64_t than_at) {
@@ -678,12 +687,19 @@ __global__ __launch_bounds__(kMergeBlock) void beam_merge_kernel(Rows r, Out out
     };
     const int n = entries;
     if (n <= kList) {
-      for (int e = tid; e < n; e += kMergeBlock) {
-        const uint64_t mo = list_o[e], ma = list_at[e];
+      // 16 lanes for an entry
+      const int part = tid & 15;
+      for (int e0 = 0; e0 < n; e0 += kMergeBlock / 16) {
+        const int e = e0 + tid / 16;
+        const bool in = e < n;
+        const uint64_t mo = in ? list_o[e] : 0, ma = in ? list_at[e] : 0;
         int rank = 0;
-#pragma unroll 4
-        for (int i = 0; i < n; ++i) rank += better(list_o[i], list_at[i], mo, ma) ? 1 : 0;
-        if (rank < r.n) take(rank, mo, ma);
+        for (int i = part; i < n; i += 16) rank += better(list_o[i], list_at[i], mo, ma) ? 1 : 0;
+        rank += (int)lane_xor<1>((uint32_t)rank);
+        rank += (int)lane_xor<2>((uint32_t)rank);
+        rank += (int)lane_xor<4>((uint32_t)rank);
+        rank += (int)lane_xor<8>((uint32_t)rank);
+        if (in && part == 0 && rank < r.n) take(rank, mo, ma);
       }
     } else {
       // (many equal scores) one after the other: the best behind the last
@@ -907,6 +923,8 @@ int run(const gtp_beam_rows* q, const Out& out, const gtp_beam_state* step, void
   r.S = (int32_t)S;
   r.slots = (int32_t)slots_of(r.n);
   r.L = L;
+  const uint32_t per_row = (uint32_t)(r.S * r.slots);  // (below 2^13: exact)
+  r.row_magic = per_row > 1 ? (uint32_t)(((1ull << 32) + per_row - 1) / per_row) : 0;
   const int64_t slices = (int64_t)r.G * r.K * S;
   r.keys = reinterpret_cast<uint64_t*>(workspace);
   r.sums = reinterpret_cast<float2*>(r.keys + slices * r.slots);
