@@ -146,13 +146,18 @@ struct Few {
   __device__ __forceinline__ void make(const void* ids, int ids64, int B, int S, int T, int E,
                                        int lane) {
     c = lane < B ? class_at(ids, ids64, lane, E) : E + 2;
-    before = same = place = 0;
-    for (int j = 0; j < B; ++j) {
-      const int o = __builtin_amdgcn_readlane(c, j);
-      before += o < c;
-      same += o == c;
-      place += o == c && j < lane;
+    // by the classes' bits, the highest first: which lanes are alike so far, and
+    // how many left them for a lower class
+    uint64_t alike = ~0ull;
+    before = 0;
+    for (int b = 31 - __builtin_clz(E + 2); b >= 0; --b) {
+      const bool bit = (c >> b) & 1;
+      const uint64_t on = __ballot(bit);
+      before += bit ? __popcll(alike & ~on) : 0;
+      alike &= bit ? on : ~on;
     }
+    same = __popcll(alike);
+    place = __popcll(alike & ((1ull << lane) - 1));
     tiles = lane < B ? (same * S + T - 1) / T : 0;
     tiles_before = 0;
     for (uint64_t m = __ballot(lane < B && place == 0); m; m &= m - 1) {
@@ -484,13 +489,12 @@ __global__ __launch_bounds__(kBlock) void shrink_kernel(Plan plan, const T* x, i
   }
 }
 
-// kE low-rank values of a position from k on: the splits' sums, scaled, as the
-// parts' operands; zeros past the rank.
+// kE low-rank values of a position from k on, the splits' sums; zeros past the
+// rank.
 template <typename T>
-__device__ __forceinline__ void low_units(const float* low, int64_t split_stride, int splits,
-                                          int r, int k, float scale, u32x4 (&unit)[Mat<T>::kParts]) {
-  constexpr int E = Mat<T>::kE, P = Mat<T>::kParts;
-  float v[E];
+__device__ __forceinline__ void low_sum(const float* low, int64_t split_stride, int splits, int r,
+                                        int k, float (&v)[Mat<T>::kE]) {
+  constexpr int E = Mat<T>::kE;
 #pragma unroll
   for (int j = 0; j < E; ++j) v[j] = 0.0f;
   if (k + E <= r) {
@@ -506,6 +510,12 @@ __device__ __forceinline__ void low_units(const float* low, int64_t split_stride
       for (int j = 0; j < E; ++j)
         if (k + j < r) v[j] += low[i * split_stride + k + j];
   }
+}
+// Scaled, as the parts' operands.
+template <typename T>
+__device__ __forceinline__ void low_parts(const float (&v)[Mat<T>::kE], float scale,
+                                          u32x4 (&unit)[Mat<T>::kParts]) {
+  constexpr int E = Mat<T>::kE, P = Mat<T>::kParts;
 #pragma unroll
   for (int h = 0; h < P; ++h) unit[h] = u32x4{0u, 0u, 0u, 0u};
 #pragma unroll
@@ -539,7 +549,9 @@ __device__ __forceinline__ void low_operands(const Plan& plan, const float* low,
   const bool in = t.e >= 0 && t.e < plan.E;
   u32x4 u[P];
   if (in && t.at + (int)(p % plan.T) < t.rows) {
-    low_units<T>(low + p * r, n * r, splits, r, c * E, scales[t.e], u);
+    float v[E];
+    low_sum<T>(low + p * r, n * r, splits, r, c * E, v);
+    low_parts<T>(v, scales[t.e], u);
   } else {
 #pragma unroll
     for (int h = 0; h < P; ++h) u[h] = u32x4{0u, 0u, 0u, 0u};
@@ -577,7 +589,7 @@ __global__ __launch_bounds__(kBlock) void low_kernel(Plan plan, const float* low
 // ready: low_kernel's units; null: summed here, which takes less than a launch
 // where a thread has few of them.  turned: as low_kernel's (with ready null).
 template <typename T, int RB>
-__global__ __launch_bounds__(kBlock) void expand_kernel(Plan plan, const float* low, int splits,
+__global__ __launch_bounds__(kBlock, 4) void expand_kernel(Plan plan, const float* low, int splits,
                                                         const float* scales, const T* W, int C,
                                                         int r, const T* base, int64_t ld_base,
                                                         T* out, int strips, int blocks,
@@ -588,6 +600,14 @@ __global__ __launch_bounds__(kBlock) void expand_kernel(Plan plan, const float* 
   extern __shared__ u32x4 frags[];  // [kRows][units + 1]
   const int lane = threadIdx.x & (kWave - 1), w = threadIdx.x / kWave;
   const int block = blockIdx.x % blocks, tile = blockIdx.x / blocks;
+  const int chunks = (r + E - 1) / E, units = P * chunks, ld = units + 1;
+  // a thread's low-rank values, ahead of the look at the plan (of a tile without
+  // an adapter they are any values, and not used)
+  const int n_low = threadIdx.x / chunks, c_low = threadIdx.x - n_low * chunks;
+  float v_low[E];
+  if (!ready && n_low < kRows)
+    low_sum<T>(low + ((int64_t)tile * kRows + n_low) * r, (int64_t)plan.tiles * kRows * r, splits,
+               r, c_low * E, v_low);
   const Where at(plan, tile, lane);
   const int e = at.tile.e;
   if (e < 0) return;
@@ -604,23 +624,28 @@ __global__ __launch_bounds__(kBlock) void expand_kernel(Plan plan, const float* 
       vb[b] = row[b] >= 0 ? load16(base + row[b] * ld_base + c, C - c) : u32x4{0u, 0u, 0u, 0u};
   };
   if (base) load_base(first);
-  const int chunks = (r + E - 1) / E, units = P * chunks, ld = units + 1;
+  // the weights of a strip's units u0 .. u0 + 3: M index m of block b is column
+  // E (m / 4) + 4 b + m % 4 of the strip
+  auto load_w = [&](int strip, int u0, u32x4 (&to)[MB]) {
+    const int u = u0 + q, k = u >= chunks ? u - chunks : u;
+#pragma unroll
+    for (int b = 0; b < MB; ++b) {
+      int64_t o = (int64_t)strip * kStrip + E * (m >> 2) + 4 * b + (m & 3);
+      if (o >= C) o = C - 1;
+      to[b] = load16(W + ((int64_t)e * C + o) * r + k * E, u < units ? r - k * E : 0);
+    }
+  };
   const bool adapted = e < plan.E;
   if (adapted) {
     if (ready) {
       const u32x4* from = ready + (int64_t)tile * kRows * units;
       for (int i = threadIdx.x; i < kRows * units; i += kBlock)
         frags[i / units * ld + i % units] = from[i];
-    } else {
-      const float scale = scales[e];
-      const int64_t split_stride = (int64_t)plan.tiles * kRows * r;
-      for (int i = threadIdx.x; i < kRows * chunks; i += kBlock) {
-        const int n = i / chunks, c = i - n * chunks;
-        u32x4 u[P];
-        low_units<T>(low + ((int64_t)tile * kRows + n) * r, split_stride, splits, r, c * E, scale, u);
+    } else if (n_low < kRows) {
+      u32x4 u[P];
+      low_parts<T>(v_low, scales[e], u);
 #pragma unroll
-        for (int h = 0; h < P; ++h) frags[n * ld + h * chunks + c] = u[h];
-      }
+      for (int h = 0; h < P; ++h) frags[n_low * ld + h * chunks + c_low] = u[h];
     }
     __syncthreads();
     if (turned && block == 0 && w == 0) {
@@ -651,23 +676,13 @@ __global__ __launch_bounds__(kBlock) void expand_kernel(Plan plan, const float* 
 #pragma unroll
       for (int b = 0; b < MB; ++b) acc[a][b] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     if (adapted) {
-      const T* pw[MB];
-#pragma unroll
-      for (int b = 0; b < MB; ++b) {
-        // M index m of block b is column E (m / 4) + 4 b + m % 4 of the strip
-        int64_t o = c0 + E * (m >> 2) + 4 * b + (m & 3);
-        if (o >= C) o = C - 1;
-        pw[b] = W + ((int64_t)e * C + o) * r;
-      }
       for (int u0 = 0; u0 < units; u0 += 4) {
-        const int u = u0 + q, k = u >= chunks ? u - chunks : u;
-        const bool in = u < units;
+        const int u = u0 + q;
         u32x4 vw[MB], vl[RB];
-#pragma unroll
-        for (int b = 0; b < MB; ++b) vw[b] = load16(pw[b] + k * E, in ? r - k * E : 0);
+        load_w(strip, u0, vw);
 #pragma unroll
         for (int a = 0; a < RB; ++a)
-          vl[a] = in ? frags[(a * 16 + m) * ld + u] : u32x4{0u, 0u, 0u, 0u};
+          vl[a] = u < units ? frags[(a * 16 + m) * ld + u] : u32x4{0u, 0u, 0u, 0u};
 #pragma unroll
         for (int a = 0; a < RB; ++a)
 #pragma unroll
