@@ -18,9 +18,11 @@
 // of the requests), each adapter's run padded to whole tiles, so a tile has one
 // adapter and every sum an order that the ids fix.
 //
-// u and v are fp32 sums.  As 16-bit operands they are two parts, hi + lo (16
-// bits or more of them): rounded once, u alone would cost as much as the
-// output's own rounding where base is small.
+// u and v are fp32 sums.  As 16-bit operands they are two bf16 parts, hi + lo (16
+// bits of them, over fp32's range): rounded once, u alone would cost as much as
+// the output's own rounding where base is small, and in fp16 a v below 2^-14,
+// as small b or gradients give, would lose its bits.  fp16 values meet them as
+// two bf16 parts as well, 8 bits and the other 3, which is exact.
 #include "tokpath_gemm.h"
 
 namespace gtp {
@@ -44,6 +46,8 @@ struct Mat<uint16_t> {
   __device__ static __forceinline__ f32x4 mma(u32x4 a, u32x4 b, f32x4 c) {
     return gemm::Bf16::mul(__builtin_bit_cast(s16x8, a), __builtin_bit_cast(s16x8, b), c);
   }
+  // with a low-rank operand
+  __device__ static __forceinline__ f32x4 meet(u32x4 a, u32x4 low, f32x4 c) { return mma(a, low, c); }
   __device__ static __forceinline__ float to(uint16_t v) { return gemm::Bf16::to(v); }
   __device__ static __forceinline__ uint16_t from(float v) { return gemm::Bf16::from(v); }
 };
@@ -53,6 +57,24 @@ struct Mat<_Float16> {
   static constexpr int kParts = 2;
   __device__ static __forceinline__ f32x4 mma(u32x4 a, u32x4 b, f32x4 c) {
     return gemm::F16::mul(__builtin_bit_cast(s16x8, a), __builtin_bit_cast(s16x8, b), c);
+  }
+  __device__ static __forceinline__ f32x4 meet(u32x4 a, u32x4 low, f32x4 c) {
+    u32x4 hi, lo;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      uint32_t f[2], d[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        f[h] = f2u(f16_to_f32((uint16_t)(a[k] >> (16 * h))));
+        const float top = u2f(f[h] & 0xFFFF0000u);
+        // (an infinity has no second part)
+        d[h] = top == u2f(f[h]) ? 0u : f2u(u2f(f[h]) - top);
+      }
+      hi[k] = __builtin_amdgcn_perm(f[1], f[0], 0x07060302u);
+      lo[k] = __builtin_amdgcn_perm(d[1], d[0], 0x07060302u);
+    }
+    c = Mat<uint16_t>::mma(hi, low, c);
+    return Mat<uint16_t>::mma(lo, low, c);
   }
   __device__ static __forceinline__ float to(_Float16 v) { return (float)v; }
   __device__ static __forceinline__ _Float16 from(float v) { return (_Float16)v; }
@@ -67,6 +89,7 @@ struct Mat<float> {
       c = __builtin_amdgcn_mfma_f32_16x16x4f32(u2f(a[j]), u2f(b[j]), c, 0, 0, 0);
     return c;
   }
+  __device__ static __forceinline__ f32x4 meet(u32x4 a, u32x4 low, f32x4 c) { return mma(a, low, c); }
   __device__ static __forceinline__ float to(float v) { return v; }
   __device__ static __forceinline__ float from(float v) { return v; }
 };
@@ -524,9 +547,9 @@ __device__ __forceinline__ void low_parts(const float (&v)[Mat<T>::kE], float sc
     if constexpr (E == 4) {
       unit[0][j] = f2u(x);
     } else {
-      const T hi = Mat<T>::from(x), lo = Mat<T>::from(x - Mat<T>::to(hi));
-      unit[0][j / 2] |= (uint32_t)__builtin_bit_cast(uint16_t, hi) << (16 * (j & 1));
-      unit[1][j / 2] |= (uint32_t)__builtin_bit_cast(uint16_t, lo) << (16 * (j & 1));
+      const uint16_t hi = gemm::Bf16::from(x), lo = gemm::Bf16::from(x - gemm::Bf16::to(hi));
+      unit[0][j / 2] |= (uint32_t)hi << (16 * (j & 1));
+      unit[1][j / 2] |= (uint32_t)lo << (16 * (j & 1));
     }
   }
 }
@@ -589,7 +612,7 @@ __global__ __launch_bounds__(kBlock) void low_kernel(Plan plan, const float* low
 // ready: low_kernel's units; null: summed here, which takes less than a launch
 // where a thread has few of them.  turned: as low_kernel's (with ready null).
 template <typename T, int RB>
-__global__ __launch_bounds__(kBlock, 4) void expand_kernel(Plan plan, const float* low, int splits,
+__global__ __launch_bounds__(kBlock, __is_same(T, _Float16) ? 3 : 4) void expand_kernel(Plan plan, const float* low, int splits,
                                                         const float* scales, const T* W, int C,
                                                         int r, const T* base, int64_t ld_base,
                                                         T* out, int strips, int blocks,
@@ -686,7 +709,7 @@ __global__ __launch_bounds__(kBlock, 4) void expand_kernel(Plan plan, const floa
 #pragma unroll
         for (int a = 0; a < RB; ++a)
 #pragma unroll
-          for (int b = 0; b < MB; ++b) acc[a][b] = Mat<T>::mma(vw[b], vl[a], acc[a][b]);
+          for (int b = 0; b < MB; ++b) acc[a][b] = Mat<T>::meet(vw[b], vl[a], acc[a][b]);
       }
     }
     const float bad = e > plan.E ? __builtin_nanf("") : 0.0f;
@@ -848,7 +871,7 @@ __global__ __launch_bounds__(kBlock) void outer_kernel(Plan plan, Side one, Side
 #pragma unroll
           for (int b = 0; b < NB; ++b)
 #pragma unroll
-            for (int h = 0; h < P; ++h) acc[j][b] = Mat<T>::mma(o, vl[b][h][0], acc[j][b]);
+            for (int h = 0; h < P; ++h) acc[j][b] = Mat<T>::meet(o, vl[b][h][0], acc[j][b]);
         }
       } else {
 #pragma unroll
@@ -857,7 +880,7 @@ __global__ __launch_bounds__(kBlock) void outer_kernel(Plan plan, Side one, Side
           for (int h = 0; h < 2; ++h) {
             const u32x4 o = {v[4 * h][j], v[4 * h + 1][j], v[4 * h + 2][j], v[4 * h + 3][j]};
 #pragma unroll
-            for (int b = 0; b < NB; ++b) acc[j][b] = Mat<T>::mma(o, vl[b][0][h], acc[j][b]);
+            for (int b = 0; b < NB; ++b) acc[j][b] = Mat<T>::meet(o, vl[b][0][h], acc[j][b]);
           }
       }
     }

@@ -1657,8 +1657,8 @@ bool same_shape(const gtp_state_shape& a, const gtp_state_shape& b) {
 
 void check_states(at::TensorList states, int64_t rows, const char* what) {
   for (const at::Tensor& t : states) {
-    TORCH_CHECK(t.is_cuda() && t.layout() == at::kStrided, "graspo_tokpath.", what,
-                ": states must be dense GPU tensors");
+    TORCH_CHECK(t.is_cuda() && t.layout() == at::kStrided && !t.is_conj() && !t.is_neg(),
+                "graspo_tokpath.", what, ": states must be dense GPU tensors");
     check_same_device(states[0], t, "every state");
     TORCH_CHECK(t.dim() >= 1 && (rows < 0 || t.size(0) == rows), "graspo_tokpath.", what,
                 ": a state's first dimension must count the rows (", rows, "), got ", t.sizes());

@@ -246,6 +246,30 @@ def test_values_where_the_low_part_matters():
         assert rel < 0.45 * torch.finfo(dtype).eps, rel
 
 
+def test_low_rank_values_past_fp16s_range():
+    """u above 65504 with b that brings it back, v far below 2^-14: the parts are
+    bf16's, so neither is lost."""
+    for up, down, grad in ((2.0 ** 12, 2.0 ** -14, 2.0 ** -4), (2.0 ** -8, 2.0 ** -12, 2.0 ** -6)):
+        d = make(2, 200, 256, 64, 1, 16, HF, seed=31, none=0.0)
+        d["ids"].zero_()
+        d["base"].zero_()
+        d["a"] = (d["a"].double() * up).to(HF)
+        d["b"] = (d["b"].double() * down).to(HF)
+        d["g"] = (d["g"].double() * grad).to(HF)
+        check(d, HF)
+        want = expect(d, HF)
+        u = (d["x"][0].double() @ d["a"][0].double().t()).abs().max()
+        v = (d["g"][0].double() @ d["b"][0].double()).abs().median()
+        assert u > 65504 or v < 2.0 ** -13
+        for got, (w, _), name in zip(run(d), want, ("out", "gx", "ga", "gb")):
+            # as far as the values themselves are normal numbers: one rounding of
+            # them, and 2^-16 of what is summed
+            ok = w.abs() > 2.0 ** -13
+            if ok.any():
+                rel = float((got.double().cpu() - w)[ok].norm() / w[ok].norm())
+                assert rel < 2.0 ** -11, (name, rel)
+
+
 def test_infinities_and_nan_stay_in_their_rows():
     d = make(4, 20, 64, 72, 2, 8, BF, seed=6, none=0.0)
     clean = run(d)
