@@ -896,12 +896,11 @@ void launch_slices(const Rows& r, hipStream_t s) {
 int run(const gtp_beam_rows* q, const Out& out, const gtp_beam_state* step, void* workspace,
         size_t workspace_bytes, void* stream) {
   const int rc = check_data(q);
-  if (rc != GTP_OK) return rc;
+  if (rc != GTP_OK || q->groups == 0) return rc;
   if (step) {
     const int rs = check_state(step);
     if (rs != GTP_OK) return rs;
   }
-  if (q->groups == 0) return GTP_OK;
   if (!workspace || workspace_bytes < gtp_beam_workspace_bytes(q) ||
       (reinterpret_cast<uintptr_t>(workspace) & 7u))
     return GTP_ERR_INVALID_ARGUMENT;
@@ -977,9 +976,9 @@ extern "C" int gtp_beam_advance(const float* scores, const int32_t* beams, const
   if (groups < 0 || num_beams < 1 || candidates < 1) return GTP_ERR_INVALID_ARGUMENT;
   if (num_beams > beam::kMaxK || candidates > beam::kMaxN || groups * num_beams > (1 << 24))
     return GTP_ERR_UNSUPPORTED;
+  if (groups == 0) return GTP_OK;
   const int rc = beam::check_state(state);
   if (rc != GTP_OK) return rc;
-  if (groups == 0) return GTP_OK;
   if (!scores || !beams || !tokens) return GTP_ERR_INVALID_ARGUMENT;
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   hipLaunchKernelGGL(beam::beam_advance_kernel, dim3((uint32_t)groups), dim3(kWave), 0, s,

@@ -304,8 +304,7 @@ class BeamDecodeState:
         done, status = self._done[t % 2], self._status[t % 2]
         done.copy_(got.state.done, non_blocking=True)
         status.copy_(got.status, non_blocking=True)
-        ev = torch.cuda.Event()
-        ev.record()
+        ev = torch.cuda.current_stream(self.attn.device).record_event()
         self._pending = (ev, done, status)
         return got
 

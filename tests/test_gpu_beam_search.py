@@ -208,6 +208,18 @@ def test_layouts():
                   given=one.to(DEV).unsqueeze(1).expand(G, K, V))
 
 
+def test_steps_without_a_group():
+    st = beam_start(0, 4, DEV)
+    got = beam_step(torch.zeros(0, 50, device=DEV), st, eos_token_id=1, pad_token_id=0)
+    assert got.tokens.shape == (0,) and got.state.scores.shape == (0, 4) and got.state.step == 1
+    cand = ops.beam_candidates(torch.zeros(0, 50, device=DEV), st.scores)
+    assert ops.beam_advance(cand, *st[:5], eos_token_id=1, pad_token_id=0, length=1.0,
+                            step=0).done.shape == (0,)
+    none = torch.zeros(1, 0, dtype=torch.int64, device=DEV)
+    out = beam_finish(got.state, none, none.int(), eos_token_id=1, pad_token_id=0)
+    assert out.tokens.shape == (0, 1, 1)
+
+
 def test_no_groups_and_no_live_beam():
     out = ops.beam_candidates(torch.zeros(0, 50, device=DEV), torch.zeros(0, 4, device=DEV))
     assert out.scores.shape == (0, 8)
