@@ -23,6 +23,16 @@
 // the output's own rounding where base is small, and in fp16 a v below 2^-14,
 // as small b or gradients give, would lose its bits.  fp16 values meet them as
 // two bf16 parts as well, 8 bits and the other 3, which is exact.
+//
+// Measured, bf16, 8192 rows of 4096 x 4096 of rank 16 with all gradients: shrink
+// 22 and 19 us (64 MB each), expand 35 (128 MB read and written) and 22 (64 MB
+// written), outer 31 (128 MB), the rest 10; 138 in all, where 403 MB at the
+// card's copying rate are 79.  fp32, 2000 rows of 2048 x 5632, rank 64: 170 us,
+// of which the products at fp32's matrix rate are about half.  A few rows: two
+// launches of 4-5 us.  Tried without gain: strips' weights loaded ahead (the
+// registers cost a wave per SIMD: 35 -> 41 us), 16 rows per wave with more waves
+// (48), neighbouring strips in one wave (42), 8 or 16 waves side by side, stores
+// past the caches.
 #include "tokpath_gemm.h"
 
 namespace gtp {
