@@ -860,7 +860,7 @@ int check_rows(const gtp_beam_rows* q) {
   if (q->dtype != GTP_DTYPE_F32 && q->dtype != GTP_DTYPE_BF16 && q->dtype != GTP_DTYPE_F16)
     return GTP_ERR_INVALID_ARGUMENT;
   if (q->beams > kMaxK || q->candidates > kMaxN || q->vocab > 0x7FFFFFFFll - 4096 ||
-      q->groups * q->beams > (1 << 24))
+      q->groups > (1 << 24) / q->beams)
     return GTP_ERR_UNSUPPORTED;
   return GTP_OK;
 }
@@ -982,7 +982,7 @@ extern "C" int gtp_beam_advance(const float* scores, const int32_t* beams, const
                                 int64_t groups, int32_t num_beams, int32_t candidates,
                                 const gtp_beam_state* state, void* stream) {
   if (groups < 0 || num_beams < 1 || candidates < 1) return GTP_ERR_INVALID_ARGUMENT;
-  if (num_beams > beam::kMaxK || candidates > beam::kMaxN || groups * num_beams > (1 << 24))
+  if (num_beams > beam::kMaxK || candidates > beam::kMaxN || groups > (1 << 24) / num_beams)
     return GTP_ERR_UNSUPPORTED;
   if (groups == 0) return GTP_OK;
   const int rc = beam::check_state(state);
@@ -1004,7 +1004,7 @@ extern "C" int gtp_beam_finish(const float* scores, const float* pool_scores,
   if (groups < 0 || num_beams < 1 || steps < 0 || give < 1 || give > num_beams ||
       out_stride < steps || !(length > 0.0))
     return GTP_ERR_INVALID_ARGUMENT;
-  if (num_beams > beam::kMaxK || groups * num_beams > (1 << 24)) return GTP_ERR_UNSUPPORTED;
+  if (num_beams > beam::kMaxK || groups > (1 << 24) / num_beams) return GTP_ERR_UNSUPPORTED;
   if (groups == 0) return GTP_OK;
   if (!scores || !pool_scores || !pool_rows || !pool_steps || !done || !out_scores ||
       !out_lengths || (steps > 0 && (!tokens || !parents || !out_tokens)))

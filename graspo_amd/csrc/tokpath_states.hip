@@ -184,7 +184,7 @@ int shape_of(const gtp_state_shape* q, uintptr_t addresses, Shape& s, int& bytes
 int check(const gtp_state_shape* q, int64_t count, int64_t groups, int32_t beams) {
   if (!q || count < 0 || groups < 0 || beams < 1 || q->run_bytes < 0)
     return GTP_ERR_INVALID_ARGUMENT;
-  if (beams > kMaxBeams || groups * beams > 0x7FFFFFFF) return GTP_ERR_UNSUPPORTED;
+  if (beams > kMaxBeams || groups > 0x7FFFFFFF / beams) return GTP_ERR_UNSUPPORTED;
   return GTP_OK;
 }
 

@@ -196,3 +196,20 @@ def test_no_cpu_path():
                                             False)):
         with pytest.raises(RuntimeError, match="no CPU path"):
             call()
+
+
+def test_counts_whose_rows_would_wrap():
+    """groups * beams past 64 bits, to few or to none."""
+    L = lib()
+    for groups in ((1 << 62), (1 << 62) + 2, (1 << 61) + (1 << 20)):
+        r = rows(groups=groups, done=4096)
+        assert L.gtp_beam_workspace_bytes(r) == 0
+        assert L.gtp_beam_candidates(r, 4096, 4096, 4096, None, 4096, 1 << 40, None) == UNSUPPORTED
+        assert L.gtp_beam_step(r, state(), None, 4096, 1 << 40, None) == UNSUPPORTED
+        assert L.gtp_beam_advance(4096, 4096, 4096, groups, 4, 8, state(), None) == UNSUPPORTED
+        assert L.gtp_beam_finish(*(4096,) * 7, groups, 4, 5, 1.0, 1, 0, 2, *(4096,) * 3, 5,
+                                 None) == UNSUPPORTED
+        shape = Shape(64, 64, (I64 * 4)(1, 1, 1, 1), (I64 * 4)(0, 0, 0, 0))
+        p = (VP * 1)(4096)
+        assert L.gtp_reorder_states(p, 1, shape, 4096, groups, 4, None, None) == UNSUPPORTED
+        assert L.gtp_expand_states(p, p, 1, shape, groups, 4, None) == UNSUPPORTED
