@@ -11,6 +11,10 @@ extension (``torch.ops.graspo_tokpath``).
 * :mod:`graspo_amd.embedding` / :mod:`graspo_amd.grad_clip` -- the other ends
   of a training step: the embedding lookup with its table's gradient, and the
   global gradient norm with clipping.
+* :mod:`graspo_amd.beam_search` -- a beam search's step, its finished
+  hypotheses and the models' states that follow its beams.
+* :mod:`graspo_amd.lora` -- low-rank adapters of many requests beside a shared
+  projection.
 * :mod:`graspo_amd.integration` -- installs the drop-ins into an imported
   ``graspo`` package without editing its call sites.
 
