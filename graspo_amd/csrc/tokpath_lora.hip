@@ -27,7 +27,7 @@
 // Measured, bf16, 8192 rows of 4096 x 4096 of rank 16 with all gradients: shrink
 // 22 and 19 us (64 MB each), expand 35 (128 MB read and written) and 22 (64 MB
 // written), outer 31 (128 MB), the rest 10; 138 in all, where 403 MB at the
-// card's copying rate are 79.  fp32, 2000 rows of 2048 x 5632, rank 64: 170 us,
+// card's copying rate are 79.  fp32, 2000 rows of 2048 x 5632, rank 64: 154 us,
 // of which the products at fp32's matrix rate are about half.  A few rows: two
 // launches of 4-5 us.  Tried without gain: strips' weights loaded ahead (the
 // registers cost a wave per SIMD: 35 -> 41 us), 16 rows per wave with more waves
@@ -46,6 +46,7 @@ constexpr int kBlock = kWaves * kWave;
 constexpr int kMaxAdapters = 1024;
 constexpr int kMaxRank = 256;
 constexpr int kRankStep = 64;   // of shrink and outer
+constexpr int kWideRank = 32;   // past it both hold four blocks of ranks
 
 template <typename T>
 struct Mat;
@@ -458,7 +459,7 @@ __global__ __launch_bounds__(kBlock) void shrink_kernel(Plan plan, const T* x, i
   for (int a = 0; a < RB; ++a)
 #pragma unroll
     for (int b = 0; b < NB; ++b) acc[a][b] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-  // tiles of 64 rows load a turn ahead; those of 16 mostly have one turn
+  // tiles of 32 and 64 rows load a turn ahead; those of 16 mostly have one turn
   constexpr bool kAhead = RB > 1;
   u32x4 nx[kSteps][RB][2], nw[kSteps][NB][2];
   auto load = [&](int s0) {
@@ -845,7 +846,7 @@ __global__ __launch_bounds__(kBlock) void outer_kernel(Plan plan, Side one, Side
     const int mine = p + w * share, until = mine + share < to ? mine + share : to;
     u32x4 next_v[8];
     auto load = [&](int s0) {
-      // (positions are whole tiles of 16 or 64: 8 of them are there or not)
+      // (positions are whole tiles of 16, 32 or 64: 8 of them are there or not)
       const bool in = s0 + q * 8 < until;
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
@@ -953,12 +954,15 @@ struct Sizes {
 int64_t round_up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
 
 // Workgroups for the chip, of at least one turn of their waves (shrink_kernel's
-// kSteps steps of 128 bytes each).
-int32_t splits_of(int64_t tiles, int64_t C, int64_t size, int T) {
+// kSteps steps of 128 bytes each).  Every split is a sum more for each low-rank
+// value: of tiles of many rows 8 at most, and about 256 workgroups for ranks past
+// 32, whose waves have a SIMD to themselves (fp32, 2000 rows, rank 64, all: 154 us,
+// with twice or 3/4 of them 162 and 163; bf16, 4096 rows, rank 64: 163 for 174).
+int32_t splits_of(int64_t tiles, int64_t C, int64_t size, int T, int r) {
   const int64_t turn = kWaves * (T == 16 ? 4 : 1);
   const int64_t steps = (C * size + 127) / 128;
   int64_t s = (512 + tiles - 1) / tiles, most = (steps + turn - 1) / turn;
-  // (every split is a sum more for each low-rank value)
+  if (T != 16 && r > kWideRank) s = (256 + tiles / 2) / tiles;
   if (T != 16 && most > 8) most = 8;
   if (s > most) s = most;
   return (int32_t)(s < 1 ? 1 : s);
@@ -967,12 +971,14 @@ int32_t splits_of(int64_t tiles, int64_t C, int64_t size, int T) {
 Sizes sizes_of(const gtp_lora* q) {
   Sizes z;
   const int64_t N = q->requests * q->rows, size = q->dtype == GTP_DTYPE_F32 ? 4 : 2;
-  // (and what a tile's low-rank rows take of LDS: 33 KB at a rank of 128)
-  z.T = N <= 1024 || q->rank > 128 ? 16 : 64;
+  // 64 rows of fp32 and a rank past 32 take 230 registers in shrink_kernel, 32 rows
+  // let three waves run for two (154 us against 163, as above); 16-bit
+  // types are level.  (A tile's low-rank rows take 33 KB of LDS at a rank of 128.)
+  z.T = N <= 1024 || q->rank > 128 ? 16 : size == 4 && q->rank > kWideRank ? 32 : 64;
   int64_t runs = q->adapters + 2 < q->requests ? q->adapters + 2 : q->requests;
   z.tiles = (int32_t)((N + z.T - 1) / z.T + (q->ids ? runs : 0));
-  z.splits_x = splits_of(z.tiles, q->in, size, z.T);
-  z.splits_g = splits_of(z.tiles, q->out, size, z.T);
+  z.splits_x = splits_of(z.tiles, q->in, size, z.T, q->rank);
+  z.splits_g = splits_of(z.tiles, q->out, size, z.T, q->rank);
   z.plan_bytes = q->ids ? round_up(Plan::words(q->requests, q->adapters, z.tiles) * 4, 256) : 0;
   z.scale_bytes = round_up((int64_t)q->adapters * 4, 256);
   z.low_bytes = round_up((int64_t)z.splits_x * z.tiles * z.T * q->rank * 4, 256);
@@ -1015,25 +1021,20 @@ Plan plan_of(const gtp_lora* q, const Sizes& z, const void* state, bool few) {
   return p;
 }
 
-template <typename T, int RB>
+template <typename T, int RB, int NB>
 void shrink(const Plan& p, const T* x, int64_t ld, const T* W, int64_t C, int r, int splits,
             float* low, Scale scale, int32_t* kept, hipStream_t s) {
   const dim3 grid((uint32_t)((int64_t)p.tiles * splits + (scale.to ? 1 : 0)), (uint32_t)((r + kRankStep - 1) / kRankStep));
-  if (r <= 16)
-    hipLaunchKernelGGL((shrink_kernel<T, RB, 1>), grid, dim3(kBlock), 0, s, p, x, ld, W, (int)C, r,
-                       splits, low, scale, kept);
-  else if (r <= 32)
-    hipLaunchKernelGGL((shrink_kernel<T, RB, 2>), grid, dim3(kBlock), 0, s, p, x, ld, W, (int)C, r,
-                       splits, low, scale, kept);
-  else
-    hipLaunchKernelGGL((shrink_kernel<T, RB, 4>), grid, dim3(kBlock), 0, s, p, x, ld, W, (int)C, r,
-                       splits, low, scale, kept);
+  hipLaunchKernelGGL((shrink_kernel<T, RB, NB>), grid, dim3(kBlock), 0, s, p, x, ld, W, (int)C, r,
+                     splits, low, scale, kept);
 }
 template <typename T>
 void shrink(const Plan& p, const T* x, int64_t ld, const T* W, int64_t C, int r, int splits,
             float* low, Scale scale, int32_t* kept, hipStream_t s) {
-  if (p.T == 16) shrink<T, 1>(p, x, ld, W, C, r, splits, low, scale, kept, s);
-  else shrink<T, 4>(p, x, ld, W, C, r, splits, low, scale, kept, s);
+  const auto run = [&](auto kernel) { kernel(p, x, ld, W, C, r, splits, low, scale, kept, s); };
+  constexpr int kLarge = sizeof(T) == 4 ? 2 : 4;
+  if (p.T == 16) run(r <= 16 ? shrink<T, 1, 1> : r <= kWideRank ? shrink<T, 1, 2> : shrink<T, 1, 4>);
+  else run(r <= 16 ? shrink<T, 4, 1> : r <= kWideRank ? shrink<T, 4, 2> : shrink<T, kLarge, 4>);
 }
 
 template <typename T>
@@ -1048,14 +1049,17 @@ void expand(const Plan& p, const float* low, int splits, const float* scales, co
   blocks = (wave_strips + strips - 1) / strips;
   const size_t lds = (size_t)p.T * (P * ((r + E - 1) / E) + 1) * 16;
   const dim3 grid((uint32_t)(p.tiles * blocks));
-  if (p.T == 16)
-    hipLaunchKernelGGL((expand_kernel<T, 1>), grid, dim3(kBlock), lds, s, p, low, splits, scales, W,
-                       (int)C, r, base, ld_base, out, strips, (int)blocks, ready,
-                       turned);
-  else
-    hipLaunchKernelGGL((expand_kernel<T, 4>), grid, dim3(kBlock), lds, s, p, low, splits, scales, W,
-                       (int)C, r, base, ld_base, out, strips, (int)blocks, ready,
-                       turned);
+  const auto run = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel, grid, dim3(kBlock), lds, s, p, low, splits, scales, W, (int)C, r,
+                       base, ld_base, out, strips, (int)blocks, ready, turned);
+  };
+  if (p.T == 16) {
+    run(expand_kernel<T, 1>);
+  } else if (p.T == 64) {
+    run(expand_kernel<T, 4>);
+  } else {
+    if constexpr (sizeof(T) == 4) run(expand_kernel<T, 2>);
+  }
 }
 
 template <typename T>
@@ -1120,12 +1124,15 @@ Work work_of(const gtp_lora* q, const Sizes& z) {
   k.units_v = take(z.units_bytes);
   k.low_tu = take(n * r * size * parts);
   k.low_tv = take(n * r * size * parts);
-  // chunks of rows: workgroups for the chip, of at least 128 rows
+  // chunks of rows: workgroups for the chip, of at least 128 rows; past a rank of
+  // 32 outer_kernel runs two to a CU, which 512 fill once, and its four waves have
+  // whole steps (fp32, 2000 rows of 2048 x 5632, rank 64: 37 us for 43; at lower
+  // ranks 768 are as good, fp32 with a rank of 128 is level)
   const int64_t cols = 16 * (16 / size), blocks = (q->in + cols - 1) / cols + (q->out + cols - 1) / cols;
-  int64_t chunks = (768 + blocks - 1) / blocks;
+  int64_t chunks = r > kWideRank ? 512 / blocks : (768 + blocks - 1) / blocks;
   if (chunks > (n + 127) / 128) chunks = (n + 127) / 128;
   if (chunks < 1) chunks = 1;
-  k.chunk = (int)round_up((n + chunks - 1) / chunks, 64);
+  k.chunk = (int)round_up((n + chunks - 1) / chunks, r > kWideRank ? 128 : 64);
   if (k.chunk > kMaxChunk) k.chunk = kMaxChunk;
   k.chunks = (int)((n + k.chunk - 1) / k.chunk);
   k.part_a = take((k.chunks + E) * r * q->in * 4);

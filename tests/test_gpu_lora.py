@@ -124,6 +124,16 @@ def test_rows_and_gradients(B, S, K, N, E, r, dtype):
     check(make(B, S, K, N, E, r, dtype, seed=K + r), dtype)
 
 
+@pytest.mark.parametrize("dtype", [BF, HF, F4], ids=["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("B,S,K,N,E,r", [
+    (1, 2049, 520, 1000, 1, 128), (7, 300, 1027, 515, 3, 33), (90, 20, 136, 264, 5, 48),
+    (1030, 1, 264, 136, 70, 40), (5, 411, 2048, 72, 2, 64),
+])
+def test_many_rows_of_larger_ranks(B, S, K, N, E, r, dtype):
+    print("lora", B, S, K, N, E, r, dtype, flush=True)
+    check(make(B, S, K, N, E, r, dtype, seed=K + r), dtype)
+
+
 @pytest.mark.parametrize("dtype", [BF, F4], ids=["bf16", "fp32"])
 @pytest.mark.parametrize("S", [1, 15, 64, 1024, 1025, 2049])
 def test_one_adapter_for_all(S, dtype):
