@@ -21,7 +21,7 @@
 // The rows' bytes bound the large calls, two launches and the merge's chain of
 // LDS steps the small ones.  bf16 [32 x 8, 248320]: 31 + 9 us (4.1 TB/s; without
 // any candidates 28, without exponentials either 27); [1 x 4, 151936]: 7.5 + 6.6
-// us, 14 with the host's part.  What brought the slices there, [256, 248320] and
+// us, 16 with the host's part.  What brought the slices there, [256, 248320] and
 // [64, 151936]: every value above the threshold appended by ballots 63 and 27 us;
 // the code a quarter of that size (a wave that runs for 10 us waits for its
 // instructions, too) 50 and 27; only vectors noted, the list cut to between n and

@@ -10,6 +10,7 @@ are further apart than twice that have to come in their order.
 
 from __future__ import annotations
 
+import io
 import math
 
 import pytest
@@ -465,3 +466,18 @@ def test_finish_of_references_out_of_range():
     parents = torch.full((4, 6), -5, dtype=torch.int32, device=DEV)
     out = beam_finish(st, tokens, parents, eos_token_id=1, pad_token_id=0, num_return=3)
     assert out.tokens.ge(0).all()
+
+
+def test_outputs_have_storages_of_their_own():
+    G, K, V = 3, 4, 500
+    x = torch.randn(G * K, V, device=DEV)
+    got = beam_step(x, beam_start(G, K, DEV, all_beams=True), eos_token_id=1, pad_token_id=0)
+    outs = [got.tokens, got.parents, *got.state[:5], got.status]
+    assert len({t.untyped_storage().data_ptr() for t in outs}) == len(outs)
+    for t in outs:
+        assert t.storage_offset() == 0
+        assert t.untyped_storage().nbytes() == t.numel() * t.element_size()
+    f = io.BytesIO()
+    torch.save(outs, f)
+    f.seek(0)
+    assert all(torch.equal(a, b) for a, b in zip(torch.load(f, weights_only=True), outs))

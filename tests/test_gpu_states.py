@@ -197,3 +197,12 @@ def test_nested_caches():
     assert torch.equal(got[1]["k"], b + 1) and got[1]["n"] == 4
     with pytest.raises(TypeError, match="cache"):
         map_states([object()], lambda ts: ts)
+
+
+def test_copies_have_storages_of_their_own():
+    states = [values((2, 5, 7), dt, 0).to(DEV) for dt in (torch.float32, torch.bfloat16, torch.uint8)]
+    outs = expand_states(states, 3)
+    assert len({t.untyped_storage().data_ptr() for t in outs}) == 3
+    for t in outs:
+        assert t.storage_offset() == 0
+        assert t.untyped_storage().nbytes() == t.numel() * t.element_size()
