@@ -291,6 +291,21 @@ __device__ __forceinline__ void load_group(const T* row, int64_t G, int64_t V, b
   }
 }
 
+// Workgroup of a grid that goes on in y: a launch holds fewer than 2^32 work
+// items in one dimension (2^24 workgroups of 256).  One with more was seen to
+// report no error and leave work undone.  The last row of y may hold workgroups
+// past the end, which have nothing to do.
+constexpr int64_t kGridItems = 1ll << 31;
+template <int kThreads>
+__device__ __forceinline__ int64_t flat_workgroup() {
+  return blockIdx.x + (int64_t)blockIdx.y * (kGridItems / kThreads);
+}
+template <int kThreads>
+inline dim3 flat_grid(int64_t n) {
+  constexpr int64_t x = kGridItems / kThreads;
+  return n <= x ? dim3((unsigned)n) : dim3((unsigned)x, (unsigned)((n + x - 1) / x));
+}
+
 // Events that the next launch through launch_timed records at its start and
 // end (hipExtLaunchKernelGGL takes them from the dispatch itself), set by
 // gtp_time_next_launch; per host thread, cleared by the launch that uses them.

@@ -220,16 +220,6 @@ struct TokenRows {
   }
 };
 
-// Workgroup of a grid that goes on in y: a launch holds fewer than 2^32 work
-// items in one dimension, 2^24 workgroups of 256.
-constexpr int64_t kGridX = 1 << 23;
-__device__ __forceinline__ int64_t flat_workgroup() {
-  return blockIdx.x + (int64_t)blockIdx.y * gridDim.x;
-}
-inline dim3 flat_grid(int64_t n) {
-  return n <= kGridX ? dim3((unsigned)n) : dim3((unsigned)kGridX, (unsigned)((n + kGridX - 1) / kGridX));
-}
-
 // What a row's state gives: logprob, entropy and status.
 struct TokenOut {
   float* lp;
@@ -289,7 +279,7 @@ __global__ __launch_bounds__(kLpBlock) void token_logprob_kernel(TokenRows a, To
                                                                  float* __restrict__ partial) {
   __shared__ float red[kLpBlock / kWave][kMaxChunks][3];
   // (rows in slices are few: one dimension)
-  const int64_t n = slices > 1 ? blockIdx.x / (uint32_t)slices : flat_workgroup();
+  const int64_t n = slices > 1 ? blockIdx.x / (uint32_t)slices : flat_workgroup<kLpBlock>();
   if (n >= a.rows()) return;
   const int k = slices > 1 ? (int)(blockIdx.x - n * slices) : 0;
   int64_t b, s;
@@ -526,7 +516,7 @@ __global__ __launch_bounds__(kLpBlock) void token_logprob_backward_kernel(
     TokenRows a, int64_t St, const float* __restrict__ lp, const float* __restrict__ grad_lp,
     const int64_t* __restrict__ count, T* __restrict__ grad, int64_t gbstride, int64_t grstride,
     int slices) {
-  const int64_t n = slices > 1 ? blockIdx.x / (uint32_t)slices : flat_workgroup();
+  const int64_t n = slices > 1 ? blockIdx.x / (uint32_t)slices : flat_workgroup<kLpBlock>();
   if (n >= a.rows()) return;
   int64_t b, s;
   a.at(n, b, s);
@@ -680,7 +670,7 @@ template <typename T>
 void token_logprob_launch(const TokenRows& a, const TokenOut& out, int64_t N, int slices,
                           uint32_t* ctr, hipStream_t s) {
   const Chunks ch = chunks_of<T>(a.V);
-  const dim3 grid = flat_grid(N * slices), block(kLpBlock);
+  const dim3 grid = flat_grid<kLpBlock>(N * slices), block(kLpBlock);
   float* partial = reinterpret_cast<float*>(ctr + (slices > 1 ? N : 0));
   if (out.H)
     launch_timed(token_logprob_kernel<T, true>, grid, block, s, a, out, ch, slices, ctr, partial);
@@ -838,7 +828,7 @@ extern "C" int gtp_token_logprob_backward(const gtp_token_rows* rows, int64_t po
   if (a.B == 1) positions = positions == rows->S ? a.S : positions;
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   const int slices = row_slices(rows->dtype, N, a.V);
-  const dim3 grid = flat_grid(N * slices), block(kLpBlock);
+  const dim3 grid = flat_grid<kLpBlock>(N * slices), block(kLpBlock);
   switch (rows->dtype) {
     case GTP_DTYPE_BF16:
       launch_timed(token_logprob_backward_kernel<uint16_t>, grid, block, s, a, positions, logprob,

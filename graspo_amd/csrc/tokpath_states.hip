@@ -70,14 +70,26 @@ struct Unit<2> { typedef uint16_t type; };
 template <>
 struct Unit<1> { typedef uint8_t type; };
 
-// tiles: workgroups per (tensor, group).  kMany: more than 16 beams.
+// The workgroup's tile, group and tensor, `tiles` workgroups for each (tensor, group).
+struct Place {
+  uint32_t tile, group, tensor;
+  __device__ __forceinline__ Place(uint32_t tiles, uint32_t groups) {
+    const uint32_t at = (uint32_t)flat_workgroup<kBlock>(), rest = at / tiles;
+    tile = at - rest * tiles;
+    tensor = rest / groups;
+    group = rest - tensor * groups;
+  }
+};
+
+// kMany: more than 16 beams.
 template <int kBytes, bool kMany>
 __global__ __launch_bounds__(kBlock) void reorder_kernel(List l, Shape s, const int32_t* parents,
                                                          uint32_t groups, int K, uint32_t tiles,
-                                                         int32_t* bad) {
+                                                         uint32_t count, int32_t* bad) {
   using U = typename Unit<kBytes>::type;
-  const uint32_t tile = blockIdx.x % tiles, rest = blockIdx.x / tiles;
-  const uint32_t g = rest % groups, t = rest / groups;
+  const Place place(tiles, groups);
+  const uint32_t tile = place.tile, g = place.group, t = place.tensor;
+  if (t >= count) return;
   const int64_t base = (int64_t)g * K;
   // lane k: where row k comes from
   const int lane = threadIdx.x & (kWave - 1);
@@ -143,12 +155,12 @@ __global__ __launch_bounds__(kBlock) void reorder_kernel(List l, Shape s, const 
 // The copies are contiguous: row_units units of kBytes each.
 template <int kBytes>
 __global__ __launch_bounds__(kBlock) void expand_kernel(Pairs l, Shape s, uint32_t groups, int K,
-                                                        uint32_t tiles) {
+                                                        uint32_t tiles, uint32_t count) {
   using U = typename Unit<kBytes>::type;
-  const uint32_t tile = blockIdx.x % tiles, rest = blockIdx.x / tiles;
-  const uint32_t g = rest % groups, t = rest / groups;
-  const uint32_t u = tile * kBlock + threadIdx.x;
-  if (u >= s.units) return;
+  const Place place(tiles, groups);
+  const uint32_t g = place.group, t = place.tensor;
+  const uint32_t u = place.tile * kBlock + threadIdx.x;
+  if (t >= count || u >= s.units) return;
   const U v = *reinterpret_cast<const U*>(reinterpret_cast<const char*>(l.from[t]) +
                                           (int64_t)g * s.row_stride + offset_of(s, u, kBytes));
   U* to = reinterpret_cast<U*>(l.to[t]) + (int64_t)g * K * s.units + u;
@@ -192,16 +204,16 @@ template <int kBytes>
 void reorder(const List& l, const Shape& s, const int32_t* parents, int64_t n, int64_t groups,
              int K, int32_t* bad, hipStream_t st) {
   const uint32_t tiles = (s.units + kBlock - 1) / kBlock;
-  const dim3 grid((uint32_t)(tiles * groups * n));
+  const dim3 grid = flat_grid<kBlock>(tiles * groups * n);
   if (K <= 16)
     hipLaunchKernelGGL((reorder_kernel<kBytes, false>), grid, dim3(kBlock), 0, st, l, s, parents,
-                       (uint32_t)groups, K, tiles, bad);
+                       (uint32_t)groups, K, tiles, (uint32_t)n, bad);
   else
     hipLaunchKernelGGL((reorder_kernel<kBytes, true>), grid, dim3(kBlock), 0, st, l, s, parents,
-                       (uint32_t)groups, K, tiles, bad);
+                       (uint32_t)groups, K, tiles, (uint32_t)n, bad);
 }
 
-// tensors per launch: their workgroups fit a grid
+// tensors per launch: their workgroups are counted in 31 bits
 int64_t per_launch(const Shape& s, int64_t groups, int64_t count) {
   const int64_t each = ((int64_t)s.units + kBlock - 1) / kBlock * groups;
   int64_t n = 0x7FFFFFFFll / (each > 0 ? each : 1);
@@ -275,24 +287,17 @@ extern "C" int gtp_expand_states(const void* const* tensors, void* const* outs, 
       l.from[i] = tensors[first + i];
       l.to[i] = outs[first + i];
     }
-    const dim3 grid((uint32_t)(tiles * groups * n)), block(states::kBlock);
-    const uint32_t G = (uint32_t)groups;
+    const dim3 grid = flat_grid<states::kBlock>(tiles * groups * n), block(states::kBlock);
+    const auto run = [&](auto kernel) {
+      hipLaunchKernelGGL(kernel, grid, block, 0, st, l, s, (uint32_t)groups, beams, tiles,
+                         (uint32_t)n);
+    };
     switch (bytes) {
-      case 16:
-        hipLaunchKernelGGL(states::expand_kernel<16>, grid, block, 0, st, l, s, G, beams, tiles);
-        break;
-      case 8:
-        hipLaunchKernelGGL(states::expand_kernel<8>, grid, block, 0, st, l, s, G, beams, tiles);
-        break;
-      case 4:
-        hipLaunchKernelGGL(states::expand_kernel<4>, grid, block, 0, st, l, s, G, beams, tiles);
-        break;
-      case 2:
-        hipLaunchKernelGGL(states::expand_kernel<2>, grid, block, 0, st, l, s, G, beams, tiles);
-        break;
-      default:
-        hipLaunchKernelGGL(states::expand_kernel<1>, grid, block, 0, st, l, s, G, beams, tiles);
-        break;
+      case 16: run(states::expand_kernel<16>); break;
+      case 8: run(states::expand_kernel<8>); break;
+      case 4: run(states::expand_kernel<4>); break;
+      case 2: run(states::expand_kernel<2>); break;
+      default: run(states::expand_kernel<1>); break;
     }
   }
   return hipGetLastError() == hipSuccess ? GTP_OK : GTP_ERR_LAUNCH;
