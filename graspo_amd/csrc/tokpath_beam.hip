@@ -572,7 +572,9 @@ __global__ __launch_bounds__(kMergeBlock) void beam_merge_kernel(Rows r, Out out
   __shared__ Candidates c;
   __shared__ int entries;
   __shared__ int row_any[kMaxK], row_status[kMaxK];
-  const int g = blockIdx.x, tid = threadIdx.x, lane = tid & (kWave - 1);
+  const int g = (int)flat_workgroup<kMergeBlock>();
+  if (g >= r.G) return;
+  const int tid = threadIdx.x, lane = tid & (kWave - 1);
   const int wid = __builtin_amdgcn_readfirstlane(tid / kWave);
   const int per_row = r.S * r.slots, total = r.K * per_row;
   const int64_t base = (int64_t)g * r.K;
@@ -939,10 +941,11 @@ int run(const gtp_beam_rows* q, const Out& out, const gtp_beam_state* step, void
   else if (q->dtype == GTP_DTYPE_F16) launch_slices<_Float16>(r, s);
   else launch_slices<float>(r, s);
   const State st = step ? state_of(step) : State{};
+  const dim3 grid = flat_grid<kMergeBlock>(r.G);
   if (step)
-    hipLaunchKernelGGL(beam_merge_kernel<true>, dim3(r.G), dim3(kMergeBlock), 0, s, r, out, st);
+    hipLaunchKernelGGL(beam_merge_kernel<true>, grid, dim3(kMergeBlock), 0, s, r, out, st);
   else
-    hipLaunchKernelGGL(beam_merge_kernel<false>, dim3(r.G), dim3(kMergeBlock), 0, s, r, out, st);
+    hipLaunchKernelGGL(beam_merge_kernel<false>, grid, dim3(kMergeBlock), 0, s, r, out, st);
   return hipGetLastError() == hipSuccess ? GTP_OK : GTP_ERR_LAUNCH;
 }
 
