@@ -761,16 +761,17 @@ struct Turn {
 };
 
 // Ahead of the backward's products, in one launch: a turned, b turned, and
-// low_kernel's `turned` of the forward's sums.
+// low_kernel's `turned` of the forward's sums (to null: not).
 template <typename T>
 __global__ __launch_bounds__(kBlock) void turn_kernel(Turn one, Turn two, Plan plan,
                                                       const float* low, int splits,
                                                       const float* scales, int r, T* to) {
   __shared__ T tile[32][33];
-  const int64_t block = blockIdx.x;
+  const int64_t block = flat_workgroup<kBlock>();
   if (block >= one.tiles + two.tiles) {
-    low_operands<T>(plan, low, splits, scales, r,
-                    (block - one.tiles - two.tiles) * kBlock + threadIdx.x, nullptr, to);
+    if (to)
+      low_operands<T>(plan, low, splits, scales, r,
+                      (block - one.tiles - two.tiles) * kBlock + threadIdx.x, nullptr, to);
     return;
   }
   const Turn t = block < one.tiles ? one : two;
@@ -816,11 +817,10 @@ __global__ __launch_bounds__(kBlock) void outer_kernel(Plan plan, Side one, Side
   __shared__ float sum[kWaves][16][kCols + 4];
   __shared__ int rows[kMaxChunk];
   const int lane = threadIdx.x & (kWave - 1), w = threadIdx.x / kWave;
-  const int all = one.blocks + two.blocks;
-  const int i = blockIdx.x / all, at = blockIdx.x % all;
+  const int i = blockIdx.y, at = blockIdx.x;
   const Side s = at < one.blocks ? one : two;
   const int c0 = (at < one.blocks ? at : at - one.blocks) * kCols;
-  const int r0 = blockIdx.y * kRankStep;
+  const int r0 = blockIdx.z * kRankStep;
   const int64_t n = (int64_t)plan.tiles * plan.T;
   const int m = lane & 15, q = lane >> 4;
   const T* y = reinterpret_cast<const T*>(s.y) + c0 + m * E;
@@ -927,7 +927,8 @@ struct Sum {
 };
 template <typename T>
 __global__ __launch_bounds__(kBlock) void outer_sum_kernel(Plan plan, Sum one, Sum two, int chunk) {
-  const int64_t block = blockIdx.x;
+  const int64_t block = flat_workgroup<kBlock>();
+  if (block >= one.blocks + two.blocks) return;
   const Sum s = block < one.blocks ? one : two;
   const int64_t t = (block < one.blocks ? block : block - one.blocks) * kBlock + threadIdx.x;
   if (t >= s.each * plan.E) return;
@@ -1164,8 +1165,8 @@ void backward(const gtp_lora* q, const gtp_lora_grads* d, const Sizes& z, const 
   const Turn tb{q->b, turned_b, need_v ? p.E * tiles_of(q->out, r) : 0, (int)q->out, r};
   const int64_t turns = ta.tiles + tb.tiles + (d->grad_b ? blocks_of(nl) : 0);
   if (turns > 0)
-    hipLaunchKernelGGL(turn_kernel<T>, dim3((uint32_t)turns), dim3(kBlock), 0, s, ta, tb, p, low_u,
-                       z.splits_x, scales, r, tu);
+    hipLaunchKernelGGL(turn_kernel<T>, flat_grid<kBlock>(turns), dim3(kBlock), 0, s, ta, tb, p,
+                       low_u, z.splits_x, scales, r, d->grad_b ? tu : nullptr);
   if (need_v) {
     u32x4* units = reinterpret_cast<u32x4*>(ws + k.units_v);
     shrink<T>(p, reinterpret_cast<const T*>(d->grad), d->grad_stride, turned_b, q->out, r,
@@ -1186,7 +1187,7 @@ void backward(const gtp_lora* q, const gtp_lora_grads* d, const Sizes& z, const 
                d->grad_a ? (int32_t)((q->in + cols - 1) / cols) : 0, 0};
   const Side b{d->grad, tu, part_b, d->grad_stride, (int32_t)q->out,
                d->grad_b ? (int32_t)((q->out + cols - 1) / cols) : 0, 1};
-  const dim3 grid((uint32_t)((int64_t)k.chunks * (a.blocks + b.blocks)),
+  const dim3 grid((uint32_t)(a.blocks + b.blocks), (uint32_t)k.chunks,
                   (uint32_t)((r + kRankStep - 1) / kRankStep));
   if (r <= 16)
     hipLaunchKernelGGL((outer_kernel<T, 1>), grid, dim3(kBlock), 0, s, p, a, b, r, k.chunk);
@@ -1196,8 +1197,8 @@ void backward(const gtp_lora* q, const gtp_lora_grads* d, const Sizes& z, const 
     hipLaunchKernelGGL((outer_kernel<T, 4>), grid, dim3(kBlock), 0, s, p, a, b, r, k.chunk);
   const Sum sa{part_a, d->grad_a, (int64_t)r * q->in, d->grad_a ? blocks_of(na) : 0};
   const Sum sb{part_b, d->grad_b, (int64_t)r * q->out, d->grad_b ? blocks_of(nb) : 0};
-  hipLaunchKernelGGL(outer_sum_kernel<T>, dim3((uint32_t)(sa.blocks + sb.blocks)), dim3(kBlock), 0,
-                     s, p, sa, sb, k.chunk);
+  hipLaunchKernelGGL(outer_sum_kernel<T>, flat_grid<kBlock>(sa.blocks + sb.blocks), dim3(kBlock),
+                     0, s, p, sa, sb, k.chunk);
 }
 
 }  // namespace lora
