@@ -221,35 +221,59 @@ int64_t per_launch(const Shape& s, int64_t groups, int64_t count) {
   return n < count ? n : count;
 }
 
+// What a call launches: `most` tensors at a time (0: nothing to do).  outs: null
+// where the tensors are moved in place.
+struct Call {
+  Shape s;
+  int bytes;
+  int64_t most;
+};
+int look(const void* const* tensors, const void* const* outs, bool in_place, int64_t count,
+         const gtp_state_shape* shape, int64_t groups, int32_t beams, Call& c) {
+  c.most = 0;
+  int rc = check(shape, count, groups, beams);
+  if (rc != GTP_OK) return rc;
+  if (count == 0 || groups == 0 || shape->run_bytes == 0) return GTP_OK;
+  if (!tensors || (!in_place && !outs)) return GTP_ERR_INVALID_ARGUMENT;
+  uintptr_t all = 0;
+  for (int64_t i = 0; i < count; ++i) {
+    if (!tensors[i] || (!in_place && !outs[i])) return GTP_ERR_INVALID_ARGUMENT;
+    all |= reinterpret_cast<uintptr_t>(tensors[i]);
+    if (!in_place) all |= reinterpret_cast<uintptr_t>(outs[i]);
+  }
+  rc = shape_of(shape, all, c.s, c.bytes);
+  if (rc != GTP_OK) return rc;
+  c.most = per_launch(c.s, groups, count);
+  return c.most < 1 ? GTP_ERR_UNSUPPORTED : GTP_OK;
+}
+
 }  // namespace states
 }  // namespace gtp
 
 using namespace gtp;
 
+extern "C" int gtp_reorder_states_check(const void* const* tensors, int64_t count,
+                                        const gtp_state_shape* shape, int64_t groups,
+                                        int32_t beams) {
+  states::Call c;
+  return states::look(tensors, nullptr, true, count, shape, groups, beams, c);
+}
+
 extern "C" int gtp_reorder_states(void* const* tensors, int64_t count,
                                   const gtp_state_shape* shape, const int32_t* parents,
                                   int64_t groups, int32_t beams, int32_t* bad, void* stream) {
-  int rc = states::check(shape, count, groups, beams);
-  if (rc != GTP_OK) return rc;
-  if (count == 0 || groups == 0 || shape->run_bytes == 0) return GTP_OK;
-  if (!tensors || !parents) return GTP_ERR_INVALID_ARGUMENT;
-  uintptr_t all = 0;
-  for (int64_t i = 0; i < count; ++i) {
-    if (!tensors[i]) return GTP_ERR_INVALID_ARGUMENT;
-    all |= reinterpret_cast<uintptr_t>(tensors[i]);
-  }
-  states::Shape s;
-  int bytes;
-  rc = states::shape_of(shape, all, s, bytes);
-  if (rc != GTP_OK) return rc;
-  const int64_t most = states::per_launch(s, groups, count);
-  if (most < 1) return GTP_ERR_UNSUPPORTED;
+  states::Call c;
+  const int rc = states::look(tensors, nullptr, true, count, shape, groups, beams, c);
+  if (rc != GTP_OK || c.most == 0) return rc;
+  if (!parents) return GTP_ERR_INVALID_ARGUMENT;
+  const states::Shape& s = c.s;
+  const int64_t most = c.most;
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   for (int64_t first = 0; first < count; first += most) {
     const int64_t n = count - first < most ? count - first : most;
     states::List l;
     for (int64_t i = 0; i < n; ++i) l.p[i] = tensors[first + i];
-    switch (bytes) {
+    switch (c.bytes) {
       case 16: states::reorder<16>(l, s, parents, n, groups, beams, bad, st); break;
       case 8: states::reorder<8>(l, s, parents, n, groups, beams, bad, st); break;
       case 4: states::reorder<4>(l, s, parents, n, groups, beams, bad, st); break;
@@ -263,21 +287,11 @@ extern "C" int gtp_reorder_states(void* const* tensors, int64_t count,
 extern "C" int gtp_expand_states(const void* const* tensors, void* const* outs, int64_t count,
                                  const gtp_state_shape* shape, int64_t groups, int32_t beams,
                                  void* stream) {
-  int rc = states::check(shape, count, groups, beams);
-  if (rc != GTP_OK) return rc;
-  if (count == 0 || groups == 0 || shape->run_bytes == 0) return GTP_OK;
-  if (!tensors || !outs) return GTP_ERR_INVALID_ARGUMENT;
-  uintptr_t all = 0;
-  for (int64_t i = 0; i < count; ++i) {
-    if (!tensors[i] || !outs[i]) return GTP_ERR_INVALID_ARGUMENT;
-    all |= reinterpret_cast<uintptr_t>(tensors[i]) | reinterpret_cast<uintptr_t>(outs[i]);
-  }
-  states::Shape s;
-  int bytes;
-  rc = states::shape_of(shape, all, s, bytes);
-  if (rc != GTP_OK) return rc;
-  const int64_t most = states::per_launch(s, groups, count);
-  if (most < 1) return GTP_ERR_UNSUPPORTED;
+  states::Call c;
+  const int rc = states::look(tensors, outs, false, count, shape, groups, beams, c);
+  if (rc != GTP_OK || c.most == 0) return rc;
+  const states::Shape& s = c.s;
+  const int64_t most = c.most;
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   const uint32_t tiles = (s.units + states::kBlock - 1) / states::kBlock;
   for (int64_t first = 0; first < count; first += most) {
@@ -292,7 +306,7 @@ extern "C" int gtp_expand_states(const void* const* tensors, void* const* outs, 
       hipLaunchKernelGGL(kernel, grid, block, 0, st, l, s, (uint32_t)groups, beams, tiles,
                          (uint32_t)n);
     };
-    switch (bytes) {
+    switch (c.bytes) {
       case 16: run(states::expand_kernel<16>); break;
       case 8: run(states::expand_kernel<8>); break;
       case 4: run(states::expand_kernel<4>); break;

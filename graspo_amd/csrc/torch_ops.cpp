@@ -1695,16 +1695,24 @@ void reorder_states_(at::TensorList states, const at::Tensor& parents, int64_t b
   if (check) bad = at::zeros({1}, parents.options());
   std::vector<void*> p;
   p.reserve(states.size());
-  for (size_t i = 0; i < states.size();) {
-    p.clear();
-    size_t j = i;
-    for (; j < states.size() && same_shape(shapes[i], shapes[j]); ++j) p.push_back(states[j].data_ptr());
-    check_rc(gtp_reorder_states(p.data(), (int64_t)p.size(), &shapes[i], parents.data_ptr<int32_t>(),
-                                R / beams, (int32_t)beams,
-                                check ? bad.data_ptr<int32_t>() : nullptr, st),
-             "gtp_reorder_states");
-    i = j;
-  }
+  for (const at::Tensor& t : states) p.push_back(t.data_ptr());
+  // neighbours of one shape in a call; of several shapes all are looked at before
+  // any is moved
+  const auto alike = [&](auto call) {
+    for (size_t i = 0, j = 0; i < p.size(); i = j) {
+      while (j < p.size() && same_shape(shapes[i], shapes[j])) ++j;
+      check_rc(call(&p[i], (int64_t)(j - i), &shapes[i]), "gtp_reorder_states");
+    }
+  };
+  const int64_t groups = R / beams;
+  alike([&](void** q, int64_t n, const gtp_state_shape* s) {
+    return n == (int64_t)p.size() ? GTP_OK
+                                  : gtp_reorder_states_check(q, n, s, groups, (int32_t)beams);
+  });
+  alike([&](void** q, int64_t n, const gtp_state_shape* s) {
+    return gtp_reorder_states(q, n, s, parents.data_ptr<int32_t>(), groups, (int32_t)beams,
+                              check ? bad.data_ptr<int32_t>() : nullptr, st);
+  });
   for (const at::Tensor& t : states)
     if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
   TORCH_CHECK(!check || bad.item<int32_t>() == 0,

@@ -851,13 +851,20 @@ typedef struct gtp_state_shape {
  * (`tensors` is a HOST array, read during the call) becomes row parents[r], for
  * the groups * beams rows r, all at once.  parents[r] lies in r's group of
  * `beams` rows; where it does not, the row stays and *bad (or NULL; the caller
- * zeroes it) is set to 1.  The tensors must not overlap.  beams <= 64.
+ * zeroes it) is set to 1.  The tensors must not overlap.  beams <= 64; rows of
+ * 2^31 units or more (of 16 bytes, or what alignment, strides and lengths leave
+ * of them) return GTP_ERR_UNSUPPORTED.
+ * gtp_reorder_states_check -- what gtp_reorder_states would say of its
+ * arguments, nothing launched: for states of several shapes, of which none is
+ * to be moved where one is refused.
  * gtp_expand_states -- outs[i] [groups * beams] contiguous rows: row
  * g * beams + k is row g of tensors[i].
  */
 int gtp_reorder_states(void* const* tensors, int64_t count, const gtp_state_shape* shape,
                        const int32_t* parents, int64_t groups, int32_t beams, int32_t* bad,
                        void* stream);
+int gtp_reorder_states_check(const void* const* tensors, int64_t count,
+                             const gtp_state_shape* shape, int64_t groups, int32_t beams);
 int gtp_expand_states(const void* const* tensors, void* const* outs, int64_t count,
                       const gtp_state_shape* shape, int64_t groups, int32_t beams, void* stream);
 
