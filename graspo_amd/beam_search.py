@@ -83,7 +83,7 @@ def beam_step(logits: torch.Tensor, state: BeamState, *, eos_token_id: int, pad_
     join the pool at score / (tokens so far) ** ``length_penalty``, and the
     first K others become the beams.  A group is done when its pool is full and
     no live beam's score, divided by the present length, is above the pool's
-    last (``early_stopping``: when it is full).  ``logits``: [G * K, V] or
+    last (``early_stopping``, a bool: when it is full).  ``logits``: [G * K, V] or
     [G, K, V] (bf16, fp16, fp32; beams may share a row by a stride of 0).
     ``allow_mask``: as :func:`ops.sample`'s, tokens that may follow; the softmax
     is over all."""

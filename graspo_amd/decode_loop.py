@@ -255,6 +255,7 @@ class BeamDecodeState:
     def __init__(self, sequences: torch.Tensor, num_beams: int, eos_token_id: int,
                  pad_token_id: int, max_new_tokens: int, length_penalty: float,
                  early_stopping: bool):
+        self.early_stopping = ops.truth(early_stopping, "early_stopping")
         if sequences.device.type != "cuda":
             raise RuntimeError("graspo_amd decode loop: sequences must be on a GPU; "
                                "there is no CPU path")
@@ -264,7 +265,6 @@ class BeamDecodeState:
         length_of(max(T, 1), length_penalty)  # (a penalty that the last step would refuse)
         self.args = dict(eos_token_id=int(eos_token_id), pad_token_id=int(pad_token_id),
                          length_penalty=float(length_penalty))
-        self.early_stopping = bool(early_stopping)
         self.tokens = torch.empty((T, G * K), dtype=torch.int64, device=dev)
         self.parents = torch.empty((T, G * K), dtype=torch.int32, device=dev)
         self.prompt = sequences
@@ -337,6 +337,7 @@ def generate_beams_with_kv_cache(self, *, sequences: torch.Tensor, eos_token_id:
     sampling loops'): ``num_beams`` beams of each, of which the ``num_return``
     best hypotheses by logprob / length ** ``length_penalty`` are returned:
     ``(sequences [G * num_return, S], scores [G, num_return], timings)``.
+    ``early_stopping`` is :func:`beam_search.beam_step`'s, a bool.
 
     The prompts are read once, their states expanded to the beams; from then on
     the cache's tensors (nested in tuples, lists and dicts, rows first) follow

@@ -507,6 +507,14 @@ def beam_candidates(logits: torch.Tensor, scores: torch.Tensor, *, candidates: i
                                                   _stream(logits)))
 
 
+def truth(value, name: str) -> bool:
+    """``value``, a bool and nothing that only passes for one: the word "never"
+    would."""
+    if not isinstance(value, bool):
+        raise ValueError(f"{name} must be True or False, got {value!r}")
+    return value
+
+
 class BeamAdvance(NamedTuple):
     tokens: torch.Tensor       # int64 [G * K], what each slot goes on with
     parents: torch.Tensor      # int32 [G * K], the row that each slot continues
@@ -525,10 +533,10 @@ def beam_advance(candidates: BeamCandidates, scores: torch.Tensor, pool_scores: 
     """Moves every group on by its candidates (include/graspo_tokpath.h has the
     rules), into new tensors; ``length`` is what finished scores are divided
     by.  ``tokens_out`` and ``parents_out``: written in the new ones' place."""
-    c = candidates
+    c, early = candidates, truth(early_stopping, "early_stopping")
     return BeamAdvance(*load().beam_advance(
         c.scores, c.beams, c.tokens, scores, pool_scores, pool_rows, pool_steps, done,
-        int(eos_token_id), int(pad_token_id), float(length), int(step), bool(early_stopping),
+        int(eos_token_id), int(pad_token_id), float(length), int(step), early,
         tokens_out, parents_out, _stream(scores)))
 
 
@@ -540,9 +548,10 @@ def beam_step(logits: torch.Tensor, scores: torch.Tensor, pool_scores: torch.Ten
               ) -> tuple[BeamAdvance, torch.Tensor]:
     """:func:`beam_candidates` (2 K of them) and :func:`beam_advance` in two
     launches; also the rows' status."""
+    early = truth(early_stopping, "early_stopping")
     out = load().beam_step(
         logits, scores, pool_scores, pool_rows, pool_steps, done, 2 * scores.shape[-1],
-        int(eos_token_id), int(pad_token_id), float(length), int(step), bool(early_stopping),
+        int(eos_token_id), int(pad_token_id), float(length), int(step), early,
         allow_mask, tokens_out, parents_out, _stream(logits))
     return BeamAdvance(*out[:7]), out[7]
 
