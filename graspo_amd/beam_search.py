@@ -16,6 +16,7 @@ replaced are moved.
 
 from __future__ import annotations
 
+import copy
 import math
 from typing import Any, Callable, NamedTuple
 
@@ -185,7 +186,10 @@ def map_states(cache: Any, change: Callable[[list[torch.Tensor]], list[torch.Ten
         if isinstance(c, torch.Tensor):
             return next(new)
         if isinstance(c, dict):
-            return type(c)((k, rebuild(v)) for k, v in c.items())
+            d = copy.copy(c)  # (of its own kind, with what that keeps beside the items)
+            for k, v in c.items():
+                d[k] = rebuild(v)
+            return d
         if isinstance(c, tuple) and hasattr(c, "_fields"):
             return type(c)(*(rebuild(v) for v in c))
         if isinstance(c, (list, tuple)):
