@@ -287,6 +287,8 @@ class BeamDecodeState:
         out = dict(tokens_out=self.tokens[t], parents_out=self.parents[t])
         if dist.is_available() and dist.is_initialized():
             # rank 0's candidates everywhere, as the sampling loops' tokens
+            if logits.shape[-1] > 1 and logits.stride(-1) != 1:
+                logits = logits.contiguous()
             c = ops.beam_candidates(logits, old.scores, done=old.done)
             for x in c[:3]:
                 dist.broadcast(x, src=0)
