@@ -296,6 +296,10 @@ __device__ __forceinline__ void load_group(const T* row, int64_t G, int64_t V, b
 // report no error and leave work undone.  The last row of y may hold workgroups
 // past the end, which have nothing to do.
 constexpr int64_t kGridItems = 1ll << 31;
+// Where a grid has one dimension: the entry point refuses what does not fit.
+inline bool fits_one_dimension(int64_t workgroups, int64_t threads) {
+  return workgroups < (1ll << 32) / threads;
+}
 template <int kThreads>
 __device__ __forceinline__ int64_t flat_workgroup() {
   return blockIdx.x + (int64_t)blockIdx.y * (kGridItems / kThreads);

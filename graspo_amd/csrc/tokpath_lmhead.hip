@@ -577,7 +577,8 @@ int lm_head_run(const uint16_t* hidden, int64_t N, int64_t K, int64_t hidden_str
   a.ldl = logits_stride;
   float* xt = reinterpret_cast<float*>(reinterpret_cast<unsigned char*>(workspace) + p.partial_bytes);
   const int64_t grid = lmh::grid_of(p.n_vg + a.tail, p.n_tt, p.blocks);
-  if (grid > 0x7FFFFFFFll) return GTP_ERR_UNSUPPORTED;
+  if (!fits_one_dimension(grid, lmh::kThreads) || !fits_one_dimension((N + 3) / 4, 256))
+    return GTP_ERR_UNSUPPORTED;
   if (out_logits)
     launch_timed(lmh::lm_head_lse_kernel<true>, dim3((unsigned)grid), dim3(lmh::kThreads), s, a);
   else

@@ -920,7 +920,7 @@ extern "C" int gtp_stream_read_rows(const void* data, int64_t rows, int64_t row_
     return GTP_ERR_INVALID_ARGUMENT;
   if ((reinterpret_cast<uintptr_t>(data) & 15u) || (row_bytes & 15) || (row_stride_bytes & 15))
     return GTP_ERR_UNSUPPORTED;
-  if (rows > 0x7FFFFFFFll) return GTP_ERR_UNSUPPORTED;
+  if (!fits_one_dimension(rows, 1024)) return GTP_ERR_UNSUPPORTED;
   if (rows == 0 || row_bytes == 0) return GTP_OK;
   launch_timed(stream_read_kernel, dim3((unsigned)rows), dim3(1024),
                reinterpret_cast<hipStream_t>(stream), reinterpret_cast<const unsigned char*>(data),
@@ -933,7 +933,7 @@ extern "C" int gtp_lse_partial_rows(const void* logits, int dtype, int64_t N, in
                                     int targets_int64, float* state, int accumulate, void* stream) {
   if (N < 0 || Vc <= 0 || row_stride < Vc || col_offset < 0 || (N > 0 && (!logits || !state)))
     return GTP_ERR_INVALID_ARGUMENT;
-  if (N > 0x7FFFFFFFll) return GTP_ERR_UNSUPPORTED;
+  if (!fits_one_dimension(N, kLpBlock)) return GTP_ERR_UNSUPPORTED;
   if (N == 0) return GTP_OK;
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   const dim3 grid((unsigned)N), block(kLpBlock);
@@ -982,7 +982,7 @@ extern "C" int gtp_logprob_backward_split_rows(const float* logits, int64_t N, i
   if (N < 0 || V <= 0 || row_stride < V || grad_stride < V ||
       (N > 0 && (!logits || !targets || !grad_logprob || !lse || !grad_hi || !grad_lo)))
     return GTP_ERR_INVALID_ARGUMENT;
-  if (N > 0x7FFFFFFFll) return GTP_ERR_UNSUPPORTED;
+  if (!fits_one_dimension(N, kLpBlock)) return GTP_ERR_UNSUPPORTED;
   if (N == 0) return GTP_OK;
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   hipLaunchKernelGGL(logprob_backward_split_kernel, dim3((unsigned)N), dim3(kLpBlock), 0, s,
@@ -1164,10 +1164,10 @@ extern "C" int gtp_logprob_backward_rows(const void* logits, int dtype, int64_t 
   if (N < 0 || V <= 0 || row_stride < V || grad_stride < V ||
       (N > 0 && (!logits || !targets || !grad_logprob || !lse || !grad)))
     return GTP_ERR_INVALID_ARGUMENT;
-  if (N > 0x7FFFFFFFll) return GTP_ERR_UNSUPPORTED;
+  if (!fits_one_dimension(N, kLpBlock)) return GTP_ERR_UNSUPPORTED;
   if (N == 0) return GTP_OK;
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  const int slices = N <= 0x3FFFFFF ? row_slices(dtype, N, V) : 1;
+  const int slices = row_slices(dtype, N, V);  // (more than one: of few rows)
   const dim3 grid((unsigned)(N * slices)), block(kLpBlock);
   switch (dtype) {
     case GTP_DTYPE_BF16:

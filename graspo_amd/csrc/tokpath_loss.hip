@@ -130,7 +130,7 @@ extern "C" int gtp_graspo_loss_forward(const float* logp, const float* old_logp,
                                        void* stream) {
   if (B <= 0 || T <= 0 || !logp || !old_logp || !adv || !out_loss || !per_seq || !inv_denom)
     return GTP_ERR_INVALID_ARGUMENT;
-  if (B > 0x7FFFFFFFll) return GTP_ERR_UNSUPPORTED;
+  if (!fits_one_dimension(B, kLsBlock)) return GTP_ERR_UNSUPPORTED;
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   hipLaunchKernelGGL(graspo_loss_rows_kernel, dim3((unsigned)B), dim3(kLsBlock), 0, s, logp,
                      old_logp, adv, MaskIn{mask, mask_u8 ? 1 : 0}, T, clip_lo, clip_hi, per_seq,
@@ -146,7 +146,7 @@ extern "C" int gtp_graspo_loss_backward(const float* logp, const float* old_logp
                                         float* grad_logp, void* stream) {
   if (B <= 0 || T <= 0 || !logp || !old_logp || !adv || !inv_denom || !grad_loss || !grad_logp)
     return GTP_ERR_INVALID_ARGUMENT;
-  if (T > (int64_t)0x7FFFFFFF * kLsBlock / B) return GTP_ERR_UNSUPPORTED;  // grid <= 2^31 - 1
+  if (T > ((1ll << 32) - kLsBlock) / B) return GTP_ERR_UNSUPPORTED;  // B T in one dimension
   const int64_t n = B * T;
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   hipLaunchKernelGGL(graspo_loss_backward_kernel, dim3((unsigned)((n + kLsBlock - 1) / kLsBlock)),

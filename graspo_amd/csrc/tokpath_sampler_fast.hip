@@ -1427,7 +1427,7 @@ extern "C" int gtp_sample_route(int dtype, int64_t B, int64_t V, int aligned, in
   if (!params || !out_route || B <= 0 || V <= 0 || hist_len < 0) return GTP_ERR_INVALID_ARGUMENT;
   if (dtype != GTP_DTYPE_F32 && dtype != GTP_DTYPE_BF16 && dtype != GTP_DTYPE_F16)
     return GTP_ERR_INVALID_ARGUMENT;
-  if (V > GTP_SAMPLER_MAX_V || B > 0x7FFFFFFFll) return GTP_ERR_UNSUPPORTED;
+  if (V > GTP_SAMPLER_MAX_V || !fits_one_dimension(B, 1024)) return GTP_ERR_UNSUPPORTED;
   if (greedy_takes(dtype, B, V, params, aligned != 0, hist_len, has_mask != 0)) {
     const FastPlan gp = plan_fast(dtype, B, V, params, true);
     *out_route = GTP_ROUTE_SPLIT_TOPK;
@@ -1557,8 +1557,8 @@ int sampler_args(SamplerArgs& a, const void* logits, int dtype, int64_t B, int64
     return GTP_ERR_INVALID_ARGUMENT;
   if (B > 0 && (!logits || !out_ids)) return GTP_ERR_INVALID_ARGUMENT;
   if (!(params->repetition_penalty > 0.0f)) return GTP_ERR_INVALID_ARGUMENT;
-  // bounded before any size arithmetic below
-  if (V > GTP_SAMPLER_MAX_V || B > 0x7FFFFFFFll) return GTP_ERR_UNSUPPORTED;
+  // bounded before any size arithmetic below (most kernels: 1024 threads a row)
+  if (V > GTP_SAMPLER_MAX_V || !fits_one_dimension(B, 1024)) return GTP_ERR_UNSUPPORTED;
   if (allow_mask && mask_stride < (V + 31) / 32) return GTP_ERR_INVALID_ARGUMENT;
   if (hist_len < 0) return GTP_ERR_INVALID_ARGUMENT;
   if (history && hist_len > 0 && hist_stride < hist_len) return GTP_ERR_INVALID_ARGUMENT;
