@@ -14,10 +14,10 @@
 //   last of them.  Within a row the order by logit is the order by score, so n
 //   per slice do.
 // - beam_merge_kernel: a workgroup per group turns the slices' sums into each
-//   row's log-sum-exp in 64 bits (scores of different beams are compared, and
-//   a sum rounded to 32 bits would decide near-ties), takes the n best of
-//   K S n candidates and, in its first wave, one lane per candidate, moves the
-//   group on.
+//   row's log-sum-exp in 64 bits (scores of different beams are compared; what
+//   is left of fp32 in them are the slices' sums and their exponentials), takes
+//   the n best of K S n candidates and, in its first wave, one lane per
+//   candidate, moves the group on.
 // The rows' bytes bound the large calls, two launches and the merge's chain of
 // LDS steps the small ones.  bf16 [32 x 8, 248320]: 31 + 9 us (4.1 TB/s; without
 // any candidates 28, without exponentials either 27); [1 x 4, 151936]: 7.5 + 6.6
@@ -40,7 +40,7 @@ constexpr int kNoted = 320;     // vectors noted per wave: 63 and a chunk's 256
 constexpr int kCap = 640;       // list entries per wave: kMaxSlots and a batch's 512
 constexpr int kMaxN = 64;       // candidates: one lane each
 constexpr int kMaxK = 32;
-constexpr int kMaxSlots = 80;   // keys that a slice gives: n and up to a quarter or half more
+constexpr int kMaxSlots = 80;   // keys that a slice gives: n and some more (slots_of)
 constexpr int kMaxKeys = 8192;  // K S slots: what the merge holds in registers
 
 struct Rows {
@@ -531,9 +531,8 @@ __device__ __forceinline__ void advance(const State& st, const Before& old, cons
     }
   }
   // the best that a live beam's score reaches at this length
-  const float best = going ? (float)((double)lane_float(score, __ffsll((unsigned long long)going) - 1) /
-                                     st.length)
-                           : kNegInf;
+  const int first = going ? __ffsll((unsigned long long)going) - 1 : 0;
+  const float best = going ? (float)((double)lane_float(score, first) / st.length) : kNegInf;
   if (lane == 0)
     st.new_done[g] = (last > kNegInf && (st.early || last >= best)) || !going ? 1 : 0;
 }
@@ -959,7 +958,8 @@ extern "C" size_t gtp_beam_workspace_bytes(const gtp_beam_rows* rows) {
   if (rows->groups == 0) return 8;
   int64_t S, L;
   beam::slices_of(rows->groups, rows->beams, rows->candidates, rows->vocab, S, L);
-  return (size_t)(rows->groups * rows->beams * S) * (size_t)(beam::slots_of(rows->candidates) + 1) * 8;
+  const int64_t slots = beam::slots_of(rows->candidates);
+  return (size_t)(rows->groups * rows->beams * S) * (size_t)(slots + 1) * 8;
 }
 
 extern "C" int gtp_beam_candidates(const gtp_beam_rows* rows, float* out_scores,

@@ -6,13 +6,17 @@
 //   v = s_e g B_e              [N, r]       dx  = v A_e              [N, K]
 //   dA_e = sum_n v_n^T x_n     [r, K]       dB_e = sum_n g_n^T u_n   [O, r]
 // (base's gradient is g).  r is small: every product reads or writes one long
-// matrix once and is bound by that, so there are three kernels, each on the
-// matrix cores (16x16x32 for 16-bit types, 16x16x4 for fp32):
+// matrix once (a backward's two read g, for v and for dB) and is bound by that, so
+// there are three kernels, each on the matrix cores (16x16x32 for 16-bit types,
+// 16x16x4 for fp32):
 //
 // - shrink_kernel: rows x long axis -> [rows, r], the long axis split over
 //   waves and workgroups, fp32 partial sums.
 // - expand_kernel: [rows, r] -> rows x long axis, added to base.
 // - outer_kernel: two tall matrices -> [r, long], rows split over workgroups.
+//   Each block of 64 (fp32) or 128 columns loads all of the low-rank operand,
+//   which is small beside them at a rank of 16 in 16 bits (a quarter of their
+//   bytes) and as much as they are at 64 in fp32.
 //
 // Rows are sorted by adapter on the device (plan_kernel: a stable counting sort
 // of the requests), each adapter's run padded to whole tiles, so a tile has one
@@ -29,8 +33,8 @@
 //
 // Measured, bf16, 8192 rows of 4096 x 4096 of rank 16 with all gradients: shrink
 // 22 and 19 us (64 MB each), expand 35 (128 MB read and written) and 22 (64 MB
-// written), outer 31 (128 MB), the rest 10; 138 in all, where 403 MB at the
-// card's copying rate are 79.  fp32, 2000 rows of 2048 x 5632, rank 64: 154 us,
+// written), outer 31 (128 MB), the rest 10; 138 in all, where 403 MB, and
+// g once more, at the card's copying rate are 92.  fp32, 2000 rows of 2048 x 5632, rank 64: 154 us,
 // of which the products at fp32's matrix rate are about half.  A few rows: two
 // launches of 4-5 us.  Tried without gain: strips' weights loaded ahead (the
 // registers cost a wave per SIMD: 35 -> 41 us), 16 rows per wave with more waves
@@ -68,7 +72,9 @@ struct Mat<uint16_t> {
     return gemm::Bf16::mul(__builtin_bit_cast(s16x8, a), __builtin_bit_cast(s16x8, b), c);
   }
   // with a low-rank operand
-  __device__ static __forceinline__ f32x4 meet(u32x4 a, u32x4 low, f32x4 c) { return mma(a, low, c); }
+  __device__ static __forceinline__ f32x4 meet(u32x4 a, u32x4 low, f32x4 c) {
+    return mma(a, low, c);
+  }
   __device__ static __forceinline__ float to(uint16_t v) { return gemm::Bf16::to(v); }
   __device__ static __forceinline__ uint16_t from(float v) { return gemm::Bf16::from(v); }
 };
@@ -110,7 +116,9 @@ struct Mat<float> {
       c = __builtin_amdgcn_mfma_f32_16x16x4f32(u2f(a[j]), u2f(b[j]), c, 0, 0, 0);
     return c;
   }
-  __device__ static __forceinline__ f32x4 meet(u32x4 a, u32x4 low, f32x4 c) { return mma(a, low, c); }
+  __device__ static __forceinline__ f32x4 meet(u32x4 a, u32x4 low, f32x4 c) {
+    return mma(a, low, c);
+  }
   __device__ static __forceinline__ float to(float v) { return v; }
   __device__ static __forceinline__ float from(float v) { return v; }
 };
@@ -461,7 +469,8 @@ __global__ __launch_bounds__(kBlock) void shrink_kernel(Plan plan, const T* x, i
   }
   // the workgroup's steps, its waves by turns
   const int steps = (C + 8 * E - 1) / (8 * E);
-  const int share = (steps + splits * kWaves * kSteps - 1) / (splits * kWaves * kSteps) * kWaves * kSteps;
+  const int turns = (steps + splits * kWaves * kSteps - 1) / (splits * kWaves * kSteps);
+  const int share = turns * kWaves * kSteps;
   const int from = split * share;
   const int to = from + share < steps ? from + share : steps;
   f32x4 acc[RB][NB];
@@ -634,11 +643,9 @@ __global__ __launch_bounds__(kBlock) void low_kernel(Plan plan, const float* low
 // ready: low_kernel's units; null: summed here, which takes less than a launch
 // where a thread has few of them.  turned: as low_kernel's (with ready null).
 template <typename T, int RB>
-__global__ __launch_bounds__(kBlock, __is_same(T, _Float16) ? 3 : 4) void expand_kernel(Plan plan, const float* low, int splits,
-                                                        const float* scales, const T* W, int C,
-                                                        int r, const T* base, int64_t ld_base,
-                                                        T* out, int strips, int blocks,
-                                                        const u32x4* ready, T* turned) {
+__global__ __launch_bounds__(kBlock, __is_same(T, _Float16) ? 3 : 4) void expand_kernel(
+    Plan plan, const float* low, int splits, const float* scales, const T* W, int C, int r,
+    const T* base, int64_t ld_base, T* out, int strips, int blocks, const u32x4* ready, T* turned) {
   constexpr int E = Mat<T>::kE, P = Mat<T>::kParts, MB = E / 4;
   constexpr int kRows = RB * 16;
   constexpr int kStrip = 4 * E;  // columns
@@ -1006,7 +1013,8 @@ int check(const gtp_lora* q) {
     return GTP_ERR_INVALID_ARGUMENT;
   if (q->dtype != GTP_DTYPE_F32 && q->dtype != GTP_DTYPE_BF16 && q->dtype != GTP_DTYPE_F16)
     return GTP_ERR_INVALID_ARGUMENT;
-  if (!q->ids && q->adapters != 1 && q->requests > 0 && q->rows > 0) return GTP_ERR_INVALID_ARGUMENT;
+  if (!q->ids && q->adapters != 1 && q->requests > 0 && q->rows > 0)
+    return GTP_ERR_INVALID_ARGUMENT;
   if (q->rank > kMaxRank || q->adapters > kMaxAdapters || q->in > (1 << 24) ||
       q->out > (1 << 24) || q->requests > (1 << 24) || q->rows > (1 << 24) ||
       q->requests * q->rows > (1 << 24) - 131072 ||
@@ -1016,7 +1024,9 @@ int check(const gtp_lora* q) {
   return GTP_OK;
 }
 
-bool aligned(const void* p, uintptr_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; }
+bool aligned(const void* p, uintptr_t to) {
+  return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0;
+}
 
 // few: the plan is not yet in the state, and need not be
 Plan plan_of(const gtp_lora* q, const Sizes& z, const void* state, bool few) {
@@ -1036,7 +1046,8 @@ Plan plan_of(const gtp_lora* q, const Sizes& z, const void* state, bool few) {
 template <typename T, int RB, int NB>
 void shrink(const Plan& p, const T* x, int64_t ld, const T* W, int64_t C, int r, int splits,
             float* low, Scale scale, int32_t* kept, hipStream_t s) {
-  const dim3 grid((uint32_t)((int64_t)p.tiles * splits + (scale.to ? 1 : 0)), (uint32_t)((r + kRankStep - 1) / kRankStep));
+  const dim3 grid((uint32_t)((int64_t)p.tiles * splits + (scale.to ? 1 : 0)),
+                  (uint32_t)((r + kRankStep - 1) / kRankStep));
   hipLaunchKernelGGL((shrink_kernel<T, RB, NB>), grid, dim3(kBlock), 0, s, p, x, ld, W, (int)C, r,
                      splits, low, scale, kept);
 }
@@ -1045,13 +1056,16 @@ void shrink(const Plan& p, const T* x, int64_t ld, const T* W, int64_t C, int r,
             float* low, Scale scale, int32_t* kept, hipStream_t s) {
   const auto run = [&](auto kernel) { kernel(p, x, ld, W, C, r, splits, low, scale, kept, s); };
   constexpr int kLarge = sizeof(T) == 4 ? 2 : 4;
-  if (p.T == 16) run(r <= 16 ? shrink<T, 1, 1> : r <= kWideRank ? shrink<T, 1, 2> : shrink<T, 1, 4>);
-  else run(r <= 16 ? shrink<T, 4, 1> : r <= kWideRank ? shrink<T, 4, 2> : shrink<T, kLarge, 4>);
+  if (p.T == 16)
+    run(r <= 16 ? shrink<T, 1, 1> : r <= kWideRank ? shrink<T, 1, 2> : shrink<T, 1, 4>);
+  else
+    run(r <= 16 ? shrink<T, 4, 1> : r <= kWideRank ? shrink<T, 4, 2> : shrink<T, kLarge, 4>);
 }
 
 template <typename T>
-void expand(const Plan& p, const float* low, int splits, const float* scales, const T* W, int64_t C, int r,
-            const T* base, int64_t ld_base, T* out, const u32x4* ready, T* turned, hipStream_t s) {
+void expand(const Plan& p, const float* low, int splits, const float* scales, const T* W, int64_t C,
+            int r, const T* base, int64_t ld_base, T* out, const u32x4* ready, T* turned,
+            hipStream_t s) {
   constexpr int E = Mat<T>::kE, P = Mat<T>::kParts;
   const int64_t wave_strips = (C + 4 * E * kWaves - 1) / (4 * E * kWaves);
   // strips per wave: fewer where there are few tiles
@@ -1140,7 +1154,8 @@ Work work_of(const gtp_lora* q, const Sizes& z) {
   // 32 outer_kernel runs two to a CU, which 512 fill once, and its four waves have
   // whole steps (fp32, 2000 rows of 2048 x 5632, rank 64: 37 us for 43; at lower
   // ranks 768 are as good, fp32 with a rank of 128 is level)
-  const int64_t cols = 16 * (16 / size), blocks = (q->in + cols - 1) / cols + (q->out + cols - 1) / cols;
+  const int64_t cols = 16 * (16 / size);
+  const int64_t blocks = (q->in + cols - 1) / cols + (q->out + cols - 1) / cols;
   int64_t chunks = r > kWideRank ? 512 / blocks : (768 + blocks - 1) / blocks;
   if (chunks > (n + 127) / 128) chunks = (n + 127) / 128;
   if (chunks < 1) chunks = 1;
@@ -1263,7 +1278,8 @@ extern "C" int gtp_lora_backward(const gtp_lora* q, const gtp_lora_grads* d, con
   if (!q->x || !q->a || !q->b || !d->grad || !state || !workspace ||
       q->x_stride < 0 || d->grad_stride < 0 || state_bytes < gtp_lora_state_bytes(q) ||
       workspace_bytes < gtp_lora_backward_workspace_bytes(q) || !lora::aligned(state, 16) ||
-      !lora::aligned(workspace, 256) || !lora::aligned(q->x, size) || !lora::aligned(q->a, size) || !lora::aligned(q->b, size) ||
+      !lora::aligned(workspace, 256) || !lora::aligned(q->x, size) ||
+      !lora::aligned(q->a, size) || !lora::aligned(q->b, size) ||
       !lora::aligned(d->grad, size) || (d->grad_x && !lora::aligned(d->grad_x, size)) ||
       (d->grad_a && !lora::aligned(d->grad_a, size)) ||
       (d->grad_b && !lora::aligned(d->grad_b, size)))

@@ -5,17 +5,20 @@
 // as bytes.
 //
 // - reorder_kernel, in place: row g K + k becomes row parent[g K + k], of the
-//   same group.  A thread holds the same few bytes of all K rows: it loads those
-//   that go elsewhere, then stores, so any map of a group onto itself (swaps,
-//   cycles) needs no second buffer; where every source stays, as the parents of
-//   a beam step do, rows that stay are neither read nor written.
+//   same group.  A thread holds the same few bytes of all K rows.  Where every
+//   source stays, as the parents of a beam step do, it loads and stores those
+//   that go elsewhere, four at a time, and rows that stay are neither read nor
+//   written.  Any other map of a group onto itself (swaps, cycles) needs no
+//   second buffer either: all rows are loaded, moving or not, then the moving
+//   ones stored.
 // - expand_kernel: row g of a prompt's state to the K rows of its beams, each
 //   byte read once.
 // Bound by memory: the bytes of the rows that change, read and written.  3 of 8
 // beams of 4 groups, 16 tensors of 268 MB filled to 4001 of 4096: 545 us, 5.2
 // TB/s; a prompt's 24 tensors to 4 beams, 0.98 GB: 180 us, 5.4 TB/s (the card
 // copies at 5.1).  One row of moves at a time and conditional loads took 234
-// registers for 8 beams; lists of four moves take 76.
+// registers for 8 beams; lists of four moves take 76.  The same 16 tensors with
+// all rows of a group in a cycle: 1.73 ms, 4.8 TB/s; two of each 8 swapped: 1.06.
 #include "tokpath_common.h"
 
 namespace gtp {

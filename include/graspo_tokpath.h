@@ -883,7 +883,8 @@ int gtp_expand_states(const void* const* tensors, void* const* outs, int64_t cou
  *   ids   [requests] int32 / int64, or NULL: all rows have adapter 0 of 1
  * all of `dtype` but scales and ids, any alignment of whole elements.  Rows
  * without an adapter are base's; an id outside [-1, adapters) gives rows of NaN.
- * Sums in fp32; the rank-sized ones meet 16-bit operands as two 16-bit parts.
+ * Sums in fp32; the rank-sized ones meet 16-bit operands as two 16-bit parts,
+ * 16 bits of them (infinities and NaN are the formula's).
  * rank <= 256, adapters <= 1024, in and out <= 2^24, requests * rows <= 2^24 -
  * 2^17: others return GTP_ERR_UNSUPPORTED.
  */

@@ -39,7 +39,8 @@ def test_equal_rows(G, K, V, n, above, dtype):
     want = ranked(x, allowed, G, K, n)
     assert [list(zip(b, t)) for b, t in zip(got.beams.tolist(), got.tokens.tolist())] == want
     lse = math.log(above * math.e + (V - above))
-    exact = torch.tensor([[-3.0 + float(x[t]) - lse for _, t in w] for w in want], dtype=torch.float64)
+    exact = torch.tensor([[-3.0 + float(x[t]) - lse for _, t in w] for w in want],
+                         dtype=torch.float64)
     # V exponentials, 256 steps of 2^-24 in all, and c's own rounding
     assert (got.scores.double().cpu() - exact).abs().max() <= 256 * 2.0 ** -24 + 32 * 2.0 ** -24
     assert not got.status.any()

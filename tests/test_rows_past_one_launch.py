@@ -24,7 +24,8 @@ def entry(name, *types):
 def test_rows_of_256_threads(N):
     f = entry("gtp_lse_partial_rows", VP, I32, I64, I64, I64, I64, VP, I32, VP, I32, VP)
     assert f(P, 0, N, 8, 8, 0, P, 1, P, 0, None) == UNSUPPORTED
-    f = entry("gtp_logprob_backward_rows", VP, I32, I64, I64, I64, I64, VP, I32, VP, VP, VP, I64, VP)
+    f = entry("gtp_logprob_backward_rows", VP, I32, I64, I64, I64, I64, VP, I32, VP, VP, VP, I64,
+              VP)
     assert f(P, 0, N, 8, 8, 0, P, 1, P, P, P, 8, None) == UNSUPPORTED
     f = entry("gtp_logprob_backward_split_rows", VP, I64, I64, I64, I64, VP, I32, VP, VP, VP, VP,
               I64, VP)
@@ -57,4 +58,5 @@ def test_rows_of_1024_threads(B):
 def test_rows_of_the_matrix_products():
     f = entry("gtp_lm_head_logprob_rows", VP, I64, I64, I64, VP, I64, I64, VP, I32, VP, VP, VP, VP,
               VP, SZ, VP)
-    assert f(P, (1 << 26) + 1, 128, 128, P, 64, 128, P, 1, P, P, P, P, P, 1 << 60, None) == UNSUPPORTED
+    rc = f(P, (1 << 26) + 1, 128, 128, P, 64, 128, P, 1, P, P, P, P, P, 1 << 60, None)
+    assert rc == UNSUPPORTED

@@ -37,4 +37,5 @@ def test_check(code, change):
     assert L.gtp_reorder_states_check(p, 2, None, 2, 3) == INVALID
     if code != OK:  # refused before anything is launched
         L.gtp_reorder_states.argtypes = [VP, I64, ctypes.POINTER(Shape), VP, I64, I32, VP, VP]
-        assert L.gtp_reorder_states(p, a["count"], s, 4096, a["groups"], a["beams"], None, None) == code
+        got = L.gtp_reorder_states(p, a["count"], s, 4096, a["groups"], a["beams"], None, None)
+        assert got == code
